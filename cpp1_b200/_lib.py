@@ -38,6 +38,8 @@ STATUS_NAMES = {
 MODES = {"3xtf32": 0, "tf32": 1, "bf16": 2}
 FMT_PACKED = 0
 FMT_DENSE = 1
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
 STRUCTS = {"upper": 0, "lower": 1, "symm": 2, "diag": 3, "toeplitz": 4}
 
 
@@ -155,6 +157,12 @@ SIGNATURES = [
     ("smm_gen_x_toeplitz_host", _i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz]),
     ("smm_diag_cols_host_workspace_size", _sz, [_i, _i]),
     ("smm_diag_cols_host", _i, [_vp, _vp, _vp, _i, _i, _vp, _sz]),
+    ("smm_causal_conv", _i, [_vp] * 8 + [_ll, _i, _i, _i, _i, _ll, _ll, _i, _i, _vp]),
+    ("smm_causal_conv_step", _i, [_vp] * 7 + [_i, _i, _i, _i, _ll, _ll, _i, _i, _vp]),
+    ("smm_selective_scan_workspace_size", _sz, [_ll, _i, _i, _i, _i, _i, _i]),
+    ("smm_selective_scan", _i, [_vp] * 13 + [_ll] + [_i] * 6 + [_ll] * 6 + [_i, _i, _i, _vp, _sz, _vp]),
+    ("smm_selective_step", _i, [_vp] * 12 + [_i] * 6 + [_ll] * 6 + [_i, _i, _i, _vp]),
+    ("smm_q4_matvec", _i, [_vp] * 5 + [_i] * 4 + [_ll, _ll, _i, _i, _vp]),
 ]
 
 _lib = None

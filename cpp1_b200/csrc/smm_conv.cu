@@ -1,0 +1,324 @@
+// Short causal convolution: y[t][c] = act(bias[c] + sum_j w[c][j] x[t-W+1+j][c]),
+// per channel a banded lower-triangular Toeplitz matrix of W diagonals.  For
+// packed prompts, and for one new token of each sequence.
+//
+// Bound by memory: each element is read once and written once (W multiplies
+// per element).  A thread owns 16 bytes of channels and walks down a run of
+// consecutive tokens with the last W-1 rows in registers, so a row is read
+// from memory once and W-1 rows per run again from L2.
+//
+// The first min(W-1, length) tokens of a sequence need the state it starts
+// from, and the state it ends with may overwrite that.  Both are done by the
+// threads whose run holds the sequence's last token: they read the old state
+// first and write the new one last, so an update in place has no race, and
+// needs no second launch.  An empty sequence belongs to the run that holds
+// its position (the last run, behind the last row).
+#include "smm_seq.cuh"
+
+namespace smm {
+namespace {
+
+struct ConvParams {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const int* offsets;
+  const void* state_in;
+  void* state_out;
+  const int* slots;
+  void* y;
+  long long tokens, ldx, ldy;
+  int channels, nseq, nslots, run, nruns, ctiles, silu;
+  uint32_t* status;
+};
+
+constexpr int kConvThreads = 128;
+
+template <typename T, int VEC, int W>
+struct ConvLane {
+  static constexpr bool kVec = VEC > 1;
+  float w[W][VEC];  // tap j of each channel
+  float bias[VEC];
+
+  __device__ void load(const ConvParams& p, int c) {
+    float wt[VEC * W];  // [channel][tap]
+    load_f32<T, VEC * W, kVec>(static_cast<const T*>(p.w) + static_cast<long long>(c) * W, wt);
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[j][i] = wt[i * W + j];
+    if (p.bias) {
+      load_f32<T, VEC, kVec>(static_cast<const T*>(p.bias) + c, bias);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) bias[i] = 0.0f;
+    }
+  }
+  // One output row from the W-1 rows before it and its own; the window moves on.
+  __device__ void row(float (&win)[W - 1][VEC], const float (&cur)[VEC], float (&out)[VEC], bool act) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      float a = bias[i];
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) a = fmaf(w[j][i], win[j][i], a);
+      a = fmaf(w[W - 1][i], cur[i], a);
+      out[i] = act ? silu(a) : a;
+#pragma unroll
+      for (int j = 0; j < W - 2; ++j) win[j][i] = win[j + 1][i];
+      win[W - 2][i] = cur[i];
+    }
+  }
+};
+
+template <typename T, int VEC, int W>
+__global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) {
+  constexpr bool kVec = VEC > 1;
+  const int ctile = static_cast<int>(blockIdx.x % p.ctiles);
+  const long long r = static_cast<long long>(blockIdx.x / p.ctiles) * blockDim.y + threadIdx.y;
+  const int c = (ctile * blockDim.x + threadIdx.x) * VEC;
+  if (c >= p.channels || r >= p.nruns) return;
+  const long long t0 = r * p.run;
+  const long long t1 = t0 + p.run < p.tokens ? t0 + p.run : p.tokens;
+  const bool last_run = r == p.nruns - 1;
+  const T* x = static_cast<const T*>(p.x) + c;
+  T* y = static_cast<T*>(p.y) + c;
+  const bool act = p.silu != 0;
+  ConvLane<T, VEC, W> lane;
+  lane.load(p, c);
+
+  // first sequence that reaches into this run or is empty at its start
+  int s = 0;
+  if (p.offsets) {
+    int lo = 0, hi = p.nseq;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(p.offsets + mid + 1) > t0 || __ldg(p.offsets + mid) >= t0)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    s = lo;
+  }
+  for (; s < p.nseq; ++s) {
+    long long b, e;
+    seq_range(p.offsets, s, p.tokens, &b, &e);
+    if (b > t1 || (b == t1 && !last_run)) break;
+    float win[W - 1][VEC];
+    const long long lo = b + W - 1 > t0 ? b + W - 1 : t0;
+    const long long hi = e < t1 ? e : t1;
+    if (lo < hi) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) load_f32<T, VEC, kVec>(x + (lo - (W - 1) + j) * p.ldx, win[j]);
+      long long t = lo;
+      constexpr int U = 4;  // rows in flight
+      for (; t + U <= hi; t += U) {
+        float cur[U][VEC], out[VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_f32<T, VEC, kVec>(x + (t + u) * p.ldx, cur[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          lane.row(win, cur[u], out, act);
+          store_f32<T, VEC, kVec>(y + (t + u) * p.ldy, out);
+        }
+      }
+      for (; t < hi; ++t) {
+        float cur[VEC], out[VEC];
+        load_f32<T, VEC, kVec>(x + t * p.ldx, cur);
+        lane.row(win, cur, out, act);
+        store_f32<T, VEC, kVec>(y + t * p.ldy, out);
+      }
+    }
+    const bool owner = e > b ? (e > t0 && e <= t1) : (b >= t0 && (b < t1 || last_run));
+    if (!owner) continue;
+    const int slot = (p.state_in || p.state_out) ? seq_slot(p.slots, s, p.nslots, p.status) : -1;
+    const long long at = (static_cast<long long>(slot) * p.channels + c) * (W - 1);
+    float old[VEC * (W - 1)];
+    if (p.state_in && slot >= 0) {
+      load_f32<T, VEC*(W - 1), kVec>(static_cast<const T*>(p.state_in) + at, old);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC * (W - 1); ++i) old[i] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) win[j][i] = old[i * (W - 1) + j];
+    const long long len = e - b;
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      if (j < len) {
+        float cur[VEC], out[VEC];
+        load_f32<T, VEC, kVec>(x + (b + j) * p.ldx, cur);
+        lane.row(win, cur, out, act);
+        store_f32<T, VEC, kVec>(y + (b + j) * p.ldy, out);
+      }
+    }
+    if (p.state_out && slot >= 0) {
+      // the window now ends at row b + min(len, W-1); a longer sequence ends later
+      if (len > W - 1) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) load_f32<T, VEC, kVec>(x + (e - (W - 1) + j) * p.ldx, win[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) old[i * (W - 1) + j] = win[j][i];
+      store_f32<T, VEC*(W - 1), kVec>(static_cast<T*>(p.state_out) + at, old);
+    }
+  }
+}
+
+// One token of each sequence: a thread per 16 bytes of channels of one row.
+template <typename T, int VEC, int W>
+__global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvParams p) {
+  constexpr bool kVec = VEC > 1;
+  const int b = static_cast<int>(blockIdx.x / p.ctiles);
+  const int c = (static_cast<int>(blockIdx.x % p.ctiles) * blockDim.x + threadIdx.x) * VEC;
+  if (c >= p.channels) return;
+  const int slot = seq_slot(p.slots, b, p.nslots, p.status);
+  const long long at = (static_cast<long long>(slot) * p.channels + c) * (W - 1);
+  float old[VEC * (W - 1)], win[W - 1][VEC], cur[VEC], out[VEC];
+  if (p.state_in && slot >= 0) {
+    load_f32<T, VEC*(W - 1), kVec>(static_cast<const T*>(p.state_in) + at, old);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC * (W - 1); ++i) old[i] = 0.0f;
+  }
+  load_f32<T, VEC, kVec>(static_cast<const T*>(p.x) + b * p.ldx + c, cur);
+  ConvLane<T, VEC, W> lane;
+  lane.load(p, c);
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) win[j][i] = old[i * (W - 1) + j];
+  lane.row(win, cur, out, p.silu != 0);
+  store_f32<T, VEC, kVec>(static_cast<T*>(p.y) + b * p.ldy + c, out);
+  if (p.state_out && slot >= 0) {
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) old[i * (W - 1) + j] = win[j][i];
+    store_f32<T, VEC*(W - 1), kVec>(static_cast<T*>(p.state_out) + at, old);
+  }
+}
+
+template <typename T, int VEC, bool STEP>
+void launch_width(int width, dim3 grid, dim3 block, const ConvParams& p, cudaStream_t st) {
+  auto go = [&](auto w) {
+    constexpr int W = decltype(w)::value;
+    if constexpr (STEP)
+      conv_step_kernel<T, VEC, W><<<grid, block, 0, st>>>(p);
+    else
+      conv_kernel<T, VEC, W><<<grid, block, 0, st>>>(p);
+  };
+  switch (width) {
+    case 2: return go(std::integral_constant<int, 2>{});
+    case 3: return go(std::integral_constant<int, 3>{});
+    case 4: return go(std::integral_constant<int, 4>{});
+    case 5: return go(std::integral_constant<int, 5>{});
+    case 6: return go(std::integral_constant<int, 6>{});
+    case 7: return go(std::integral_constant<int, 7>{});
+    default: return go(std::integral_constant<int, 8>{});
+  }
+}
+
+// Checks shared by both entries; rows is tokens or batch, nseq sequences.
+int check_conv(const char* who, const ConvParams& p, int width, int dtype, int act, bool step) {
+  if (p.tokens < 0 || p.channels < 0 || p.nseq < 0 || p.nslots < 0)
+    return set_error(SMM_ERR_INVALID, "%s: negative size", who);
+  if (width < 2 || width > 8) return set_error(SMM_ERR_INVALID, "%s: width %d is not in 2..8", who, width);
+  if (!valid_dtype(dtype)) return set_error(SMM_ERR_INVALID, "%s: unknown element type %d", who, dtype);
+  if (act != SMM_ACT_NONE && act != SMM_ACT_SILU)
+    return set_error(SMM_ERR_INVALID, "%s: unknown activation %d", who, act);
+  if (p.ldx < p.channels || p.ldy < p.channels)
+    return set_error(SMM_ERR_INVALID, "%s: row stride shorter than %d channels", who, p.channels);
+  if (!step && !p.offsets && p.nseq > 1)
+    return set_error(SMM_ERR_INVALID, "%s: %d sequences without offsets", who, p.nseq);
+  if ((p.state_in || p.state_out) && !p.slots && p.nslots < p.nseq)
+    return set_error(SMM_ERR_INVALID, "%s: %d states for %d sequences", who, p.nslots, p.nseq);
+  if (p.channels == 0 || (p.tokens == 0 && p.nseq == 0)) return SMM_OK;
+  if (!p.w || (p.tokens > 0 && (!p.x || !p.y))) return set_error(SMM_ERR_INVALID, "%s: null pointer", who);
+  const size_t e = dtype_size(dtype);
+  const Span x{p.x, span_bytes(p.tokens, p.channels, p.ldx, e)}, y{p.y, span_bytes(p.tokens, p.channels, p.ldy, e)};
+  const size_t sb = static_cast<size_t>(p.nslots) * p.channels * (width - 1) * e;
+  const Span si{p.state_in, sb}, so{p.state_out, sb};
+  const Span wv{p.w, static_cast<size_t>(p.channels) * width * e}, bv{p.bias, p.channels * e};
+  const Span off{p.offsets, (static_cast<size_t>(p.nseq) + 1) * 4}, sl{p.slots, static_cast<size_t>(p.nseq) * 4};
+  if (overlaps(y, x) || overlaps(y, si) || overlaps(y, so) || overlaps(y, wv) || overlaps(y, bv) ||
+      overlaps(y, off) || overlaps(y, sl) || overlaps(so, x) || overlaps(so, wv) || overlaps(so, bv) ||
+      overlaps(so, off) || overlaps(so, sl) || (p.state_in != p.state_out && overlaps(si, so)))
+    return set_error(SMM_ERR_INVALID, "%s: an output overlaps an input", who);
+  return SMM_OK;
+}
+
+template <bool STEP>
+int run_conv(ConvParams& p, int width, int dtype, cudaStream_t st) {
+  if (p.channels == 0 || p.nseq == 0) return SMM_OK;
+  p.status = device_status_word();
+  if (!p.status) return set_error(SMM_ERR_CUDA, "device status word unavailable");
+  const int per16 = static_cast<int>(16 / dtype_size(dtype));
+  // 16-byte accesses where every row, the weights and the states keep to them
+  const bool vec = p.channels % per16 == 0 && p.ldx % per16 == 0 && p.ldy % per16 == 0 && aligned_to(p.x, 16) &&
+                   aligned_to(p.y, 16) && aligned_to(p.w, 16) && aligned_to(p.bias, 16) &&
+                   aligned_to(p.state_in, 16) && aligned_to(p.state_out, 16);
+  const int cv = vec ? p.channels / per16 : p.channels;
+  int bx = 32;
+  while (bx < kConvThreads && bx < cv) bx *= 2;
+  const int by = STEP ? 1 : kConvThreads / bx;
+  p.ctiles = (cv + bx - 1) / bx;
+  long long blocks;
+  if (STEP) {
+    blocks = static_cast<long long>(p.ctiles) * p.nseq;
+  } else {
+    // Runs of 16 rows read W-1 of 16 rows twice; shorter ones only where the
+    // GPU would otherwise be short of threads.
+    p.run = 16;
+    while (p.run > 4 && static_cast<long long>(cv) * (p.tokens / p.run) < 148LL * 1024) p.run /= 2;
+    p.nruns = static_cast<int>(p.tokens > 0 ? (p.tokens + p.run - 1) / p.run : 1);
+    blocks = static_cast<long long>(p.ctiles) * ((p.nruns + by - 1) / by);
+  }
+  if (blocks > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "convolution too large for one launch");
+  const dim3 grid(static_cast<unsigned>(blocks)), block(bx, by);
+  if (dtype == SMM_DTYPE_F32) {
+    if (vec)
+      launch_width<float, 4, STEP>(width, grid, block, p, st);
+    else
+      launch_width<float, 1, STEP>(width, grid, block, p, st);
+  } else {
+    if (vec)
+      launch_width<__nv_bfloat16, 8, STEP>(width, grid, block, p, st);
+    else
+      launch_width<__nv_bfloat16, 1, STEP>(width, grid, block, p, st);
+  }
+  count_launch();
+  SMM_CUDA_TRY(cudaGetLastError(), STEP ? "conv_step launch" : "conv launch");
+  return SMM_OK;
+}
+
+}  // namespace
+}  // namespace smm
+
+using namespace smm;
+
+extern "C" int smm_causal_conv(const void* x, const void* w, const void* bias, const int* offsets,
+                               const void* state_in, void* state_out, const int* slots, void* y, long long tokens,
+                               int channels, int width, int nseq, int nslots, long long ldx, long long ldy, int dtype,
+                               int act, void* stream) {
+  SMM_RANGE("smm_causal_conv");
+  ConvParams p{x, w, bias, offsets, state_in, state_out, slots, y, tokens, ldx, ldy, channels, nseq, nslots};
+  p.silu = act == SMM_ACT_SILU;
+  if (int rc = check_conv("smm_causal_conv", p, width, dtype, act, false)) return rc;
+  if (tokens > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "smm_causal_conv: %lld tokens exceed 31 bits", tokens);
+  return run_conv<false>(p, width, dtype, as_stream(stream));
+}
+
+extern "C" int smm_causal_conv_step(const void* x, const void* w, const void* bias, const void* state_in,
+                                    void* state_out, const int* slots, void* y, int batch, int channels, int width,
+                                    int nslots, long long ldx, long long ldy, int dtype, int act, void* stream) {
+  SMM_RANGE("smm_causal_conv_step");
+  ConvParams p{x, w, bias, nullptr, state_in, state_out, slots, y, batch, ldx, ldy, channels, batch, nslots};
+  p.silu = act == SMM_ACT_SILU;
+  if (int rc = check_conv("smm_causal_conv_step", p, width, dtype, act, true)) return rc;
+  if (batch == 0) return SMM_OK;
+  return run_conv<true>(p, width, dtype, as_stream(stream));
+}

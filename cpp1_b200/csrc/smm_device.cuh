@@ -16,6 +16,7 @@ enum : uint32_t {
   kBoundsA = 1u << 16,       // structured left operand (packed triangle / Toeplitz generator)
   kBoundsB = 1u << 17,       // structured right operand
   kBoundsExpand = 1u << 18,  // packed-operand expansion
+  kBoundsSlot = 1u << 19,    // state slot of a sequence (checked in every build)
   // Which wait gave up (ORed with kDevErrTimeout).
   kWaitProducer = 1u << 8,   // producer waiting for a free stage
   kWaitMma = 1u << 9,        // MMA issuer waiting for a staged k-block

@@ -1,0 +1,121 @@
+// Selective state space scan: what the two prompt kernels (smm_scan.cu on the
+// fp32 pipes, smm_scan_umma.cu on the tensor cores) share.
+//
+// Long sequences are split into segments of seg_len tokens so that few heads
+// still fill the GPU.  A segment's work needs the state before it, which is
+// linear in the states that the earlier segments would end with when started
+// from zero:  S_before(j) = exp(a_0+..+a_{j-1}) S_in + sum_k exp(a_{k+1}+..+a_{j-1}) F_k
+// with a_k the sum of d A over segment k and F_k its final state from zero.
+// A first launch writes every F_k and a_k (all but the last segment of each
+// sequence), a second one forms S_before and computes the outputs.
+#pragma once
+#include "smm_seq.cuh"
+
+namespace smm {
+
+struct ScanParams {
+  const void* x;
+  const void* dt;
+  const float* A;
+  const void* B;
+  const void* C;
+  const float* D;
+  const void* z;
+  const float* dt_bias;
+  const int* offsets;
+  const float* state_in;
+  float* state_out;
+  const int* slots;
+  void* y;
+  long long tokens, ldx, lddt, ldb, ldc, ldz, ldy;
+  int nseq, nslots, heads, dim, groups, state_dim;
+  int dt_f32, softplus;
+  int seg_len;       // tokens per segment (tokens or more: no sequence is split)
+  int split;         // seg_len < tokens
+  float* seg_state;  // [segment][head][dim][state_dim]: F_k
+  float* seg_log;    // [segment][head]: a_k
+  uint32_t* status;
+  unsigned long long wait_limit_ns;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float scan_dt(const ScanParams& p, long long t, int h) {
+  const long long i = t * p.lddt + h;
+  float d = p.dt_f32 ? __ldg(static_cast<const float*>(p.dt) + i)
+                     : to_f32(static_cast<const __nv_bfloat16*>(p.dt)[i]);
+  if (p.dt_bias) d += __ldg(p.dt_bias + h);
+  return p.softplus ? softplus(d) : d;
+}
+
+// One segment: sequence, its index in the sequence, how many the sequence
+// has, the index of the sequence's first segment, and the rows.
+struct Segment {
+  int seq, j, count, first;
+  long long begin, end;
+  bool valid;
+};
+
+// Finds segment `seg`: sequences have max(1, ceil(length / seg_len)) each.
+// Called by one full warp.
+__device__ __forceinline__ Segment find_segment(const ScanParams& p, int seg) {
+  Segment r;
+  r.valid = false;
+  r.seq = r.j = r.first = 0;
+  r.count = 1;
+  r.begin = r.end = 0;
+  if (!p.split) {
+    if (seg >= p.nseq) return r;
+    r.seq = seg;
+    r.first = seg;
+    seq_range(p.offsets, seg, p.tokens, &r.begin, &r.end);
+    r.valid = true;
+    return r;
+  }
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int s0 = 0; s0 < p.nseq; s0 += 32) {
+    long long b = 0, e = 0;
+    int n = 0;
+    if (s0 + lane < p.nseq) {
+      seq_range(p.offsets, s0 + lane, p.tokens, &b, &e);
+      n = e > b ? static_cast<int>((e - b + p.seg_len - 1) / p.seg_len) : 1;
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned hit = __ballot_sync(0xFFFFFFFFu, seg < base + incl && n > 0);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int end_incl = __shfl_sync(0xFFFFFFFFu, incl, src);
+      r.count = __shfl_sync(0xFFFFFFFFu, n, src);
+      b = __shfl_sync(0xFFFFFFFFu, b, src);
+      e = __shfl_sync(0xFFFFFFFFu, e, src);
+      r.seq = s0 + src;
+      r.first = base + end_incl - r.count;
+      r.j = seg - r.first;
+      r.begin = b + static_cast<long long>(r.j) * p.seg_len;
+      r.end = r.begin + p.seg_len < e ? r.begin + p.seg_len : e;
+      // overlapping sequences (offsets that decrease) could count past the
+      // workspace's segments; those beyond it have no work
+      r.valid = true;
+      return r;
+    }
+    base += __shfl_sync(0xFFFFFFFFu, incl, 31);
+  }
+  return r;
+}
+
+// Segments that the grid and the workspace provide for.
+inline long long max_segments(long long tokens, int nseq, int seg_len) {
+  return seg_len >= tokens ? nseq : nseq + tokens / seg_len;
+}
+
+// smm_scan_umma.cu
+bool scan_umma_fits(const ScanParams& p, int dtype);
+int scan_umma_launch(ScanParams& p, cudaStream_t st);
+
+}  // namespace smm

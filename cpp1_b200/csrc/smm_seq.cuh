@@ -1,0 +1,129 @@
+// Helpers of the sequence operators (short convolution, selective scan, 4-bit
+// matrix-vector product): vectors of fp32 or bf16 elements widened to fp32,
+// sequence boundaries and state slots, host-side overlap checks.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "smm_device.cuh"
+#include "smm_host.h"
+
+namespace smm {
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  return static_cast<float>(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// N consecutive elements as fp32.  The compiler merges the element loads of
+// an aligned vector type; N * sizeof(T) is a multiple of 16 where VEC loads
+// are used, and the pointer is then 16-byte aligned.
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_f32(const T* p, float (&v)[N]) {
+  if constexpr (VEC && (N * sizeof(T)) % 16 == 0) {
+    constexpr int Q = N * sizeof(T) / 16;
+    uint4 raw[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (sizeof(T) == 4)
+        v[i] = __uint_as_float(w[i]);
+      else
+        v[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32(p[i]);
+  }
+}
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void store_f32(T* p, const float (&v)[N]) {
+  if constexpr (VEC && (N * sizeof(T)) % 16 == 0) {
+    constexpr int Q = N * sizeof(T) / 16;
+    uint32_t w[Q * 4];
+#pragma unroll
+    for (int i = 0; i < Q * 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(v[i]);
+      } else {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = from_f32<T>(v[i]);
+  }
+}
+
+// v * sigmoid(v).  exp(-v) overflows to infinity for v below -88 and the
+// quotient is then the right limit, -0.
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
+// log(1 + exp(v)); above 20 the correction is below half a step of v.
+__device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
+
+// Rows [begin, end) of sequence s, kept inside [0, tokens) whatever the
+// offsets hold.
+__device__ __forceinline__ void seq_range(const int* __restrict__ offsets, int s, long long tokens, long long* begin,
+                                          long long* end) {
+  if (!offsets) {
+    *begin = 0;
+    *end = tokens;
+    return;
+  }
+  long long b = __ldg(offsets + s), e = __ldg(offsets + s + 1);
+  b = b < 0 ? 0 : (b > tokens ? tokens : b);
+  e = e < b ? b : (e > tokens ? tokens : e);
+  *begin = b;
+  *end = e;
+}
+
+// State entry of sequence s, or -1 when it has none.
+__device__ __forceinline__ int seq_slot(const int* __restrict__ slots, int s, int nslots, uint32_t* status) {
+  const int i = slots ? __ldg(slots + s) : s;
+  if (i >= nslots) {
+    if (status) atomicOr(status, kDevErrBounds | kBoundsSlot);
+    return -1;
+  }
+  return i < 0 ? -1 : i;
+}
+
+// ---------------------------------------------------------------- host checks
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+// Bytes from the first to behind the last element of `rows` rows of `width`
+// elements, ld apart.
+inline size_t span_bytes(long long rows, long long width, long long ld, size_t esz) {
+  return rows <= 0 || width <= 0 ? 0 : (static_cast<size_t>(rows - 1) * ld + width) * esz;
+}
+inline bool overlaps(Span a, Span b) {
+  if (!a.p || !b.p || !a.bytes || !b.bytes) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return x < y + b.bytes && y < x + a.bytes;
+}
+inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+inline bool valid_dtype(int d) { return d == SMM_DTYPE_F32 || d == SMM_DTYPE_BF16; }
+inline size_t dtype_size(int d) { return d == SMM_DTYPE_F32 ? 4 : 2; }
+
+}  // namespace smm

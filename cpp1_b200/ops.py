@@ -9,6 +9,7 @@ matrices are their 2N-1 generator with ``T[i][j] = g[(N-1) + (j-i)]``.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -357,6 +358,337 @@ def device_status(stream=None) -> None:
 
 def launch_count() -> int:
     return int(_lib.load().smm_launch_count())
+
+
+# ---------------------------------------------------------------- state-space blocks
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+_ACTS = {None: 0, "silu": 1}
+
+
+def _check_seq(name: str, t: torch.Tensor, like: torch.Tensor, dtype, shape) -> torch.Tensor:
+    """A tensor of this type and shape on like's device; None in shape: any size."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != len(shape) or any(e is not None and n != e for n, e in zip(t.shape, shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+                         f"({', '.join('*' if e is None else str(e) for e in shape)})")
+    return t
+
+
+def _check_x(x: torch.Tensor, dims: int) -> int:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    if x.dim() != dims:
+        raise ValueError(f"x has shape {tuple(x.shape)}, expected {dims} dimensions")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"x must be float32 or bfloat16, got {x.dtype}")
+    return _DTYPES[x.dtype]
+
+
+def _is_rows(t: torch.Tensor) -> bool:
+    """Whether the elements of one row (all dimensions but the first) are
+    contiguous and rows do not overlap; dimensions of size one may have any stride."""
+    shape, stride, width = t.shape, t.stride(), 1
+    for i in range(len(shape) - 1, 0, -1):
+        if shape[i] != 1 and stride[i] != width:
+            return False
+        width *= shape[i]
+    return shape[0] <= 1 or stride[0] >= width
+
+
+def _rows(t: torch.Tensor):
+    """t with contiguous rows (copied if it is laid out otherwise), and the row stride."""
+    if not _is_rows(t):
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else math.prod(t.shape[1:])
+
+
+def _seq_out(out: Optional[torch.Tensor], x: torch.Tensor, shape) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=x.dtype, device=x.device)
+    _check_seq("out", out, x, x.dtype, shape)
+    if not _is_rows(out):
+        raise ValueError("out must have contiguous rows that do not overlap")
+    return out
+
+
+def _states(x, dtype, entry, state, state_out, in_place: bool):
+    """The checked pair of state tensors and their number of entries."""
+    for name, t in (("state", state), ("state_out", state_out)):
+        if t is not None:
+            _check_seq(name, t, x, dtype, (None, *entry))
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+    if state is not None and state_out is not None and state.shape[0] != state_out.shape[0]:
+        raise ValueError(f"state has {state.shape[0]} entries, state_out {state_out.shape[0]}")
+    if state_out is None and in_place:
+        state_out = state
+    n = state.shape[0] if state is not None else state_out.shape[0] if state_out is not None else 0
+    return state, state_out, n
+
+
+def _index(name: str, t: Optional[torch.Tensor], like: torch.Tensor, n: Optional[int]) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    _check_seq(name, t, like, torch.int32, (n,))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _opt(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _on(x: torch.Tensor, stream: Optional[torch.cuda.Stream], call):
+    """call(stream pointer) with x's device current.  Whatever call allocates belongs
+    to the stream that its kernels run on."""
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    if stream is not None:
+        if stream.device != x.device:
+            raise ValueError(f"stream is on {stream.device}, x on {x.device}")
+        with torch.cuda.stream(stream):
+            return call(stream.cuda_stream or None)
+    if x.device.index == torch.cuda.current_device():
+        return call(torch.cuda.current_stream().cuda_stream or None)
+    with torch.cuda.device(x.device):
+        return call(torch.cuda.current_stream().cuda_stream or None)
+
+
+def _sequences(offsets, x):
+    offsets = _index("offsets", offsets, x, None)
+    if offsets is None:
+        return None, 1
+    if offsets.shape[0] < 1:
+        raise ValueError("offsets must have at least one element")
+    return offsets, offsets.shape[0] - 1
+
+
+def _act(activation) -> int:
+    try:
+        return _ACTS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"unknown activation {activation!r}; expected None or 'silu'") from None
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                offsets: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+                state_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                activation: Optional[str] = "silu", out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """y[t, c] = act(bias[c] + sum_j weight[c, j] x[t-W+1+j, c]): a banded
+    lower-triangular Toeplitz matrix per channel, over packed sequences.
+
+    x (tokens, channels) float32 or bfloat16; weight (channels, W), W in 2..8,
+    and bias (channels) of the same type.  Sequence s is the rows
+    [offsets[s], offsets[s+1]) (int32, not decreasing; None: all rows are one sequence).  state (entries,
+    channels, W-1), of x's type, holds the rows before each sequence, oldest first
+    (None: zeros), and state_out receives the rows that each one ends with (None:
+    state is updated in place).  Sequence s uses entry slots[s] (int32; None: s;
+    negative: no state); no two may share one.  Rows outside every sequence are
+    left as they are in `out`, and have no defined values without it."""
+    dt = _check_x(x, 2)
+    tokens, channels = x.shape
+    _check_seq("weight", weight, x, x.dtype, (channels, None))
+    width = weight.shape[1]
+    if not 2 <= width <= 8:
+        raise ValueError(f"weight has {width} taps, expected 2 to 8")
+    if bias is not None:
+        _check_seq("bias", bias, x, x.dtype, (channels,))
+    act = _act(activation)
+    state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out, True)
+    offsets, nseq = _sequences(offsets, x)
+    slots = _index("slots", slots, x, nseq)
+
+    def call(st):
+        xr, ldx = _rows(x)
+        w = weight.contiguous()
+        b = None if bias is None else bias.contiguous()
+        y = _seq_out(out, x, (tokens, channels))
+        _lib.check(_lib.load().smm_causal_conv(
+            _ptr(xr), _ptr(w), _opt(b), _opt(offsets), _opt(state), _opt(state_out), _opt(slots), _ptr(y), tokens,
+            channels, width, nseq, entries, ldx, _rows(y)[1], dt, act, st), "smm_causal_conv")
+        return y
+    return _on(x, stream, call)
+
+
+def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                     state: torch.Tensor, state_out: Optional[torch.Tensor] = None,
+                     slots: Optional[torch.Tensor] = None, activation: Optional[str] = "silu",
+                     out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """causal_conv for one new token of each sequence: row b of x (batch,
+    channels) continues the state at entry slots[b] (None: b), which is updated in
+    place unless state_out is given.  A row with a negative slot starts from zero and leaves no state."""
+    dt = _check_x(x, 2)
+    batch, channels = x.shape
+    _check_seq("weight", weight, x, x.dtype, (channels, None))
+    width = weight.shape[1]
+    if not 2 <= width <= 8:
+        raise ValueError(f"weight has {width} taps, expected 2 to 8")
+    if bias is not None:
+        _check_seq("bias", bias, x, x.dtype, (channels,))
+    act = _act(activation)
+    if state is None:
+        raise TypeError("state must be a torch.Tensor")
+    state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out, True)
+    slots = _index("slots", slots, x, batch)
+
+    def call(st):
+        xr, ldx = _rows(x)
+        w = weight.contiguous()
+        b = None if bias is None else bias.contiguous()
+        y = _seq_out(out, x, (batch, channels))
+        _lib.check(_lib.load().smm_causal_conv_step(
+            _ptr(xr), _ptr(w), _opt(b), _opt(state), _opt(state_out), _opt(slots), _ptr(y), batch, channels, width,
+            entries, ldx, _rows(y)[1], dt, act, st), "smm_causal_conv_step")
+        return y
+    return _on(x, stream, call)
+
+
+def _scan_args(x, dt, A, B, C, D, z, dt_bias):
+    """Checks shared by the scan and the step; returns (dtype, dt's dtype, groups, state_dim)."""
+    ty = _check_x(x, 3)
+    t, heads, dim = x.shape
+    if not isinstance(dt, torch.Tensor):
+        raise TypeError("dt must be a torch.Tensor")
+    if dt.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"dt must be {x.dtype} or float32, got {dt.dtype}")
+    _check_seq("dt", dt, x, dt.dtype, (t, heads))
+    _check_seq("A", A, x, torch.float32, (heads,))
+    _check_seq("B", B, x, x.dtype, (t, None, None))
+    groups, n = B.shape[1], B.shape[2]
+    _check_seq("C", C, x, x.dtype, (t, groups, n))
+    if not (1 <= dim <= 256 and 1 <= n <= 256):
+        raise ValueError(f"head dim {dim} and state dim {n} must be 1 to 256")
+    if groups < 1 or heads % groups:
+        raise ValueError(f"{heads} heads do not divide into {groups} groups")
+    for name, v in (("D", D), ("dt_bias", dt_bias)):
+        if v is not None:
+            _check_seq(name, v, x, torch.float32, (heads,))
+    if z is not None:
+        _check_seq("z", z, x, x.dtype, (t, heads, dim))
+    return ty, _DTYPES[dt.dtype], groups, n
+
+
+def _vec(v: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return v if v is None or v.is_contiguous() else v.contiguous()
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+                   D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                   dt_bias: Optional[torch.Tensor] = None, dt_softplus: bool = False,
+                   offsets: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+                   state_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Selective state space scan over packed sequences: per head a
+    lower-triangular semiseparable matrix times x.  With d = dt + dt_bias (through
+    softplus if dt_softplus) and g the head's group,
+
+        S_t = exp(d_t A_h) S_{t-1} + d_t x_t (outer) B_t,g
+        y_t = (S_t C_t,g + D_h x_t) * silu(z_t)
+
+    x, z, y (tokens, heads, dim) and B, C (tokens, groups, state_dim) float32 or
+    bfloat16, dt (tokens, heads) of the same type or float32; A, D, dt_bias
+    (heads) float32.  dim and state_dim are 1 to 256.  Rows may be strided (x, B and
+    C columns of one matrix).  Sums, decays and states are float32.
+
+    offsets, slots, out, state (entries, heads, dim, state_dim; float32) and state_out are as in causal_conv.
+    A non-finite input makes the rest of its sequence non-finite, and may
+    do so for up to 127 tokens before it."""
+    ty, dty, groups, n = _scan_args(x, dt, A, B, C, D, z, dt_bias)
+    tokens, heads, dim = x.shape
+    state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out, True)
+    offsets, nseq = _sequences(offsets, x)
+    slots = _index("slots", slots, x, nseq)
+
+    def call(st):
+        L = _lib.load()
+        (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x), _rows(dt), _rows(B), _rows(C)
+        zr, ldz = (None, 0) if z is None else _rows(z)
+        a, dd, db = _vec(A), _vec(D), _vec(dt_bias)
+        y = _seq_out(out, x, (tokens, heads, dim))
+        nws = L.smm_selective_scan_workspace_size(tokens, nseq, heads, dim, groups, n, ty)
+        # of this call alone: streams and captured graphs share nothing
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
+        _lib.check(L.smm_selective_scan(
+            _ptr(xr), _ptr(dr), _ptr(a), _ptr(br), _ptr(cr), _opt(dd), _opt(zr), _opt(db), _opt(offsets), _opt(state),
+            _opt(state_out), _opt(slots), _ptr(y), tokens, nseq, entries, heads, dim, groups, n, ldx, ldd, ldb, ldc,
+            ldz, _rows(y)[1], ty, dty, int(dt_softplus), _opt(ws), nws, st), "smm_selective_scan")
+        return y
+    return _on(x, stream, call)
+
+
+def selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+                   state: torch.Tensor, D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
+                   dt_bias: Optional[torch.Tensor] = None, dt_softplus: bool = False,
+                   state_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """selective_scan for one new token of each sequence: row b of x (batch,
+    heads, dim) continues the state at entry slots[b] (None: b), which is updated
+    in place unless state_out is given.  A row with a negative slot starts from
+    zero and leaves no state."""
+    ty, dty, groups, n = _scan_args(x, dt, A, B, C, D, z, dt_bias)
+    batch, heads, dim = x.shape
+    if state is None:
+        raise TypeError("state must be a torch.Tensor")
+    state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out, True)
+    slots = _index("slots", slots, x, batch)
+
+    def call(st):
+        (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x), _rows(dt), _rows(B), _rows(C)
+        zr, ldz = (None, 0) if z is None else _rows(z)
+        a, dd, db = _vec(A), _vec(D), _vec(dt_bias)
+        y = _seq_out(out, x, (batch, heads, dim))
+        _lib.check(_lib.load().smm_selective_step(
+            _ptr(xr), _ptr(dr), _ptr(a), _ptr(br), _ptr(cr), _opt(dd), _opt(zr), _opt(db), _opt(state),
+            _opt(state_out), _opt(slots), _ptr(y), batch, entries, heads, dim, groups, n, ldx, ldd, ldb, ldc, ldz,
+            _rows(y)[1], ty, dty, int(dt_softplus), st), "smm_selective_step")
+        return y
+    return _on(x, stream, call)
+
+
+def q4_matvec(q: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
+              out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """y = x W^T for a few rows x (batch, cols) and W held in 4 bits:
+    W[r, k] = (code[r, k] - zero[r, k // group]) * scales[r, k // group].
+
+    q (rows, cols/2) uint8 holds code 2i of a row in the low half of byte i; scales
+    (rows, cols/group), of x's type or float32, and zeros (same shape, uint8, 0..15; None:
+    8 everywhere) give the group, a multiple of 32.  x float32 or bfloat16; products are
+    exact and sums float32 in both.  Returns (batch, rows)."""
+    ty = _check_x(x, 2)
+    batch, cols = x.shape
+    if not isinstance(q, torch.Tensor) or not isinstance(scales, torch.Tensor):
+        raise TypeError("q and scales must be torch.Tensors")
+    if cols % 2:
+        raise ValueError(f"x has an odd number of columns, {cols}")
+    _check_seq("q", q, x, torch.uint8, (None, cols // 2))
+    rows = q.shape[0]
+    if scales.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"scales must be {x.dtype} or float32, got {scales.dtype}")
+    _check_seq("scales", scales, x, scales.dtype, (rows, None))
+    groups = scales.shape[1]
+    if groups < 1 or cols % groups or (cols // groups) % 32 or cols == 0:
+        raise ValueError(f"{cols} columns do not divide into {groups} groups of a multiple of 32")
+    if zeros is not None:
+        _check_seq("zeros", zeros, x, torch.uint8, (rows, groups))
+
+    def call(st):
+        xr, ldx = _rows(x)
+        if xr.data_ptr() % 16 or (batch > 1 and ldx * xr.element_size() % 16):
+            xr = xr.contiguous().clone() if xr.data_ptr() % 16 else xr.contiguous()
+            ldx = cols
+        qc, sc, zc = q.contiguous(), scales.contiguous(), _vec(zeros)
+        if qc.data_ptr() % 16:
+            qc = qc.clone()
+        y = _seq_out(out, x, (batch, rows))
+        _lib.check(_lib.load().smm_q4_matvec(
+            _ptr(qc), _ptr(sc), _opt(zc), _ptr(xr), _ptr(y), batch, rows, cols, cols // groups, ldx, _rows(y)[1], ty,
+            _DTYPES[scales.dtype], st), "smm_q4_matvec")
+        return y
+    return _on(x, stream, call)
 
 
 # ---------------------------------------------------------------- host buffers

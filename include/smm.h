@@ -472,6 +472,83 @@ int smm_pack(const float* D, int s_fmt, float* P, int N, void* stream);
  * toeplitz_matmul2.cpp:34-41). */
 int smm_toeplitz_compact(const float* T, float* g, int rows, int cols, void* stream);
 
+/* ---- operators of a state-space block ----------------------------------- */
+
+/* Element types of these entry points' inputs and outputs.  Sums, decays and
+ * states are fp32 in both. */
+typedef enum { SMM_DTYPE_F32 = 0, SMM_DTYPE_BF16 = 1 } smm_dtype;
+typedef enum { SMM_ACT_NONE = 0, SMM_ACT_SILU = 1 } smm_act;
+
+/* Conventions shared by the four sequence entry points below.
+ *   Rows are tokens; ld* is the distance between two tokens' rows in elements
+ *   (the elements of one token are contiguous).  Prompts are packed one after
+ *   another: sequence s is the rows [offsets[s], offsets[s+1]) (offsets: nseq + 1
+ *   device ints, not decreasing; NULL: one sequence of all rows).  A sequence may be
+ *   empty.  Rows outside every sequence are neither read nor written.
+ *   state_in is what a sequence starts from (NULL: zero), state_out what it ends
+ *   with (NULL: not wanted); both have nslots entries, may be the same memory (an
+ *   update in place) but must not overlap otherwise.  Sequence s uses entry slots[s]
+ *   (device ints; NULL: entry s).  A sequence with a negative slot starts from
+ *   zero and leaves no state.  So does one whose slot is nslots or more, which
+ *   also makes smm_device_status report SMM_ERR_BOUNDS.  Two sequences of one
+ *   call must not share an entry.  Outputs must not overlap inputs. */
+
+/* y[t][c] = act(bias[c] + sum_j w[c][j] x[t-width+1+j][c]): per channel a banded
+ * lower-triangular Toeplitz matrix of `width` (2..8) diagonals times a column.
+ * Rows before the sequence come from its state, [channels][width-1] elements of
+ * the same type, oldest first.  w is channels x width, bias (NULL: none) has
+ * channels elements.  tokens counts x's rows.  No counterpart in the reference. */
+int smm_causal_conv(const void* x, const void* w, const void* bias, const int* offsets, const void* state_in,
+                    void* state_out, const int* slots, void* y, long long tokens, int channels, int width, int nseq,
+                    int nslots, long long ldx, long long ldy, int dtype, int act, void* stream);
+
+/* The same for one new token of each of `batch` sequences: row b belongs to
+ * sequence b. */
+int smm_causal_conv_step(const void* x, const void* w, const void* bias, const void* state_in, void* state_out,
+                         const int* slots, void* y, int batch, int channels, int width, int nslots, long long ldx,
+                         long long ldy, int dtype, int act, void* stream);
+
+/* Selective state space scan, per head h with its group g = h / (heads/groups):
+ *   d_t = dt[t][h] + dt_bias[h], through log(1 + exp(d)) if dt_softplus
+ *   S_t = exp(d_t A[h]) S_{t-1} + d_t x[t][h] (outer) B[t][g]    (dim x state_dim)
+ *   y[t][h] = (S_t C[t][g] + D[h] x[t][h]) * silu(z[t][h])
+ * that is, a lower-triangular semiseparable matrix times x.  x, z and y have rows
+ * of heads x dim elements, B and C of groups x state_dim, dt of heads; A, D and
+ * dt_bias are fp32.  D, z and dt_bias may be NULL.  A state is heads x dim x
+ * state_dim fp32.  dim and state_dim are 1..256.  dt_dtype is dt's own type.
+ *
+ * A non-finite x, B, C or dt of a token makes the rest of its sequence
+ * non-finite, and may do so for the up to 127 tokens before it as well.
+ *
+ * The workspace holds the states between the parts that a long sequence is
+ * split into (0 bytes: no split at these sizes).  No counterpart in the reference. */
+size_t smm_selective_scan_workspace_size(long long tokens, int nseq, int heads, int dim, int groups, int state_dim,
+                                         int dtype);
+int smm_selective_scan(const void* x, const void* dt, const float* A, const void* B, const void* C, const float* D,
+                       const void* z, const float* dt_bias, const int* offsets, const float* state_in,
+                       float* state_out, const int* slots, void* y, long long tokens, int nseq, int nslots, int heads,
+                       int dim, int groups, int state_dim, long long ldx, long long lddt, long long ldb, long long ldc,
+                       long long ldz, long long ldy, int dtype, int dt_dtype, int dt_softplus, void* ws,
+                       size_t ws_bytes, void* stream);
+
+/* The same for one new token of each of `batch` sequences. */
+int smm_selective_step(const void* x, const void* dt, const float* A, const void* B, const void* C, const float* D,
+                       const void* z, const float* dt_bias, const float* state_in, float* state_out, const int* slots,
+                       void* y, int batch, int nslots, int heads, int dim, int groups, int state_dim, long long ldx,
+                       long long lddt, long long ldb, long long ldc, long long ldz, long long ldy, int dtype,
+                       int dt_dtype, int dt_softplus, void* stream);
+
+/* ---- 4-bit operand ------------------------------------------------------- */
+
+/* y[b][r] = sum_k W[r][k] x[b][k], W[r][k] = (code[r][k] - zero[r][k/group]) scale[r][k/group]
+ * (X W^T for a few rows x).  q holds rows x cols/2 bytes, code 2i of a row in
+ * the low half of byte i; scales and zeros (bytes; NULL: 8 everywhere) are rows x
+ * cols/group.  group is a multiple of 32 and divides cols.  x and y have dtype
+ * elements, scales scale_dtype.  Products are exact and sums fp32, also for fp32 x.
+ * q 16-byte aligned.  y must not overlap an input.  No counterpart in the reference. */
+int smm_q4_matvec(const void* q, const void* scales, const void* zeros, const void* x, void* y, int batch, int rows,
+                  int cols, int group, long long ldx, long long ldy, int dtype, int scale_dtype, void* stream);
+
 /* ---- reference-compatible wrappers (synchronous, timed) ---------------- */
 
 /* One per operation the DSL's CUDA runner generates, with the generated
