@@ -178,6 +178,9 @@ thread_local unsigned long long g_wait_next = 0;
 
 }  // namespace
 
+// cuTensorMapEncodeTiled, or null (for the translation units with maps of their own).
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
+
 bool valid_mode(int mode) { return mode == SMM_MODE_3XTF32 || mode == SMM_MODE_TF32 || mode == SMM_MODE_BF16; }
 
 int check_packed(const char* who, int N) {

@@ -140,7 +140,12 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
   const T* gC = static_cast<const T*>(p.C) + static_cast<long long>(g) * N;
   const T* gx = static_cast<const T*>(p.x) + static_cast<long long>(h) * p.dim + p0;
   const T* gz = p.z ? static_cast<const T*>(p.z) + static_cast<long long>(h) * p.dim + p0 : nullptr;
-  float rB[NE], rC[NE], rx[XE], rz[XE], cx[XE], cz[XE], rd = 0.0f, la = 0.0f;
+  // elements as loaded: nothing waits for them before stage() widens them
+  T rB[NE], rC[NE], rx[XE], rz[XE], cx[XE], cz[XE];
+  uint32_t rd = 0;
+  float la = 0.0f;
+  const float bias = p.dt_bias ? __ldg(p.dt_bias + h) : 0.0f;
+  const T zero = from_f32<T>(0.0f);
   const int pdims = p.dim - p0 < PT ? p.dim - p0 : PT;
   auto fetch = [&](long long t0) {
     const int nt = sg.end - t0 < kTile ? static_cast<int>(sg.end - t0) : kTile;
@@ -148,36 +153,37 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
     for (int i = 0; i < NE; ++i) {
       const int e = tid + i * THREADS, t = e / NP, n = e % NP;
       const bool ok = t < nt && n < N;
-      rB[i] = ok ? to_f32(gB[(t0 + t) * p.ldb + n]) : 0.0f;
-      if constexpr (!STATES) rC[i] = ok ? to_f32(gC[(t0 + t) * p.ldc + n]) : 0.0f;
+      rB[i] = ok ? gB[(t0 + t) * p.ldb + n] : zero;
+      if constexpr (!STATES) rC[i] = ok ? gC[(t0 + t) * p.ldc + n] : zero;
     }
 #pragma unroll
     for (int i = 0; i < XE; ++i) {
       const int e = tid + i * THREADS, t = e / PT, q = e % PT;
       const bool ok = t < nt && q < pdims;
-      rx[i] = ok ? to_f32(gx[(t0 + t) * p.ldx + q]) : 0.0f;
-      if constexpr (!STATES) rz[i] = ok && gz ? to_f32(gz[(t0 + t) * p.ldz + q]) : 0.0f;
+      rx[i] = ok ? gx[(t0 + t) * p.ldx + q] : zero;
+      if constexpr (!STATES) rz[i] = ok && gz ? gz[(t0 + t) * p.ldz + q] : zero;
     }
-    if (tid < kTile) rd = tid < nt ? scan_dt(p, t0 + tid, h) : 0.0f;
+    if (tid < nt) rd = scan_dt_raw(p, t0 + tid, h);
   };
   auto stage = [&](int nt) {
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       const int e = tid + i * THREADS;
       if (e < kTile * NP) {
-        sB[e] = rB[i];
-        if constexpr (!STATES) sC[e] = rC[i];
+        sB[e] = to_f32(rB[i]);
+        if constexpr (!STATES) sC[e] = to_f32(rC[i]);
       }
     }
 #pragma unroll
     for (int i = 0; i < XE; ++i) {
-      sx[tid + i * THREADS] = rx[i];
+      sx[tid + i * THREADS] = to_f32(rx[i]);
       cx[i] = rx[i];
       if constexpr (!STATES) cz[i] = rz[i];
     }
     if (tid < kTile) {
-      sad[tid] = tid < nt ? make_float2(expf(rd * A), rd) : make_float2(1.0f, 0.0f);
-      if (tid < nt) la += rd * A;
+      const float d = scan_dt(p, rd, bias);
+      sad[tid] = make_float2(expf(d * A), d);
+      if (tid < nt) la += d * A;
     }
   };
 
@@ -233,8 +239,8 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
       for (int i = 0; i < XE; ++i) {
         const int e = tid + i * THREADS, t = e / PT, q = e % PT;
         if (t < nt && q < pdims) {
-          float v = fmaf(Dh, cx[i], sy[e]);
-          if (gz) v *= silu(cz[i]);
+          float v = fmaf(Dh, to_f32(cx[i]), sy[e]);
+          if (gz) v *= silu(to_f32(cz[i]));
           gy[(t0 + t) * p.ldy + q] = from_f32<T>(v);
         }
       }
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, 
       bv[k][i] = n < N ? to_f32(static_cast<const T*>(p.B)[b * p.ldb + static_cast<long long>(g) * N + n]) : 0.0f;
       cv[k][i] = n < N ? to_f32(static_cast<const T*>(p.C)[b * p.ldc + static_cast<long long>(g) * N + n]) : 0.0f;
     }
-  const float d = scan_dt(p, b, h);
+  const float d = scan_dt(p, scan_dt_raw(p, b, h), p.dt_bias ? __ldg(p.dt_bias + h) : 0.0f);
   const float a = expf(d * __ldg(p.A + h));
   const float Dh = p.D ? __ldg(p.D + h) : 0.0f;
   // every thread of the CTA makes the same number of turns (the shuffles)

@@ -40,11 +40,15 @@ struct ScanParams {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float scan_dt(const ScanParams& p, long long t, int h) {
+// dt as it lies (the 16 bits of a bf16 element, or an fp32 one), and d from it
+// and the head's bias: loads stay ahead of the arithmetic that waits for them.
+__device__ __forceinline__ uint32_t scan_dt_raw(const ScanParams& p, long long t, int h) {
   const long long i = t * p.lddt + h;
-  float d = p.dt_f32 ? __ldg(static_cast<const float*>(p.dt) + i)
-                     : to_f32(static_cast<const __nv_bfloat16*>(p.dt)[i]);
-  if (p.dt_bias) d += __ldg(p.dt_bias + h);
+  return p.dt_f32 ? __ldg(static_cast<const uint32_t*>(p.dt) + i)
+                  : static_cast<uint32_t>(__ldg(static_cast<const unsigned short*>(p.dt) + i));
+}
+__device__ __forceinline__ float scan_dt(const ScanParams& p, uint32_t raw, float bias) {
+  const float d = __uint_as_float(p.dt_f32 ? raw : raw << 16) + bias;
   return p.softplus ? softplus(d) : d;
 }
 
