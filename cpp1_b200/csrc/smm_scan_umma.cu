@@ -22,14 +22,16 @@
 // (2^-16), because the state is an fp32 result that is carried on.  The state
 // itself stays in fp32 registers, S, Y, Yo and dS are fp32 in tensor memory.
 //
-// Warps: 0 loads (TMA), 1 issues the products, 2 computes the decays, 4-7 and 8-11
-// form G and write y of the even and the odd chunks, 12-15 form Xw, 16-19 carry
+// Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the decays in turn, 4-7 and 8-11
+// form G and write y of the even and the odd chunks, 12-19 form Xw, 20-23 carry
 // the state.  Every wait is bounded; on expiry the CTA records it and leaves.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 
 #include "smm_scan.cuh"
 
@@ -41,7 +43,7 @@ namespace {
 
 constexpr int kQ = 128;         // tokens per chunk
 constexpr int kP = 64;          // dims per CTA
-constexpr int kThreads = 640;
+constexpr int kThreads = 768;
 constexpr uint32_t kAtom = kQ * 128;  // one 64-element wide tile of 128 rows: 16 KiB
 // tensor memory columns; G[k] overlays the first half of S[k]
 constexpr uint32_t kColS = 0, kColY = 256, kColYo = 384, kColDs = 448, kCols = 512;
@@ -57,7 +59,7 @@ struct Scal {
 };
 
 struct Bars {
-  uint64_t full_bc[2], full_x[2], done[2], xfree[2], s_full[2], g_full[2];
+  uint64_t full_bc[2], full_x[2], full_z[2], done[2], xfree[2], bfree[2], zfree[2], s_full[2], g_full[2];
   uint64_t xw_full, ds_full, ds_free, h_full, yo_free;
   uint64_t sc_full[3], sc_free[3];
   uint64_t drain;
@@ -77,7 +79,7 @@ struct Smem {
 };
 
 struct Tmaps {
-  CUtensorMap x, b, c;
+  CUtensorMap x, b, c, y, z;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
@@ -88,16 +90,63 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-  umma_lohi<false, true>(d, static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b),
-                         static_cast<uint32_t>(b >> 32), idesc, acc ? 1u : 0u);
+// Tile in shared memory -> global; returns once the tile has been read.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n\t"
+      "cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// The whole warp reaches these together and only lane `leader` issues: with the
+// predicate on the instruction, control flow stays uniform and the compiler
+// keeps the descriptors in uniform registers.  (From one lane's branch, each
+// product cost 65 to 110 cycles of register moves, 2600 and more a chunk.)
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b32 t;\n\telect.sync t|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r;
+}
+// The descriptors are given as their low word of the stage's first product and
+// their high word; the step's offset is added inside, so that the compiler
+// does not keep a register for every step of every product.
+template <uint32_t OA, uint32_t OB, bool FIRST>
+__device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
+                                        uint32_t b_hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
+      "add.u32 x, %1, %7;\n\tadd.u32 y, %3, %8;\n\tmov.b64 da, {x, %2};\n\tmov.b64 db, {y, %4};\n\t"
+      "setp.ne.b32 p, %9, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}\n" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "n"(OA), "n"(OB), "n"(FIRST ? 0 : 1)
+      : "memory");
 }
 // A from tensor memory (bf16, two per column), B from shared memory
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+template <uint32_t OA, uint32_t OB, bool FIRST>
+__device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                        uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 db;\n\t"
+      "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\tmov.b64 db, {y, %3};\n\t"
+      "setp.ne.b32 p, %8, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "n"(OA), "n"(OB), "n"(FIRST ? 0 : 1)
+      : "memory");
+}
+template <int... K, typename F>
+__device__ __forceinline__ void steps_of(std::integer_sequence<int, K...>, F&& f) {
+  (f(std::integral_constant<int, K>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void steps(F&& f) {
+  steps_of(std::make_integer_sequence<int, N>{}, f);
+}
+__device__ __forceinline__ void umma_commit_by(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -108,6 +157,35 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+// Whether to give up a wait (called every 64 tries, out of line: a dozen roles' waits
+// share it).  t0 is 0 before the first call.
+__device__ __forceinline__ bool give_up(const WaitCtx& w, uint64_t& t0) {
+  if (*w.abort_flag) return true;
+  const uint64_t t = globaltimer_ns();
+  if (t0 == 0) t0 = t;
+  if (t - t0 <= w.limit_ns) return false;
+  *w.abort_flag = 1;
+  if (w.status) atomicOr(w.status, kDevErrTimeout | w.where);
+  return true;
+}
+// mbar_wait with a short inline path.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const WaitCtx& w) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, parity)) return true;
+  uint64_t t0 = 0;
+  uint32_t n = 0;
+  while (!mbar_try_wait(a, parity))
+    if ((++n & 63u) == 0 && give_up(w, t0)) return false;
+  return true;
+}
+template <int R>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -129,13 +207,14 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(r));
   return o;
 }
+// Registers into 32 lanes x 8 consecutive columns of tensor memory.
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
 }
 
 // STATES: the first launch of a split scan (B, x and the state only).
@@ -145,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using L = Smem<NA>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Segment sseg;
+  __shared__ float seg_sum[2];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   Scal* scal = reinterpret_cast<Scal*>(smem + L::kScal);
@@ -187,18 +267,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->full_bc[i], 1);
       mbar_init(&bars->full_x[i], 1);
       mbar_init(&bars->done[i], 1);
-      mbar_init(&bars->xfree[i], 4);
+      mbar_init(&bars->full_z[i], 1);
+      mbar_init(&bars->xfree[i], 1);
+      mbar_init(&bars->bfree[i], 1);
+      mbar_init(&bars->zfree[i], 4);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->g_full[i], 4);
     }
-    mbar_init(&bars->xw_full, 4);
+    mbar_init(&bars->xw_full, 8);
     mbar_init(&bars->ds_full, 1);
     mbar_init(&bars->ds_free, 4);
     mbar_init(&bars->h_full, 4);
     mbar_init(&bars->yo_free, 4);
     for (int i = 0; i < 3; ++i) {
       mbar_init(&bars->sc_full[i], 1);
-      mbar_init(&bars->sc_free[i], STATES ? 8 : 12);
+      mbar_init(&bars->sc_free[i], STATES ? 12 : 16);
     }
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
@@ -211,139 +294,174 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = bars->tmem;
 
   WaitCtx w{&bars->abort_flag, p.status, p.wait_limit_ns, 0};
-  const uint32_t stage_c = 0, stage_b = NA * kAtom, stage_x = 2 * NA * kAtom;
+  constexpr uint32_t stage_c = 0, stage_b = NA * kAtom, stage_x = 2 * NA * kAtom;
 
+  // The launch's 6 x 80 registers per warpgroup's thread, shared out by need:
+  // 64 (loads, products, decays), 2 x 96 (G and y), 2 x 64 (Xw), 96 (state) = 480.
+  // A spill costs a trip to L2 here: shared memory leaves L1 too small for the stacks.
+  if (warp < 4) {
+    regs_dec<64>();
   if (warp == 0) {
     // ------------------------------------------------------------ loads
     if (lane == 0) {
       w.where = kWaitProducer;
-      tma_prefetch_desc(&maps.x);
-      tma_prefetch_desc(&maps.b);
-      if (!STATES) tma_prefetch_desc(&maps.c);
-      int issued = 0;
-      for (int c = 0; c < nc; ++c) {
-        const int s = c & 1;
-        if (c >= 2 && !mbar_wait(&bars->done[s], ((c >> 1) - 1) & 1, w)) break;
-        const uint32_t st = sbase + s * L::kStage;
-        const int t0 = static_cast<int>(sg.begin) + c * kQ;
-        mbar_arrive_expect_tx(&bars->full_bc[s], (STATES ? 1 : 2) * NA * kAtom);
-#pragma unroll
-        for (int a = 0; a < NA; ++a) {
-          if (!STATES) tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_bc[s], a * 64, g, t0);
-          tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_bc[s], a * 64, g, t0);
+      const bool gated = !STATES && p.z != nullptr;
+      // next chunk of each kind of load; z goes where B was, once dS has read it
+      int c_bc = 0, c_x = 0, c_z = 0;
+      uint32_t idle = 0;
+      uint64_t t0 = 0;
+      const int row0 = static_cast<int>(sg.begin);
+      while (c_bc < nc || c_x < nc || (gated && c_z < nc)) {
+        bool did = false;
+        if (gated && c_z < c_bc && mbar_test(&bars->bfree[c_z & 1], (c_z >> 1) & 1)) {
+          const int s = c_z & 1;
+          mbar_arrive_expect_tx(&bars->full_z[s], kAtom);
+          tma_load_3d(sbase + s * L::kStage + stage_b, &maps.z, &bars->full_z[s], p0, h, row0 + c_z * kQ);
+          ++c_z;
+          did = true;
         }
-        issued = c + 1;
-        if (!STATES && c >= 2 && !mbar_wait(&bars->xfree[s], ((c >> 1) - 1) & 1, w)) break;
-        mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
-        tma_load_3d(st + stage_x, &maps.x, &bars->full_x[s], p0, h, t0);
+        if (c_bc < nc &&
+            (c_bc < 2 || (mbar_test(&bars->done[c_bc & 1], ((c_bc >> 1) - 1) & 1) &&
+                          (!gated || (c_z > c_bc - 2 && mbar_test(&bars->zfree[c_bc & 1], ((c_bc >> 1) - 1) & 1)))))) {
+          const int s = c_bc & 1;
+          const uint32_t st = sbase + s * L::kStage;
+          mbar_arrive_expect_tx(&bars->full_bc[s], (STATES ? 1 : 2) * NA * kAtom);
+#pragma unroll
+          for (int a = 0; a < NA; ++a) {
+            if (!STATES) tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_bc[s], a * 64, g, row0 + c_bc * kQ);
+            tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_bc[s], a * 64, g, row0 + c_bc * kQ);
+          }
+          ++c_bc;
+          did = true;
+        }
+        if (c_x < c_bc && (c_x < 2 || STATES || mbar_test(&bars->xfree[c_x & 1], ((c_x >> 1) - 1) & 1))) {
+          const int s = c_x & 1;
+          mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
+          tma_load_3d(sbase + s * L::kStage + stage_x, &maps.x, &bars->full_x[s], p0, h, row0 + c_x * kQ);
+          ++c_x;
+          did = true;
+        }
+        if (did)
+          idle = 0, t0 = 0;
+        else if ((++idle & 255u) == 0 && give_up(w, t0))
+          break;
       }
       // after an abort, copies in flight land before the CTA leaves
-      if (bars->abort_flag) {
+      if (*w.abort_flag) {
         int none = 0;
         WaitCtx dw{&none, p.status, p.wait_limit_ns > 1000000000ull ? p.wait_limit_ns : 1000000000ull, kWaitDrain};
-        for (int c = issued >= 2 ? issued - 2 : 0; c < issued; ++c) {
-          mbar_wait(&bars->full_bc[c & 1], (c >> 1) & 1, dw);
-          // x's copy of the newest chunk may not have been issued
-          if (c < issued - 1) mbar_wait(&bars->full_x[c & 1], (c >> 1) & 1, dw);
-        }
-        const int c = issued - 1;
-        if (c >= 0) {
-          none = 0;
-          dw.limit_ns = 1000000;
-          dw.status = nullptr;
-          mbar_wait(&bars->full_x[c & 1], (c >> 1) & 1, dw);
-        }
+        for (int c = c_bc > 2 ? c_bc - 2 : 0; c < c_bc; ++c) wait_bar(&bars->full_bc[c & 1], (c >> 1) & 1, dw);
+        for (int c = c_x > 2 ? c_x - 2 : 0; c < c_x; ++c) wait_bar(&bars->full_x[c & 1], (c >> 1) & 1, dw);
+        for (int c = c_z > 2 ? c_z - 2 : 0; c < c_z; ++c) wait_bar(&bars->full_z[c & 1], (c >> 1) & 1, dw);
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
-      constexpr uint32_t idS = make_idesc(kFmtBF16, 128, 128, 0, 0);
-      constexpr uint32_t idY = make_idesc(kFmtBF16, 128, kP, 0, 1);
-      constexpr uint32_t idD = make_idesc(kFmtBF16, 128, kP, 1, 1);
-      const int ksteps = (N + 15) / 16;
-      int s_next = STATES ? nc : 0, g_next = 0, sub = 0;
-      uint64_t t_idle = 0;
-      while (g_next < nc) {
-        bool did = false;
-        if (!STATES && s_next < nc && s_next < g_next + 2 &&
-            mbar_test(&bars->full_bc[s_next & 1], (s_next >> 1) & 1)) {
-          // the loads of chunk c waited for every product of chunk c - 2, so S and G are free
-          tc_fence_after_sync();
-          const int s = s_next & 1;
-          const uint32_t st = sbase + s * L::kStage;
-          for (int k = 0; k < ksteps; ++k) {
-            const uint32_t off = (k >> 2) * kAtom + (k & 3) * 32;
-            umma_ss(tmem + kColS + s * 128, make_smem_desc(st + stage_c + off, 16, 1024, kLayoutSw128),
-                    make_smem_desc(st + stage_b + off, 16, 1024, kLayoutSw128), idS, k > 0);
-          }
-          umma_commit(&bars->s_full[s]);
-          ++s_next;
-          did = true;
-        } else if (STATES || g_next < s_next) {
-          const int c = g_next, s = c & 1;
-          const uint32_t st = sbase + s * L::kStage;
-          if (sub == 0) {
-            if (mbar_test(&bars->xw_full, c & 1) && (c == 0 || mbar_test(&bars->ds_free, (c - 1) & 1)) &&
-                mbar_test(&bars->full_bc[s], (c >> 1) & 1) && mbar_test(&bars->full_x[s], (c >> 1) & 1)) {
-              tc_fence_after_sync();
-              for (int k = 0; k < 16; ++k) {
-                const uint32_t kk = (k & 7) * 2048;
-                umma_ss(tmem + kColDs, make_smem_desc(st + stage_b + kk, kAtom, 1024, kLayoutSw128),
-                        make_smem_desc(sbase + L::kXw + (k >> 3) * kAtom + kk, kAtom, 1024, kLayoutSw128), idD, k > 0);
-              }
-              umma_commit(&bars->ds_full);
-              if (STATES) {
-                umma_commit(&bars->done[s]);
-                ++g_next;
-              } else {
-                sub = 1;
-              }
-              did = true;
-            }
-          } else if (sub == 1) {
-            if (mbar_test(&bars->g_full[s], (c >> 1) & 1)) {
-              tc_fence_after_sync();
-              for (int k = 0; k < 8; ++k)
-                umma_ts(tmem + kColY + s * kP, tmem + kColS + s * 128 + k * 8,
-                        make_smem_desc(st + stage_x + k * 2048, kAtom, 1024, kLayoutSw128), idY, k > 0);
-              sub = 2;
-              did = true;
-            }
-          } else {
-            if (mbar_test(&bars->h_full, c & 1) && (c == 0 || mbar_test(&bars->yo_free, (c - 1) & 1))) {
-              tc_fence_after_sync();
-              for (int k = 0; k < ksteps; ++k) {
-                const uint32_t off = (k >> 2) * kAtom + (k & 3) * 32;
-                umma_ss(tmem + kColYo, make_smem_desc(st + stage_c + off, 16, 1024, kLayoutSw128),
-                        make_smem_desc(sbase + L::kH + k * 2048, kAtom, 1024, kLayoutSw128), idY, k > 0);
-              }
-              umma_commit(&bars->done[s]);
-              sub = 0;
+    constexpr uint32_t idS = make_idesc(kFmtBF16, 128, 128, 0, 0);
+    constexpr uint32_t idY = make_idesc(kFmtBF16, 128, kP, 0, 1);
+    constexpr uint32_t idD = make_idesc(kFmtBF16, 128, kP, 1, 1);
+    const int ksteps = (N + 15) / 16;
+    const uint32_t leader = elect_one();
+    // descriptors of stage 0; a stage is kSt further.  Only the low word, the
+    // start address in 16-byte units, changes with stage and step.
+    constexpr uint32_t kSt = L::kStage >> 4;
+    auto lo = [](uint64_t d) { return static_cast<uint32_t>(d); };
+    const uint64_t dK = make_smem_desc(sbase, 16, 1024, kLayoutSw128);      // K-major
+    const uint64_t dM = make_smem_desc(sbase, kAtom, 1024, kLayoutSw128);   // MN-major
+    const uint32_t hK = static_cast<uint32_t>(dK >> 32), hM = static_cast<uint32_t>(dM >> 32);
+    auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xFFFFFFFFu, mbar_test(bar, parity)) != 0; };
+    int s_next = STATES ? nc : 0, g_next = 0, sub = 0;
+    uint32_t idle = 0;
+    uint64_t t_idle = 0;
+    while (g_next < nc) {
+      bool did = false;
+      if (!STATES && s_next < nc && s_next < g_next + 2 && ready(&bars->full_bc[s_next & 1], (s_next >> 1) & 1)) {
+        // the loads of chunk c waited for every product of chunk c - 2, so S and G are free
+        tc_fence_after_sync();
+        const int s = s_next & 1;
+        const uint32_t base = lo(dK) + s * kSt;
+        steps<4 * NA>([&](auto kc) {
+          constexpr int k = decltype(kc)::value;
+          constexpr uint32_t off = ((k >> 2) * kAtom + (k & 3) * 32) >> 4;
+          if (k < ksteps)
+            umma_ss<off + (stage_c >> 4), off + (stage_b >> 4), k == 0>(leader, tmem + kColS + s * 128, base, hK, base, hK,
+                                                                       idS);
+        });
+        umma_commit_by(leader, &bars->s_full[s]);
+        ++s_next;
+        did = true;
+      } else if (STATES || g_next < s_next) {
+        const int c = g_next, s = c & 1;
+        if (sub == 0) {
+          if (ready(&bars->xw_full, c & 1) && (c == 0 || ready(&bars->ds_free, (c - 1) & 1)) &&
+              ready(&bars->full_bc[s], (c >> 1) & 1) && ready(&bars->full_x[s], (c >> 1) & 1)) {
+            tc_fence_after_sync();
+            const uint32_t base = lo(dM) + s * kSt;
+            steps<16>([&](auto kc) {
+              constexpr int k = decltype(kc)::value;
+              constexpr uint32_t kk = (k & 7) * 128;
+              umma_ss<(stage_b >> 4) + kk, (L::kXw >> 4) + (k >> 3) * (kAtom >> 4) + kk, k == 0>(
+                  leader, tmem + kColDs, base, hM, lo(dM), hM, idD);
+            });
+            umma_commit_by(leader, &bars->ds_full);
+            if (!STATES) umma_commit_by(leader, &bars->bfree[s]);
+            if (STATES) {
+              umma_commit_by(leader, &bars->done[s]);
               ++g_next;
-              did = true;
+            } else {
+              sub = 1;
             }
+            did = true;
           }
-        }
-        if (did) {
-          t_idle = 0;
+        } else if (sub == 1) {
+          if (ready(&bars->g_full[s], (c >> 1) & 1)) {
+            tc_fence_after_sync();
+            const uint32_t base = lo(dM) + s * kSt;
+            steps<8>([&](auto kc) {
+              constexpr int k = decltype(kc)::value;
+              umma_ts<k * 8, (stage_x >> 4) + k * 128, k == 0>(leader, tmem + kColY + s * kP, tmem + kColS + s * 128, base,
+                                                               hM, idY);
+            });
+            sub = 2;
+            did = true;
+          }
         } else {
-          if (t_idle == 0) t_idle = globaltimer_ns();
-          if (*w.abort_flag) break;
-          if (globaltimer_ns() - t_idle > w.limit_ns) {
-            *w.abort_flag = 1;
-            if (w.status) atomicOr(w.status, kDevErrTimeout | kWaitMma);
-            break;
+          if (ready(&bars->h_full, c & 1) && (c == 0 || ready(&bars->yo_free, (c - 1) & 1))) {
+            tc_fence_after_sync();
+            const uint32_t base = lo(dK) + s * kSt;
+            steps<4 * NA>([&](auto kc) {
+              constexpr int k = decltype(kc)::value;
+              constexpr uint32_t off = ((k >> 2) * kAtom + (k & 3) * 32) >> 4;
+              if (k < ksteps)
+                umma_ss<off + (stage_c >> 4), (L::kH >> 4) + k * 128, k == 0>(leader, tmem + kColYo, base, hK, lo(dM), hM,
+                                                                             idY);
+            });
+            umma_commit_by(leader, &bars->done[s]);
+            sub = 0;
+            ++g_next;
+            did = true;
           }
         }
       }
-      // every product has completed, and its arrivals have landed, before the CTA leaves
-      int none = 0;
-      WaitCtx dw{&none, p.status, p.wait_limit_ns > 1000000000ull ? p.wait_limit_ns : 1000000000ull, kWaitDrain};
-      umma_commit(&bars->drain);
-      mbar_wait(&bars->drain, 0, dw);
+      if (did) {
+        idle = 0;
+      } else if ((++idle & 1023u) == 0) {
+        // the timer is slow to read: now and then is enough for the limit
+        if (__any_sync(0xFFFFFFFFu, *w.abort_flag != 0)) break;
+        if (idle == 1024u) t_idle = globaltimer_ns();
+        if (__any_sync(0xFFFFFFFFu, globaltimer_ns() - t_idle > w.limit_ns)) {
+          *w.abort_flag = 1;
+          if (w.status && lane == 0) atomicOr(w.status, kDevErrTimeout | kWaitMma);
+          break;
+        }
+      }
     }
-  } else if (warp == 2) {
+    // every product has completed, and its arrivals have landed, before the CTA leaves
+    int none = 0;
+    WaitCtx dw{&none, p.status, p.wait_limit_ns > 1000000000ull ? p.wait_limit_ns : 1000000000ull, kWaitDrain};
+    umma_commit_by(leader, &bars->drain);
+    wait_bar(&bars->drain, 0, dw);
+  } else {
     // ------------------------------------------------------------ decays
     w.where = kWaitTransform;
     const float A2 = __ldg(p.A + h) * kLog2e;
@@ -358,11 +476,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (t < sg.end) raw[i] = scan_dt_raw(p, t, h);
       }
     };
-    if (nc > 0) fetch(0);
-    for (int c = 0; c < nc; ++c) {
+    if (warp - 2 < nc) fetch(warp - 2);
+    for (int c = warp - 2; c < nc; c += 2) {
       const int b3 = c % 3;
       if (c >= 3) {
-        ok = mbar_wait(&bars->sc_free[b3], (c / 3 - 1) & 1, w);
+        ok = wait_bar(&bars->sc_free[b3], (c / 3 - 1) & 1, w);
         if (!ok) break;
       }
       Scal& sc = scal[b3];
@@ -372,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const long long t = sg.begin + static_cast<long long>(c) * kQ + lane * 4 + i;
         d[i] = t < sg.end ? scan_dt(p, raw[i], bias) : 0.0f;
       }
-      if (c + 1 < nc) fetch(c + 1);
+      if (c + 2 < nc) fetch(c + 2);
       // sums within blocks of 32 tokens (8 lanes): inclusive before, exclusive behind
       float run = 0.0f;
 #pragma unroll
@@ -427,9 +545,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->sc_full[b3]);
     }
-    if (STATES && ok && pt == 0 && lane == 0)
-      p.seg_log[static_cast<long long>(seg) * p.heads + h] = log_sum * (1.0f / kLog2e);
-  } else if (warp >= 4 && warp < 12) {
+    if (lane == 0) seg_sum[warp - 2] = log_sum;
+  }
+  } else if (warp < 12) {
+    regs_inc<96>();
     // ------------------------------------------------------------ G, then y
     if constexpr (!STATES) {
       w.where = kWaitEpilogue;
@@ -440,148 +559,159 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t sYo = tmem + lanes + kColYo;
       const float Dh = p.D ? __ldg(p.D + h) : 0.0f;
       __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + static_cast<long long>(h) * p.dim + p0;
-      const __nv_bfloat16* gz =
-          p.z ? static_cast<const __nv_bfloat16*>(p.z) + static_cast<long long>(h) * p.dim + p0 : nullptr;
+      const bool gated = p.z != nullptr;
       for (int c = wg; c < nc; c += 2) {
         const int b3 = c % 3;
         const uint32_t par = (c >> 1) & 1;
-        if (!mbar_wait(&bars->sc_full[b3], (c / 3) & 1, w)) break;
-        if (!mbar_wait(&bars->s_full[wg], par, w)) break;
+        if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, w)) break;
+        if (!wait_bar(&bars->s_full[wg], par, w)) break;
         tc_fence_after_sync();
         const Scal& sc = scal[b3];
         const float u = sc.u[t], lt = sc.l[t];
-        for (int b = 0; b < 4; ++b) {
-          uint32_t o[16];
+        // 16 columns at a time: the block of columns b is off the diagonal for b < q
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+          const int b = j >> 1;
+          uint32_t o[8];
           if (b <= q) {
-            uint32_t r[2][16];
-            tmem_ld_32x32b_x16(sS + 32 * b, r[0]);
-            tmem_ld_32x32b_x16(sS + 32 * b + 16, r[1]);
-            tmem_wait_ld();
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(sS + 16 * j, r);
+            const float2* f = reinterpret_cast<const float2*>((b < q ? sc.f[q - 1] : sc.d) + 16 * j);
             if (b < q) {
-              const float2* f = reinterpret_cast<const float2*>(sc.f[q - 1] + 32 * b);
               const float2 u2 = make_float2(u, u);
+              tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 s2 = make_float2(__uint_as_float(r[i >> 3][2 * (i & 7)]),
-                                              __uint_as_float(r[i >> 3][2 * (i & 7) + 1]));
-                const float2 v = mul2(mul2(s2, f[i]), u2);
+              for (int i = 0; i < 8; ++i) {
+                const float2 v = mul2(
+                    mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f[i]), u2);
                 o[i] = bf16_pair(v.x, v.y);
               }
             } else {
-              const float2* ls = reinterpret_cast<const float2*>(sc.l + 32 * b);
-              const float2* ds = reinterpret_cast<const float2*>(sc.d + 32 * b);
+              const float2* ls = reinterpret_cast<const float2*>(sc.l + 16 * j);
+              const int top = lane - 16 * (j & 1);  // columns up to here are at or before this row
+              float2 g2[8];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 l2 = ls[i], d2 = ds[i];
-                const float a = __uint_as_float(r[i >> 3][2 * (i & 7)]) * (ex2(lt - l2.x) * d2.x);
-                const float z = __uint_as_float(r[i >> 3][2 * (i & 7) + 1]) * (ex2(lt - l2.y) * d2.y);
-                o[i] = bf16_pair(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f);
+              for (int i = 0; i < 8; ++i) {
+                const float2 l2 = ls[i], d2 = f[i];
+                g2[i] = make_float2(ex2(lt - l2.x) * d2.x, ex2(lt - l2.y) * d2.y);
               }
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                o[i] = bf16_pair(2 * i <= top ? __uint_as_float(r[2 * i]) * g2[i].x : 0.0f,
+                                 2 * i + 1 <= top ? __uint_as_float(r[2 * i + 1]) * g2[i].y : 0.0f);
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = 0;
+            for (int i = 0; i < 8; ++i) o[i] = 0;
           }
-          // columns 16 b .. 16 b + 15 of S have been read by this lane already
-          tmem_st_32x32b_x16(sS + 16 * b, o);
+          // columns 8 j .. 8 j + 7 of S have been read by this lane already
+          tmem_st_32x32b_x8(sS + 8 * j, o);
         }
         tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->g_full[wg]);
 
-        const long long row = sg.begin + static_cast<long long>(c) * kQ + t;
-        const bool live = row < sg.end;
-        uint4 zv[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (gz && live && 8 * i < pdims) zv[i] = __ldcs(reinterpret_cast<const uint4*>(gz + row * p.ldz) + i);
-        if (!mbar_wait(&bars->done[wg], par, w)) break;
+        // y takes x's place in shared memory, row by row, and leaves as one tile (or by
+        // rows where the chunk ends before the tile)
+        if (!wait_bar(&bars->full_x[wg], par, w)) break;
+        if (gated && !wait_bar(&bars->full_z[wg], par, w)) break;
+        if (!wait_bar(&bars->done[wg], par, w)) break;
         tc_fence_after_sync();
         const float e = sc.e[t];
-        const uint32_t xrow = sbase + wg * L::kStage + stage_x;
-#pragma unroll
-        for (int pc = 0; pc < 4; ++pc) {
-          uint32_t ry[16], ro[16];
-          tmem_ld_32x32b_x16(sY + 16 * pc, ry);
-          tmem_ld_32x32b_x16(sYo + 16 * pc, ro);
-          uint4 xv[2];
-          xv[0] = ld_shared_v4(xrow + swz_offset(t, 2 * pc, 128));
-          xv[1] = ld_shared_v4(xrow + swz_offset(t, 2 * pc + 1, 128));
+        uint8_t* xt = smem + wg * L::kStage + stage_x;
+        const uint8_t* zt = smem + wg * L::kStage + stage_b;
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          uint32_t ry[16], ro[16], xw[8], zw[8], out[8];
+          tmem_ld_32x32b_x16(sY + 16 * k, ry);
+          tmem_ld_32x32b_x16(sYo + 16 * k, ro);
+          const uint32_t o0 = swz_offset(t, 2 * k, 128), o1 = swz_offset(t, 2 * k + 1, 128);
+          *reinterpret_cast<uint4*>(xw) = *reinterpret_cast<const uint4*>(xt + o0);
+          *reinterpret_cast<uint4*>(xw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
+          if (gated) {
+            *reinterpret_cast<uint4*>(zw) = *reinterpret_cast<const uint4*>(zt + o0);
+            *reinterpret_cast<uint4*>(zw + 4) = *reinterpret_cast<const uint4*>(zt + o1);
+          }
           tmem_wait_ld();
-          uint32_t out[8];
-          const uint32_t* xw = reinterpret_cast<const uint32_t*>(xv);
-          const uint32_t* zw = reinterpret_cast<const uint32_t*>(zv) + 8 * pc;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float a = fmaf(e, __uint_as_float(ro[2 * i]), __uint_as_float(ry[2 * i]));
-            float b = fmaf(e, __uint_as_float(ro[2 * i + 1]), __uint_as_float(ry[2 * i + 1]));
-            a = fmaf(Dh, bf_lo(xw[i]), a);
-            b = fmaf(Dh, bf_hi(xw[i]), b);
-            if (gz) {
+            float a = fmaf(Dh, bf_lo(xw[i]), fmaf(e, __uint_as_float(ro[2 * i]), __uint_as_float(ry[2 * i])));
+            float b = fmaf(Dh, bf_hi(xw[i]), fmaf(e, __uint_as_float(ro[2 * i + 1]), __uint_as_float(ry[2 * i + 1])));
+            if (gated) {
               a *= silu(bf_lo(zw[i]));
               b *= silu(bf_hi(zw[i]));
             }
             out[i] = bf16_pair(a, b);
           }
-          if (live) {
-            uint4* dst = reinterpret_cast<uint4*>(gy + row * p.ldy + 16 * pc);
-            if (16 * pc < pdims) dst[0] = make_uint4(out[0], out[1], out[2], out[3]);
-            if (16 * pc + 8 < pdims) dst[1] = make_uint4(out[4], out[5], out[6], out[7]);
+          *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
+          *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
+        }
+        tc_fence_before_sync();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->yo_free);
+          mbar_arrive(&bars->sc_free[b3]);
+          if (gated) mbar_arrive(&bars->zfree[wg]);
+        }
+        const long long t0 = sg.begin + static_cast<long long>(c) * kQ;
+        if (t0 + kQ <= sg.end) {
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");  // the four warps' rows are written
+          if (q == 0 && lane == 0) {
+            tma_store_3d(&maps.y, sbase + wg * L::kStage + stage_x, p0, h, static_cast<int>(t0));
+            mbar_arrive(&bars->xfree[wg]);
           }
-          if (pc == 3) {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(&bars->yo_free);
-              mbar_arrive(&bars->xfree[wg]);
-              mbar_arrive(&bars->sc_free[b3]);
-            }
+        } else {
+          if (t0 + t < sg.end) {
+            __nv_bfloat16* yr = gy + (t0 + t) * p.ldy;
+#pragma unroll 1
+            for (int i = 0; 8 * i < pdims; ++i)
+              *reinterpret_cast<uint4*>(yr + 8 * i) = *reinterpret_cast<const uint4*>(xt + swz_offset(t, i, 128));
           }
+          // a partial chunk is the last: nothing waits for its x tile
         }
       }
     }
-  } else if (warp >= 12 && warp < 16) {
+  } else if (warp < 20) {
+    regs_dec<64>();
     // ------------------------------------------------------------ Xw
     w.where = kWaitTransform;
-    const int s = threadIdx.x - 384;  // row
-    const uint32_t hi = sbase + L::kXw, lo = hi + kAtom;
+    const int s = (threadIdx.x - 384) & 127;     // row
+    const int i0 = warp < 16 ? 0 : 4;            // first of this thread's 16-byte pieces
     for (int c = 0; c < nc; ++c) {
       const int b3 = c % 3, sb = c & 1;
       const uint32_t st = sbase + sb * L::kStage;
       const long long left = sg.end - sg.begin - static_cast<long long>(c) * kQ;
-      if (!mbar_wait(&bars->sc_full[b3], (c / 3) & 1, w)) break;
-      if (!mbar_wait(&bars->full_x[sb], (c >> 1) & 1, w)) break;
+      if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, w)) break;
+      if (!wait_bar(&bars->full_x[sb], (c >> 1) & 1, w)) break;
       const float ws = scal[b3].f[3][s];
-      uint32_t vh[32], vl[32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 x = ld_shared_v4(st + stage_x + swz_offset(s, i, 128));
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float a = 0.0f, b = 0.0f;
-          if (s < left) a = ws * bf_lo(xs[k]), b = ws * bf_hi(xs[k]);
-          const uint32_t hp = bf16_pair(a, b);
-          vh[4 * i + k] = hp;
-          vl[4 * i + k] = bf16_pair(a - bf_lo(hp), b - bf_hi(hp));
-        }
-      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->sc_free[b3]);
-      if (c >= 1 && !mbar_wait(&bars->ds_full, (c - 1) & 1, w)) break;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      if (c >= 1 && !wait_bar(&bars->ds_full, (c - 1) & 1, w)) break;
+      const bool live = s < left;
+#pragma unroll 2
+      for (int i = i0; i < i0 + 4; ++i) {
         const uint32_t off = swz_offset(s, i, 128);
-        st_shared_v4(hi + off, vh[4 * i], vh[4 * i + 1], vh[4 * i + 2], vh[4 * i + 3]);
-        st_shared_v4(lo + off, vl[4 * i], vl[4 * i + 1], vl[4 * i + 2], vl[4 * i + 3]);
+        const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+        uint32_t vh[4], vl[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float a = live ? ws * bf_lo(xs[k]) : 0.0f, b = live ? ws * bf_hi(xs[k]) : 0.0f;
+          vh[k] = bf16_pair(a, b);
+          vl[k] = bf16_pair(a - bf_lo(vh[k]), b - bf_hi(vh[k]));
+        }
+        *reinterpret_cast<uint4*>(smem + L::kXw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
+        *reinterpret_cast<uint4*>(smem + L::kXw + kAtom + off) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
       }
       if (left < kQ) {
         // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-        if (!mbar_wait(&bars->full_bc[sb], (c >> 1) & 1, w)) break;
+        if (!wait_bar(&bars->full_bc[sb], (c >> 1) & 1, w)) break;
         if (s >= left) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = i0; i < i0 + 4; ++i) {
             const uint32_t off = swz_offset(s, i, 128);
             st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
 #pragma unroll
@@ -593,10 +723,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->xw_full);
     }
-  } else if (warp >= 16) {
+  } else {
+    regs_inc<96>();
     // ------------------------------------------------------------ state
     w.where = kWaitTransform;
-    const int n = threadIdx.x - 512;  // state element (lane of tensor memory)
+    const int n = threadIdx.x - 640;  // state element (lane of tensor memory)
     const int q = warp & 3;
     const bool wlive = 32 * q < N;    // this warp has state elements
     const bool live = n < N;
@@ -604,10 +735,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     float hv[kP];
 #pragma unroll
     for (int i = 0; i < kP; ++i) hv[i] = 0.0f;
+    // eight rows at a time (pdims is a multiple of 8): more loads in flight would not fit the registers
     auto add_state = [&](const float* src, float decay) {
 #pragma unroll
-      for (int i = 0; i < kP; ++i)
-        if (live && i < pdims) hv[i] = fmaf(hv[i], decay, src[i * N + n]);
+      for (int g8 = 0; g8 < kP / 8; ++g8) {
+        if (live && 8 * g8 < pdims) {
+          const float* at = src + 8 * g8 * N + n;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = at[i * N];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) hv[8 * g8 + i] = fmaf(hv[8 * g8 + i], decay, v[i]);
+        }
+        asm volatile("" ::: "memory");
+      }
     };
     if (!STATES) {
       if (sg.count == 1) {
@@ -631,14 +772,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->h_full);
     };
-    if (!STATES && nc > 0) put_h();
     bool ok = true;
     for (int c = 0; c < nc; ++c) {
       const int b3 = c % 3;
-      ok = mbar_wait(&bars->sc_full[b3], (c / 3) & 1, w);
+      if (!STATES) {
+        // the product that reads the old H is done
+        ok = c == 0 || wait_bar(&bars->done[(c - 1) & 1], ((c - 1) >> 1) & 1, w);
+        if (!ok) break;
+        put_h();
+      }
+      ok = wait_bar(&bars->sc_full[b3], (c / 3) & 1, w);
       if (!ok) break;
       const float decay = scal[b3].total;
-      ok = mbar_wait(&bars->ds_full, c & 1, w);
+      ok = wait_bar(&bars->ds_full, c & 1, w);
       if (!ok) break;
       tc_fence_after_sync();
       if (wlive) {
@@ -658,19 +804,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&bars->ds_free);
         mbar_arrive(&bars->sc_free[b3]);
       }
-      if (!STATES && c + 1 < nc) {
-        ok = mbar_wait(&bars->done[c & 1], (c >> 1) & 1, w);  // the product that reads the old H
-        if (!ok) break;
-        put_h();
-      }
     }
     if (ok) {
       float* dst = STATES ? p.seg_state + seg * per_slot + head_at
                           : (last && p.state_out && slot >= 0 ? p.state_out + slot * per_slot + head_at : nullptr);
-      if (dst && live) {
 #pragma unroll
-        for (int i = 0; i < kP; ++i)
-          if (i < pdims) dst[i * N + n] = hv[i];
+      for (int g8 = 0; g8 < kP / 8; ++g8) {
+        if (dst && live && 8 * g8 < pdims) {
+          float* at = dst + 8 * g8 * N + n;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) at[i * N] = hv[8 * g8 + i];
+        }
+        asm volatile("" ::: "memory");
       }
     }
   }
@@ -679,6 +824,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   if (warp == 1) tmem_dealloc(tmem, kCols);
+  if (STATES && pt == 0 && threadIdx.x == 0)
+    p.seg_log[static_cast<long long>(seg) * p.heads + h] = (seg_sum[0] + seg_sum[1]) * (1.0f / kLog2e);
 }
 
 int make_map(CUtensorMap* m, const void* base, int inner, int mid, long long rows, long long ld, const char* what) {
@@ -752,10 +899,13 @@ int scan_umma_launch(ScanParams& p, cudaStream_t st) {
   const int ptiles = (p.dim + kP - 1) / kP;
   const long long blocks = max_segments(p.tokens, p.nseq, p.seg_len) * p.heads * ptiles;
   if (blocks > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "selective scan too large for one launch");
-  Tmaps maps;
+  Tmaps maps{};
   if (int rc = make_map(&maps.x, p.x, p.dim, p.heads, p.tokens, p.ldx, "x")) return rc;
   if (int rc = make_map(&maps.b, p.B, p.state_dim, p.groups, p.tokens, p.ldb, "B")) return rc;
   if (int rc = make_map(&maps.c, p.C, p.state_dim, p.groups, p.tokens, p.ldc, "C")) return rc;
+  if (int rc = make_map(&maps.y, p.y, p.dim, p.heads, p.tokens, p.ldy, "y")) return rc;
+  if (p.z)
+    if (int rc = make_map(&maps.z, p.z, p.dim, p.heads, p.tokens, p.ldz, "z")) return rc;
   const unsigned grid = static_cast<unsigned>(blocks);
   if (p.state_dim <= 64) {
     if (p.split)
