@@ -30,8 +30,6 @@
 
 #include <algorithm>
 #include <mutex>
-#include <type_traits>
-#include <utility>
 
 #include "smm_scan.cuh"
 
@@ -45,8 +43,9 @@ constexpr int kQ = 128;         // tokens per chunk
 constexpr int kP = 64;          // dims per CTA
 constexpr int kThreads = 768;
 constexpr uint32_t kAtom = kQ * 128;  // one 64-element wide tile of 128 rows: 16 KiB
-// tensor memory columns; G[k] overlays the first half of S[k]
-constexpr uint32_t kColS = 0, kColY = 256, kColYo = 384, kColDs = 448, kCols = 512;
+// tensor memory columns, for two chunks: S is 128 wide; G takes the place of its
+// first half while it is read, Yo that of its second half afterwards
+constexpr uint32_t kColS = 0, kColYo = 64, kColY = 256, kColDs = 384, kCols = 512;
 
 struct Scal {
   float f[4][kQ];  // f[b-1][s], b = 1..4
@@ -59,8 +58,8 @@ struct Scal {
 };
 
 struct Bars {
-  uint64_t full_bc[2], full_x[2], full_z[2], done[2], xfree[2], bfree[2], zfree[2], s_full[2], g_full[2];
-  uint64_t xw_full, ds_full, ds_free, h_full, yo_free;
+  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], cfree[2], xfree[2], done[2], s_full[2], g_full[2], yo_free[2];
+  uint64_t xw_full, ds_full, ds_free, h_full;
   uint64_t sc_full[3], sc_free[3];
   uint64_t drain;
   uint32_t tmem;
@@ -79,7 +78,7 @@ struct Smem {
 };
 
 struct Tmaps {
-  CUtensorMap x, b, c, y, z;
+  CUtensorMap x, b, c, y;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
@@ -108,39 +107,25 @@ __device__ __forceinline__ uint32_t elect_one() {
       "{\n\t.reg .pred p;\n\t.reg .b32 t;\n\telect.sync t|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
   return r;
 }
-// The descriptors are given as their low word of the stage's first product and
-// their high word; the step's offset is added inside, so that the compiler
-// does not keep a register for every step of every product.
-template <uint32_t OA, uint32_t OB, bool FIRST>
+// Descriptors are given as two words: only the low one (the start address) changes.
 __device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
-                                        uint32_t b_hi, uint32_t idesc) {
+                                        uint32_t b_hi, uint32_t idesc, int acc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
-      "add.u32 x, %1, %7;\n\tadd.u32 y, %3, %8;\n\tmov.b64 da, {x, %2};\n\tmov.b64 db, {y, %4};\n\t"
-      "setp.ne.b32 p, %9, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+      "setp.ne.b32 p, %7, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}\n" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "n"(OA), "n"(OB), "n"(FIRST ? 0 : 1)
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "r"(acc)
       : "memory");
 }
 // A from tensor memory (bf16, two per column), B from shared memory
-template <uint32_t OA, uint32_t OB, bool FIRST>
 __device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
-                                        uint32_t idesc) {
+                                        uint32_t idesc, int acc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 db;\n\t"
-      "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\tmov.b64 db, {y, %3};\n\t"
-      "setp.ne.b32 p, %8, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, p;\n\t}\n" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "n"(OA), "n"(OB), "n"(FIRST ? 0 : 1)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "r"(acc)
       : "memory");
-}
-template <int... K, typename F>
-__device__ __forceinline__ void steps_of(std::integer_sequence<int, K...>, F&& f) {
-  (f(std::integral_constant<int, K>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void steps(F&& f) {
-  steps_of(std::make_integer_sequence<int, N>{}, f);
 }
 __device__ __forceinline__ void umma_commit_by(uint32_t leader, uint64_t* bar) {
   asm volatile(
@@ -158,26 +143,43 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Whether to give up a wait (called every 64 tries, out of line: a dozen roles' waits
-// share it).  t0 is 0 before the first call.
-__device__ __forceinline__ bool give_up(const WaitCtx& w, uint64_t& t0) {
-  if (*w.abort_flag) return true;
-  const uint64_t t = globaltimer_ns();
-  if (t0 == 0) t0 = t;
-  if (t - t0 <= w.limit_ns) return false;
-  *w.abort_flag = 1;
-  if (w.status) atomicOr(w.status, kDevErrTimeout | w.where);
+// Waits of all roles but the two below: every one of them depends on loads or
+// products still to come, so the loading and the issuing warp keep the time, and
+// raise the flag for all.  (The code of a dozen timers is what instruction fetches
+// have no room for.)
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const volatile int* abort_flag) {
+  const uint32_t a = smem_u32(bar);
+  while (!mbar_try_wait(a, parity))
+    if (*abort_flag) return false;
   return true;
 }
-// mbar_wait with a short inline path.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const WaitCtx& w) {
-  const uint32_t a = smem_u32(bar);
-  if (mbar_try_wait(a, parity)) return true;
+// Time since the first of a run of fruitless polls; true once the limit has passed
+// or another role has given up.
+struct Patience {
   uint64_t t0 = 0;
-  uint32_t n = 0;
+  uint32_t idle = 0;
+  __device__ __forceinline__ void progress() { idle = 0; }
+  __device__ __forceinline__ bool out(const ScanParams& p, volatile int* abort_flag, uint32_t where) {
+    if ((++idle & 255u) != 0) return false;  // the timer is slow to read
+    if (*abort_flag) return true;
+    const uint64_t t = globaltimer_ns();
+    if (idle == 256u) t0 = t;
+    if (t - t0 <= p.wait_limit_ns) return false;
+    *abort_flag = 1;
+    if (p.status) atomicOr(p.status, kDevErrTimeout | where);
+    return true;
+  }
+};
+// Until what has been issued has landed; gives up (for all) after the limit, a second at least.
+__device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t parity, const ScanParams& p, volatile int* abort_flag) {
+  const uint32_t a = smem_u32(bar);
+  const uint64_t t0 = globaltimer_ns(), limit = p.wait_limit_ns > 1000000000ull ? p.wait_limit_ns : 1000000000ull;
   while (!mbar_try_wait(a, parity))
-    if ((++n & 63u) == 0 && give_up(w, t0)) return false;
-  return true;
+    if (globaltimer_ns() - t0 > limit) {
+      *abort_flag = 1;
+      if (p.status) atomicOr(p.status, kDevErrTimeout | kWaitDrain);
+      break;
+    }
 }
 template <int R>
 __device__ __forceinline__ void regs_inc() {
@@ -187,10 +189,23 @@ template <int R>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
+template <int R>
+__device__ __forceinline__ void regs_to() {
+  if constexpr (R < 80)
+    regs_dec<R>();
+  else
+    regs_inc<R>();
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// v sigmoid(v) in five instructions; 0 once 1 + exp(-v) passes 2^126.
+__device__ __forceinline__ float gate(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(-kLog2e * v)));
+  return v * r;
 }
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -207,11 +222,18 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(r));
   return o;
 }
-// Registers into 32 lanes x 8 consecutive columns of tensor memory.
-__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
+// 32 lanes x 32 consecutive columns of tensor memory into registers.
+__device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -230,7 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   Scal* scal = reinterpret_cast<Scal*>(smem + L::kScal);
   Bars* bars = reinterpret_cast<Bars*>(smem + L::kBars);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a shuffle from a fixed lane tells the compiler that the warp's role, and all that
+  // follows from it, is uniform
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int pt = static_cast<int>(blockIdx.x % ptiles);
   const int hs = static_cast<int>(blockIdx.x / ptiles);
   const int h = hs % p.heads, seg = hs / p.heads;
@@ -264,21 +288,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->full_bc[i], 1);
+      mbar_init(&bars->full_b[i], 1);
+      mbar_init(&bars->full_c[i], 1);
       mbar_init(&bars->full_x[i], 1);
-      mbar_init(&bars->done[i], 1);
-      mbar_init(&bars->full_z[i], 1);
-      mbar_init(&bars->xfree[i], 1);
       mbar_init(&bars->bfree[i], 1);
-      mbar_init(&bars->zfree[i], 4);
+      mbar_init(&bars->cfree[i], 1);
+      mbar_init(&bars->xfree[i], 1);
+      mbar_init(&bars->done[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->g_full[i], 4);
+      mbar_init(&bars->yo_free[i], 4);
     }
     mbar_init(&bars->xw_full, 8);
     mbar_init(&bars->ds_full, 1);
     mbar_init(&bars->ds_free, 4);
     mbar_init(&bars->h_full, 4);
-    mbar_init(&bars->yo_free, 4);
     for (int i = 0; i < 3; ++i) {
       mbar_init(&bars->sc_full[i], 1);
       mbar_init(&bars->sc_free[i], STATES ? 12 : 16);
@@ -291,50 +315,48 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = bars->tmem;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, bars->tmem, 0);
 
-  WaitCtx w{&bars->abort_flag, p.status, p.wait_limit_ns, 0};
+  volatile int* const flag = &bars->abort_flag;
   constexpr uint32_t stage_c = 0, stage_b = NA * kAtom, stage_x = 2 * NA * kAtom;
 
-  // The launch's 6 x 80 registers per warpgroup's thread, shared out by need:
-  // 64 (loads, products, decays), 2 x 96 (G and y), 2 x 64 (Xw), 96 (state) = 480.
+  // The launch's 6 x 80 registers per warpgroup's thread, shared out by need.
   // A spill costs a trip to L2 here: shared memory leaves L1 too small for the stacks.
+  constexpr int kRegsMisc = 56, kRegsG = STATES ? 24 : 112, kRegsXw = 56, kRegsState = STATES ? 152 : 88;
+  static_assert(kRegsMisc + 2 * kRegsG + 2 * kRegsXw + kRegsState <= 6 * 80, "more registers than the launch has");
   if (warp < 4) {
-    regs_dec<64>();
+    regs_dec<kRegsMisc>();
   if (warp == 0) {
     // ------------------------------------------------------------ loads
     if (lane == 0) {
-      w.where = kWaitProducer;
-      const bool gated = !STATES && p.z != nullptr;
-      // next chunk of each kind of load; z goes where B was, once dS has read it
-      int c_bc = 0, c_x = 0, c_z = 0;
-      uint32_t idle = 0;
-      uint64_t t0 = 0;
+      // next chunk of each operand: each place is free at its own time
+      int c_b = 0, c_c = STATES ? nc : 0, c_x = 0;
+      Patience time;
       const int row0 = static_cast<int>(sg.begin);
-      while (c_bc < nc || c_x < nc || (gated && c_z < nc)) {
+      auto space = [&](uint64_t* free, int c) { return c < 2 || mbar_test(free + (c & 1), ((c >> 1) - 1) & 1); };
+      while (c_b < nc || c_c < nc || c_x < nc) {
         bool did = false;
-        if (gated && c_z < c_bc && mbar_test(&bars->bfree[c_z & 1], (c_z >> 1) & 1)) {
-          const int s = c_z & 1;
-          mbar_arrive_expect_tx(&bars->full_z[s], kAtom);
-          tma_load_3d(sbase + s * L::kStage + stage_b, &maps.z, &bars->full_z[s], p0, h, row0 + c_z * kQ);
-          ++c_z;
-          did = true;
-        }
-        if (c_bc < nc &&
-            (c_bc < 2 || (mbar_test(&bars->done[c_bc & 1], ((c_bc >> 1) - 1) & 1) &&
-                          (!gated || (c_z > c_bc - 2 && mbar_test(&bars->zfree[c_bc & 1], ((c_bc >> 1) - 1) & 1)))))) {
-          const int s = c_bc & 1;
-          const uint32_t st = sbase + s * L::kStage;
-          mbar_arrive_expect_tx(&bars->full_bc[s], (STATES ? 1 : 2) * NA * kAtom);
+        if (c_b < nc && space(bars->bfree, c_b)) {
+          const int s = c_b & 1;
+          mbar_arrive_expect_tx(&bars->full_b[s], NA * kAtom);
 #pragma unroll
-          for (int a = 0; a < NA; ++a) {
-            if (!STATES) tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_bc[s], a * 64, g, row0 + c_bc * kQ);
-            tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_bc[s], a * 64, g, row0 + c_bc * kQ);
-          }
-          ++c_bc;
+          for (int a = 0; a < NA; ++a)
+            tma_load_3d(sbase + s * L::kStage + stage_b + a * kAtom, &maps.b, &bars->full_b[s], a * 64, g,
+                        row0 + c_b * kQ);
+          ++c_b;
           did = true;
         }
-        if (c_x < c_bc && (c_x < 2 || STATES || mbar_test(&bars->xfree[c_x & 1], ((c_x >> 1) - 1) & 1))) {
+        if (c_c < nc && space(bars->cfree, c_c)) {
+          const int s = c_c & 1;
+          mbar_arrive_expect_tx(&bars->full_c[s], NA * kAtom);
+#pragma unroll
+          for (int a = 0; a < NA; ++a)
+            tma_load_3d(sbase + s * L::kStage + stage_c + a * kAtom, &maps.c, &bars->full_c[s], a * 64, g,
+                        row0 + c_c * kQ);
+          ++c_c;
+          did = true;
+        }
+        if (c_x < nc && space(STATES ? bars->bfree : bars->xfree, c_x)) {
           const int s = c_x & 1;
           mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
           tma_load_3d(sbase + s * L::kStage + stage_x, &maps.x, &bars->full_x[s], p0, h, row0 + c_x * kQ);
@@ -342,17 +364,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           did = true;
         }
         if (did)
-          idle = 0, t0 = 0;
-        else if ((++idle & 255u) == 0 && give_up(w, t0))
+          time.progress();
+        else if (time.out(p, flag, kWaitProducer))
           break;
       }
       // after an abort, copies in flight land before the CTA leaves
-      if (*w.abort_flag) {
-        int none = 0;
-        WaitCtx dw{&none, p.status, p.wait_limit_ns > 1000000000ull ? p.wait_limit_ns : 1000000000ull, kWaitDrain};
-        for (int c = c_bc > 2 ? c_bc - 2 : 0; c < c_bc; ++c) wait_bar(&bars->full_bc[c & 1], (c >> 1) & 1, dw);
-        for (int c = c_x > 2 ? c_x - 2 : 0; c < c_x; ++c) wait_bar(&bars->full_x[c & 1], (c >> 1) & 1, dw);
-        for (int c = c_z > 2 ? c_z - 2 : 0; c < c_z; ++c) wait_bar(&bars->full_z[c & 1], (c >> 1) & 1, dw);
+      if (*flag) {
+        const int n[3] = {c_b, STATES ? 0 : c_c, c_x};
+#pragma unroll 1
+        for (int k = 0; k < 6; ++k) {  // full_b, full_c, full_x, two of each
+          const int last_use = ((n[k >> 1] - (k & 1) + 1) >> 1) - 1;
+          if (last_use >= 0) drain_bar(&bars->full_b[0] + k, last_use & 1, p, flag);
+        }
       }
     }
   } else if (warp == 1) {
@@ -371,22 +394,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t hK = static_cast<uint32_t>(dK >> 32), hM = static_cast<uint32_t>(dM >> 32);
     auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xFFFFFFFFu, mbar_test(bar, parity)) != 0; };
     int s_next = STATES ? nc : 0, g_next = 0, sub = 0;
-    uint32_t idle = 0;
-    uint64_t t_idle = 0;
+    Patience time;
     while (g_next < nc) {
       bool did = false;
-      if (!STATES && s_next < nc && s_next < g_next + 2 && ready(&bars->full_bc[s_next & 1], (s_next >> 1) & 1)) {
-        // the loads of chunk c waited for every product of chunk c - 2, so S and G are free
+      if (!STATES && s_next < nc && s_next < g_next + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
+          ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1) &&
+          (s_next < 2 || ready(&bars->yo_free[s_next & 1], ((s_next >> 1) - 1) & 1))) {
+        // y of chunk c - 2 has left S's place, which its G and Yo shared
         tc_fence_after_sync();
         const int s = s_next & 1;
         const uint32_t base = lo(dK) + s * kSt;
-        steps<4 * NA>([&](auto kc) {
-          constexpr int k = decltype(kc)::value;
-          constexpr uint32_t off = ((k >> 2) * kAtom + (k & 3) * 32) >> 4;
-          if (k < ksteps)
-            umma_ss<off + (stage_c >> 4), off + (stage_b >> 4), k == 0>(leader, tmem + kColS + s * 128, base, hK, base, hK,
-                                                                       idS);
-        });
+#pragma unroll 2
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t off = base + (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
+          umma_ss(leader, tmem + kColS + s * 128, off + (stage_c >> 4), hK, off + (stage_b >> 4), hK, idS, k);
+        }
         umma_commit_by(leader, &bars->s_full[s]);
         ++s_next;
         did = true;
@@ -394,85 +416,61 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int c = g_next, s = c & 1;
         if (sub == 0) {
           if (ready(&bars->xw_full, c & 1) && (c == 0 || ready(&bars->ds_free, (c - 1) & 1)) &&
-              ready(&bars->full_bc[s], (c >> 1) & 1) && ready(&bars->full_x[s], (c >> 1) & 1)) {
+              ready(&bars->full_b[s], (c >> 1) & 1) && ready(&bars->full_x[s], (c >> 1) & 1)) {
             tc_fence_after_sync();
             const uint32_t base = lo(dM) + s * kSt;
-            steps<16>([&](auto kc) {
-              constexpr int k = decltype(kc)::value;
-              constexpr uint32_t kk = (k & 7) * 128;
-              umma_ss<(stage_b >> 4) + kk, (L::kXw >> 4) + (k >> 3) * (kAtom >> 4) + kk, k == 0>(
-                  leader, tmem + kColDs, base, hM, lo(dM), hM, idD);
-            });
+#pragma unroll 2
+            for (int k = 0; k < 16; ++k)  // Xw's low term lies 8 steps behind its high one
+              umma_ss(leader, tmem + kColDs, base + (stage_b >> 4) + (k & 7) * 128, hM, lo(dM) + (L::kXw >> 4) + k * 128,
+                      hM, idD, k);
             umma_commit_by(leader, &bars->ds_full);
-            if (!STATES) umma_commit_by(leader, &bars->bfree[s]);
+            umma_commit_by(leader, &bars->bfree[s]);
             if (STATES) {
-              umma_commit_by(leader, &bars->done[s]);
               ++g_next;
             } else {
               sub = 1;
             }
             did = true;
           }
-        } else if (sub == 1) {
-          if (ready(&bars->g_full[s], (c >> 1) & 1)) {
-            tc_fence_after_sync();
-            const uint32_t base = lo(dM) + s * kSt;
-            steps<8>([&](auto kc) {
-              constexpr int k = decltype(kc)::value;
-              umma_ts<k * 8, (stage_x >> 4) + k * 128, k == 0>(leader, tmem + kColY + s * kP, tmem + kColS + s * 128, base,
-                                                               hM, idY);
-            });
-            sub = 2;
-            did = true;
-          }
-        } else {
-          if (ready(&bars->h_full, c & 1) && (c == 0 || ready(&bars->yo_free, (c - 1) & 1))) {
-            tc_fence_after_sync();
-            const uint32_t base = lo(dK) + s * kSt;
-            steps<4 * NA>([&](auto kc) {
-              constexpr int k = decltype(kc)::value;
-              constexpr uint32_t off = ((k >> 2) * kAtom + (k & 3) * 32) >> 4;
-              if (k < ksteps)
-                umma_ss<off + (stage_c >> 4), (L::kH >> 4) + k * 128, k == 0>(leader, tmem + kColYo, base, hK, lo(dM), hM,
-                                                                             idY);
-            });
-            umma_commit_by(leader, &bars->done[s]);
-            sub = 0;
-            ++g_next;
-            did = true;
-          }
+        } else if (ready(&bars->g_full[s], (c >> 1) & 1) && ready(&bars->h_full, c & 1)) {
+          tc_fence_after_sync();
+          const uint32_t base = lo(dK) + s * kSt;
+#pragma unroll 2
+          for (int k = 0; k < ksteps; ++k)
+            umma_ss(leader, tmem + kColYo + s * 128, base + (stage_c >> 4) + (k >> 2) * (kAtom >> 4) + (k & 3) * 2, hK,
+                    lo(dM) + (L::kH >> 4) + k * 128, hM, idY, k);
+          umma_commit_by(leader, &bars->cfree[s]);
+          const uint32_t basex = lo(dM) + s * kSt;
+#pragma unroll 2
+          for (int k = 0; k < 8; ++k)
+            umma_ts(leader, tmem + kColY + s * kP, tmem + kColS + s * 128 + k * 8, basex + (stage_x >> 4) + k * 128, hM, idY,
+                    k);
+          umma_commit_by(leader, &bars->done[s]);
+          sub = 0;
+          ++g_next;
+          did = true;
         }
       }
-      if (did) {
-        idle = 0;
-      } else if ((++idle & 1023u) == 0) {
-        // the timer is slow to read: now and then is enough for the limit
-        if (__any_sync(0xFFFFFFFFu, *w.abort_flag != 0)) break;
-        if (idle == 1024u) t_idle = globaltimer_ns();
-        if (__any_sync(0xFFFFFFFFu, globaltimer_ns() - t_idle > w.limit_ns)) {
-          *w.abort_flag = 1;
-          if (w.status && lane == 0) atomicOr(w.status, kDevErrTimeout | kWaitMma);
-          break;
-        }
-      }
+      if (did)
+        time.progress();
+      else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitMma)))
+        break;
     }
     // every product has completed, and its arrivals have landed, before the CTA leaves
-    int none = 0;
-    WaitCtx dw{&none, p.status, p.wait_limit_ns > 1000000000ull ? p.wait_limit_ns : 1000000000ull, kWaitDrain};
     umma_commit_by(leader, &bars->drain);
-    wait_bar(&bars->drain, 0, dw);
+    drain_bar(&bars->drain, 0, p, flag);
   } else {
     // ------------------------------------------------------------ decays
-    w.where = kWaitTransform;
     const float A2 = __ldg(p.A + h) * kLog2e;
     float log_sum = 0.0f;  // log2 of the segment's decay
     bool ok = true;
     const float bias = p.dt_bias ? __ldg(p.dt_bias + h) : 0.0f;
+    // lane -> token 32 b + lane of each block b
     uint32_t raw[4] = {};
     auto fetch = [&](int c) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const long long t = sg.begin + static_cast<long long>(c) * kQ + lane * 4 + i;
+        const long long t = sg.begin + static_cast<long long>(c) * kQ + 32 * i + lane;
         if (t < sg.end) raw[i] = scan_dt_raw(p, t, h);
       }
     };
@@ -480,63 +478,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int c = warp - 2; c < nc; c += 2) {
       const int b3 = c % 3;
       if (c >= 3) {
-        ok = wait_bar(&bars->sc_free[b3], (c / 3 - 1) & 1, w);
+        ok = wait_bar(&bars->sc_free[b3], (c / 3 - 1) & 1, flag);
         if (!ok) break;
       }
       Scal& sc = scal[b3];
-      float d[4], inc[4], suf[4];
+      const long long left = sg.end - sg.begin - static_cast<long long>(c) * kQ - lane;
+      float bt[4], head = 0.0f;
+#pragma unroll 1
+      for (int b = 0; b < 4; ++b) {
+        const float d = 32 * b < left ? scan_dt(p, raw[0], bias) : 0.0f;
+        raw[0] = raw[1], raw[1] = raw[2], raw[2] = raw[3];
+        // sums within the block: inclusive up to the token, exclusive behind it
+        float inc = d * A2, suf = inc;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const long long t = sg.begin + static_cast<long long>(c) * kQ + lane * 4 + i;
-        d[i] = t < sg.end ? scan_dt(p, raw[i], bias) : 0.0f;
+        for (int o = 1; o < 32; o <<= 1) {
+          const float x = __shfl_up_sync(0xFFFFFFFFu, inc, o), z = __shfl_down_sync(0xFFFFFFFFu, suf, o);
+          if (lane >= o) inc += x;
+          if (lane + o < 32) suf += z;
+        }
+        bt[0] = bt[1], bt[1] = bt[2], bt[2] = bt[3], bt[3] = __shfl_sync(0xFFFFFFFFu, inc, 31);
+        suf = __shfl_down_sync(0xFFFFFFFFu, suf, 1);
+        const int t = 32 * b + lane;
+        sc.l[t] = inc;
+        sc.u[t] = ex2(inc);
+        sc.e[t] = ex2(head + inc);
+        sc.d[t] = d;
+        sc.f[3][t] = lane < 31 ? suf : 0.0f;  // the exponent, until the blocks' sums are known
+        head += bt[3];
       }
       if (c + 2 < nc) fetch(c + 2);
-      // sums within blocks of 32 tokens (8 lanes): inclusive before, exclusive behind
-      float run = 0.0f;
+#pragma unroll 1
+      for (int b = 0; b < 4; ++b) {
+        const int t = 32 * b + lane;
+        const float suf = sc.f[3][t], d = sc.d[t];
+        float between = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) inc[i] = (run += d[i] * A2);
-      float back = 0.0f;
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        suf[i] = back;
-        back += d[i] * A2;
-      }
-      float pre = run, post = back;  // scans of the lanes' sums
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        const float a = __shfl_up_sync(0xFFFFFFFFu, pre, o, 8), z = __shfl_down_sync(0xFFFFFFFFu, post, o, 8);
-        if ((lane & 7) >= o) pre += a;
-        if ((lane & 7) + o < 8) post += z;
-      }
-      const float before = __shfl_up_sync(0xFFFFFFFFu, pre, 1, 8), behind = __shfl_down_sync(0xFFFFFFFFu, post, 1, 8);
-      if (lane & 7) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) inc[i] += before;
-      }
-      if ((lane & 7) != 7) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) suf[i] += behind;
-      }
-      float bt[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) bt[k] = __shfl_sync(0xFFFFFFFFu, pre, 8 * k + 7);
-      const int blk = lane >> 3;
-      const float head = (blk > 0 ? bt[0] : 0.0f) + (blk > 1 ? bt[1] : 0.0f) + (blk > 2 ? bt[2] : 0.0f);
-      float4 v;
-      v = make_float4(inc[0], inc[1], inc[2], inc[3]);
-      reinterpret_cast<float4*>(sc.l)[lane] = v;
-      reinterpret_cast<float4*>(sc.u)[lane] = make_float4(ex2(v.x), ex2(v.y), ex2(v.z), ex2(v.w));
-      reinterpret_cast<float4*>(sc.e)[lane] =
-          make_float4(ex2(head + v.x), ex2(head + v.y), ex2(head + v.z), ex2(head + v.w));
-      reinterpret_cast<float4*>(sc.d)[lane] = make_float4(d[0], d[1], d[2], d[3]);
-      float between = 0.0f;
-#pragma unroll
-      for (int b = 1; b <= 4; ++b) {
-        if (b > blk) {
-          if (b - 1 > blk) between += bt[b - 1];
-          reinterpret_cast<float4*>(sc.f[b - 1])[lane] =
-              make_float4(d[0] * ex2(suf[0] + between), d[1] * ex2(suf[1] + between), d[2] * ex2(suf[2] + between),
-                          d[3] * ex2(suf[3] + between));
+        for (int k = 1; k <= 4; ++k) {
+          if (k > b) {
+            if (k - 1 > b) between += bt[k - 1];
+            sc.f[k - 1][t] = d * ex2(suf + between);
+          }
         }
       }
       const float total = bt[0] + bt[1] + bt[2] + bt[3];
@@ -548,80 +529,90 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) seg_sum[warp - 2] = log_sum;
   }
   } else if (warp < 12) {
-    regs_inc<96>();
+    regs_to<kRegsG>();
     // ------------------------------------------------------------ G, then y
     if constexpr (!STATES) {
-      w.where = kWaitEpilogue;
       const int wg = (warp - 4) >> 2, q = warp & 3;
       const int t = 32 * q + lane;
       const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
       const uint32_t sS = tmem + lanes + kColS + wg * 128, sY = tmem + lanes + kColY + wg * kP;
-      const uint32_t sYo = tmem + lanes + kColYo;
+      const uint32_t sYo = sS + kColYo;
       const float Dh = p.D ? __ldg(p.D + h) : 0.0f;
       __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + static_cast<long long>(h) * p.dim + p0;
       const bool gated = p.z != nullptr;
+      const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + static_cast<long long>(h) * p.dim + p0;
       for (int c = wg; c < nc; c += 2) {
         const int b3 = c % 3;
         const uint32_t par = (c >> 1) & 1;
-        if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, w)) break;
-        if (!wait_bar(&bars->s_full[wg], par, w)) break;
+        if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
+        if (!wait_bar(&bars->s_full[wg], par, flag)) break;
         tc_fence_after_sync();
         const Scal& sc = scal[b3];
         const float u = sc.u[t], lt = sc.l[t];
-        // 16 columns at a time: the block of columns b is off the diagonal for b < q
 #pragma unroll 1
-        for (int j = 0; j < 8; ++j) {
-          const int b = j >> 1;
-          uint32_t o[8];
+        for (int b = 0; b < 4; ++b) {
+          uint32_t o[16];
           if (b <= q) {
-            uint32_t r[16];
-            tmem_ld_32x32b_x16(sS + 16 * j, r);
-            const float2* f = reinterpret_cast<const float2*>((b < q ? sc.f[q - 1] : sc.d) + 16 * j);
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(sS + 32 * b, r);
+            const float4* f = reinterpret_cast<const float4*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
             if (b < q) {
               const float2 u2 = make_float2(u, u);
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float2 v = mul2(
-                    mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), f[i]), u2);
-                o[i] = bf16_pair(v.x, v.y);
+                const float4 f4 = f[i];
+                const float2 v0 = mul2(
+                    mul2(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), make_float2(f4.x, f4.y)),
+                    u2);
+                const float2 v1 = mul2(mul2(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
+                                            make_float2(f4.z, f4.w)),
+                                       u2);
+                o[2 * i] = bf16_pair(v0.x, v0.y);
+                o[2 * i + 1] = bf16_pair(v1.x, v1.y);
               }
             } else {
-              const float2* ls = reinterpret_cast<const float2*>(sc.l + 16 * j);
-              const int top = lane - 16 * (j & 1);  // columns up to here are at or before this row
-              float2 g2[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float2 l2 = ls[i], d2 = f[i];
-                g2[i] = make_float2(ex2(lt - l2.x) * d2.x, ex2(lt - l2.y) * d2.y);
-              }
+              const float4* ls = reinterpret_cast<const float4*>(sc.l + 32 * b);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                o[i] = bf16_pair(2 * i <= top ? __uint_as_float(r[2 * i]) * g2[i].x : 0.0f,
-                                 2 * i + 1 <= top ? __uint_as_float(r[2 * i + 1]) * g2[i].y : 0.0f);
+              for (int i = 0; i < 8; ++i) {
+                const float4 l4 = ls[i], d4 = f[i];
+                // columns up to this row
+                const float g0 = 4 * i <= lane ? __uint_as_float(r[4 * i]) * (ex2(lt - l4.x) * d4.x) : 0.0f;
+                const float g1 = 4 * i + 1 <= lane ? __uint_as_float(r[4 * i + 1]) * (ex2(lt - l4.y) * d4.y) : 0.0f;
+                const float g2 = 4 * i + 2 <= lane ? __uint_as_float(r[4 * i + 2]) * (ex2(lt - l4.z) * d4.z) : 0.0f;
+                const float g3 = 4 * i + 3 <= lane ? __uint_as_float(r[4 * i + 3]) * (ex2(lt - l4.w) * d4.w) : 0.0f;
+                o[2 * i] = bf16_pair(g0, g1);
+                o[2 * i + 1] = bf16_pair(g2, g3);
+              }
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = 0;
+            for (int i = 0; i < 16; ++i) o[i] = 0;
           }
-          // columns 8 j .. 8 j + 7 of S have been read by this lane already
-          tmem_st_32x32b_x8(sS + 8 * j, o);
+          // columns 16 b .. 16 b + 15 of S have been read by this lane already
+          tmem_st_32x32b_x16(sS + 16 * b, o);
         }
         tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->g_full[wg]);
 
+        const long long t0 = sg.begin + static_cast<long long>(c) * kQ;
+        // z's own row, on its way while the products run
+        uint4 zv[8];
+        if (gated) {
+          const uint4* zr = reinterpret_cast<const uint4*>(gz + (t0 + t) * p.ldz);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) zv[i] = t0 + t < sg.end && 8 * i < pdims ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
+        }
         // y takes x's place in shared memory, row by row, and leaves as one tile (or by
         // rows where the chunk ends before the tile)
-        if (!wait_bar(&bars->full_x[wg], par, w)) break;
-        if (gated && !wait_bar(&bars->full_z[wg], par, w)) break;
-        if (!wait_bar(&bars->done[wg], par, w)) break;
+        if (!wait_bar(&bars->full_x[wg], par, flag)) break;
+        if (!wait_bar(&bars->done[wg], par, flag)) break;
         tc_fence_after_sync();
         const float e = sc.e[t];
         uint8_t* xt = smem + wg * L::kStage + stage_x;
-        const uint8_t* zt = smem + wg * L::kStage + stage_b;
 #pragma unroll 1
         for (int k = 0; k < 4; ++k) {
           uint32_t ry[16], ro[16], xw[8], zw[8], out[8];
@@ -631,8 +622,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(xw) = *reinterpret_cast<const uint4*>(xt + o0);
           *reinterpret_cast<uint4*>(xw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
           if (gated) {
-            *reinterpret_cast<uint4*>(zw) = *reinterpret_cast<const uint4*>(zt + o0);
-            *reinterpret_cast<uint4*>(zw + 4) = *reinterpret_cast<const uint4*>(zt + o1);
+            *reinterpret_cast<uint4*>(zw) = zv[0];
+            *reinterpret_cast<uint4*>(zw + 4) = zv[1];
+#pragma unroll
+            for (int i = 0; i < 6; ++i) zv[i] = zv[i + 2];
           }
           tmem_wait_ld();
 #pragma unroll
@@ -640,8 +633,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             float a = fmaf(Dh, bf_lo(xw[i]), fmaf(e, __uint_as_float(ro[2 * i]), __uint_as_float(ry[2 * i])));
             float b = fmaf(Dh, bf_hi(xw[i]), fmaf(e, __uint_as_float(ro[2 * i + 1]), __uint_as_float(ry[2 * i + 1])));
             if (gated) {
-              a *= silu(bf_lo(zw[i]));
-              b *= silu(bf_hi(zw[i]));
+              a *= gate(bf_lo(zw[i]));
+              b *= gate(bf_hi(zw[i]));
             }
             out[i] = bf16_pair(a, b);
           }
@@ -652,11 +645,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bars->yo_free);
+          mbar_arrive(&bars->yo_free[wg]);
           mbar_arrive(&bars->sc_free[b3]);
-          if (gated) mbar_arrive(&bars->zfree[wg]);
         }
-        const long long t0 = sg.begin + static_cast<long long>(c) * kQ;
         if (t0 + kQ <= sg.end) {
           asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");  // the four warps' rows are written
           if (q == 0 && lane == 0) {
@@ -675,23 +666,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp < 20) {
-    regs_dec<64>();
+    regs_dec<kRegsXw>();
     // ------------------------------------------------------------ Xw
-    w.where = kWaitTransform;
     const int s = (threadIdx.x - 384) & 127;     // row
     const int i0 = warp < 16 ? 0 : 4;            // first of this thread's 16-byte pieces
     for (int c = 0; c < nc; ++c) {
       const int b3 = c % 3, sb = c & 1;
       const uint32_t st = sbase + sb * L::kStage;
       const long long left = sg.end - sg.begin - static_cast<long long>(c) * kQ;
-      if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, w)) break;
-      if (!wait_bar(&bars->full_x[sb], (c >> 1) & 1, w)) break;
+      if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
+      if (!wait_bar(&bars->full_x[sb], (c >> 1) & 1, flag)) break;
       const float ws = scal[b3].f[3][s];
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->sc_free[b3]);
-      if (c >= 1 && !wait_bar(&bars->ds_full, (c - 1) & 1, w)) break;
+      if (c >= 1 && !wait_bar(&bars->ds_full, (c - 1) & 1, flag)) break;
       const bool live = s < left;
-#pragma unroll 2
+#pragma unroll 1
       for (int i = i0; i < i0 + 4; ++i) {
         const uint32_t off = swz_offset(s, i, 128);
         const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
@@ -708,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (left < kQ) {
         // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-        if (!wait_bar(&bars->full_bc[sb], (c >> 1) & 1, w)) break;
+        if (!wait_bar(&bars->full_b[sb], (c >> 1) & 1, flag)) break;
         if (s >= left) {
 #pragma unroll
           for (int i = i0; i < i0 + 4; ++i) {
@@ -724,9 +714,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&bars->xw_full);
     }
   } else {
-    regs_inc<96>();
+    regs_inc<kRegsState>();
     // ------------------------------------------------------------ state
-    w.where = kWaitTransform;
     const int n = threadIdx.x - 640;  // state element (lane of tensor memory)
     const int q = warp & 3;
     const bool wlive = 32 * q < N;    // this warp has state elements
@@ -751,13 +740,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     if (!STATES) {
-      if (sg.count == 1) {
-        if (in) add_state(in, 0.0f);
-      } else {
-        add_state(p.seg_state + (sg.first + sg.count - 1) * per_slot + head_at, 0.0f);
-        for (int k = 0; k < sg.j; ++k)
-          add_state(p.seg_state + (sg.first + k) * per_slot + head_at,
-                    expf(p.seg_log[static_cast<long long>(sg.first + k) * p.heads + h]));
+      // Horner over the earlier segments' final states; the first term is what the sequence starts from
+      const float* src = sg.count == 1 ? in : p.seg_state + (sg.first + sg.count - 1) * per_slot + head_at;
+      const int terms = sg.count > 1 ? 1 + sg.j : in ? 1 : 0;
+#pragma unroll 1
+      for (int k = 0; k < terms; ++k) {
+        const float decay = k ? expf(p.seg_log[static_cast<long long>(sg.first + k - 1) * p.heads + h]) : 0.0f;
+        add_state(src, decay);
+        src = p.seg_state + (sg.first + k) * per_slot + head_at;
       }
     }
     auto put_h = [&]() {
@@ -777,14 +767,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b3 = c % 3;
       if (!STATES) {
         // the product that reads the old H is done
-        ok = c == 0 || wait_bar(&bars->done[(c - 1) & 1], ((c - 1) >> 1) & 1, w);
+        ok = c == 0 || wait_bar(&bars->cfree[(c - 1) & 1], ((c - 1) >> 1) & 1, flag);
         if (!ok) break;
         put_h();
       }
-      ok = wait_bar(&bars->sc_full[b3], (c / 3) & 1, w);
+      ok = wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag);
       if (!ok) break;
       const float decay = scal[b3].total;
-      ok = wait_bar(&bars->ds_full, c & 1, w);
+      ok = wait_bar(&bars->ds_full, c & 1, flag);
       if (!ok) break;
       tc_fence_after_sync();
       if (wlive) {
@@ -795,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            hv[16 * pc + i] = live ? fmaf(hv[16 * pc + i], decay, __uint_as_float(r[i])) : 0.0f;
+            hv[16 * pc + i] = fmaf(hv[16 * pc + i], decay, __uint_as_float(r[i]));
         }
       }
       tc_fence_before_sync();
@@ -904,8 +894,6 @@ int scan_umma_launch(ScanParams& p, cudaStream_t st) {
   if (int rc = make_map(&maps.b, p.B, p.state_dim, p.groups, p.tokens, p.ldb, "B")) return rc;
   if (int rc = make_map(&maps.c, p.C, p.state_dim, p.groups, p.tokens, p.ldc, "C")) return rc;
   if (int rc = make_map(&maps.y, p.y, p.dim, p.heads, p.tokens, p.ldy, "y")) return rc;
-  if (p.z)
-    if (int rc = make_map(&maps.z, p.z, p.dim, p.heads, p.tokens, p.ldz, "z")) return rc;
   const unsigned grid = static_cast<unsigned>(blocks);
   if (p.state_dim <= 64) {
     if (p.split)
