@@ -22,8 +22,8 @@
 // (2^-16), because the state is an fp32 result that is carried on.  The state
 // itself stays in fp32 registers, S, Y, Yo and dS are fp32 in tensor memory.
 //
-// Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the decays in turn, 4-7 and 8-11
-// form G and write y of the even and the odd chunks, 12-19 form Xw, 20-23 carry
+// Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the decays in turn,
+// 4-11 form G and write y of the chunk before, half of the columns each, 12-19 form Xw, 20-23 carry
 // the state.  Every wait is bounded; on expiry the CTA records it and leaves.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -43,9 +43,9 @@ constexpr int kQ = 128;         // tokens per chunk
 constexpr int kP = 64;          // dims per CTA
 constexpr int kThreads = 768;
 constexpr uint32_t kAtom = kQ * 128;  // one 64-element wide tile of 128 rows: 16 KiB
-// tensor memory columns, for two chunks: S is 128 wide; G takes the place of its
-// first half while it is read, Yo that of its second half afterwards
-constexpr uint32_t kColS = 0, kColYo = 64, kColY = 256, kColDs = 384, kCols = 512;
+// Tensor memory columns.  S is 128 wide and double; G takes the place of the first
+// quarter and the third one of S, each written by the warps that have read its half.
+constexpr uint32_t kColS = 0, kColY = 256, kColDs = 384, kColYo = 448, kCols = 512;
 
 struct Scal {
   float f[4][kQ];  // f[b-1][s], b = 1..4
@@ -58,8 +58,8 @@ struct Scal {
 };
 
 struct Bars {
-  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], cfree[2], xfree[2], done[2], s_full[2], g_full[2], yo_free[2];
-  uint64_t xw_full, ds_full, ds_free, h_full;
+  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], xfree[2], done[2], s_full[2], g_full[2];
+  uint64_t xw_full, ds_full, ds_free, h_full, yo_free, y_full;
   uint64_t sc_full[3], sc_free[3];
   uint64_t drain;
   uint32_t tmem;
@@ -292,20 +292,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->full_c[i], 1);
       mbar_init(&bars->full_x[i], 1);
       mbar_init(&bars->bfree[i], 1);
-      mbar_init(&bars->cfree[i], 1);
       mbar_init(&bars->xfree[i], 1);
       mbar_init(&bars->done[i], 1);
       mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->g_full[i], 4);
-      mbar_init(&bars->yo_free[i], 4);
+      mbar_init(&bars->g_full[i], 8);
     }
     mbar_init(&bars->xw_full, 8);
     mbar_init(&bars->ds_full, 1);
     mbar_init(&bars->ds_free, 4);
     mbar_init(&bars->h_full, 4);
+    mbar_init(&bars->yo_free, 8);
+    mbar_init(&bars->y_full, 8);
     for (int i = 0; i < 3; ++i) {
       mbar_init(&bars->sc_full[i], 1);
-      mbar_init(&bars->sc_free[i], STATES ? 12 : 16);
+      mbar_init(&bars->sc_free[i], STATES ? 12 : 20);
     }
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++c_b;
           did = true;
         }
-        if (c_c < nc && space(bars->cfree, c_c)) {
+        if (c_c < nc && space(bars->done, c_c)) {
           const int s = c_c & 1;
           mbar_arrive_expect_tx(&bars->full_c[s], NA * kAtom);
 #pragma unroll
@@ -367,6 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           time.progress();
         else if (time.out(p, flag, kWaitProducer))
           break;
+        else
+          __nanosleep(100);  // polling takes issue slots from the warps that compute
       }
       // after an abort, copies in flight land before the CTA leaves
       if (*flag) {
@@ -398,9 +400,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (g_next < nc) {
       bool did = false;
       if (!STATES && s_next < nc && s_next < g_next + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
-          ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1) &&
-          (s_next < 2 || ready(&bars->yo_free[s_next & 1], ((s_next >> 1) - 1) & 1))) {
-        // y of chunk c - 2 has left S's place, which its G and Yo shared
+          ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1)) {
+        // C was loaded once every product of chunk c - 2 was done: S's place, where its G was, is free
         tc_fence_after_sync();
         const int s = s_next & 1;
         const uint32_t base = lo(dK) + s * kSt;
@@ -432,19 +433,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             did = true;
           }
-        } else if (ready(&bars->g_full[s], (c >> 1) & 1) && ready(&bars->h_full, c & 1)) {
+        } else if (sub == 1) {
+          if (ready(&bars->g_full[s], (c >> 1) & 1)) {
+            tc_fence_after_sync();
+            const uint32_t base = lo(dM) + s * kSt;
+#pragma unroll 2
+            for (int k = 0; k < 8; ++k)
+              umma_ts(leader, tmem + kColY + s * kP, tmem + kColS + s * 128 + (k >> 2) * 64 + (k & 3) * 8,
+                      base + (stage_x >> 4) + k * 128, hM, idY, k);
+            sub = 2;
+            did = true;
+          }
+        } else if (ready(&bars->h_full, c & 1) && (c == 0 || ready(&bars->yo_free, (c - 1) & 1))) {
           tc_fence_after_sync();
           const uint32_t base = lo(dK) + s * kSt;
 #pragma unroll 2
           for (int k = 0; k < ksteps; ++k)
-            umma_ss(leader, tmem + kColYo + s * 128, base + (stage_c >> 4) + (k >> 2) * (kAtom >> 4) + (k & 3) * 2, hK,
+            umma_ss(leader, tmem + kColYo, base + (stage_c >> 4) + (k >> 2) * (kAtom >> 4) + (k & 3) * 2, hK,
                     lo(dM) + (L::kH >> 4) + k * 128, hM, idY, k);
-          umma_commit_by(leader, &bars->cfree[s]);
-          const uint32_t basex = lo(dM) + s * kSt;
-#pragma unroll 2
-          for (int k = 0; k < 8; ++k)
-            umma_ts(leader, tmem + kColY + s * kP, tmem + kColS + s * 128 + k * 8, basex + (stage_x >> 4) + k * 128, hM, idY,
-                    k);
           umma_commit_by(leader, &bars->done[s]);
           sub = 0;
           ++g_next;
@@ -455,6 +461,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         time.progress();
       else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitMma)))
         break;
+      else
+        __nanosleep(20);
     }
     // every product has completed, and its arrivals have landed, before the CTA leaves
     umma_commit_by(leader, &bars->drain);
@@ -530,138 +538,147 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else if (warp < 12) {
     regs_to<kRegsG>();
-    // ------------------------------------------------------------ G, then y
+    // ------------------------------------------------------------ G, and y of the chunk before
     if constexpr (!STATES) {
-      const int wg = (warp - 4) >> 2, q = warp & 3;
+      const int half = (warp - 4) >> 2, q = warp & 3;  // columns 64 half.. of G, 32 half.. of y
       const int t = 32 * q + lane;
       const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
-      const uint32_t sS = tmem + lanes + kColS + wg * 128, sY = tmem + lanes + kColY + wg * kP;
-      const uint32_t sYo = sS + kColYo;
+      const uint32_t sYo = tmem + lanes + kColYo + 32 * half;
       const float Dh = p.D ? __ldg(p.D + h) : 0.0f;
-      __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + static_cast<long long>(h) * p.dim + p0;
       const bool gated = p.z != nullptr;
-      const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + static_cast<long long>(h) * p.dim + p0;
-      for (int c = wg; c < nc; c += 2) {
-        const int b3 = c % 3;
-        const uint32_t par = (c >> 1) & 1;
-        if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
-        if (!wait_bar(&bars->s_full[wg], par, flag)) break;
-        tc_fence_after_sync();
-        const Scal& sc = scal[b3];
-        const float u = sc.u[t], lt = sc.l[t];
-#pragma unroll 1
-        for (int b = 0; b < 4; ++b) {
-          uint32_t o[16];
-          if (b <= q) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(sS + 32 * b, r);
-            const float4* f = reinterpret_cast<const float4*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
-            if (b < q) {
-              const float2 u2 = make_float2(u, u);
-              tmem_wait_ld();
+      const long long col = static_cast<long long>(h) * p.dim + p0 + 32 * half;
+      const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + (sg.begin + t) * p.ldz + col;
+      const int wdims = pdims - 32 * half;  // columns of this half
+      for (int c = 0; c <= nc; ++c) {
+        // z's own row for the chunk before, on its way while G is formed
+        uint4 zv[4];
+        if (gated && c > 0) {
+          const bool live = sg.begin + static_cast<long long>(c - 1) * kQ + t < sg.end;
+          const uint4* zr = reinterpret_cast<const uint4*>(gz + static_cast<long long>(c - 1) * kQ * p.ldz);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 f4 = f[i];
-                const float2 v0 = mul2(
-                    mul2(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), make_float2(f4.x, f4.y)),
-                    u2);
-                const float2 v1 = mul2(mul2(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
-                                            make_float2(f4.z, f4.w)),
-                                       u2);
-                o[2 * i] = bf16_pair(v0.x, v0.y);
-                o[2 * i + 1] = bf16_pair(v1.x, v1.y);
+          for (int i = 0; i < 4; ++i) zv[i] = live && 8 * i < wdims ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
+        }
+        if (c < nc) {
+          const int b3 = c % 3, s = c & 1;
+          if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
+          if (!wait_bar(&bars->s_full[s], (c >> 1) & 1, flag)) break;
+          tc_fence_after_sync();
+          const Scal& sc = scal[b3];
+          const float u = sc.u[t], lt = sc.l[t];
+          const uint32_t sS = tmem + lanes + kColS + s * 128 + 64 * half;
+#pragma unroll 1
+          for (int i2 = 0; i2 < 2; ++i2) {
+            const int b = 2 * half + i2;  // block of 32 columns: off the diagonal for b < q
+            uint32_t o[16];
+            if (b <= q) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(sS + 32 * i2, r);
+              const float4* f = reinterpret_cast<const float4*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
+              if (b < q) {
+                const float2 u2 = make_float2(u, u);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float4 f4 = f[i];
+                  const float2 v0 = mul2(mul2(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])),
+                                              make_float2(f4.x, f4.y)),
+                                         u2);
+                  const float2 v1 = mul2(mul2(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
+                                              make_float2(f4.z, f4.w)),
+                                         u2);
+                  o[2 * i] = bf16_pair(v0.x, v0.y);
+                  o[2 * i + 1] = bf16_pair(v1.x, v1.y);
+                }
+              } else {
+                const float4* ls = reinterpret_cast<const float4*>(sc.l + 32 * b);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float4 l4 = ls[i], d4 = f[i];
+                  // columns up to this row
+                  const float g0 = 4 * i <= lane ? __uint_as_float(r[4 * i]) * (ex2(lt - l4.x) * d4.x) : 0.0f;
+                  const float g1 = 4 * i + 1 <= lane ? __uint_as_float(r[4 * i + 1]) * (ex2(lt - l4.y) * d4.y) : 0.0f;
+                  const float g2 = 4 * i + 2 <= lane ? __uint_as_float(r[4 * i + 2]) * (ex2(lt - l4.z) * d4.z) : 0.0f;
+                  const float g3 = 4 * i + 3 <= lane ? __uint_as_float(r[4 * i + 3]) * (ex2(lt - l4.w) * d4.w) : 0.0f;
+                  o[2 * i] = bf16_pair(g0, g1);
+                  o[2 * i + 1] = bf16_pair(g2, g3);
+                }
               }
             } else {
-              const float4* ls = reinterpret_cast<const float4*>(sc.l + 32 * b);
-              tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 l4 = ls[i], d4 = f[i];
-                // columns up to this row
-                const float g0 = 4 * i <= lane ? __uint_as_float(r[4 * i]) * (ex2(lt - l4.x) * d4.x) : 0.0f;
-                const float g1 = 4 * i + 1 <= lane ? __uint_as_float(r[4 * i + 1]) * (ex2(lt - l4.y) * d4.y) : 0.0f;
-                const float g2 = 4 * i + 2 <= lane ? __uint_as_float(r[4 * i + 2]) * (ex2(lt - l4.z) * d4.z) : 0.0f;
-                const float g3 = 4 * i + 3 <= lane ? __uint_as_float(r[4 * i + 3]) * (ex2(lt - l4.w) * d4.w) : 0.0f;
-                o[2 * i] = bf16_pair(g0, g1);
-                o[2 * i + 1] = bf16_pair(g2, g3);
+              for (int i = 0; i < 16; ++i) o[i] = 0;
+            }
+            // these columns of S have been read by this lane already
+            tmem_st_32x32b_x16(sS + 16 * i2, o);
+          }
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->g_full[s]);
+        }
+        if (c > 0) {
+          const int d = c - 1, b3 = d % 3, s = d & 1;
+          // y takes x's place in shared memory, row by row, and leaves as one tile (or by
+          // rows where the chunk ends before the tile)
+          if (!wait_bar(&bars->full_x[s], (d >> 1) & 1, flag)) break;
+          if (!wait_bar(&bars->done[s], (d >> 1) & 1, flag)) break;
+          tc_fence_after_sync();
+          const float e = scal[b3].e[t];
+          const uint32_t sY = tmem + lanes + kColY + s * kP + 32 * half;
+          uint8_t* xt = smem + s * L::kStage + stage_x;
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            uint32_t ry[16], ro[16], xw[8], zw[8], out[8];
+            tmem_ld_32x32b_x16(sY + 16 * k, ry);
+            tmem_ld_32x32b_x16(sYo + 16 * k, ro);
+            const uint32_t o0 = swz_offset(t, 4 * half + 2 * k, 128), o1 = swz_offset(t, 4 * half + 2 * k + 1, 128);
+            *reinterpret_cast<uint4*>(xw) = *reinterpret_cast<const uint4*>(xt + o0);
+            *reinterpret_cast<uint4*>(xw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
+            if (gated) {
+              *reinterpret_cast<uint4*>(zw) = zv[0];
+              *reinterpret_cast<uint4*>(zw + 4) = zv[1];
+              zv[0] = zv[2];
+              zv[1] = zv[3];
+            }
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float a = fmaf(Dh, bf_lo(xw[i]), fmaf(e, __uint_as_float(ro[2 * i]), __uint_as_float(ry[2 * i])));
+              float b = fmaf(Dh, bf_hi(xw[i]), fmaf(e, __uint_as_float(ro[2 * i + 1]), __uint_as_float(ry[2 * i + 1])));
+              if (gated) {
+                a *= gate(bf_lo(zw[i]));
+                b *= gate(bf_hi(zw[i]));
+              }
+              out[i] = bf16_pair(a, b);
+            }
+            *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
+            *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
+          }
+          tc_fence_before_sync();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bars->yo_free);
+            mbar_arrive(&bars->sc_free[b3]);
+            mbar_arrive(&bars->y_full);
+          }
+          const long long t0 = sg.begin + static_cast<long long>(d) * kQ;
+          if (t0 + kQ <= sg.end) {
+            if (warp == 4) {
+              if (!wait_bar(&bars->y_full, d & 1, flag)) break;  // all of the tile is written
+              if (lane == 0) {
+                tma_store_3d(&maps.y, sbase + s * L::kStage + stage_x, p0, h, static_cast<int>(t0));
+                mbar_arrive(&bars->xfree[s]);
               }
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = 0;
-          }
-          // columns 16 b .. 16 b + 15 of S have been read by this lane already
-          tmem_st_32x32b_x16(sS + 16 * b, o);
-        }
-        tmem_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->g_full[wg]);
-
-        const long long t0 = sg.begin + static_cast<long long>(c) * kQ;
-        // z's own row, on its way while the products run
-        uint4 zv[8];
-        if (gated) {
-          const uint4* zr = reinterpret_cast<const uint4*>(gz + (t0 + t) * p.ldz);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) zv[i] = t0 + t < sg.end && 8 * i < pdims ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
-        }
-        // y takes x's place in shared memory, row by row, and leaves as one tile (or by
-        // rows where the chunk ends before the tile)
-        if (!wait_bar(&bars->full_x[wg], par, flag)) break;
-        if (!wait_bar(&bars->done[wg], par, flag)) break;
-        tc_fence_after_sync();
-        const float e = sc.e[t];
-        uint8_t* xt = smem + wg * L::kStage + stage_x;
+          } else if (t0 + t < sg.end) {
+            // a partial chunk is the last: nothing waits for its x tile
+            __nv_bfloat16* yr = static_cast<__nv_bfloat16*>(p.y) + (t0 + t) * p.ldy + col;
 #pragma unroll 1
-        for (int k = 0; k < 4; ++k) {
-          uint32_t ry[16], ro[16], xw[8], zw[8], out[8];
-          tmem_ld_32x32b_x16(sY + 16 * k, ry);
-          tmem_ld_32x32b_x16(sYo + 16 * k, ro);
-          const uint32_t o0 = swz_offset(t, 2 * k, 128), o1 = swz_offset(t, 2 * k + 1, 128);
-          *reinterpret_cast<uint4*>(xw) = *reinterpret_cast<const uint4*>(xt + o0);
-          *reinterpret_cast<uint4*>(xw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
-          if (gated) {
-            *reinterpret_cast<uint4*>(zw) = zv[0];
-            *reinterpret_cast<uint4*>(zw + 4) = zv[1];
-#pragma unroll
-            for (int i = 0; i < 6; ++i) zv[i] = zv[i + 2];
+            for (int i = 0; i < 4 && 8 * i < wdims; ++i)
+              *reinterpret_cast<uint4*>(yr + 8 * i) =
+                  *reinterpret_cast<const uint4*>(xt + swz_offset(t, 4 * half + i, 128));
           }
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float a = fmaf(Dh, bf_lo(xw[i]), fmaf(e, __uint_as_float(ro[2 * i]), __uint_as_float(ry[2 * i])));
-            float b = fmaf(Dh, bf_hi(xw[i]), fmaf(e, __uint_as_float(ro[2 * i + 1]), __uint_as_float(ry[2 * i + 1])));
-            if (gated) {
-              a *= gate(bf_lo(zw[i]));
-              b *= gate(bf_hi(zw[i]));
-            }
-            out[i] = bf16_pair(a, b);
-          }
-          *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
-          *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
-        }
-        tc_fence_before_sync();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->yo_free[wg]);
-          mbar_arrive(&bars->sc_free[b3]);
-        }
-        if (t0 + kQ <= sg.end) {
-          asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");  // the four warps' rows are written
-          if (q == 0 && lane == 0) {
-            tma_store_3d(&maps.y, sbase + wg * L::kStage + stage_x, p0, h, static_cast<int>(t0));
-            mbar_arrive(&bars->xfree[wg]);
-          }
-        } else {
-          if (t0 + t < sg.end) {
-            __nv_bfloat16* yr = gy + (t0 + t) * p.ldy;
-#pragma unroll 1
-            for (int i = 0; 8 * i < pdims; ++i)
-              *reinterpret_cast<uint4*>(yr + 8 * i) = *reinterpret_cast<const uint4*>(xt + swz_offset(t, i, 128));
-          }
-          // a partial chunk is the last: nothing waits for its x tile
         }
       }
     }
@@ -767,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b3 = c % 3;
       if (!STATES) {
         // the product that reads the old H is done
-        ok = c == 0 || wait_bar(&bars->cfree[(c - 1) & 1], ((c - 1) >> 1) & 1, flag);
+        ok = c == 0 || wait_bar(&bars->done[(c - 1) & 1], ((c - 1) >> 1) & 1, flag);
         if (!ok) break;
         put_h();
       }
