@@ -366,75 +366,88 @@ _ACTS = {None: 0, "silu": 1}
 
 
 def _check_seq(name: str, t: torch.Tensor, like: torch.Tensor, dtype, shape) -> torch.Tensor:
-    """A tensor of this type and shape on like's device; None in shape: any size."""
+    """A tensor of this type and shape on like's device."""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.device == like.device:
+            return t
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != len(shape) or any(e is not None and n != e for n, e in zip(t.shape, shape)):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
-                         f"({', '.join('*' if e is None else str(e) for e in shape)})")
-    return t
+    raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
-def _check_x(x: torch.Tensor, dims: int) -> int:
-    if not isinstance(x, torch.Tensor):
-        raise TypeError("x must be a torch.Tensor")
-    if x.dim() != dims:
-        raise ValueError(f"x has shape {tuple(x.shape)}, expected {dims} dimensions")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"x must be float32 or bfloat16, got {x.dtype}")
-    return _DTYPES[x.dtype]
+def _dims(name: str, t: torch.Tensor, dims: int):
+    """The shape of a tensor of so many dimensions."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    shape = t.shape
+    if len(shape) != dims:
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected {dims} dimensions")
+    return shape
 
 
-def _is_rows(t: torch.Tensor) -> bool:
-    """Whether the elements of one row (all dimensions but the first) are
-    contiguous and rows do not overlap; dimensions of size one may have any stride."""
-    shape, stride, width = t.shape, t.stride(), 1
+def _x_dtype(x: torch.Tensor) -> int:
+    try:
+        return _DTYPES[x.dtype]
+    except KeyError:
+        raise TypeError(f"x must be float32 or bfloat16, got {x.dtype}") from None
+
+
+def _row_stride(t: torch.Tensor, width: int) -> Optional[int]:
+    """The distance of t's rows (its first dimension), or None where the elements of
+    a row are not contiguous or rows overlap.  Dimensions of size one may have any stride."""
+    if t.is_contiguous():
+        return width
+    shape, stride, w = t.shape, t.stride(), 1
     for i in range(len(shape) - 1, 0, -1):
-        if shape[i] != 1 and stride[i] != width:
-            return False
-        width *= shape[i]
-    return shape[0] <= 1 or stride[0] >= width
+        if shape[i] != 1 and stride[i] != w:
+            return None
+        w *= shape[i]
+    if shape[0] <= 1:
+        return width
+    return stride[0] if stride[0] >= width else None
 
 
-def _rows(t: torch.Tensor):
+def _rows(t: torch.Tensor, width: int):
     """t with contiguous rows (copied if it is laid out otherwise), and the row stride."""
-    if not _is_rows(t):
-        t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else math.prod(t.shape[1:])
+    ld = _row_stride(t, width)
+    return (t, ld) if ld is not None else (t.contiguous(), width)
 
 
-def _seq_out(out: Optional[torch.Tensor], x: torch.Tensor, shape) -> torch.Tensor:
+def _seq_out(out: Optional[torch.Tensor], x: torch.Tensor, shape, width: int):
     if out is None:
-        return torch.empty(shape, dtype=x.dtype, device=x.device)
+        return x.new_empty(shape), width
     _check_seq("out", out, x, x.dtype, shape)
-    if not _is_rows(out):
+    ld = _row_stride(out, width)
+    if ld is None:
         raise ValueError("out must have contiguous rows that do not overlap")
-    return out
+    return out, ld
 
 
-def _states(x, dtype, entry, state, state_out, in_place: bool):
-    """The checked pair of state tensors and their number of entries."""
+def _states(x, dtype, entry, state, state_out):
+    """The checked pair of state tensors (in place without state_out) and their number of entries."""
+    n = None
     for name, t in (("state", state), ("state_out", state_out)):
         if t is not None:
-            _check_seq(name, t, x, dtype, (None, *entry))
+            m = _dims(name, t, 1 + len(entry))[0]
+            _check_seq(name, t, x, dtype, (m, *entry))
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
-    if state is not None and state_out is not None and state.shape[0] != state_out.shape[0]:
-        raise ValueError(f"state has {state.shape[0]} entries, state_out {state_out.shape[0]}")
-    if state_out is None and in_place:
-        state_out = state
-    n = state.shape[0] if state is not None else state_out.shape[0] if state_out is not None else 0
-    return state, state_out, n
+            if n is not None and n != m:
+                raise ValueError(f"state has {n} entries, state_out {m}")
+            n = m
+    return state, state if state_out is None else state_out, n or 0
 
 
 def _index(name: str, t: Optional[torch.Tensor], like: torch.Tensor, n: Optional[int]) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    _check_seq(name, t, like, torch.int32, (n,))
+    _check_seq(name, t, like, torch.int32, _dims(name, t, 1) if n is None else (n,))
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -442,34 +455,53 @@ def _opt(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _vec(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+# A small call's time is the host's: the stream's handle without a Stream object.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _on(x: torch.Tensor, stream: Optional[torch.cuda.Stream], call):
     """call(stream pointer) with x's device current.  Whatever call allocates belongs
     to the stream that its kernels run on."""
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
+    index = x.device.index
     if stream is not None:
         if stream.device != x.device:
             raise ValueError(f"stream is on {stream.device}, x on {x.device}")
         with torch.cuda.stream(stream):
             return call(stream.cuda_stream or None)
-    if x.device.index == torch.cuda.current_device():
-        return call(torch.cuda.current_stream().cuda_stream or None)
-    with torch.cuda.device(x.device):
-        return call(torch.cuda.current_stream().cuda_stream or None)
+    if index == torch.cuda.current_device():
+        return call(_raw_stream(index) or None)
+    with torch.cuda.device(index):
+        return call(_raw_stream(index) or None)
 
 
 def _sequences(offsets, x):
-    offsets = _index("offsets", offsets, x, None)
     if offsets is None:
         return None, 1
+    offsets = _index("offsets", offsets, x, None)
     if offsets.shape[0] < 1:
         raise ValueError("offsets must have at least one element")
     return offsets, offsets.shape[0] - 1
 
 
-def _act(activation) -> int:
+def _conv_args(x, weight, bias, activation):
+    """Checks shared by the convolution and its step; returns (rows, channels, width, dtype, act)."""
+    rows, channels = _dims("x", x, 2)
+    ty = _x_dtype(x)
+    width = _dims("weight", weight, 2)[1]
+    _check_seq("weight", weight, x, x.dtype, (channels, width))
+    if not 2 <= width <= 8:
+        raise ValueError(f"weight has {width} taps, expected 2 to 8")
+    if bias is not None:
+        _check_seq("bias", bias, x, x.dtype, (channels,))
     try:
-        return _ACTS[activation]
+        return rows, channels, width, ty, _ACTS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"unknown activation {activation!r}; expected None or 'silu'") from None
 
@@ -489,27 +521,18 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     state is updated in place).  Sequence s uses entry slots[s] (int32; None: s;
     negative: no state); no two may share one.  Rows outside every sequence are
     left as they are in `out`, and have no defined values without it."""
-    dt = _check_x(x, 2)
-    tokens, channels = x.shape
-    _check_seq("weight", weight, x, x.dtype, (channels, None))
-    width = weight.shape[1]
-    if not 2 <= width <= 8:
-        raise ValueError(f"weight has {width} taps, expected 2 to 8")
-    if bias is not None:
-        _check_seq("bias", bias, x, x.dtype, (channels,))
-    act = _act(activation)
-    state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out, True)
+    tokens, channels, width, ty, act = _conv_args(x, weight, bias, activation)
+    state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out)
     offsets, nseq = _sequences(offsets, x)
     slots = _index("slots", slots, x, nseq)
 
     def call(st):
-        xr, ldx = _rows(x)
-        w = weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        y = _seq_out(out, x, (tokens, channels))
+        xr, ldx = _rows(x, channels)
+        w, b = _vec(weight), _vec(bias)
+        y, ldy = _seq_out(out, x, (tokens, channels), channels)
         _lib.check(_lib.load().smm_causal_conv(
-            _ptr(xr), _ptr(w), _opt(b), _opt(offsets), _opt(state), _opt(state_out), _opt(slots), _ptr(y), tokens,
-            channels, width, nseq, entries, ldx, _rows(y)[1], dt, act, st), "smm_causal_conv")
+            xr.data_ptr(), w.data_ptr(), _opt(b), _opt(offsets), _opt(state), _opt(state_out), _opt(slots),
+            y.data_ptr(), tokens, channels, width, nseq, entries, ldx, ldy, ty, act, st), "smm_causal_conv")
         return y
     return _on(x, stream, call)
 
@@ -521,59 +544,47 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     """causal_conv for one new token of each sequence: row b of x (batch,
     channels) continues the state at entry slots[b] (None: b), which is updated in
     place unless state_out is given.  A row with a negative slot starts from zero and leaves no state."""
-    dt = _check_x(x, 2)
-    batch, channels = x.shape
-    _check_seq("weight", weight, x, x.dtype, (channels, None))
-    width = weight.shape[1]
-    if not 2 <= width <= 8:
-        raise ValueError(f"weight has {width} taps, expected 2 to 8")
-    if bias is not None:
-        _check_seq("bias", bias, x, x.dtype, (channels,))
-    act = _act(activation)
+    batch, channels, width, ty, act = _conv_args(x, weight, bias, activation)
     if state is None:
         raise TypeError("state must be a torch.Tensor")
-    state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out, True)
+    state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out)
     slots = _index("slots", slots, x, batch)
 
     def call(st):
-        xr, ldx = _rows(x)
-        w = weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        y = _seq_out(out, x, (batch, channels))
+        xr, ldx = _rows(x, channels)
+        w, b = _vec(weight), _vec(bias)
+        y, ldy = _seq_out(out, x, (batch, channels), channels)
         _lib.check(_lib.load().smm_causal_conv_step(
-            _ptr(xr), _ptr(w), _opt(b), _opt(state), _opt(state_out), _opt(slots), _ptr(y), batch, channels, width,
-            entries, ldx, _rows(y)[1], dt, act, st), "smm_causal_conv_step")
+            xr.data_ptr(), w.data_ptr(), _opt(b), state.data_ptr(), state_out.data_ptr(), _opt(slots), y.data_ptr(),
+            batch, channels, width, entries, ldx, ldy, ty, act, st), "smm_causal_conv_step")
         return y
     return _on(x, stream, call)
 
 
 def _scan_args(x, dt, A, B, C, D, z, dt_bias):
-    """Checks shared by the scan and the step; returns (dtype, dt's dtype, groups, state_dim)."""
-    ty = _check_x(x, 3)
-    t, heads, dim = x.shape
+    """Checks shared by the scan and the step; returns (rows, heads, dim, groups, state_dim, dtype, dt's dtype)."""
+    t, heads, dim = _dims("x", x, 3)
+    ty = _x_dtype(x)
     if not isinstance(dt, torch.Tensor):
         raise TypeError("dt must be a torch.Tensor")
-    if dt.dtype not in (x.dtype, torch.float32):
+    if dt.dtype is not x.dtype and dt.dtype is not torch.float32:
         raise TypeError(f"dt must be {x.dtype} or float32, got {dt.dtype}")
     _check_seq("dt", dt, x, dt.dtype, (t, heads))
     _check_seq("A", A, x, torch.float32, (heads,))
-    _check_seq("B", B, x, x.dtype, (t, None, None))
-    groups, n = B.shape[1], B.shape[2]
-    _check_seq("C", C, x, x.dtype, (t, groups, n))
+    _, groups, n = shape = _dims("B", B, 3)
+    _check_seq("B", B, x, x.dtype, (t, groups, n))
+    _check_seq("C", C, x, x.dtype, shape)
     if not (1 <= dim <= 256 and 1 <= n <= 256):
         raise ValueError(f"head dim {dim} and state dim {n} must be 1 to 256")
     if groups < 1 or heads % groups:
         raise ValueError(f"{heads} heads do not divide into {groups} groups")
-    for name, v in (("D", D), ("dt_bias", dt_bias)):
-        if v is not None:
-            _check_seq(name, v, x, torch.float32, (heads,))
+    if D is not None:
+        _check_seq("D", D, x, torch.float32, (heads,))
+    if dt_bias is not None:
+        _check_seq("dt_bias", dt_bias, x, torch.float32, (heads,))
     if z is not None:
         _check_seq("z", z, x, x.dtype, (t, heads, dim))
-    return ty, _DTYPES[dt.dtype], groups, n
-
-
-def _vec(v: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return v if v is None or v.is_contiguous() else v.contiguous()
+    return t, heads, dim, groups, n, ty, _DTYPES[dt.dtype]
 
 
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
@@ -597,25 +608,26 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     offsets, slots, out, state (entries, heads, dim, state_dim; float32) and state_out are as in causal_conv.
     A non-finite input makes the rest of its sequence non-finite, and may
     do so for up to 127 tokens before it."""
-    ty, dty, groups, n = _scan_args(x, dt, A, B, C, D, z, dt_bias)
-    tokens, heads, dim = x.shape
-    state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out, True)
+    tokens, heads, dim, groups, n, ty, dty = _scan_args(x, dt, A, B, C, D, z, dt_bias)
+    state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out)
     offsets, nseq = _sequences(offsets, x)
     slots = _index("slots", slots, x, nseq)
 
     def call(st):
         L = _lib.load()
-        (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x), _rows(dt), _rows(B), _rows(C)
-        zr, ldz = (None, 0) if z is None else _rows(z)
+        wx, wb = heads * dim, groups * n
+        (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x, wx), _rows(dt, heads), _rows(B, wb), _rows(C, wb)
+        zr, ldz = (None, 0) if z is None else _rows(z, wx)
         a, dd, db = _vec(A), _vec(D), _vec(dt_bias)
-        y = _seq_out(out, x, (tokens, heads, dim))
+        y, ldy = _seq_out(out, x, (tokens, heads, dim), wx)
         nws = L.smm_selective_scan_workspace_size(tokens, nseq, heads, dim, groups, n, ty)
         # of this call alone: streams and captured graphs share nothing
         ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
         _lib.check(L.smm_selective_scan(
-            _ptr(xr), _ptr(dr), _ptr(a), _ptr(br), _ptr(cr), _opt(dd), _opt(zr), _opt(db), _opt(offsets), _opt(state),
-            _opt(state_out), _opt(slots), _ptr(y), tokens, nseq, entries, heads, dim, groups, n, ldx, ldd, ldb, ldc,
-            ldz, _rows(y)[1], ty, dty, int(dt_softplus), _opt(ws), nws, st), "smm_selective_scan")
+            xr.data_ptr(), dr.data_ptr(), a.data_ptr(), br.data_ptr(), cr.data_ptr(), _opt(dd), _opt(zr), _opt(db),
+            _opt(offsets), _opt(state), _opt(state_out), _opt(slots), y.data_ptr(), tokens, nseq, entries, heads, dim,
+            groups, n, ldx, ldd, ldb, ldc, ldz, ldy, ty, dty, 1 if dt_softplus else 0, _opt(ws), nws, st),
+            "smm_selective_scan")
         return y
     return _on(x, stream, call)
 
@@ -629,22 +641,22 @@ def selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     heads, dim) continues the state at entry slots[b] (None: b), which is updated
     in place unless state_out is given.  A row with a negative slot starts from
     zero and leaves no state."""
-    ty, dty, groups, n = _scan_args(x, dt, A, B, C, D, z, dt_bias)
-    batch, heads, dim = x.shape
+    batch, heads, dim, groups, n, ty, dty = _scan_args(x, dt, A, B, C, D, z, dt_bias)
     if state is None:
         raise TypeError("state must be a torch.Tensor")
-    state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out, True)
+    state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out)
     slots = _index("slots", slots, x, batch)
 
     def call(st):
-        (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x), _rows(dt), _rows(B), _rows(C)
-        zr, ldz = (None, 0) if z is None else _rows(z)
+        wx, wb = heads * dim, groups * n
+        (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x, wx), _rows(dt, heads), _rows(B, wb), _rows(C, wb)
+        zr, ldz = (None, 0) if z is None else _rows(z, wx)
         a, dd, db = _vec(A), _vec(D), _vec(dt_bias)
-        y = _seq_out(out, x, (batch, heads, dim))
+        y, ldy = _seq_out(out, x, (batch, heads, dim), wx)
         _lib.check(_lib.load().smm_selective_step(
-            _ptr(xr), _ptr(dr), _ptr(a), _ptr(br), _ptr(cr), _opt(dd), _opt(zr), _opt(db), _opt(state),
-            _opt(state_out), _opt(slots), _ptr(y), batch, entries, heads, dim, groups, n, ldx, ldd, ldb, ldc, ldz,
-            _rows(y)[1], ty, dty, int(dt_softplus), st), "smm_selective_step")
+            xr.data_ptr(), dr.data_ptr(), a.data_ptr(), br.data_ptr(), cr.data_ptr(), _opt(dd), _opt(zr), _opt(db),
+            state.data_ptr(), state_out.data_ptr(), _opt(slots), y.data_ptr(), batch, entries, heads, dim, groups, n,
+            ldx, ldd, ldb, ldc, ldz, ldy, ty, dty, 1 if dt_softplus else 0, st), "smm_selective_step")
         return y
     return _on(x, stream, call)
 
@@ -658,35 +670,32 @@ def q4_matvec(q: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, zeros: Opt
     (rows, cols/group), of x's type or float32, and zeros (same shape, uint8, 0..15; None:
     8 everywhere) give the group, a multiple of 32.  x float32 or bfloat16; products are
     exact and sums float32 in both.  Returns (batch, rows)."""
-    ty = _check_x(x, 2)
-    batch, cols = x.shape
-    if not isinstance(q, torch.Tensor) or not isinstance(scales, torch.Tensor):
-        raise TypeError("q and scales must be torch.Tensors")
+    batch, cols = _dims("x", x, 2)
+    ty = _x_dtype(x)
     if cols % 2:
         raise ValueError(f"x has an odd number of columns, {cols}")
-    _check_seq("q", q, x, torch.uint8, (None, cols // 2))
-    rows = q.shape[0]
-    if scales.dtype not in (x.dtype, torch.float32):
+    rows = _dims("q", q, 2)[0]
+    _check_seq("q", q, x, torch.uint8, (rows, cols // 2))
+    _, groups = shape = _dims("scales", scales, 2)
+    if scales.dtype is not x.dtype and scales.dtype is not torch.float32:
         raise TypeError(f"scales must be {x.dtype} or float32, got {scales.dtype}")
-    _check_seq("scales", scales, x, scales.dtype, (rows, None))
-    groups = scales.shape[1]
+    _check_seq("scales", scales, x, scales.dtype, (rows, groups))
     if groups < 1 or cols % groups or (cols // groups) % 32 or cols == 0:
         raise ValueError(f"{cols} columns do not divide into {groups} groups of a multiple of 32")
     if zeros is not None:
-        _check_seq("zeros", zeros, x, torch.uint8, (rows, groups))
+        _check_seq("zeros", zeros, x, torch.uint8, shape)
 
     def call(st):
-        xr, ldx = _rows(x)
+        xr, ldx = _rows(x, cols)
         if xr.data_ptr() % 16 or (batch > 1 and ldx * xr.element_size() % 16):
-            xr = xr.contiguous().clone() if xr.data_ptr() % 16 else xr.contiguous()
-            ldx = cols
-        qc, sc, zc = q.contiguous(), scales.contiguous(), _vec(zeros)
+            xr, ldx = xr.clone(memory_format=torch.contiguous_format), cols
+        qc, sc, zc = _vec(q), _vec(scales), _vec(zeros)
         if qc.data_ptr() % 16:
             qc = qc.clone()
-        y = _seq_out(out, x, (batch, rows))
+        y, ldy = _seq_out(out, x, (batch, rows), rows)
         _lib.check(_lib.load().smm_q4_matvec(
-            _ptr(qc), _ptr(sc), _opt(zc), _ptr(xr), _ptr(y), batch, rows, cols, cols // groups, ldx, _rows(y)[1], ty,
-            _DTYPES[scales.dtype], st), "smm_q4_matvec")
+            qc.data_ptr(), sc.data_ptr(), _opt(zc), xr.data_ptr(), y.data_ptr(), batch, rows, cols, cols // groups, ldx,
+            ldy, ty, _DTYPES[scales.dtype], st), "smm_q4_matvec")
         return y
     return _on(x, stream, call)
 
