@@ -3,7 +3,7 @@
 // packed prompts, and for one new token of each sequence.
 //
 // Bound by memory: each element is read once and written once (W multiplies
-// per element).  A thread owns 16 bytes of channels and walks down a run of
+// per element).  A thread owns four channels and walks down a run of
 // consecutive tokens with the last W-1 rows in registers, so a row is read
 // from memory once and W-1 rows per run again from L2.
 //
@@ -14,6 +14,8 @@
 // needs no second launch.  An empty sequence belongs to the run that holds
 // its position (the last run, behind the last row).
 #include "smm_seq.cuh"
+
+#include <type_traits>
 
 namespace smm {
 namespace {
@@ -34,38 +36,114 @@ struct ConvParams {
 
 constexpr int kConvThreads = 128;
 
+// VEC channels of a thread, in pairs where there are pairs.  Four: with the eight of a
+// 16-byte bf16 vector, registers left nine warps on an SM and the loads' latency showed.
 template <typename T, int VEC, int W>
 struct ConvLane {
   static constexpr bool kVec = VEC > 1;
-  float w[W][VEC];  // tap j of each channel
-  float bias[VEC];
+  static constexpr int kPiece = VEC * sizeof(T) % 16 == 0 ? 16 : 8;  // bytes of one access
+  static constexpr int NP = kVec ? VEC / 2 : 1;
+  using E = typename std::conditional<kVec, unsigned long long, float>::type;
+  E w[W][NP];  // tap j of each channel
+  E bias[NP];
 
-  __device__ void load(const ConvParams& p, int c) {
-    float wt[VEC * W];  // [channel][tap]
-    load_f32<T, VEC * W, kVec>(static_cast<const T*>(p.w) + static_cast<long long>(c) * W, wt);
+  static __device__ __forceinline__ void put(E (&d)[NP], const float (&v)[VEC]) {
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) w[j][i] = wt[i * W + j];
-    if (p.bias) {
-      load_f32<T, VEC, kVec>(static_cast<const T*>(p.bias) + c, bias);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) bias[i] = 0.0f;
+    for (int i = 0; i < NP; ++i) {
+      if constexpr (kVec)
+        d[i] = pack2(v[2 * i], v[2 * i + 1]);
+      else
+        d[i] = v[i];
     }
   }
+  static __device__ __forceinline__ void get(const E (&d)[NP], float (&v)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      if constexpr (kVec)
+        unpack2(d[i], v[2 * i], v[2 * i + 1]);
+      else
+        v[i] = d[i];
+    }
+  }
+  __device__ void load(const ConvParams& p, int c) {
+    float wt[VEC * W], one[VEC];  // [channel][tap]
+    load_f32<T, VEC * W, kVec, kPiece>(static_cast<const T*>(p.w) + static_cast<long long>(c) * W, wt);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) one[i] = wt[i * W + j];
+      put(w[j], one);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) one[i] = 0.0f;
+    if (p.bias) load_f32<T, VEC, kVec>(static_cast<const T*>(p.bias) + c, one);
+    put(bias, one);
+  }
+  // a row's channels as they lie (narrower than fp32 pairs while on their way)
+  using Raw = typename std::conditional<kVec, RawVec<T, kVec ? VEC : 16 / sizeof(T), kPiece>, T>::type;
+  static __device__ __forceinline__ void load_raw(const T* x, Raw& r) {
+    if constexpr (kVec)
+      r.load(x);
+    else
+      r = *x;
+  }
+  static __device__ __forceinline__ void from_raw(const Raw& r, E (&d)[NP]) {
+    if constexpr (kVec) {
+      float v[VEC];
+      r.get(v);
+      put(d, v);
+    } else {
+      d[0] = to_f32(r);
+    }
+  }
+  static __device__ __forceinline__ void load_row(const T* x, E (&d)[NP]) {
+    Raw r;
+    load_raw(x, r);
+    from_raw(r, d);
+  }
   // One output row from the W-1 rows before it and its own; the window moves on.
-  __device__ void row(float (&win)[W - 1][VEC], const float (&cur)[VEC], float (&out)[VEC], bool act) const {
+  __device__ __forceinline__ void row(E (&win)[W - 1][NP], const E (&cur)[NP], T* y, bool act) const {
+    E a[NP];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float a = bias[i];
+    for (int i = 0; i < NP; ++i) {
+      a[i] = bias[i];
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) a = fmaf(w[j][i], win[j][i], a);
-      a = fmaf(w[W - 1][i], cur[i], a);
-      out[i] = act ? silu(a) : a;
+      for (int j = 0; j < W; ++j) {
+        const E in = j < W - 1 ? win[j < W - 1 ? j : 0][i] : cur[i];
+        if constexpr (kVec)
+          a[i] = fma2(w[j][i], in, a[i]);
+        else
+          a[i] = fmaf(w[j][i], in, a[i]);
+      }
 #pragma unroll
       for (int j = 0; j < W - 2; ++j) win[j][i] = win[j + 1][i];
       win[W - 2][i] = cur[i];
+    }
+    float out[VEC];
+    get(a, out);
+    if (act) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) out[i] = silu(out[i]);
+    }
+    store_f32<T, VEC, kVec>(y, out);
+  }
+  // The window to and from a state's [channel][W-1] elements.
+  static __device__ __forceinline__ void from_state(const float (&old)[VEC * (W - 1)], E (&win)[W - 1][NP]) {
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = old[i * (W - 1) + j];
+      put(win[j], v);
+    }
+  }
+  static __device__ __forceinline__ void to_state(const E (&win)[W - 1][NP], float (&old)[VEC * (W - 1)]) {
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+      get(win[j], v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) old[i * (W - 1) + j] = v[i];
     }
   }
 };
@@ -83,7 +161,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
   const T* x = static_cast<const T*>(p.x) + c;
   T* y = static_cast<T*>(p.y) + c;
   const bool act = p.silu != 0;
-  ConvLane<T, VEC, W> lane;
+  using Lane = ConvLane<T, VEC, W>;
+  Lane lane;
   lane.load(p, c);
 
   // first sequence that reaches into this run or is empty at its start
@@ -103,29 +182,29 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
     long long b, e;
     seq_range(p.offsets, s, p.tokens, &b, &e);
     if (b > t1 || (b == t1 && !last_run)) break;
-    float win[W - 1][VEC];
+    typename Lane::E win[W - 1][Lane::NP];
     const long long lo = b + W - 1 > t0 ? b + W - 1 : t0;
     const long long hi = e < t1 ? e : t1;
     if (lo < hi) {
 #pragma unroll
-      for (int j = 0; j < W - 1; ++j) load_f32<T, VEC, kVec>(x + (lo - (W - 1) + j) * p.ldx, win[j]);
+      for (int j = 0; j < W - 1; ++j) Lane::load_row(x + (lo - (W - 1) + j) * p.ldx, win[j]);
       long long t = lo;
-      constexpr int U = 4;  // rows in flight
+      constexpr int U = kVec ? 8 : 4;  // rows in flight
       for (; t + U <= hi; t += U) {
-        float cur[U][VEC], out[VEC];
+        typename Lane::Raw raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) load_f32<T, VEC, kVec>(x + (t + u) * p.ldx, cur[u]);
+        for (int u = 0; u < U; ++u) Lane::load_raw(x + (t + u) * p.ldx, raw[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          lane.row(win, cur[u], out, act);
-          store_f32<T, VEC, kVec>(y + (t + u) * p.ldy, out);
+          typename Lane::E cur[Lane::NP];
+          Lane::from_raw(raw[u], cur);
+          lane.row(win, cur, y + (t + u) * p.ldy, act);
         }
       }
       for (; t < hi; ++t) {
-        float cur[VEC], out[VEC];
-        load_f32<T, VEC, kVec>(x + t * p.ldx, cur);
-        lane.row(win, cur, out, act);
-        store_f32<T, VEC, kVec>(y + t * p.ldy, out);
+        typename Lane::E cur[Lane::NP];
+        Lane::load_row(x + t * p.ldx, cur);
+        lane.row(win, cur, y + t * p.ldy, act);
       }
     }
     const bool owner = e > b ? (e > t0 && e <= t1) : (b >= t0 && (b < t1 || last_run));
@@ -134,41 +213,34 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
     const long long at = (static_cast<long long>(slot) * p.channels + c) * (W - 1);
     float old[VEC * (W - 1)];
     if (p.state_in && slot >= 0) {
-      load_f32<T, VEC*(W - 1), kVec>(static_cast<const T*>(p.state_in) + at, old);
+      load_f32<T, VEC*(W - 1), kVec, Lane::kPiece>(static_cast<const T*>(p.state_in) + at, old);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC * (W - 1); ++i) old[i] = 0.0f;
     }
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) win[j][i] = old[i * (W - 1) + j];
+    Lane::from_state(old, win);
     const long long len = e - b;
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) {
       if (j < len) {
-        float cur[VEC], out[VEC];
-        load_f32<T, VEC, kVec>(x + (b + j) * p.ldx, cur);
-        lane.row(win, cur, out, act);
-        store_f32<T, VEC, kVec>(y + (b + j) * p.ldy, out);
+        typename Lane::E cur[Lane::NP];
+        Lane::load_row(x + (b + j) * p.ldx, cur);
+        lane.row(win, cur, y + (b + j) * p.ldy, act);
       }
     }
     if (p.state_out && slot >= 0) {
       // the window now ends at row b + min(len, W-1); a longer sequence ends later
       if (len > W - 1) {
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) load_f32<T, VEC, kVec>(x + (e - (W - 1) + j) * p.ldx, win[j]);
+        for (int j = 0; j < W - 1; ++j) Lane::load_row(x + (e - (W - 1) + j) * p.ldx, win[j]);
       }
-#pragma unroll
-      for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) old[i * (W - 1) + j] = win[j][i];
-      store_f32<T, VEC*(W - 1), kVec>(static_cast<T*>(p.state_out) + at, old);
+      Lane::to_state(win, old);
+      store_f32<T, VEC*(W - 1), kVec, Lane::kPiece>(static_cast<T*>(p.state_out) + at, old);
     }
   }
 }
 
-// One token of each sequence: a thread per 16 bytes of channels of one row.
+// One token of each sequence: a thread per four channels of one row.
 template <typename T, int VEC, int W>
 __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvParams p) {
   constexpr bool kVec = VEC > 1;
@@ -177,28 +249,23 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvParam
   if (c >= p.channels) return;
   const int slot = seq_slot(p.slots, b, p.nslots, p.status);
   const long long at = (static_cast<long long>(slot) * p.channels + c) * (W - 1);
-  float old[VEC * (W - 1)], win[W - 1][VEC], cur[VEC], out[VEC];
+  using Lane = ConvLane<T, VEC, W>;
+  float old[VEC * (W - 1)];
+  typename Lane::E win[W - 1][Lane::NP], cur[Lane::NP];
   if (p.state_in && slot >= 0) {
-    load_f32<T, VEC*(W - 1), kVec>(static_cast<const T*>(p.state_in) + at, old);
+    load_f32<T, VEC*(W - 1), kVec, Lane::kPiece>(static_cast<const T*>(p.state_in) + at, old);
   } else {
 #pragma unroll
     for (int i = 0; i < VEC * (W - 1); ++i) old[i] = 0.0f;
   }
-  load_f32<T, VEC, kVec>(static_cast<const T*>(p.x) + b * p.ldx + c, cur);
-  ConvLane<T, VEC, W> lane;
+  Lane::load_row(static_cast<const T*>(p.x) + b * p.ldx + c, cur);
+  Lane lane;
   lane.load(p, c);
-#pragma unroll
-  for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) win[j][i] = old[i * (W - 1) + j];
-  lane.row(win, cur, out, p.silu != 0);
-  store_f32<T, VEC, kVec>(static_cast<T*>(p.y) + b * p.ldy + c, out);
+  Lane::from_state(old, win);
+  lane.row(win, cur, static_cast<T*>(p.y) + b * p.ldy + c, p.silu != 0);
   if (p.state_out && slot >= 0) {
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) old[i * (W - 1) + j] = win[j][i];
-    store_f32<T, VEC*(W - 1), kVec>(static_cast<T*>(p.state_out) + at, old);
+    Lane::to_state(win, old);
+    store_f32<T, VEC*(W - 1), kVec, Lane::kPiece>(static_cast<T*>(p.state_out) + at, old);
   }
 }
 
@@ -256,12 +323,12 @@ int run_conv(ConvParams& p, int width, int dtype, cudaStream_t st) {
   if (p.channels == 0 || p.nseq == 0) return SMM_OK;
   p.status = device_status_word();
   if (!p.status) return set_error(SMM_ERR_CUDA, "device status word unavailable");
-  const int per16 = static_cast<int>(16 / dtype_size(dtype));
-  // 16-byte accesses where every row, the weights and the states keep to them
-  const bool vec = p.channels % per16 == 0 && p.ldx % per16 == 0 && p.ldy % per16 == 0 && aligned_to(p.x, 16) &&
-                   aligned_to(p.y, 16) && aligned_to(p.w, 16) && aligned_to(p.bias, 16) &&
-                   aligned_to(p.state_in, 16) && aligned_to(p.state_out, 16);
-  const int cv = vec ? p.channels / per16 : p.channels;
+  // accesses of four channels where every row, the weights and the states keep to them
+  const size_t al = 4 * dtype_size(dtype);
+  const bool vec = p.channels % 4 == 0 && p.ldx % 4 == 0 && p.ldy % 4 == 0 && aligned_to(p.x, al) &&
+                   aligned_to(p.y, al) && aligned_to(p.w, al) && aligned_to(p.bias, al) && aligned_to(p.state_in, al) &&
+                   aligned_to(p.state_out, al);
+  const int cv = vec ? p.channels / 4 : p.channels;
   int bx = 32;
   while (bx < kConvThreads && bx < cv) bx *= 2;
   const int by = STEP ? 1 : kConvThreads / bx;
@@ -286,7 +353,7 @@ int run_conv(ConvParams& p, int width, int dtype, cudaStream_t st) {
       launch_width<float, 1, STEP>(width, grid, block, p, st);
   } else {
     if (vec)
-      launch_width<__nv_bfloat16, 8, STEP>(width, grid, block, p, st);
+      launch_width<__nv_bfloat16, 4, STEP>(width, grid, block, p, st);
     else
       launch_width<__nv_bfloat16, 1, STEP>(width, grid, block, p, st);
   }

@@ -18,8 +18,12 @@
 // done, which also keeps the tensor cores' truncating additions to one group.
 // fp32 x is the exact sum of three bf16 numbers and takes three products.
 //
-// The warps of a CTA share 16 rows and take chunks of 32 V columns in turn; their
-// sums are added through shared memory in a fixed order.
+// A CTA of 1024 threads (512 for more than eight rows of x) is four (two) teams of eight
+// warps.  A team takes a tile of 16 rows of W, its warps the tile's columns in
+// runs of U chunks of 32 V, and adds their sums through shared memory in a fixed
+// order; then it takes its next tile.  x is laid out once per CTA in shared memory in the order
+// that the products take it.  64 registers a thread leave little to prefetch with:
+// the 32 warps' loads cover for one another.
 #include "smm_seq.cuh"
 
 #include <algorithm>
@@ -44,41 +48,43 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The code pair (i, i+4) of a word, as bf16 code - zero (off = 128 + zero twice).
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, __nv_bfloat162 off) {
+__device__ __forceinline__ void mma_16816_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// The code pair (i, i+4) of a word as bf16 code - zero: off is the bf16 pair 128 + zero,
+// whose bits are 0x4300 | zero.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, uint32_t off) {
   const uint32_t u = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), off);
+  const __nv_bfloat162 v =
+      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&off));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Pairs (x[i], x[i+4]), i = 0..3, of eight consecutive elements: PARTS bf16
+// Pairs (x[i], x[i+4]), i = 0..3, of eight consecutive elements: kParts bf16
 // terms whose sum is x exactly.
 template <typename T>
 struct XWord;
 template <>
 struct XWord<__nv_bfloat16> {
   static constexpr int kParts = 1;
-  uint32_t b[1][4];
-  __device__ __forceinline__ void load(const __nv_bfloat16* p, bool ok) {
-    const uint4 v = ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-    b[0][0] = __byte_perm(v.x, v.z, 0x5410);
-    b[0][1] = __byte_perm(v.x, v.z, 0x7632);
-    b[0][2] = __byte_perm(v.y, v.w, 0x5410);
-    b[0][3] = __byte_perm(v.y, v.w, 0x7632);
+  uint4 b[1];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    b[0] = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                      __byte_perm(v.y, v.w, 0x7632));
   }
 };
 template <>
 struct XWord<float> {
   static constexpr int kParts = 3;
-  uint32_t b[3][4];
-  __device__ __forceinline__ void load(const float* p, bool ok) {
+  uint4 b[3];
+  __device__ __forceinline__ void load(const float* p) {
     float v[8];
-    if (ok) {
-      load_f32<float, 8, true>(p, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    }
+    load_f32<float, 8, true>(p, v);
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
       uint32_t hi[8];
@@ -88,143 +94,235 @@ struct XWord<float> {
         // an infinity or NaN is all in its first term
         v[i] = (hi[i] & 0x7F800000u) == 0x7F800000u ? 0.0f : v[i] - __uint_as_float(hi[i]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[part][i] = __byte_perm(hi[i], hi[i + 4], 0x7632);
+      b[part] = make_uint4(__byte_perm(hi[0], hi[4], 0x7632), __byte_perm(hi[1], hi[5], 0x7632),
+                           __byte_perm(hi[2], hi[6], 0x7632), __byte_perm(hi[3], hi[7], 0x7632));
     }
   }
 };
 
+// V words of codes of rows g and g + 8 of four chunks.  Lane (g, t) holds the scales and
+// zero points of chunk t alone, for the four lanes of its rows: a load by each for
+// each chunk had touched three times the lines that the codes lie in.
 template <int V>
-struct Words {
-  uint32_t w[V];
-  __device__ __forceinline__ void load(const uint8_t* p) {
-    if constexpr (V == 4) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (V == 2) {
-      const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
-      w[0] = v.x, w[1] = v.y;
-    } else {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    }
-  }
+struct Codes {
+  uint32_t wa[4][V], wb[4][V];
+  uint32_t sa, sb;  // scales as loaded: an fp32 or, in the low half, a bf16
+  uint32_t za, zb;
 };
-
-template <typename T, int V, int NT>
-__global__ void __launch_bounds__(512) q4_kernel(const Q4Params p) {
-  constexpr int kChunk = 32 * V;
-  constexpr int U = V == 4 ? 2 : 4;  // chunks in flight per warp
-  extern __shared__ float red[];     // [warp][NT][16][8]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int r0 = blockIdx.x * 16;
-  const int ra = r0 + g < p.rows ? r0 + g : p.rows - 1;
-  const int rb = r0 + g + 8 < p.rows ? r0 + g + 8 : p.rows - 1;
-  const int b0 = blockIdx.y * 8 * NT;
-  const int groups = p.cols / p.group;
-  const uint8_t* qa = p.q + static_cast<long long>(ra) * (p.cols / 2) + 4 * V * t;
-  const uint8_t* qb = p.q + static_cast<long long>(rb) * (p.cols / 2) + 4 * V * t;
-  const T* xp[NT];
-  bool xok[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int n = b0 + 8 * j + g;
-    xok[j] = n < p.batch;
-    xp[j] = static_cast<const T*>(p.x) + (xok[j] ? n : 0) * p.ldx + 8 * V * t;
-  }
-  auto scale_at = [&](long long i) {
-    return p.scale_f32 ? __ldg(static_cast<const float*>(p.scales) + i)
-                       : to_f32(static_cast<const __nv_bfloat16*>(p.scales)[i]);
-  };
-  float tot[NT][4] = {};
-  const int chunks = p.cols / kChunk;
-  for (int c0 = warp; c0 < chunks; c0 += U * warps) {
-    Words<V> wa[U], wb[U];
-    float sa[U], sb[U];
-    __nv_bfloat162 oa[U], ob[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * warps;
-      if (c < chunks) {
-        wa[u].load(qa + static_cast<long long>(c) * (kChunk / 2));
-        wb[u].load(qb + static_cast<long long>(c) * (kChunk / 2));
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * warps;
-      if (c < chunks) {
-        const int gr = c * kChunk / p.group;
-        const long long ia = static_cast<long long>(ra) * groups + gr, ib = static_cast<long long>(rb) * groups + gr;
-        sa[u] = scale_at(ia);
-        sb[u] = scale_at(ib);
-        oa[u] = __float2bfloat162_rn(128.0f + (p.zeros ? p.zeros[ia] & 15 : 8));
-        ob[u] = __float2bfloat162_rn(128.0f + (p.zeros ? p.zeros[ib] & 15 : 8));
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * warps;
-      if (c >= chunks) break;
-      float acc[NT][4] = {};
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        uint32_t lo[4], hi[4];
-        lo[0] = code_pair(wa[u].w[v], 0, oa[u]);
-        lo[1] = code_pair(wb[u].w[v], 0, ob[u]);
-        lo[2] = code_pair(wa[u].w[v], 1, oa[u]);
-        lo[3] = code_pair(wb[u].w[v], 1, ob[u]);
-        hi[0] = code_pair(wa[u].w[v], 2, oa[u]);
-        hi[1] = code_pair(wb[u].w[v], 2, ob[u]);
-        hi[2] = code_pair(wa[u].w[v], 3, oa[u]);
-        hi[3] = code_pair(wb[u].w[v], 3, ob[u]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          XWord<T> x;
-          x.load(xp[j] + static_cast<long long>(c) * kChunk + 8 * v, xok[j]);
-#pragma unroll
-          for (int part = XWord<T>::kParts - 1; part >= 0; --part) {
-            mma_16816(acc[j], lo, x.b[part][0], x.b[part][1]);
-            mma_16816(acc[j], hi, x.b[part][2], x.b[part][3]);
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        tot[j][0] = fmaf(sa[u], acc[j][0], tot[j][0]);
-        tot[j][1] = fmaf(sa[u], acc[j][1], tot[j][1]);
-        tot[j][2] = fmaf(sb[u], acc[j][2], tot[j][2]);
-        tot[j][3] = fmaf(sb[u], acc[j][3], tot[j][3]);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    float* o = red + (warp * NT + j) * 128;  // [column][row]
-    o[(2 * t) * 16 + g] = tot[j][0];
-    o[(2 * t + 1) * 16 + g] = tot[j][1];
-    o[(2 * t) * 16 + g + 8] = tot[j][2];
-    o[(2 * t + 1) * 16 + g + 8] = tot[j][3];
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < NT * 128; e += blockDim.x) {
-    float s = 0.0f;
-    for (int w = 0; w < warps; ++w) s += red[w * NT * 128 + e];
-    const int n = b0 + e / 16, r = r0 + e % 16;
-    if (n < p.batch && r < p.rows) static_cast<T*>(p.y)[n * p.ldy + r] = from_f32<T>(s);
+template <int V>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[V]) {
+  if constexpr (V == 4) {
+    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (V == 2) {
+    const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
   }
 }
 
-template <typename T, int V>
-void launch_q4(const Q4Params& p, int warps, cudaStream_t st) {
-  const unsigned gx = (p.rows + 15) / 16;
-  auto go = [&](auto nt) {
-    constexpr int NT = decltype(nt)::value;
-    q4_kernel<T, V, NT><<<dim3(gx, (p.batch + 8 * NT - 1) / (8 * NT)), warps * 32, warps * NT * 512, st>>>(p);
+constexpr int kTeam = 8;                  // warps that share a tile
+constexpr size_t kQ4XBytes = 192 * 1024;  // most of shared memory for x; the sums take up to 16 KB
+
+// XS: x in shared memory (else, for rows of x too long for it, read beside the products)
+template <typename T, int V, int NT, bool XS>
+__global__ void __launch_bounds__(NT == 1 ? 1024 : 512, 1) q4_kernel(const Q4Params p, int nb) {
+  constexpr int kTeams = (NT == 1 ? 1024 : 512) / (32 * kTeam);
+  constexpr int kChunk = 32 * V, U = 4, kParts = XWord<T>::kParts;
+  extern __shared__ uint4 q4_smem[];
+  // x by words of 8 columns, in the order in which lanes (g, t) take them: [chunk][v][part][row of x][t]
+  uint4* sx = q4_smem;
+  const int words = p.cols / 8;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % kTeam, team = threadIdx.x / (32 * kTeam);
+  float* red = reinterpret_cast<float*>(sx + (XS ? static_cast<size_t>(words) * kParts * nb : 0)) +
+               team * (kTeam * NT * 128);  // [warp][NT][8][16]
+  const int g = lane >> 2, t = lane & 3;
+  const int b0 = blockIdx.y * nb;
+  const int nx = p.batch - b0 < nb ? p.batch - b0 : nb;  // rows of x here
+  const int tiles = (p.rows + 15) / 16;
+  const int groups = p.cols / p.group;
+  const int chunks = p.cols / kChunk;
+  const int ratio = p.group / kChunk;  // chunks per group
+  // this warp's chunks of every tile
+  const int per_warp = (chunks + kTeam - 1) / kTeam;
+  const int c_first = warp * per_warp, c_end = c_first + per_warp < chunks ? c_first + per_warp : chunks;
+
+  // Columns of the product behind the last row of x are not stored: lanes there repeat the last row.
+  const uint4* xs[NT];
+  const T* xg[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = 8 * j + g < nx ? 8 * j + g : nx - 1;
+    xs[j] = sx + n * 4 + t;
+    xg[j] = static_cast<const T*>(p.x) + (b0 + n) * p.ldx + 8 * V * t;
+  }
+
+  Codes<V> k;
+  const uint8_t *qa, *qb, *za, *zb;
+  const char *sa, *sb;
+  // a lane's rows of a tile, at this warp's first column
+  auto seek = [&](int tile) {
+    const int ra = tile * 16 + g < p.rows ? tile * 16 + g : p.rows - 1;
+    const int rb = tile * 16 + g + 8 < p.rows ? tile * 16 + g + 8 : p.rows - 1;
+    qa = p.q + static_cast<long long>(ra) * (p.cols / 2) + 4 * V * t;
+    qb = p.q + static_cast<long long>(rb) * (p.cols / 2) + 4 * V * t;
+    const long long ia = static_cast<long long>(ra) * groups, ib = static_cast<long long>(rb) * groups;
+    sa = static_cast<const char*>(p.scales) + ia * (p.scale_f32 ? 4 : 2);
+    sb = static_cast<const char*>(p.scales) + ib * (p.scale_f32 ? 4 : 2);
+    za = p.zeros + ia;
+    zb = p.zeros + ib;
   };
-  if (p.batch <= 8) return go(std::integral_constant<int, 1>{});
-  if (p.batch <= 16) return go(std::integral_constant<int, 2>{});
-  go(std::integral_constant<int, 4>{});
+  auto fetch = [&](int c) {
+    const uint8_t* a = qa + c * (kChunk / 2);
+    const uint8_t* b = qb + c * (kChunk / 2);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c + u < c_end) {
+        load_words<V>(a + u * (kChunk / 2), k.wa[u]);
+        load_words<V>(b + u * (kChunk / 2), k.wb[u]);
+      }
+    const int ct = c + t < c_end ? c + t : c;
+    const int gr = ratio == 1 ? ct : ct / ratio;
+    if (p.scale_f32) {
+      k.sa = __ldg(reinterpret_cast<const uint32_t*>(sa) + gr);
+      k.sb = __ldg(reinterpret_cast<const uint32_t*>(sb) + gr);
+    } else {
+      k.sa = __ldg(reinterpret_cast<const unsigned short*>(sa) + gr);
+      k.sb = __ldg(reinterpret_cast<const unsigned short*>(sb) + gr);
+    }
+    if (p.zeros) {
+      k.za = __ldg(za + gr);
+      k.zb = __ldg(zb + gr);
+    }
+  };
+  const int tstep = gridDim.x * kTeams;
+  int tile = team * gridDim.x + blockIdx.x;
+  if (tile < tiles) {
+    seek(tile);
+    if (c_first < c_end) fetch(c_first);
+  }
+  if constexpr (XS) {
+    for (int n = 0; n < nx; ++n) {
+      const T* row = static_cast<const T*>(p.x) + (b0 + n) * p.ldx;
+#pragma unroll 4
+      for (int w = threadIdx.x; w < words; w += blockDim.x) {
+        XWord<T> x;
+        x.load(row + 8 * w);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+          sx[(((w / (4 * V) * V + w % V) * kParts + part) * nb + n) * 4 + w / V % 4] = x.b[part];
+      }
+    }
+    __syncthreads();
+  }
+  const int xstep = kParts * nb * 4;  // from one word to the next
+  for (; tile < tiles; tile += tstep) {
+    float tot[NT][4] = {};
+    for (int c0 = c_first; c0 < c_end; c0 += U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u;
+        if (c >= c_end) break;
+        uint32_t oa = 0x43084308u, ob = 0x43084308u;
+        if (p.zeros) {
+          oa = 0x43004300u | ((__shfl_sync(0xFFFFFFFFu, k.za, u, 4) & 15u) * 0x10001u);
+          ob = 0x43004300u | ((__shfl_sync(0xFFFFFFFFu, k.zb, u, 4) & 15u) * 0x10001u);
+        }
+        float acc[NT][4];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const uint32_t wa = k.wa[u][v], wb = k.wb[u][v];
+          const uint32_t lo[4] = {code_pair(wa, 0, oa), code_pair(wb, 0, ob), code_pair(wa, 1, oa), code_pair(wb, 1, ob)};
+          const uint32_t hi[4] = {code_pair(wa, 2, oa), code_pair(wb, 2, ob), code_pair(wa, 3, oa), code_pair(wb, 3, ob)};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            XWord<T> x;
+            if constexpr (XS) {
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) x.b[part] = xs[j][(c * V + v) * xstep + part * nb * 4];
+            } else {
+              x.load(xg[j] + static_cast<long long>(c) * kChunk + 8 * v);
+            }
+#pragma unroll
+            for (int part = kParts - 1; part >= 0; --part) {
+              if (v == 0 && part == kParts - 1)
+                mma_16816_zero(acc[j], lo, x.b[part].x, x.b[part].y);
+              else
+                mma_16816(acc[j], lo, x.b[part].x, x.b[part].y);
+              mma_16816(acc[j], hi, x.b[part].z, x.b[part].w);
+            }
+          }
+        }
+        const uint32_t ua = __shfl_sync(0xFFFFFFFFu, k.sa, u, 4), ub = __shfl_sync(0xFFFFFFFFu, k.sb, u, 4);
+        const float fa = __uint_as_float(p.scale_f32 ? ua : ua << 16);
+        const float fb = __uint_as_float(p.scale_f32 ? ub : ub << 16);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          tot[j][0] = fmaf(fa, acc[j][0], tot[j][0]);
+          tot[j][1] = fmaf(fa, acc[j][1], tot[j][1]);
+          tot[j][2] = fmaf(fb, acc[j][2], tot[j][2]);
+          tot[j][3] = fmaf(fb, acc[j][3], tot[j][3]);
+        }
+      }
+      if (c0 + U < c_end) fetch(c0 + U);
+    }
+    if (tile + tstep < tiles) {
+      seek(tile + tstep);
+      if (c_first < c_end) fetch(c_first);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float* o = red + (warp * NT + j) * 128;  // [column][row]
+      o[(2 * t) * 16 + g] = tot[j][0];
+      o[(2 * t + 1) * 16 + g] = tot[j][1];
+      o[(2 * t) * 16 + g + 8] = tot[j][2];
+      o[(2 * t + 1) * 16 + g + 8] = tot[j][3];
+    }
+    // a team's barrier: its number is the team's, its count the team's threads
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * kTeam) : "memory");
+    const int e = threadIdx.x % (32 * kTeam);
+    if (e < NT * 128) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kTeam; ++w) s += red[w * NT * 128 + e];
+      const int n = e / 16, row = tile * 16 + e % 16;
+      if (n < nx && row < p.rows) static_cast<T*>(p.y)[(b0 + n) * p.ldy + row] = from_f32<T>(s);
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * kTeam) : "memory");
+  }
+}
+
+template <typename T, int V, int NT, bool XS>
+int launch_q4(const Q4Params& p, int nb, cudaStream_t st) {
+  auto kern = q4_kernel<T, V, NT, XS>;
+  constexpr int kThreads = NT == 1 ? 1024 : 512, kTeams = kThreads / (32 * kTeam);
+  const size_t smem = (XS ? static_cast<size_t>(p.cols) / 8 * XWord<T>::kParts * nb * sizeof(uint4) : 0) +
+                      kTeams * kTeam * NT * 128 * sizeof(float);
+  if (smem > 48 * 1024) {
+    // (a cheap call, and right for whichever device is current)
+    SMM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
+                 "q4_matvec shared memory size");
+  }
+  const int tiles = (p.rows + 15) / 16;
+  // One CTA an SM.  Few tiles are spread over the SMs, one to a CTA.
+  const dim3 grid(std::min(tiles, 148), (p.batch + nb - 1) / nb);
+  kern<<<grid, kThreads, smem, st>>>(p, nb);
+  return SMM_OK;
+}
+
+template <typename T, int V>
+int launch_q4_rows(const Q4Params& p, cudaStream_t st) {
+  // up to 16 rows of x to a CTA, 8 where 16 do not fit, fewer of long rows
+  const size_t row = static_cast<size_t>(p.cols) / 8 * XWord<T>::kParts * sizeof(uint4);
+  if (p.batch > 8 && 16 * row <= kQ4XBytes) return launch_q4<T, V, 2, true>(p, std::min(p.batch, 16), st);
+  const int fit = row ? static_cast<int>(std::min<size_t>(kQ4XBytes / row, 8)) : 8;
+  if (fit >= 1) {
+    // equal shares: 9 rows by at most 8 are 5 and 4
+    const int parts = (p.batch + fit - 1) / fit;
+    return launch_q4<T, V, 1, true>(p, (p.batch + parts - 1) / parts, st);
+  }
+  return launch_q4<T, V, 1, false>(p, 8, st);
 }
 
 }  // namespace
@@ -253,21 +351,22 @@ extern "C" int smm_q4_matvec(const void* q, const void* scales, const void* zero
     return set_error(SMM_ERR_INVALID, "smm_q4_matvec: y overlaps an input");
   if (!aligned_to(q, 16) || !aligned_to(x, 16) || (batch > 1 && ldx * e % 16 != 0))
     return set_error(SMM_ERR_INVALID, "smm_q4_matvec: q, x and x's rows must be 16-byte aligned");
-  if (batch > 65535 * 32) return set_error(SMM_ERR_INVALID, "smm_q4_matvec: batch %d too large", batch);
+  if (batch > 65535) return set_error(SMM_ERR_INVALID, "smm_q4_matvec: batch %d too large", batch);
   Q4Params p{static_cast<const uint8_t*>(q), scales, static_cast<const uint8_t*>(zeros), x, y, batch, rows, cols,
              group, scale_dtype == SMM_DTYPE_F32, ldx, ldy};
-  const int warps = 8;
   cudaStream_t st = as_stream(stream);
+  // the widest load whose columns lie in one group
   const int v = group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;
-  if (dtype == SMM_DTYPE_F32) {
-    if (v == 4) launch_q4<float, 4>(p, warps, st);
-    else if (v == 2) launch_q4<float, 2>(p, warps, st);
-    else launch_q4<float, 1>(p, warps, st);
-  } else {
-    if (v == 4) launch_q4<__nv_bfloat16, 4>(p, warps, st);
-    else if (v == 2) launch_q4<__nv_bfloat16, 2>(p, warps, st);
-    else launch_q4<__nv_bfloat16, 1>(p, warps, st);
-  }
+  int rc;
+  if (dtype == SMM_DTYPE_F32)
+    rc = v == 4   ? launch_q4_rows<float, 4>(p, st)
+         : v == 2 ? launch_q4_rows<float, 2>(p, st)
+                  : launch_q4_rows<float, 1>(p, st);
+  else
+    rc = v == 4   ? launch_q4_rows<__nv_bfloat16, 4>(p, st)
+         : v == 2 ? launch_q4_rows<__nv_bfloat16, 2>(p, st)
+                  : launch_q4_rows<__nv_bfloat16, 1>(p, st);
+  if (rc) return rc;
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "q4_matvec launch");
   return SMM_OK;

@@ -9,29 +9,7 @@
 namespace smm {
 namespace {
 
-// Two fp32 lanes in one 64-bit register: one instruction does two fused
-// multiply-adds, each rounded as a scalar one is.
-struct F2 {
-  unsigned long long v;
-};
-__device__ __forceinline__ F2 pack2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(F2 x, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
+using F2 = unsigned long long;  // two fp32 lanes
 
 // ------------------------------------------------------------ prompts
 // The recurrence itself, for fp32 elements (whose accuracy bf16 products do
@@ -332,7 +310,7 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, 
         const int n = (k * lanes + sub) * VEC;
         if (in && q < pend && n < N) {
           if constexpr (VEC == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(in + static_cast<long long>(q) * N + n);
+            const float4 f = __ldcs(reinterpret_cast<const float4*>(in + static_cast<long long>(q) * N + n));
             hv[r][k][0] = f.x, hv[r][k][1] = f.y, hv[r][k][2] = f.z, hv[r][k][3] = f.w;
           } else {
             hv[r][k][0] = in[static_cast<long long>(q) * N + n];
@@ -379,8 +357,8 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, 
         const int n = (k * lanes + sub) * VEC;
         if (out && q < pend && n < N) {
           if constexpr (VEC == 4)
-            *reinterpret_cast<float4*>(out + static_cast<long long>(q) * N + n) =
-                make_float4(hv[r][k][0], hv[r][k][1], hv[r][k][2], hv[r][k][3]);
+            __stcs(reinterpret_cast<float4*>(out + static_cast<long long>(q) * N + n),
+                   make_float4(hv[r][k][0], hv[r][k][1], hv[r][k][2], hv[r][k][3]));
           else
             out[static_cast<long long>(q) * N + n] = hv[r][k][0];
         }

@@ -201,25 +201,15 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// v sigmoid(v) in five instructions; 0 once 1 + exp(-v) passes 2^126.
-__device__ __forceinline__ float gate(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2(-kLog2e * v)));
-  return v * r;
-}
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  unsigned long long x, y, r;
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
   float2 o;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(b.x), "f"(b.y));
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(r));
+  unpack2(mul2(pack2(a.x, a.y), pack2(b.x, b.y)), o.x, o.y);
   return o;
 }
 // 32 lanes x 32 consecutive columns of tensor memory into registers.
@@ -580,10 +570,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                   const float4 f4 = f[i];
-                  const float2 v0 = mul2(mul2(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])),
+                  const float2 v0 = mul_pair(mul_pair(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])),
                                               make_float2(f4.x, f4.y)),
                                          u2);
-                  const float2 v1 = mul2(mul2(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
+                  const float2 v1 = mul_pair(mul_pair(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
                                               make_float2(f4.z, f4.w)),
                                          u2);
                   o[2 * i] = bf16_pair(v0.x, v0.y);
@@ -646,8 +636,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               float a = fmaf(Dh, bf_lo(xw[i]), fmaf(e, __uint_as_float(ro[2 * i]), __uint_as_float(ry[2 * i])));
               float b = fmaf(Dh, bf_hi(xw[i]), fmaf(e, __uint_as_float(ro[2 * i + 1]), __uint_as_float(ry[2 * i + 1])));
               if (gated) {
-                a *= gate(bf_lo(zw[i]));
-                b *= gate(bf_hi(zw[i]));
+                a *= silu(bf_lo(zw[i]));
+                b *= silu(bf_hi(zw[i]));
               }
               out[i] = bf16_pair(a, b);
             }

@@ -12,6 +12,27 @@
 
 namespace smm {
 
+// Two fp32 lanes in one 64-bit register: one instruction does two multiply-adds, each
+// rounded as a scalar one is.
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(unsigned long long x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
   return static_cast<float>(v);
@@ -29,17 +50,27 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// N consecutive elements as fp32.  The compiler merges the element loads of
-// an aligned vector type; N * sizeof(T) is a multiple of 16 where VEC loads
-// are used, and the pointer is then 16-byte aligned.
-template <typename T, int N, bool VEC>
-__device__ __forceinline__ void load_f32(const T* p, float (&v)[N]) {
-  if constexpr (VEC && (N * sizeof(T)) % 16 == 0) {
-    constexpr int Q = N * sizeof(T) / 16;
-    uint4 raw[Q];
+// N consecutive elements as fp32.  With VEC they are moved in pieces of 16 bytes, or of
+// 8 where N elements are no multiple of 16 bytes; the pointer is aligned to a piece.
+template <int BYTES>
+struct Piece {
+  using type = uint4;
+};
+template <>
+struct Piece<8> {
+  using type = uint2;
+};
+// The raw pieces, and their elements.
+template <typename T, int N, int PB>
+struct RawVec {
+  static_assert(N * sizeof(T) % PB == 0, "whole pieces");
+  typename Piece<PB>::type q[N * sizeof(T) / PB];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < Q; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+    for (int i = 0; i < int(N * sizeof(T) / PB); ++i) q[i] = reinterpret_cast<const typename Piece<PB>::type*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float (&v)[N]) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(q);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if constexpr (sizeof(T) == 4)
@@ -47,18 +78,27 @@ __device__ __forceinline__ void load_f32(const T* p, float (&v)[N]) {
       else
         v[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
     }
+  }
+};
+template <typename T, int N, bool VEC, int PB = (N * sizeof(T) % 16 == 0 ? 16 : 8)>
+__device__ __forceinline__ void load_f32(const T* p, float (&v)[N]) {
+  if constexpr (VEC) {
+    RawVec<T, N, PB> r;
+    r.load(p);
+    r.get(v);
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = to_f32(p[i]);
   }
 }
-template <typename T, int N, bool VEC>
+template <typename T, int N, bool VEC, int PB = (N * sizeof(T) % 16 == 0 ? 16 : 8)>
 __device__ __forceinline__ void store_f32(T* p, const float (&v)[N]) {
-  if constexpr (VEC && (N * sizeof(T)) % 16 == 0) {
-    constexpr int Q = N * sizeof(T) / 16;
-    uint32_t w[Q * 4];
+  if constexpr (VEC) {
+    constexpr int Q = N * sizeof(T) / PB;
+    typename Piece<PB>::type q[Q];
+    uint32_t* w = reinterpret_cast<uint32_t*>(q);
 #pragma unroll
-    for (int i = 0; i < Q * 4; ++i) {
+    for (int i = 0; i < int(N * sizeof(T) / 4); ++i) {
       if constexpr (sizeof(T) == 4) {
         w[i] = __float_as_uint(v[i]);
       } else {
@@ -67,18 +107,23 @@ __device__ __forceinline__ void store_f32(T* p, const float (&v)[N]) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < Q; ++i)
-      reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    for (int i = 0; i < Q; ++i) reinterpret_cast<typename Piece<PB>::type*>(p)[i] = q[i];
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = from_f32<T>(v[i]);
   }
 }
 
-// v * sigmoid(v), by the fast quotient (2 units in the last place; the IEEE one
-// made an epilogue of 64 of them ten times as long).  The quotient is 0, the
-// right limit, once 1 + exp(-v) passes 2^126 (v below -87).
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+// v * sigmoid(v) in five instructions: exp(-v) as a power of two and the reciprocal by
+// the fast units, 2 units in the last place each.  (The IEEE quotient made an
+// epilogue of 64 of them ten times as long.)  It is 0, the right limit, once
+// 1 + exp(-v) passes 2^126 (v below -87).
+__device__ __forceinline__ float silu(float v) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return v * r;
+}
 // log(1 + exp(v)); above 20 the correction is below half a step of v.
 __device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
 

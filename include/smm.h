@@ -545,7 +545,8 @@ int smm_selective_step(const void* x, const void* dt, const float* A, const void
  * the low half of byte i; scales and zeros (bytes; NULL: 8 everywhere) are rows x
  * cols/group.  group is a multiple of 32 and divides cols.  x and y have dtype
  * elements, scales scale_dtype.  Products are exact and sums fp32, also for fp32 x.
- * q 16-byte aligned.  y must not overlap an input.  No counterpart in the reference. */
+ * q, x and x's rows are 16-byte aligned; batch is at most 65535.  y must not overlap
+ * an input.  No counterpart in the reference. */
 int smm_q4_matvec(const void* q, const void* scales, const void* zeros, const void* x, void* y, int batch, int rows,
                   int cols, int group, long long ldx, long long ldy, int dtype, int scale_dtype, void* stream);
 

@@ -199,7 +199,7 @@ def q4(q=at(0), scales=at(4096), zeros=None, x=at(8192), y=at(16384), batch=2, r
     dict(batch=-1), dict(rows=-1), dict(cols=-64), dict(group=16), dict(group=0), dict(group=48), dict(group=128),
     dict(dtype=3), dict(sd=3), dict(ldx=63), dict(ldy=7), dict(q=None), dict(scales=None), dict(x=None), dict(y=None),
     dict(q=at(8)), dict(x=at(8192 + 4)), dict(ldx=65), dict(y=at(8192 + 256)), dict(y=at(0)), dict(y=at(4096)),
-    dict(batch=65535 * 32 + 1),
+    dict(batch=65536, y=at(1 << 26)),
 ])
 def test_q4_entry_rejects(kw):
     assert q4(**kw) == _lib.SMM_ERR_INVALID
