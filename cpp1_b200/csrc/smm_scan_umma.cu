@@ -47,6 +47,8 @@ constexpr uint32_t kAtom = kQ * 128;  // one 64-element wide tile of 128 rows: 1
 // quarter and the third one of S, each written by the warps that have read its half.
 constexpr uint32_t kColS = 0, kColY = 256, kColDs = 384, kColYo = 448, kCols = 512;
 
+constexpr int kNapLoad = 100, kNapMma = 20, kNapDecay = 32, kNapG = 32, kNapXw = 32, kNapState = 32;
+
 struct Scal {
   float f[4][kQ];  // f[b-1][s], b = 1..4
   float l[kQ];     // log2 of the decay from the block's start through t
@@ -58,8 +60,8 @@ struct Scal {
 };
 
 struct Bars {
-  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], xfree[2], done[2], s_full[2], g_full[2];
-  uint64_t xw_full, ds_full, ds_free, h_full, yo_free, y_full;
+  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], xfree[2], done[2], s_full[2], g_full[2], y_full[2];
+  uint64_t xw_full, ds_full, ds_free, h_full, yo_free;
   uint64_t sc_full[3], sc_free[3];
   uint64_t drain;
   uint32_t tmem;
@@ -147,10 +149,13 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // products still to come, so the loading and the issuing warp keep the time, and
 // raise the flag for all.  (The code of a dozen timers is what instruction fetches
 // have no room for.)
+template <int NS>
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const volatile int* abort_flag) {
   const uint32_t a = smem_u32(bar);
-  while (!mbar_try_wait(a, parity))
+  while (!mbar_try_wait(a, parity)) {
+    __nanosleep(NS);
     if (*abort_flag) return false;
+  }
   return true;
 }
 // Time since the first of a run of fruitless polls; true once the limit has passed
@@ -286,13 +291,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->done[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->g_full[i], 8);
+      mbar_init(&bars->y_full[i], 8);
     }
     mbar_init(&bars->xw_full, 8);
     mbar_init(&bars->ds_full, 1);
     mbar_init(&bars->ds_free, 4);
     mbar_init(&bars->h_full, 4);
     mbar_init(&bars->yo_free, 8);
-    mbar_init(&bars->y_full, 8);
     for (int i = 0; i < 3; ++i) {
       mbar_init(&bars->sc_full[i], 1);
       mbar_init(&bars->sc_free[i], STATES ? 12 : 20);
@@ -358,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         else if (time.out(p, flag, kWaitProducer))
           break;
         else
-          __nanosleep(100);  // polling takes issue slots from the warps that compute
+          __nanosleep(kNapLoad);
       }
       // after an abort, copies in flight land before the CTA leaves
       if (*flag) {
@@ -452,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitMma)))
         break;
       else
-        __nanosleep(20);
+        __nanosleep(kNapMma);
     }
     // every product has completed, and its arrivals have landed, before the CTA leaves
     umma_commit_by(leader, &bars->drain);
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int c = warp - 2; c < nc; c += 2) {
       const int b3 = c % 3;
       if (c >= 3) {
-        ok = wait_bar(&bars->sc_free[b3], (c / 3 - 1) & 1, flag);
+        ok = wait_bar<kNapDecay>(&bars->sc_free[b3], (c / 3 - 1) & 1, flag);
         if (!ok) break;
       }
       Scal& sc = scal[b3];
@@ -535,23 +540,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
       const uint32_t sYo = tmem + lanes + kColYo + 32 * half;
       const float Dh = p.D ? __ldg(p.D + h) : 0.0f;
+      const unsigned long long D2 = pack2(Dh, Dh);
       const bool gated = p.z != nullptr;
       const long long col = static_cast<long long>(h) * p.dim + p0 + 32 * half;
       const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + (sg.begin + t) * p.ldz + col;
+      const long long zstep = static_cast<long long>(kQ) * p.ldz;
+      const int rows = static_cast<int>(sg.end - sg.begin);
       const int wdims = pdims - 32 * half;  // columns of this half
       for (int c = 0; c <= nc; ++c) {
         // z's own row for the chunk before, on its way while G is formed
         uint4 zv[4];
         if (gated && c > 0) {
-          const bool live = sg.begin + static_cast<long long>(c - 1) * kQ + t < sg.end;
-          const uint4* zr = reinterpret_cast<const uint4*>(gz + static_cast<long long>(c - 1) * kQ * p.ldz);
+          const uint4* zr = reinterpret_cast<const uint4*>(gz);
+          const int have = (c - 1) * kQ + t < rows ? wdims : 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) zv[i] = live && 8 * i < wdims ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < 4; ++i) zv[i] = 8 * i < have ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
+          gz += zstep;
         }
         if (c < nc) {
           const int b3 = c % 3, s = c & 1;
-          if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
-          if (!wait_bar(&bars->s_full[s], (c >> 1) & 1, flag)) break;
+          if (!wait_bar<kNapG>(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
+          if (!wait_bar<kNapG>(&bars->s_full[s], (c >> 1) & 1, flag)) break;
           tc_fence_after_sync();
           const Scal& sc = scal[b3];
           const float u = sc.u[t], lt = sc.l[t];
@@ -563,35 +572,29 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (b <= q) {
               uint32_t r[32];
               tmem_ld_32x32b_x32(sS + 32 * i2, r);
-              const float4* f = reinterpret_cast<const float4*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
+              const unsigned long long* f =
+                  reinterpret_cast<const unsigned long long*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
               if (b < q) {
-                const float2 u2 = make_float2(u, u);
+                const unsigned long long u2 = pack2(u, u);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const float4 f4 = f[i];
-                  const float2 v0 = mul_pair(mul_pair(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])),
-                                              make_float2(f4.x, f4.y)),
-                                         u2);
-                  const float2 v1 = mul_pair(mul_pair(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
-                                              make_float2(f4.z, f4.w)),
-                                         u2);
-                  o[2 * i] = bf16_pair(v0.x, v0.y);
-                  o[2 * i + 1] = bf16_pair(v1.x, v1.y);
+                for (int i = 0; i < 16; ++i) {
+                  const unsigned long long s2 = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                  o[i] = narrow2(mul2(mul2(s2, f[i]), u2));
                 }
               } else {
-                const float4* ls = reinterpret_cast<const float4*>(sc.l + 32 * b);
+                const unsigned long long* ls = reinterpret_cast<const unsigned long long*>(sc.l + 32 * b);
+                const unsigned long long lt2 = pack2(lt, lt), neg = pack2(-1.0f, -1.0f);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const float4 l4 = ls[i], d4 = f[i];
-                  // columns up to this row
-                  const float g0 = 4 * i <= lane ? __uint_as_float(r[4 * i]) * (ex2(lt - l4.x) * d4.x) : 0.0f;
-                  const float g1 = 4 * i + 1 <= lane ? __uint_as_float(r[4 * i + 1]) * (ex2(lt - l4.y) * d4.y) : 0.0f;
-                  const float g2 = 4 * i + 2 <= lane ? __uint_as_float(r[4 * i + 2]) * (ex2(lt - l4.z) * d4.z) : 0.0f;
-                  const float g3 = 4 * i + 3 <= lane ? __uint_as_float(r[4 * i + 3]) * (ex2(lt - l4.w) * d4.w) : 0.0f;
-                  o[2 * i] = bf16_pair(g0, g1);
-                  o[2 * i + 1] = bf16_pair(g2, g3);
+                for (int i = 0; i < 16; ++i) {
+                  // Columns up to this row.  The factors are formed for all of them and the rest is
+                  // selected away: an exponential inside a condition becomes a branch of its own.
+                  float a, z;
+                  unpack2(fma2(ls[i], neg, lt2), a, z);
+                  const unsigned long long w2 = mul2(pack2(ex2(a), ex2(z)), f[i]);
+                  unpack2(mul2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), w2), a, z);
+                  o[i] = bf16_pair(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f);
                 }
               }
             } else {
@@ -610,10 +613,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int d = c - 1, b3 = d % 3, s = d & 1;
           // y takes x's place in shared memory, row by row, and leaves as one tile (or by
           // rows where the chunk ends before the tile)
-          if (!wait_bar(&bars->full_x[s], (d >> 1) & 1, flag)) break;
-          if (!wait_bar(&bars->done[s], (d >> 1) & 1, flag)) break;
+          if (!wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag)) break;
+          if (!wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag)) break;
           tc_fence_after_sync();
           const float e = scal[b3].e[t];
+          const unsigned long long e2 = pack2(e, e);
           const uint32_t sY = tmem + lanes + kColY + s * kP + 32 * half;
           uint8_t* xt = smem + s * L::kStage + stage_x;
 #pragma unroll 1
@@ -633,13 +637,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              float a = fmaf(Dh, bf_lo(xw[i]), fmaf(e, __uint_as_float(ro[2 * i]), __uint_as_float(ry[2 * i])));
-              float b = fmaf(Dh, bf_hi(xw[i]), fmaf(e, __uint_as_float(ro[2 * i + 1]), __uint_as_float(ry[2 * i + 1])));
-              if (gated) {
-                a *= silu(bf_lo(zw[i]));
-                b *= silu(bf_hi(zw[i]));
-              }
-              out[i] = bf16_pair(a, b);
+              unsigned long long v = fma2(e2, pack2(__uint_as_float(ro[2 * i]), __uint_as_float(ro[2 * i + 1])),
+                                          pack2(__uint_as_float(ry[2 * i]), __uint_as_float(ry[2 * i + 1])));
+              v = fma2(D2, widen2(xw[i]), v);
+              if (gated) v = mul2(v, silu2(widen2(zw[i])));
+              out[i] = narrow2(v);
             }
             *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
             *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
@@ -650,18 +652,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) {
             mbar_arrive(&bars->yo_free);
             mbar_arrive(&bars->sc_free[b3]);
-            mbar_arrive(&bars->y_full);
+            mbar_arrive(&bars->y_full[s]);
           }
           const long long t0 = sg.begin + static_cast<long long>(d) * kQ;
-          if (t0 + kQ <= sg.end) {
-            if (warp == 4) {
-              if (!wait_bar(&bars->y_full, d & 1, flag)) break;  // all of the tile is written
-              if (lane == 0) {
-                tma_store_3d(&maps.y, sbase + s * L::kStage + stage_x, p0, h, static_cast<int>(t0));
-                mbar_arrive(&bars->xfree[s]);
-              }
-            }
-          } else if (t0 + t < sg.end) {
+          // a whole tile is sent off by a warp of the next role
+          if (t0 + kQ > sg.end && t0 + t < sg.end) {
             // a partial chunk is the last: nothing waits for its x tile
             __nv_bfloat16* yr = static_cast<__nv_bfloat16*>(p.y) + (t0 + t) * p.ldy + col;
 #pragma unroll 1
@@ -677,18 +672,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ Xw
     const int s = (threadIdx.x - 384) & 127;     // row
     const int i0 = warp < 16 ? 0 : 4;            // first of this thread's 16-byte pieces
+    // Warp 12 also sends y's tiles off: x of chunk c, which this role waits for, comes
+    // into the place of y of chunk c - 2.
+    auto send_y = [&](int d) {
+      if (!wait_bar<kNapXw>(&bars->y_full[d & 1], (d >> 1) & 1, flag)) return false;
+      if (lane == 0) {
+        tma_store_3d(&maps.y, sbase + (d & 1) * L::kStage + stage_x, p0, h, static_cast<int>(sg.begin) + d * kQ);
+        mbar_arrive(&bars->xfree[d & 1]);
+      }
+      __syncwarp();
+      return true;
+    };
+    const int whole = static_cast<int>((sg.end - sg.begin) / kQ);  // chunks that leave as tiles
+    bool ok = true;
     for (int c = 0; c < nc; ++c) {
       const int b3 = c % 3, sb = c & 1;
       const uint32_t st = sbase + sb * L::kStage;
+      if (!STATES && warp == 12 && c >= 2 && !send_y(c - 2)) {
+        ok = false;
+        break;
+      }
       const long long left = sg.end - sg.begin - static_cast<long long>(c) * kQ;
-      if (!wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
-      if (!wait_bar(&bars->full_x[sb], (c >> 1) & 1, flag)) break;
+      if (!wait_bar<kNapXw>(&bars->sc_full[b3], (c / 3) & 1, flag)) {
+        ok = false;
+        break;
+      }
+      if (!wait_bar<kNapXw>(&bars->full_x[sb], (c >> 1) & 1, flag)) {
+        ok = false;
+        break;
+      }
       const float ws = scal[b3].f[3][s];
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->sc_free[b3]);
-      if (c >= 1 && !wait_bar(&bars->ds_full, (c - 1) & 1, flag)) break;
-      const bool live = s < left;
-#pragma unroll 1
+      if (c >= 1 && !wait_bar<kNapXw>(&bars->ds_full, (c - 1) & 1, flag)) {
+        ok = false;
+        break;
+      }
+      const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
+#pragma unroll 2
       for (int i = i0; i < i0 + 4; ++i) {
         const uint32_t off = swz_offset(s, i, 128);
         const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
@@ -696,21 +717,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t vh[4], vl[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float a = live ? ws * bf_lo(xs[k]) : 0.0f, b = live ? ws * bf_hi(xs[k]) : 0.0f;
-          vh[k] = bf16_pair(a, b);
-          vl[k] = bf16_pair(a - bf_lo(vh[k]), b - bf_hi(vh[k]));
+          const unsigned long long v = mul2(w2, widen2(xs[k]));
+          vh[k] = narrow2(v);
+          vl[k] = narrow2(fma2(neg, widen2(vh[k]), v));
         }
         *reinterpret_cast<uint4*>(smem + L::kXw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
         *reinterpret_cast<uint4*>(smem + L::kXw + kAtom + off) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
       }
       if (left < kQ) {
         // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-        if (!wait_bar(&bars->full_b[sb], (c >> 1) & 1, flag)) break;
+        if (!wait_bar<kNapXw>(&bars->full_b[sb], (c >> 1) & 1, flag)) {
+          ok = false;
+          break;
+        }
         if (s >= left) {
 #pragma unroll
           for (int i = i0; i < i0 + 4; ++i) {
             const uint32_t off = swz_offset(s, i, 128);
             st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
+            st_shared_v4(sbase + L::kXw + off, 0, 0, 0, 0);
+            st_shared_v4(sbase + L::kXw + kAtom + off, 0, 0, 0, 0);
 #pragma unroll
             for (int a = 0; a < NA; ++a) st_shared_v4(st + stage_b + a * kAtom + off, 0, 0, 0, 0);
           }
@@ -720,6 +746,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->xw_full);
     }
+    if (!STATES && warp == 12 && ok)
+      for (int d = nc > 2 ? nc - 2 : 0; d < whole; ++d)
+        if (!send_y(d)) break;
   } else {
     regs_inc<kRegsState>();
     // ------------------------------------------------------------ state
@@ -774,14 +803,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b3 = c % 3;
       if (!STATES) {
         // the product that reads the old H is done
-        ok = c == 0 || wait_bar(&bars->done[(c - 1) & 1], ((c - 1) >> 1) & 1, flag);
+        ok = c == 0 || wait_bar<kNapState>(&bars->done[(c - 1) & 1], ((c - 1) >> 1) & 1, flag);
         if (!ok) break;
         put_h();
       }
-      ok = wait_bar(&bars->sc_full[b3], (c / 3) & 1, flag);
+      ok = wait_bar<kNapState>(&bars->sc_full[b3], (c / 3) & 1, flag);
       if (!ok) break;
       const float decay = scal[b3].total;
-      ok = wait_bar(&bars->ds_full, c & 1, flag);
+      ok = wait_bar<kNapState>(&bars->ds_full, c & 1, flag);
       if (!ok) break;
       tc_fence_after_sync();
       if (wlive) {

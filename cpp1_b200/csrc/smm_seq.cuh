@@ -33,6 +33,22 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
   return r;
 }
 
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The two elements of a bf16 pair.
+__device__ __forceinline__ unsigned long long widen2(uint32_t w) {
+  return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t narrow2(unsigned long long v) {
+  float a, b;
+  unpack2(v, a, b);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v) {
   return static_cast<float>(v);
@@ -123,6 +139,16 @@ __device__ __forceinline__ float silu(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * v));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
   return v * r;
+}
+__device__ __forceinline__ unsigned long long silu2(unsigned long long v) {
+  float a, b, ra, rb;
+  unpack2(mul2(v, pack2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(a));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(b));
+  unpack2(add2(pack2(a, b), pack2(1.0f, 1.0f)), a, b);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ra) : "f"(a));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rb) : "f"(b));
+  return mul2(v, pack2(ra, rb));
 }
 // log(1 + exp(v)); above 20 the correction is below half a step of v.
 __device__ __forceinline__ float softplus(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
