@@ -18,13 +18,17 @@
 // the block; w_s = f[4][s].  So a quarter of the exponentials remains.
 //
 // Roundings: G and H to bf16 as operands of products (relative 2^-8 of
-// each term of y, which is itself rounded to bf16); Xw as the sum of two bf16 terms
-// (2^-16), because the state is an fp32 result that is carried on.  The state
-// itself stays in fp32 registers, S, Y, Yo and dS are fp32 in tensor memory.
+// each term of y, which is itself rounded to bf16); Xw as the sum of three bf16 terms
+// (2^-24; two left an error of 2.3e-6 in the states, an fp32 result that is carried on,
+// where the plain fp32 form has 0.2 to 1.7e-6).  The state itself stays in fp32
+// registers, S, Y, Yo and dS are fp32 in tensor memory.
 //
-// Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the decays in turn,
-// 4-11 form G and write y of the chunk before, half of the columns each, 12-19 form Xw, 20-23 carry
-// the state.  Every wait is bounded; on expiry the CTA records it and leaves.
+// Persistent: a CTA an SM walks its share of the (segment, head, 64 dims) items as one
+// stream of chunks, so that the next item's loads and S are under way while an item
+// ends.  Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the decays in
+// turn, 4-11 form G and write y of the chunk before, half of the columns each, 12-19
+// form Xw, 20-23 carry the state.  Every wait is bounded; on expiry the CTA records it
+// and leaves.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -42,6 +46,7 @@ namespace {
 constexpr int kQ = 128;         // tokens per chunk
 constexpr int kP = 64;          // dims per CTA
 constexpr int kThreads = 768;
+constexpr int kSms = 148;
 constexpr uint32_t kAtom = kQ * 128;  // one 64-element wide tile of 128 rows: 16 KiB
 // Tensor memory columns.  S is 128 wide and double; G takes the place of the first
 // quarter and the third one of S, each written by the warps that have read its half.
@@ -56,12 +61,13 @@ struct Scal {
   float e[kQ];     // decay from the chunk's start through t
   float d[kQ];
   float total;     // decay of the whole chunk
-  float pad[3];
+  float log2;      // its logarithm
+  float pad[2];
 };
 
 struct Bars {
-  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], xfree[2], done[2], s_full[2], g_full[2], y_full[2];
-  uint64_t xw_full, ds_full, ds_free, h_full, yo_free;
+  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], xfree[2], done[2], s_full[2], g_full[2];
+  uint64_t xw_full, xl_full, ds_full, ds_free, h_full, yo_free;
   uint64_t sc_full[3], sc_free[3];
   uint64_t drain;
   uint32_t tmem;
@@ -72,15 +78,15 @@ struct Bars {
 template <int NA>
 struct Smem {
   static constexpr uint32_t kStage = (2 * NA + 1) * kAtom;  // C, B, x
-  static constexpr uint32_t kXw = 2 * kStage;               // high and low terms
-  static constexpr uint32_t kH = kXw + 2 * kAtom;
-  static constexpr uint32_t kScal = kH + NA * 64 * 128;
+  static constexpr uint32_t kXw = 2 * kStage;               // first and second term
+  static constexpr uint32_t kH = kXw + 2 * kAtom;           // third term of Xw, then H (in turn)
+  static constexpr uint32_t kScal = kH + kAtom;
   static constexpr uint32_t kBars = kScal + 3 * sizeof(Scal);
   static constexpr uint32_t kBytes = kBars + sizeof(Bars) + 1024;  // + alignment
 };
 
 struct Tmaps {
-  CUtensorMap x, b, c, y;
+  CUtensorMap x, b, c;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
@@ -89,14 +95,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-// Tile in shared memory -> global; returns once the tile has been read.
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n\t"
-      "cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::"l"(reinterpret_cast<uint64_t>(map)),
-      "r"(src), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 // The whole warp reaches these together and only lane `leader` issues: with the
@@ -210,13 +208,6 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
-  float2 o;
-  unpack2(mul2(pack2(a.x, a.y), pack2(b.x, b.y)), o.x, o.y);
-  return o;
-}
 // 32 lanes x 32 consecutive columns of tensor memory into registers.
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -234,14 +225,35 @@ __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y,
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// One (segment, head, 64 dims) of the work.
+struct Item {
+  Segment sg;
+  int seg, h, p0, pdims, nc;  // nc: chunks
+  long long head_at;          // of this head's and these dims' state in an entry
+  bool last;                  // the sequence's last segment
+};
+// Called by a full warp.
+template <bool STATES>
+__device__ __forceinline__ Item get_item(const ScanParams& p, int it, int ptiles) {
+  Item w;
+  const int hs = it / ptiles;
+  w.h = hs % p.heads;
+  w.seg = hs / p.heads;
+  w.p0 = (it - hs * ptiles) * kP;
+  w.pdims = p.dim - w.p0 < kP ? p.dim - w.p0 : kP;
+  w.sg = find_segment(p, w.seg);
+  w.last = w.sg.j == w.sg.count - 1;
+  w.head_at = (static_cast<long long>(w.h) * p.dim + w.p0) * p.state_dim;
+  w.nc = w.sg.valid && !(STATES && w.last) ? static_cast<int>((w.sg.end - w.sg.begin + kQ - 1) / kQ) : 0;
+  return w;
+}
+
 // STATES: the first launch of a split scan (B, x and the state only).
 template <int NA, bool STATES>
 __global__ void __launch_bounds__(kThreads, 1)
-    scan_umma_kernel(const __grid_constant__ Tmaps maps, const ScanParams p, int ptiles) {
+    scan_umma_kernel(const __grid_constant__ Tmaps maps, const ScanParams p, int items, int ptiles) {
   using L = Smem<NA>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ Segment sseg;
-  __shared__ float seg_sum[2];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   Scal* scal = reinterpret_cast<Scal*>(smem + L::kScal);
@@ -250,36 +262,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // a shuffle from a fixed lane tells the compiler that the warp's role, and all that
   // follows from it, is uniform
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int pt = static_cast<int>(blockIdx.x % ptiles);
-  const int hs = static_cast<int>(blockIdx.x / ptiles);
-  const int h = hs % p.heads, seg = hs / p.heads;
-  if (warp == 0) {
-    const Segment s = find_segment(p, seg);
-    if (lane == 0) sseg = s;
-  }
-  __syncthreads();
-  const Segment sg = sseg;
-  if (!sg.valid) return;
-  const int g = h / (p.heads / p.groups);
-  const int p0 = pt * kP;
-  const int pdims = p.dim - p0 < kP ? p.dim - p0 : kP;
   const int N = p.state_dim;
-  const bool last = sg.j == sg.count - 1;
   const long long per_slot = static_cast<long long>(p.heads) * p.dim * N;
-  const long long head_at = (static_cast<long long>(h) * p.dim + p0) * N;
-  const int slot = (p.state_in || p.state_out) ? seq_slot(p.slots, sg.seq, p.nslots, p.status) : -1;
-  const float* in = p.state_in && slot >= 0 ? p.state_in + slot * per_slot + head_at : nullptr;
-  if constexpr (STATES) {
-    // The last segment's place keeps the state the sequence started from: the
-    // second launch may overwrite it while other segments still need it.
-    if (last) {
-      if (sg.count > 1)
-        for (int i = threadIdx.x; i < pdims * N; i += kThreads)
-          p.seg_state[seg * per_slot + head_at + i] = in ? in[i] : 0.0f;
-      return;
-    }
-  }
-  const int nc = static_cast<int>((sg.end - sg.begin + kQ - 1) / kQ);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -287,13 +271,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->full_c[i], 1);
       mbar_init(&bars->full_x[i], 1);
       mbar_init(&bars->bfree[i], 1);
-      mbar_init(&bars->xfree[i], 1);
+      mbar_init(&bars->xfree[i], 8);
       mbar_init(&bars->done[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->g_full[i], 8);
-      mbar_init(&bars->y_full[i], 8);
     }
     mbar_init(&bars->xw_full, 8);
+    mbar_init(&bars->xl_full, 8);
     mbar_init(&bars->ds_full, 1);
     mbar_init(&bars->ds_free, 4);
     mbar_init(&bars->h_full, 4);
@@ -314,223 +298,272 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   volatile int* const flag = &bars->abort_flag;
   constexpr uint32_t stage_c = 0, stage_b = NA * kAtom, stage_x = 2 * NA * kAtom;
+  const int it0 = blockIdx.x, its = gridDim.x;
 
+  // In every role below, c counts the chunks of an item and cc those of the CTA: stages,
+  // buffers and barriers' phases go by cc.
+  //
   // The launch's 6 x 80 registers per warpgroup's thread, shared out by need.
   // A spill costs a trip to L2 here: shared memory leaves L1 too small for the stacks.
-  constexpr int kRegsMisc = 56, kRegsG = STATES ? 24 : 112, kRegsXw = 56, kRegsState = STATES ? 152 : 88;
+  constexpr int kRegsMisc = 48, kRegsG = STATES ? 24 : 104, kRegsXw = 64, kRegsState = STATES ? 152 : 96;
   static_assert(kRegsMisc + 2 * kRegsG + 2 * kRegsXw + kRegsState <= 6 * 80, "more registers than the launch has");
   if (warp < 4) {
     regs_dec<kRegsMisc>();
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    if (lane == 0) {
-      // next chunk of each operand: each place is free at its own time
-      int c_b = 0, c_c = STATES ? nc : 0, c_x = 0;
+    if (warp == 0) {
+      // ---------------------------------------------------------- loads
+      // B is free after dS, C after all products of its chunk, x after the y that took
+      // its place has left.  Each goes through the items at its own pace.
+      int n_b = 0, n_c = 0, n_x = 0;  // loads issued
       Patience time;
-      const int row0 = static_cast<int>(sg.begin);
-      auto space = [&](uint64_t* free, int c) { return c < 2 || mbar_test(free + (c & 1), ((c >> 1) - 1) & 1); };
-      while (c_b < nc || c_c < nc || c_x < nc) {
+      auto free_at = [&](uint64_t* bar, int cc) {
+        return cc < 2 || __any_sync(0xFFFFFFFFu, mbar_test(bar + (cc & 1), ((cc >> 1) - 1) & 1));
+      };
+      struct Walk {
+        int it, left, row, h, p0;  // chunks left of the item, next row
+      };
+      auto enter = [&](Walk& k) {
+        const Item w = get_item<STATES>(p, k.it, ptiles);
+        k.left = w.nc;
+        k.row = static_cast<int>(w.sg.begin);
+        k.h = w.h;
+        k.p0 = w.p0;
+      };
+      // on to the next item when this one is through; whether there is a chunk
+      auto settle = [&](Walk& k) {
+        while (k.left == 0 && k.it < items) {
+          k.it += its;
+          if (k.it < items) enter(k);
+        }
+        return k.it < items;
+      };
+      Walk b{it0, 0, 0, 0, 0};
+      if (it0 < items) enter(b);
+      bool more_b = settle(b), more_x = more_b, more_c = !STATES && more_b;
+      Walk x = b, cw = b;
+      const int per_group = p.heads / p.groups;
+      while (more_b || more_x || more_c) {
         bool did = false;
-        if (c_b < nc && space(bars->bfree, c_b)) {
-          const int s = c_b & 1;
-          mbar_arrive_expect_tx(&bars->full_b[s], NA * kAtom);
+        if (more_b && free_at(bars->bfree, n_b)) {
+          const int s = n_b & 1, g = b.h / per_group;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars->full_b[s], NA * kAtom);
 #pragma unroll
-          for (int a = 0; a < NA; ++a)
-            tma_load_3d(sbase + s * L::kStage + stage_b + a * kAtom, &maps.b, &bars->full_b[s], a * 64, g,
-                        row0 + c_b * kQ);
-          ++c_b;
+            for (int a = 0; a < NA; ++a)
+              tma_load_3d(sbase + s * L::kStage + stage_b + a * kAtom, &maps.b, &bars->full_b[s], a * 64, g, b.row);
+          }
+          ++n_b, --b.left, b.row += kQ;
+          more_b = settle(b);
           did = true;
         }
-        if (c_c < nc && space(bars->done, c_c)) {
-          const int s = c_c & 1;
-          mbar_arrive_expect_tx(&bars->full_c[s], NA * kAtom);
-#pragma unroll
-          for (int a = 0; a < NA; ++a)
-            tma_load_3d(sbase + s * L::kStage + stage_c + a * kAtom, &maps.c, &bars->full_c[s], a * 64, g,
-                        row0 + c_c * kQ);
-          ++c_c;
+        if (more_x && free_at(STATES ? bars->bfree : bars->xfree, n_x)) {
+          const int s = n_x & 1;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
+            tma_load_3d(sbase + s * L::kStage + stage_x, &maps.x, &bars->full_x[s], x.p0, x.h, x.row);
+          }
+          ++n_x, --x.left, x.row += kQ;
+          more_x = settle(x);
           did = true;
         }
-        if (c_x < nc && space(STATES ? bars->bfree : bars->xfree, c_x)) {
-          const int s = c_x & 1;
-          mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
-          tma_load_3d(sbase + s * L::kStage + stage_x, &maps.x, &bars->full_x[s], p0, h, row0 + c_x * kQ);
-          ++c_x;
+        if (more_c && free_at(bars->done, n_c)) {
+          const int s = n_c & 1, g = cw.h / per_group;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars->full_c[s], NA * kAtom);
+#pragma unroll
+            for (int a = 0; a < NA; ++a)
+              tma_load_3d(sbase + s * L::kStage + stage_c + a * kAtom, &maps.c, &bars->full_c[s], a * 64, g, cw.row);
+          }
+          ++n_c, --cw.left, cw.row += kQ;
+          more_c = settle(cw);
           did = true;
         }
         if (did)
           time.progress();
-        else if (time.out(p, flag, kWaitProducer))
+        else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitProducer)))
           break;
         else
           __nanosleep(kNapLoad);
       }
       // after an abort, copies in flight land before the CTA leaves
-      if (*flag) {
-        const int n[3] = {c_b, STATES ? 0 : c_c, c_x};
+      if (*flag && lane == 0) {
+        const int n[3] = {n_b, n_c, n_x};
 #pragma unroll 1
         for (int k = 0; k < 6; ++k) {  // full_b, full_c, full_x, two of each
           const int last_use = ((n[k >> 1] - (k & 1) + 1) >> 1) - 1;
           if (last_use >= 0) drain_bar(&bars->full_b[0] + k, last_use & 1, p, flag);
         }
       }
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ products
-    constexpr uint32_t idS = make_idesc(kFmtBF16, 128, 128, 0, 0);
-    constexpr uint32_t idY = make_idesc(kFmtBF16, 128, kP, 0, 1);
-    constexpr uint32_t idD = make_idesc(kFmtBF16, 128, kP, 1, 1);
-    const int ksteps = (N + 15) / 16;
-    const uint32_t leader = elect_one();
-    // descriptors of stage 0; a stage is kSt further.  Only the low word, the
-    // start address in 16-byte units, changes with stage and step.
-    constexpr uint32_t kSt = L::kStage >> 4;
-    auto lo = [](uint64_t d) { return static_cast<uint32_t>(d); };
-    const uint64_t dK = make_smem_desc(sbase, 16, 1024, kLayoutSw128);      // K-major
-    const uint64_t dM = make_smem_desc(sbase, kAtom, 1024, kLayoutSw128);   // MN-major
-    const uint32_t hK = static_cast<uint32_t>(dK >> 32), hM = static_cast<uint32_t>(dM >> 32);
-    auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xFFFFFFFFu, mbar_test(bar, parity)) != 0; };
-    int s_next = STATES ? nc : 0, g_next = 0, sub = 0;
-    Patience time;
-    while (g_next < nc) {
-      bool did = false;
-      if (!STATES && s_next < nc && s_next < g_next + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
-          ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1)) {
-        // C was loaded once every product of chunk c - 2 was done: S's place, where its G was, is free
-        tc_fence_after_sync();
-        const int s = s_next & 1;
-        const uint32_t base = lo(dK) + s * kSt;
+    } else if (warp == 1) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t idS = make_idesc(kFmtBF16, 128, 128, 0, 0);
+      constexpr uint32_t idY = make_idesc(kFmtBF16, 128, kP, 0, 1);
+      constexpr uint32_t idD = make_idesc(kFmtBF16, 128, kP, 1, 1);
+      const int ksteps = (N + 15) / 16;
+      const uint32_t leader = elect_one();
+      int total = 0;
+      for (int it = it0; it < items; it += its) total += get_item<STATES>(p, it, ptiles).nc;
+      // descriptors of stage 0; a stage is kSt further.  Only the low word, the
+      // start address in 16-byte units, changes with stage and step.
+      constexpr uint32_t kSt = L::kStage >> 4;
+      auto lo = [](uint64_t d) { return static_cast<uint32_t>(d); };
+      const uint64_t dK = make_smem_desc(sbase, 16, 1024, kLayoutSw128);     // K-major
+      const uint64_t dM = make_smem_desc(sbase, kAtom, 1024, kLayoutSw128);  // MN-major
+      const uint32_t hK = static_cast<uint32_t>(dK >> 32), hM = static_cast<uint32_t>(dM >> 32);
+      auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xFFFFFFFFu, mbar_test(bar, parity)) != 0; };
+      // terms k0 .. k1 - 1 (of 8 steps each) of dS = B^T Xw
+      auto ds_steps = [&](int s, int k0, int k1) {
+        const uint32_t base = lo(dM) + s * kSt;
 #pragma unroll 2
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = base + (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
-          umma_ss(leader, tmem + kColS + s * 128, off + (stage_c >> 4), hK, off + (stage_b >> 4), hK, idS, k);
-        }
-        umma_commit_by(leader, &bars->s_full[s]);
-        ++s_next;
-        did = true;
-      } else if (STATES || g_next < s_next) {
-        const int c = g_next, s = c & 1;
-        if (sub == 0) {
-          if (ready(&bars->xw_full, c & 1) && (c == 0 || ready(&bars->ds_free, (c - 1) & 1)) &&
-              ready(&bars->full_b[s], (c >> 1) & 1) && ready(&bars->full_x[s], (c >> 1) & 1)) {
-            tc_fence_after_sync();
-            const uint32_t base = lo(dM) + s * kSt;
-#pragma unroll 2
-            for (int k = 0; k < 16; ++k)  // Xw's low term lies 8 steps behind its high one
-              umma_ss(leader, tmem + kColDs, base + (stage_b >> 4) + (k & 7) * 128, hM, lo(dM) + (L::kXw >> 4) + k * 128,
-                      hM, idD, k);
-            umma_commit_by(leader, &bars->ds_full);
-            umma_commit_by(leader, &bars->bfree[s]);
-            if (STATES) {
-              ++g_next;
-            } else {
-              sub = 1;
-            }
-            did = true;
-          }
-        } else if (sub == 1) {
-          if (ready(&bars->g_full[s], (c >> 1) & 1)) {
-            tc_fence_after_sync();
-            const uint32_t base = lo(dM) + s * kSt;
-#pragma unroll 2
-            for (int k = 0; k < 8; ++k)
-              umma_ts(leader, tmem + kColY + s * kP, tmem + kColS + s * 128 + (k >> 2) * 64 + (k & 3) * 8,
-                      base + (stage_x >> 4) + k * 128, hM, idY, k);
-            sub = 2;
-            did = true;
-          }
-        } else if (ready(&bars->h_full, c & 1) && (c == 0 || ready(&bars->yo_free, (c - 1) & 1))) {
+        for (int k = k0; k < k1; ++k)
+          umma_ss(leader, tmem + kColDs, base + (stage_b >> 4) + (k & 7) * 128, hM, lo(dM) + (L::kXw >> 4) + k * 128, hM,
+                  idD, k);
+      };
+      int s_next = STATES ? total : 0, g_next = 0, sub = 0;
+      Patience time;
+      while (g_next < total) {
+        bool did = false;
+        if (!STATES && s_next < total && s_next < g_next + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
+            ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1)) {
+          // C was loaded once every product of chunk c - 2 was done: S's place, where its G was, is free
           tc_fence_after_sync();
+          const int s = s_next & 1;
           const uint32_t base = lo(dK) + s * kSt;
 #pragma unroll 2
-          for (int k = 0; k < ksteps; ++k)
-            umma_ss(leader, tmem + kColYo, base + (stage_c >> 4) + (k >> 2) * (kAtom >> 4) + (k & 3) * 2, hK,
-                    lo(dM) + (L::kH >> 4) + k * 128, hM, idY, k);
-          umma_commit_by(leader, &bars->done[s]);
-          sub = 0;
-          ++g_next;
+          for (int k = 0; k < ksteps; ++k) {
+            const uint32_t off = base + (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
+            umma_ss(leader, tmem + kColS + s * 128, off + (stage_c >> 4), hK, off + (stage_b >> 4), hK, idS, k);
+          }
+          umma_commit_by(leader, &bars->s_full[s]);
+          ++s_next;
           did = true;
-        }
-      }
-      if (did)
-        time.progress();
-      else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitMma)))
-        break;
-      else
-        __nanosleep(kNapMma);
-    }
-    // every product has completed, and its arrivals have landed, before the CTA leaves
-    umma_commit_by(leader, &bars->drain);
-    drain_bar(&bars->drain, 0, p, flag);
-  } else {
-    // ------------------------------------------------------------ decays
-    const float A2 = __ldg(p.A + h) * kLog2e;
-    float log_sum = 0.0f;  // log2 of the segment's decay
-    bool ok = true;
-    const float bias = p.dt_bias ? __ldg(p.dt_bias + h) : 0.0f;
-    // lane -> token 32 b + lane of each block b
-    uint32_t raw[4] = {};
-    auto fetch = [&](int c) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const long long t = sg.begin + static_cast<long long>(c) * kQ + 32 * i + lane;
-        if (t < sg.end) raw[i] = scan_dt_raw(p, t, h);
-      }
-    };
-    if (warp - 2 < nc) fetch(warp - 2);
-    for (int c = warp - 2; c < nc; c += 2) {
-      const int b3 = c % 3;
-      if (c >= 3) {
-        ok = wait_bar<kNapDecay>(&bars->sc_free[b3], (c / 3 - 1) & 1, flag);
-        if (!ok) break;
-      }
-      Scal& sc = scal[b3];
-      const long long left = sg.end - sg.begin - static_cast<long long>(c) * kQ - lane;
-      float bt[4], head = 0.0f;
-#pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
-        const float d = 32 * b < left ? scan_dt(p, raw[0], bias) : 0.0f;
-        raw[0] = raw[1], raw[1] = raw[2], raw[2] = raw[3];
-        // sums within the block: inclusive up to the token, exclusive behind it
-        float inc = d * A2, suf = inc;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const float x = __shfl_up_sync(0xFFFFFFFFu, inc, o), z = __shfl_down_sync(0xFFFFFFFFu, suf, o);
-          if (lane >= o) inc += x;
-          if (lane + o < 32) suf += z;
-        }
-        bt[0] = bt[1], bt[1] = bt[2], bt[2] = bt[3], bt[3] = __shfl_sync(0xFFFFFFFFu, inc, 31);
-        suf = __shfl_down_sync(0xFFFFFFFFu, suf, 1);
-        const int t = 32 * b + lane;
-        sc.l[t] = inc;
-        sc.u[t] = ex2(inc);
-        sc.e[t] = ex2(head + inc);
-        sc.d[t] = d;
-        sc.f[3][t] = lane < 31 ? suf : 0.0f;  // the exponent, until the blocks' sums are known
-        head += bt[3];
-      }
-      if (c + 2 < nc) fetch(c + 2);
-#pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
-        const int t = 32 * b + lane;
-        const float suf = sc.f[3][t], d = sc.d[t];
-        float between = 0.0f;
-#pragma unroll
-        for (int k = 1; k <= 4; ++k) {
-          if (k > b) {
-            if (k - 1 > b) between += bt[k - 1];
-            sc.f[k - 1][t] = d * ex2(suf + between);
+        } else if (STATES || g_next < s_next) {
+          const int cc = g_next, s = cc & 1;
+          const uint32_t par = (cc >> 1) & 1;
+          if (sub == 0) {
+            if (ready(&bars->xw_full, cc & 1) && (cc == 0 || ready(&bars->ds_free, (cc - 1) & 1)) &&
+                ready(&bars->full_b[s], par) && ready(&bars->full_x[s], par)) {
+              tc_fence_after_sync();
+              ds_steps(s, 0, 16);
+              sub = 1;
+              did = true;
+            }
+          } else if (sub == 1) {
+            if (ready(&bars->xl_full, cc & 1)) {
+              tc_fence_after_sync();
+              ds_steps(s, 16, 24);
+              umma_commit_by(leader, &bars->ds_full);
+              umma_commit_by(leader, &bars->bfree[s]);
+              sub = 2;
+              if (STATES) sub = 0, ++g_next;
+              did = true;
+            }
+          } else if (sub == 2) {
+            if (ready(&bars->g_full[s], par)) {
+              tc_fence_after_sync();
+              const uint32_t base = lo(dM) + s * kSt;
+#pragma unroll 2
+              for (int k = 0; k < 8; ++k)
+                umma_ts(leader, tmem + kColY + s * kP, tmem + kColS + s * 128 + (k >> 2) * 64 + (k & 3) * 8,
+                        base + (stage_x >> 4) + k * 128, hM, idY, k);
+              sub = 3;
+              did = true;
+            }
+          } else if (ready(&bars->h_full, cc & 1) && (cc == 0 || ready(&bars->yo_free, (cc - 1) & 1))) {
+            tc_fence_after_sync();
+            const uint32_t base = lo(dK) + s * kSt;
+#pragma unroll 2
+            for (int k = 0; k < ksteps; ++k)
+              umma_ss(leader, tmem + kColYo, base + (stage_c >> 4) + (k >> 2) * (kAtom >> 4) + (k & 3) * 2, hK,
+                      lo(dM) + (L::kH >> 4) + k * 128, hM, idY, k);
+            umma_commit_by(leader, &bars->done[s]);
+            sub = 0;
+            ++g_next;
+            did = true;
           }
         }
+        if (did)
+          time.progress();
+        else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitMma)))
+          break;
+        else
+          __nanosleep(kNapMma);
       }
-      const float total = bt[0] + bt[1] + bt[2] + bt[3];
-      log_sum += total;
-      if (lane == 0) sc.total = ex2(total);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->sc_full[b3]);
+      // every product has completed, and its arrivals have landed, before the CTA leaves
+      umma_commit_by(leader, &bars->drain);
+      drain_bar(&bars->drain, 0, p, flag);
+    } else {
+      // ---------------------------------------------------------- decays
+      // lane -> token 32 b + lane of each block b; even chunks of the stream by warp 2, odd ones by warp 3
+      int cc0 = 0;
+      bool ok = true;
+      for (int it = it0; it < items && ok; it += its) {
+        const Item w = get_item<STATES>(p, it, ptiles);
+        const float A2 = w.nc > 0 ? __ldg(p.A + w.h) * kLog2e : 0.0f;
+        const float bias = w.nc > 0 && p.dt_bias ? __ldg(p.dt_bias + w.h) : 0.0f;
+        uint32_t raw[4] = {};
+        auto fetch = [&](int c) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const long long t = w.sg.begin + static_cast<long long>(c) * kQ + 32 * i + lane;
+            if (t < w.sg.end) raw[i] = scan_dt_raw(p, t, w.h);
+          }
+        };
+        const int first = (cc0 & 1) == (warp & 1) ? 0 : 1;
+        if (first < w.nc) fetch(first);
+#pragma unroll 1
+        for (int c = first; c < w.nc; c += 2) {
+          const int cc = cc0 + c, b3 = cc % 3;
+          ok = cc < 3 || wait_bar<kNapDecay>(&bars->sc_free[b3], (cc / 3 - 1) & 1, flag);
+          if (!ok) break;
+          Scal& sc = scal[b3];
+          const long long left = w.sg.end - w.sg.begin - static_cast<long long>(c) * kQ - lane;
+          float bt[4], head = 0.0f;
+#pragma unroll 1
+          for (int b = 0; b < 4; ++b) {
+            const float d = 32 * b < left ? scan_dt(p, raw[0], bias) : 0.0f;
+            raw[0] = raw[1], raw[1] = raw[2], raw[2] = raw[3];
+            // sums within the block: inclusive up to the token, exclusive behind it
+            float inc = d * A2, suf = inc;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const float x = __shfl_up_sync(0xFFFFFFFFu, inc, o), z = __shfl_down_sync(0xFFFFFFFFu, suf, o);
+              if (lane >= o) inc += x;
+              if (lane + o < 32) suf += z;
+            }
+            bt[0] = bt[1], bt[1] = bt[2], bt[2] = bt[3], bt[3] = __shfl_sync(0xFFFFFFFFu, inc, 31);
+            suf = __shfl_down_sync(0xFFFFFFFFu, suf, 1);
+            const int t = 32 * b + lane;
+            sc.l[t] = inc;
+            sc.u[t] = ex2(inc);
+            sc.e[t] = ex2(head + inc);
+            sc.d[t] = d;
+            sc.f[3][t] = lane < 31 ? suf : 0.0f;  // the exponent, until the blocks' sums are known
+            head += bt[3];
+          }
+          if (c + 2 < w.nc) fetch(c + 2);
+#pragma unroll 1
+          for (int b = 0; b < 4; ++b) {
+            const int t = 32 * b + lane;
+            const float suf = sc.f[3][t], d = sc.d[t];
+            float between = 0.0f;
+#pragma unroll
+            for (int k = 1; k <= 4; ++k) {
+              if (k > b) {
+                if (k - 1 > b) between += bt[k - 1];
+                sc.f[k - 1][t] = d * ex2(suf + between);
+              }
+            }
+          }
+          if (lane == 0) {
+            sc.total = ex2(head);
+            sc.log2 = head;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->sc_full[b3]);
+        }
+        cc0 += w.nc;
+      }
     }
-    if (lane == 0) seg_sum[warp - 2] = log_sum;
-  }
   } else if (warp < 12) {
     regs_to<kRegsG>();
     // ------------------------------------------------------------ G, and y of the chunk before
@@ -539,132 +572,148 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = 32 * q + lane;
       const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
       const uint32_t sYo = tmem + lanes + kColYo + 32 * half;
-      const float Dh = p.D ? __ldg(p.D + h) : 0.0f;
-      const unsigned long long D2 = pack2(Dh, Dh);
       const bool gated = p.z != nullptr;
-      const long long col = static_cast<long long>(h) * p.dim + p0 + 32 * half;
-      const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + (sg.begin + t) * p.ldz + col;
-      const long long zstep = static_cast<long long>(kQ) * p.ldz;
-      const int rows = static_cast<int>(sg.end - sg.begin);
-      const int wdims = pdims - 32 * half;  // columns of this half
-      for (int c = 0; c <= nc; ++c) {
-        // z's own row for the chunk before, on its way while G is formed
-        uint4 zv[4];
-        if (gated && c > 0) {
-          const uint4* zr = reinterpret_cast<const uint4*>(gz);
-          const int have = (c - 1) * kQ + t < rows ? wdims : 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) zv[i] = 8 * i < have ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
-          gz += zstep;
-        }
-        if (c < nc) {
-          const int b3 = c % 3, s = c & 1;
-          if (!wait_bar<kNapG>(&bars->sc_full[b3], (c / 3) & 1, flag)) break;
-          if (!wait_bar<kNapG>(&bars->s_full[s], (c >> 1) & 1, flag)) break;
-          tc_fence_after_sync();
-          const Scal& sc = scal[b3];
-          const float u = sc.u[t], lt = sc.l[t];
-          const uint32_t sS = tmem + lanes + kColS + s * 128 + 64 * half;
+      const long long zstep = static_cast<long long>(kQ) * p.ldz, ystep = static_cast<long long>(kQ) * p.ldy;
+      const bool wide = p.dim % 16 == 0 && p.ldy % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31) == 0;
+      int cc0 = 0;
+      bool ok = true;
+      for (int it = it0; it < items && ok; it += its) {
+        const Item w = get_item<STATES>(p, it, ptiles);
+        if (w.nc == 0) continue;
+        const float Dh = p.D ? __ldg(p.D + w.h) : 0.0f;
+        const unsigned long long D2 = pack2(Dh, Dh);
+        const long long col = static_cast<long long>(w.h) * p.dim + w.p0 + 32 * half;
+        const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + (w.sg.begin + t) * p.ldz + col;
+        __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + (w.sg.begin + t) * p.ldy + col;
+        const int rows = static_cast<int>(w.sg.end - w.sg.begin);
+        const int wdims = w.pdims - 32 * half;  // columns of this half
 #pragma unroll 1
-          for (int i2 = 0; i2 < 2; ++i2) {
-            const int b = 2 * half + i2;  // block of 32 columns: off the diagonal for b < q
-            uint32_t o[16];
-            if (b <= q) {
-              uint32_t r[32];
-              tmem_ld_32x32b_x32(sS + 32 * i2, r);
-              const unsigned long long* f =
-                  reinterpret_cast<const unsigned long long*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
-              if (b < q) {
-                const unsigned long long u2 = pack2(u, u);
-                tmem_wait_ld();
+        for (int c = 0; c <= w.nc; ++c) {
+          // z's own row for the chunk before, on its way while G is formed
+          uint4 zv[4];
+          if (gated && c > 0) {
+            const uint4* zr = reinterpret_cast<const uint4*>(gz);
+            const int have = (c - 1) * kQ + t < rows ? wdims : 0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const unsigned long long s2 = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                  o[i] = narrow2(mul2(mul2(s2, f[i]), u2));
+            for (int i = 0; i < 4; ++i) zv[i] = 8 * i < have ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
+            gz += zstep;
+          }
+          if (c < w.nc) {
+            const int cc = cc0 + c, b3 = cc % 3, s = cc & 1;
+            ok = wait_bar<kNapG>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
+                 wait_bar<kNapG>(&bars->s_full[s], (cc >> 1) & 1, flag);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const Scal& sc = scal[b3];
+            const float u = sc.u[t], lt = sc.l[t];
+            const uint32_t sS = tmem + lanes + kColS + s * 128 + 64 * half;
+#pragma unroll 1
+            for (int i2 = 0; i2 < 2; ++i2) {
+              const int b = 2 * half + i2;  // block of 32 columns: off the diagonal for b < q
+              uint32_t o[16];
+              if (b <= q) {
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(sS + 32 * i2, r);
+                const unsigned long long* f =
+                    reinterpret_cast<const unsigned long long*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
+                if (b < q) {
+                  const unsigned long long u2 = pack2(u, u);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const unsigned long long s2 = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                    o[i] = narrow2(mul2(mul2(s2, f[i]), u2));
+                  }
+                } else {
+                  const unsigned long long* ls = reinterpret_cast<const unsigned long long*>(sc.l + 32 * b);
+                  const unsigned long long lt2 = pack2(lt, lt), neg = pack2(-1.0f, -1.0f);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    // Columns up to this row.  The factors are formed for all of them and the rest is
+                    // selected away: an exponential inside a condition becomes a branch of its own.
+                    float a, z;
+                    unpack2(fma2(ls[i], neg, lt2), a, z);
+                    const unsigned long long w2 = mul2(pack2(ex2(a), ex2(z)), f[i]);
+                    unpack2(mul2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), w2), a, z);
+                    o[i] = bf16_pair(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f);
+                  }
                 }
               } else {
-                const unsigned long long* ls = reinterpret_cast<const unsigned long long*>(sc.l + 32 * b);
-                const unsigned long long lt2 = pack2(lt, lt), neg = pack2(-1.0f, -1.0f);
-                tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  // Columns up to this row.  The factors are formed for all of them and the rest is
-                  // selected away: an exponential inside a condition becomes a branch of its own.
-                  float a, z;
-                  unpack2(fma2(ls[i], neg, lt2), a, z);
-                  const unsigned long long w2 = mul2(pack2(ex2(a), ex2(z)), f[i]);
-                  unpack2(mul2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), w2), a, z);
-                  o[i] = bf16_pair(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f);
+                for (int i = 0; i < 16; ++i) o[i] = 0;
+              }
+              // these columns of S have been read by this lane already
+              tmem_st_32x32b_x16(sS + 16 * i2, o);
+            }
+            tmem_wait_st();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->g_full[s]);
+          }
+          if (c > 0) {
+            const int d = cc0 + c - 1, b3 = d % 3, s = d & 1;
+            ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag) &&
+                 wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag);
+            if (!ok) break;
+            tc_fence_after_sync();
+            // x's own row for D x, and the tile's place goes back: the next x but one comes
+            // into it, and dS of that chunk waits for it.  (With y leaving through the same
+            // place as a TMA tile that wait was the longest of a chunk's.)
+            const uint8_t* xt = smem + s * L::kStage + stage_x;
+            uint4 xv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) xv[i] = *reinterpret_cast<const uint4*>(xt + swz_offset(t, 4 * half + i, 128));
+            const float e = scal[b3].e[t];
+            const unsigned long long e2 = pack2(e, e);
+            const uint32_t sY = tmem + lanes + kColY + s * kP + 32 * half;
+            const int have = (c - 1) * kQ + t < rows ? wdims : 0;
+            __nv_bfloat16* yr = gy;
+            gy += ystep;
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k) {
+              uint32_t ry[16], ro[16], out[8];
+              tmem_ld_32x32b_x16(sY + 16 * k, ry);
+              tmem_ld_32x32b_x16(sYo + 16 * k, ro);
+              const uint32_t xw[8] = {xv[0].x, xv[0].y, xv[0].z, xv[0].w, xv[1].x, xv[1].y, xv[1].z, xv[1].w};
+              const uint32_t zw[8] = {zv[0].x, zv[0].y, zv[0].z, zv[0].w, zv[1].x, zv[1].y, zv[1].z, zv[1].w};
+              xv[0] = xv[2], xv[1] = xv[3], zv[0] = zv[2], zv[1] = zv[3];
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                unsigned long long v = fma2(e2, pack2(__uint_as_float(ro[2 * i]), __uint_as_float(ro[2 * i + 1])),
+                                            pack2(__uint_as_float(ry[2 * i]), __uint_as_float(ry[2 * i + 1])));
+                v = fma2(D2, widen2(xw[i]), v);
+                if (gated) v = mul2(v, silu2(widen2(zw[i])));
+                out[i] = narrow2(v);
+              }
+              // a lane's own row, whole sectors where rows are aligned to them
+              if (wide && have >= 16 * k + 16) {
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(yr + 16 * k), "r"(out[0]),
+                             "r"(out[1]), "r"(out[2]), "r"(out[3]), "r"(out[4]), "r"(out[5]), "r"(out[6]), "r"(out[7])
+                             : "memory");
+              } else {
+                if (have > 16 * k)
+                  *reinterpret_cast<uint4*>(yr + 16 * k) = make_uint4(out[0], out[1], out[2], out[3]);
+                if (have > 16 * k + 8)
+                  *reinterpret_cast<uint4*>(yr + 16 * k + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+              }
+              if (k == 0) {
+                // Here, where the loaded registers have been used: an arrival does not wait
+                // for loads on their way, and the next tile then overtook them.
+                __syncwarp();
+                if (lane == 0) {
+                  mbar_arrive(&bars->xfree[s]);
+                  mbar_arrive(&bars->sc_free[b3]);
                 }
               }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = 0;
             }
-            // these columns of S have been read by this lane already
-            tmem_st_32x32b_x16(sS + 16 * i2, o);
-          }
-          tmem_wait_st();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->g_full[s]);
-        }
-        if (c > 0) {
-          const int d = c - 1, b3 = d % 3, s = d & 1;
-          // y takes x's place in shared memory, row by row, and leaves as one tile (or by
-          // rows where the chunk ends before the tile)
-          if (!wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag)) break;
-          if (!wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag)) break;
-          tc_fence_after_sync();
-          const float e = scal[b3].e[t];
-          const unsigned long long e2 = pack2(e, e);
-          const uint32_t sY = tmem + lanes + kColY + s * kP + 32 * half;
-          uint8_t* xt = smem + s * L::kStage + stage_x;
-#pragma unroll 1
-          for (int k = 0; k < 2; ++k) {
-            uint32_t ry[16], ro[16], xw[8], zw[8], out[8];
-            tmem_ld_32x32b_x16(sY + 16 * k, ry);
-            tmem_ld_32x32b_x16(sYo + 16 * k, ro);
-            const uint32_t o0 = swz_offset(t, 4 * half + 2 * k, 128), o1 = swz_offset(t, 4 * half + 2 * k + 1, 128);
-            *reinterpret_cast<uint4*>(xw) = *reinterpret_cast<const uint4*>(xt + o0);
-            *reinterpret_cast<uint4*>(xw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
-            if (gated) {
-              *reinterpret_cast<uint4*>(zw) = zv[0];
-              *reinterpret_cast<uint4*>(zw + 4) = zv[1];
-              zv[0] = zv[2];
-              zv[1] = zv[3];
-            }
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              unsigned long long v = fma2(e2, pack2(__uint_as_float(ro[2 * i]), __uint_as_float(ro[2 * i + 1])),
-                                          pack2(__uint_as_float(ry[2 * i]), __uint_as_float(ry[2 * i + 1])));
-              v = fma2(D2, widen2(xw[i]), v);
-              if (gated) v = mul2(v, silu2(widen2(zw[i])));
-              out[i] = narrow2(v);
-            }
-            *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
-            *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
-          }
-          tc_fence_before_sync();
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&bars->yo_free);
-            mbar_arrive(&bars->sc_free[b3]);
-            mbar_arrive(&bars->y_full[s]);
-          }
-          const long long t0 = sg.begin + static_cast<long long>(d) * kQ;
-          // a whole tile is sent off by a warp of the next role
-          if (t0 + kQ > sg.end && t0 + t < sg.end) {
-            // a partial chunk is the last: nothing waits for its x tile
-            __nv_bfloat16* yr = static_cast<__nv_bfloat16*>(p.y) + (t0 + t) * p.ldy + col;
-#pragma unroll 1
-            for (int i = 0; i < 4 && 8 * i < wdims; ++i)
-              *reinterpret_cast<uint4*>(yr + 8 * i) =
-                  *reinterpret_cast<const uint4*>(xt + swz_offset(t, 4 * half + i, 128));
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->yo_free);
           }
         }
+        cc0 += w.nc;
       }
     }
   } else if (warp < 20) {
@@ -672,83 +721,77 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ Xw
     const int s = (threadIdx.x - 384) & 127;     // row
     const int i0 = warp < 16 ? 0 : 4;            // first of this thread's 16-byte pieces
-    // Warp 12 also sends y's tiles off: x of chunk c, which this role waits for, comes
-    // into the place of y of chunk c - 2.
-    auto send_y = [&](int d) {
-      if (!wait_bar<kNapXw>(&bars->y_full[d & 1], (d >> 1) & 1, flag)) return false;
-      if (lane == 0) {
-        tma_store_3d(&maps.y, sbase + (d & 1) * L::kStage + stage_x, p0, h, static_cast<int>(sg.begin) + d * kQ);
-        mbar_arrive(&bars->xfree[d & 1]);
-      }
-      __syncwarp();
-      return true;
-    };
-    const int whole = static_cast<int>((sg.end - sg.begin) / kQ);  // chunks that leave as tiles
+    int cc = 0;
     bool ok = true;
-    for (int c = 0; c < nc; ++c) {
-      const int b3 = c % 3, sb = c & 1;
-      const uint32_t st = sbase + sb * L::kStage;
-      if (!STATES && warp == 12 && c >= 2 && !send_y(c - 2)) {
-        ok = false;
-        break;
-      }
-      const long long left = sg.end - sg.begin - static_cast<long long>(c) * kQ;
-      if (!wait_bar<kNapXw>(&bars->sc_full[b3], (c / 3) & 1, flag)) {
-        ok = false;
-        break;
-      }
-      if (!wait_bar<kNapXw>(&bars->full_x[sb], (c >> 1) & 1, flag)) {
-        ok = false;
-        break;
-      }
-      const float ws = scal[b3].f[3][s];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->sc_free[b3]);
-      if (c >= 1 && !wait_bar<kNapXw>(&bars->ds_full, (c - 1) & 1, flag)) {
-        ok = false;
-        break;
-      }
-      const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
-#pragma unroll 2
-      for (int i = i0; i < i0 + 4; ++i) {
-        const uint32_t off = swz_offset(s, i, 128);
-        const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-        uint32_t vh[4], vl[4];
+    for (int it = it0; it < items && ok; it += its) {
+      const Item w = get_item<STATES>(p, it, ptiles);
+#pragma unroll 1
+      for (int c = 0; c < w.nc; ++c, ++cc) {
+        const int b3 = cc % 3, sb = cc & 1;
+        const uint32_t st = sbase + sb * L::kStage;
+        const int left = static_cast<int>(w.sg.end - w.sg.begin) - c * kQ;
+        ok = wait_bar<kNapXw>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
+             wait_bar<kNapXw>(&bars->full_x[sb], (cc >> 1) & 1, flag);
+        if (!ok) break;
+        const float ws = scal[b3].f[3][s];
+        ok = cc < 1 || wait_bar<kNapXw>(&bars->ds_full, (cc - 1) & 1, flag);
+        if (!ok) break;
+        const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
+        uint32_t vl[16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned long long v = mul2(w2, widen2(xs[k]));
-          vh[k] = narrow2(v);
-          vl[k] = narrow2(fma2(neg, widen2(vh[k]), v));
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t off = swz_offset(s, i0 + i, 128);
+          const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+          uint32_t vh[4], vm[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const unsigned long long v = mul2(w2, widen2(xs[k]));
+            vh[k] = narrow2(v);
+            const unsigned long long r = fma2(neg, widen2(vh[k]), v);
+            vm[k] = narrow2(r);
+            vl[4 * i + k] = narrow2(fma2(neg, widen2(vm[k]), r));
+          }
+          *reinterpret_cast<uint4*>(smem + L::kXw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
+          *reinterpret_cast<uint4*>(smem + L::kXw + kAtom + off) = make_uint4(vm[0], vm[1], vm[2], vm[3]);
         }
-        *reinterpret_cast<uint4*>(smem + L::kXw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
-        *reinterpret_cast<uint4*>(smem + L::kXw + kAtom + off) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
-      }
-      if (left < kQ) {
-        // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-        if (!wait_bar<kNapXw>(&bars->full_b[sb], (c >> 1) & 1, flag)) {
-          ok = false;
-          break;
-        }
-        if (s >= left) {
+        if (left < kQ) {
+          // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
+          ok = wait_bar<kNapXw>(&bars->full_b[sb], (cc >> 1) & 1, flag);
+          if (!ok) break;
+          if (s >= left) {
 #pragma unroll
-          for (int i = i0; i < i0 + 4; ++i) {
-            const uint32_t off = swz_offset(s, i, 128);
-            st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
-            st_shared_v4(sbase + L::kXw + off, 0, 0, 0, 0);
-            st_shared_v4(sbase + L::kXw + kAtom + off, 0, 0, 0, 0);
+            for (int i = 0; i < 16; ++i) vl[i] = 0;
+#pragma unroll 1
+            for (int i = i0; i < i0 + 4; ++i) {
+              const uint32_t off = swz_offset(s, i, 128);
+              st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
+              st_shared_v4(sbase + L::kXw + off, 0, 0, 0, 0);
+              st_shared_v4(sbase + L::kXw + kAtom + off, 0, 0, 0, 0);
 #pragma unroll
-            for (int a = 0; a < NA; ++a) st_shared_v4(st + stage_b + a * kAtom + off, 0, 0, 0, 0);
+              for (int a = 0; a < NA; ++a) st_shared_v4(st + stage_b + a * kAtom + off, 0, 0, 0, 0);
+            }
           }
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->xw_full);
+          mbar_arrive(&bars->sc_free[b3]);
+        }
+        // the third term's place is H's until the chunk before is done
+        if (!STATES) {
+          ok = cc < 1 || wait_bar<kNapXw>(&bars->done[(cc - 1) & 1], ((cc - 1) >> 1) & 1, flag);
+          if (!ok) break;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          st_shared_v4(sbase + L::kH + swz_offset(s, i0 + i, 128), vl[4 * i], vl[4 * i + 1], vl[4 * i + 2], vl[4 * i + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->xl_full);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->xw_full);
     }
-    if (!STATES && warp == 12 && ok)
-      for (int d = nc > 2 ? nc - 2 : 0; d < whole; ++d)
-        if (!send_y(d)) break;
   } else {
     regs_inc<kRegsState>();
     // ------------------------------------------------------------ state
@@ -757,86 +800,101 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool wlive = 32 * q < N;    // this warp has state elements
     const bool live = n < N;
     const uint32_t sD = tmem + (static_cast<uint32_t>(32 * q) << 16) + kColDs;
-    float hv[kP];
+    int cc = 0;
+    bool ok = true;
+    for (int it = it0; it < items && ok; it += its) {
+      const Item w = get_item<STATES>(p, it, ptiles);
+      if (!w.sg.valid) continue;
+      const int slot = (p.state_in || p.state_out) ? seq_slot(p.slots, w.sg.seq, p.nslots, p.status) : -1;
+      const float* in = p.state_in && slot >= 0 ? p.state_in + slot * per_slot + w.head_at : nullptr;
+      float hv[kP];
 #pragma unroll
-    for (int i = 0; i < kP; ++i) hv[i] = 0.0f;
-    // eight rows at a time (pdims is a multiple of 8): more loads in flight would not fit the registers
-    auto add_state = [&](const float* src, float decay) {
-#pragma unroll
-      for (int g8 = 0; g8 < kP / 8; ++g8) {
-        if (live && 8 * g8 < pdims) {
-          const float* at = src + 8 * g8 * N + n;
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = at[i * N];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) hv[8 * g8 + i] = fmaf(hv[8 * g8 + i], decay, v[i]);
-        }
-        asm volatile("" ::: "memory");
-      }
-    };
-    if (!STATES) {
-      // Horner over the earlier segments' final states; the first term is what the sequence starts from
-      const float* src = sg.count == 1 ? in : p.seg_state + (sg.first + sg.count - 1) * per_slot + head_at;
-      const int terms = sg.count > 1 ? 1 + sg.j : in ? 1 : 0;
+      for (int i = 0; i < kP; ++i) hv[i] = 0.0f;
+      // What the state starts from: Horner over the earlier segments' final states, whose
+      // first term is the sequence's own start.  The first launch starts from zero, but
+      // copies the sequence's start into the last segment's place: the second launch
+      // may overwrite it while other segments still need it.
+      const float* src = STATES || w.sg.count == 1
+                             ? in
+                             : p.seg_state + (w.sg.first + w.sg.count - 1) * per_slot + w.head_at;
+      int terms = w.sg.count > 1 ? 1 + w.sg.j : 1;
+      if (STATES) terms = w.last && w.sg.count > 1 ? 1 : 0;
+      if (!src) terms = 0;
 #pragma unroll 1
       for (int k = 0; k < terms; ++k) {
-        const float decay = k ? expf(p.seg_log[static_cast<long long>(sg.first + k - 1) * p.heads + h]) : 0.0f;
-        add_state(src, decay);
-        src = p.seg_state + (sg.first + k) * per_slot + head_at;
-      }
-    }
-    auto put_h = [&]() {
-      if (n < 64 * NA) {
+        const float decay = k ? expf(p.seg_log[static_cast<long long>(w.sg.first + k - 1) * p.heads + w.h]) : 0.0f;
+        // eight rows at a time (pdims is a multiple of 8): more loads in flight would not fit the registers
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          st_shared_v4(sbase + L::kH + swz_offset(n, i, 128), bf16_pair(hv[8 * i], hv[8 * i + 1]),
-                       bf16_pair(hv[8 * i + 2], hv[8 * i + 3]), bf16_pair(hv[8 * i + 4], hv[8 * i + 5]),
-                       bf16_pair(hv[8 * i + 6], hv[8 * i + 7]));
+        for (int g8 = 0; g8 < kP / 8; ++g8) {
+          if (live && 8 * g8 < w.pdims) {
+            const float* at = src + 8 * g8 * N + n;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = at[i * N];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hv[8 * g8 + i] = fmaf(hv[8 * g8 + i], decay, v[i]);
+          }
+          asm volatile("" ::: "memory");
+        }
+        if (k + 1 < terms) src = p.seg_state + (w.sg.first + k) * per_slot + w.head_at;
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->h_full);
-    };
-    bool ok = true;
-    for (int c = 0; c < nc; ++c) {
-      const int b3 = c % 3;
-      if (!STATES) {
-        // the product that reads the old H is done
-        ok = c == 0 || wait_bar<kNapState>(&bars->done[(c - 1) & 1], ((c - 1) >> 1) & 1, flag);
+      float log_sum = 0.0f;
+#pragma unroll 1
+      for (int c = 0; c < w.nc; ++c, ++cc) {
+        const int b3 = cc % 3;
+        ok = wait_bar<kNapState>(&bars->ds_full, cc & 1, flag);
         if (!ok) break;
-        put_h();
-      }
-      ok = wait_bar<kNapState>(&bars->sc_full[b3], (c / 3) & 1, flag);
-      if (!ok) break;
-      const float decay = scal[b3].total;
-      ok = wait_bar<kNapState>(&bars->ds_full, c & 1, flag);
-      if (!ok) break;
-      tc_fence_after_sync();
-      if (wlive) {
+        if (!STATES) {
+          // H, the state before the chunk, where the third term of Xw has been read
+          if (n < 64 * NA) {
 #pragma unroll
-        for (int pc = 0; pc < 4; ++pc) {
-          uint32_t r[16];
-          tmem_ld_32x32b_x16(sD + 16 * pc, r);
-          tmem_wait_ld();
+            for (int i = 0; i < 8; ++i)
+              st_shared_v4(sbase + L::kH + swz_offset(n, i, 128), bf16_pair(hv[8 * i], hv[8 * i + 1]),
+                           bf16_pair(hv[8 * i + 2], hv[8 * i + 3]), bf16_pair(hv[8 * i + 4], hv[8 * i + 5]),
+                           bf16_pair(hv[8 * i + 6], hv[8 * i + 7]));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->h_full);
+        }
+        ok = wait_bar<kNapState>(&bars->sc_full[b3], (cc / 3) & 1, flag);
+        if (!ok) break;
+        const float decay = scal[b3].total;
+        log_sum += scal[b3].log2;
+        const unsigned long long decay2 = pack2(decay, decay);
+        tc_fence_after_sync();
+        if (wlive) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            hv[16 * pc + i] = fmaf(hv[16 * pc + i], decay, __uint_as_float(r[i]));
+          for (int pc = 0; pc < 4; ++pc) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(sD + 16 * pc, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              unpack2(fma2(pack2(hv[16 * pc + 2 * i], hv[16 * pc + 2 * i + 1]), decay2,
+                           pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]))),
+                      hv[16 * pc + 2 * i], hv[16 * pc + 2 * i + 1]);
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->ds_free);
+          mbar_arrive(&bars->sc_free[b3]);
         }
       }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&bars->ds_free);
-        mbar_arrive(&bars->sc_free[b3]);
+      if (!ok) break;
+      float* dst = nullptr;
+      if (STATES) {
+        if (w.sg.count > 1) dst = p.seg_state + w.seg * per_slot + w.head_at;
+        if (n == 0 && w.p0 == 0)
+          p.seg_log[static_cast<long long>(w.seg) * p.heads + w.h] = log_sum * (1.0f / kLog2e);
+      } else if (w.last && p.state_out && slot >= 0) {
+        dst = p.state_out + slot * per_slot + w.head_at;
       }
-    }
-    if (ok) {
-      float* dst = STATES ? p.seg_state + seg * per_slot + head_at
-                          : (last && p.state_out && slot >= 0 ? p.state_out + slot * per_slot + head_at : nullptr);
 #pragma unroll
       for (int g8 = 0; g8 < kP / 8; ++g8) {
-        if (dst && live && 8 * g8 < pdims) {
+        if (dst && live && 8 * g8 < w.pdims) {
           float* at = dst + 8 * g8 * N + n;
 #pragma unroll
           for (int i = 0; i < 8; ++i) at[i * N] = hv[8 * g8 + i];
@@ -850,8 +908,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after_sync();
   if (warp == 1) tmem_dealloc(tmem, kCols);
-  if (STATES && pt == 0 && threadIdx.x == 0)
-    p.seg_log[static_cast<long long>(seg) * p.heads + h] = (seg_sum[0] + seg_sum[1]) * (1.0f / kLog2e);
 }
 
 int make_map(CUtensorMap* m, const void* base, int inner, int mid, long long rows, long long ld, const char* what) {
@@ -872,7 +928,7 @@ int make_map(CUtensorMap* m, const void* base, int inner, int mid, long long row
 }
 
 template <int NA, bool STATES>
-int launch_one(const Tmaps& maps, const ScanParams& p, unsigned grid, int ptiles, cudaStream_t st) {
+int launch_one(const Tmaps& maps, const ScanParams& p, int items, int ptiles, cudaStream_t st) {
   auto kern = scan_umma_kernel<NA, STATES>;
   static std::once_flag once[64];
   int dev = 0;
@@ -882,7 +938,7 @@ int launch_one(const Tmaps& maps, const ScanParams& p, unsigned grid, int ptiles
   if (dev < 64) std::call_once(once[dev], set);
   else set();
   SMM_CUDA_TRY(err, "selective scan shared memory size");
-  kern<<<grid, kThreads, Smem<NA>::kBytes, st>>>(maps, p, ptiles);
+  kern<<<std::min(items, kSms), kThreads, Smem<NA>::kBytes, st>>>(maps, p, items, ptiles);
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "selective scan (tensor core) launch");
   return SMM_OK;
@@ -929,16 +985,15 @@ int scan_umma_launch(ScanParams& p, cudaStream_t st) {
   if (int rc = make_map(&maps.x, p.x, p.dim, p.heads, p.tokens, p.ldx, "x")) return rc;
   if (int rc = make_map(&maps.b, p.B, p.state_dim, p.groups, p.tokens, p.ldb, "B")) return rc;
   if (int rc = make_map(&maps.c, p.C, p.state_dim, p.groups, p.tokens, p.ldc, "C")) return rc;
-  if (int rc = make_map(&maps.y, p.y, p.dim, p.heads, p.tokens, p.ldy, "y")) return rc;
-  const unsigned grid = static_cast<unsigned>(blocks);
+  const int items = static_cast<int>(blocks);
   if (p.state_dim <= 64) {
     if (p.split)
-      if (int rc = launch_one<1, true>(maps, p, grid, ptiles, st)) return rc;
-    return launch_one<1, false>(maps, p, grid, ptiles, st);
+      if (int rc = launch_one<1, true>(maps, p, items, ptiles, st)) return rc;
+    return launch_one<1, false>(maps, p, items, ptiles, st);
   }
   if (p.split)
-    if (int rc = launch_one<2, true>(maps, p, grid, ptiles, st)) return rc;
-  return launch_one<2, false>(maps, p, grid, ptiles, st);
+    if (int rc = launch_one<2, true>(maps, p, items, ptiles, st)) return rc;
+  return launch_one<2, false>(maps, p, items, ptiles, st);
 }
 
 }  // namespace smm
