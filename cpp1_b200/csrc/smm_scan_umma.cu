@@ -34,6 +34,8 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 
 #include "smm_scan.cuh"
 
@@ -46,13 +48,12 @@ namespace {
 constexpr int kQ = 128;         // tokens per chunk
 constexpr int kP = 64;          // dims per CTA
 constexpr int kThreads = 768;
-constexpr int kSms = 148;
 constexpr uint32_t kAtom = kQ * 128;  // one 64-element wide tile of 128 rows: 16 KiB
 // Tensor memory columns.  S is 128 wide and double; G takes the place of the first
 // quarter and the third one of S, each written by the warps that have read its half.
 constexpr uint32_t kColS = 0, kColY = 256, kColDs = 384, kColYo = 448, kCols = 512;
 
-constexpr int kNapLoad = 100, kNapMma = 20, kNapDecay = 32, kNapG = 32, kNapXw = 32, kNapState = 32;
+constexpr int kNapLoad = 32, kNapMma = 20, kNapDecay = 100, kNapG = 32, kNapXw = 32, kNapState = 32;
 
 struct Scal {
   float f[4][kQ];  // f[b-1][s], b = 1..4
@@ -107,25 +108,39 @@ __device__ __forceinline__ uint32_t elect_one() {
       "{\n\t.reg .pred p;\n\t.reg .b32 t;\n\telect.sync t|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
   return r;
 }
-// Descriptors are given as two words: only the low one (the start address) changes.
+// Descriptors are given as two words; a step's offset is added to the low one (the start
+// address) inside, so that the compiler keeps no register for each step of each product.
+// Unrolled: in a loop, a product took 65 to 80 cycles to issue, here 28.
+template <uint32_t OA, uint32_t OB, bool ACC>
 __device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
-                                        uint32_t b_hi, uint32_t idesc, int acc) {
+                                        uint32_t b_hi, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
-      "setp.ne.b32 p, %7, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 da, db;\n\t"
+      "add.u32 x, %1, %7;\n\tadd.u32 y, %3, %8;\n\tmov.b64 da, {x, %2};\n\tmov.b64 db, {y, %4};\n\t"
+      "setp.ne.b32 p, %9, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}\n" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "r"(acc)
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "n"(OA), "n"(OB), "n"(ACC ? 1 : 0)
       : "memory");
 }
 // A from tensor memory (bf16, two per column), B from shared memory
+template <uint32_t OA, uint32_t OB, bool ACC>
 __device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
-                                        uint32_t idesc, int acc) {
+                                        uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %3};\n\t"
-      "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}\n" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 x, y;\n\t.reg .b64 db;\n\t"
+      "add.u32 x, %1, %6;\n\tadd.u32 y, %2, %7;\n\tmov.b64 db, {y, %3};\n\t"
+      "setp.ne.b32 p, %8, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [x], db, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(leader), "n"(OA), "n"(OB), "n"(ACC ? 1 : 0)
       : "memory");
+}
+template <int... K, typename F>
+__device__ __forceinline__ void steps_of(std::integer_sequence<int, K...>, F&& f) {
+  (f(std::integral_constant<int, K>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void steps(F&& f) {
+  steps_of(std::make_integer_sequence<int, N>{}, f);
 }
 __device__ __forceinline__ void umma_commit_by(uint32_t leader, uint64_t* bar) {
   asm volatile(
@@ -143,12 +158,13 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits of all roles but the two below: every one of them depends on loads or
-// products still to come, so the loading and the issuing warp keep the time, and
-// raise the flag for all.  (The code of a dozen timers is what instruction fetches
-// have no room for.)
+// Waits of all roles.  A sleep follows every fruitless try: the tries return at once, and
+// a dozen waiting warps' loops would take issue slots from those that compute.  Every
+// wait depends on loads or products still to come, so the warp that issues the products
+// keeps the time (TIMED), and raises the flag for all: the code of a dozen timers is
+// what instruction fetches have no room for.
 template <int NS>
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const volatile int* abort_flag) {
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const ScanParams& p, volatile int* abort_flag) {
   const uint32_t a = smem_u32(bar);
   while (!mbar_try_wait(a, parity)) {
     __nanosleep(NS);
@@ -156,23 +172,6 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const v
   }
   return true;
 }
-// Time since the first of a run of fruitless polls; true once the limit has passed
-// or another role has given up.
-struct Patience {
-  uint64_t t0 = 0;
-  uint32_t idle = 0;
-  __device__ __forceinline__ void progress() { idle = 0; }
-  __device__ __forceinline__ bool out(const ScanParams& p, volatile int* abort_flag, uint32_t where) {
-    if ((++idle & 255u) != 0) return false;  // the timer is slow to read
-    if (*abort_flag) return true;
-    const uint64_t t = globaltimer_ns();
-    if (idle == 256u) t0 = t;
-    if (t - t0 <= p.wait_limit_ns) return false;
-    *abort_flag = 1;
-    if (p.status) atomicOr(p.status, kDevErrTimeout | where);
-    return true;
-  }
-};
 // Until what has been issued has landed; gives up (for all) after the limit, a second at least.
 __device__ __forceinline__ void drain_bar(uint64_t* bar, uint32_t parity, const ScanParams& p, volatile int* abort_flag) {
   const uint32_t a = smem_u32(bar);
@@ -311,78 +310,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_dec<kRegsMisc>();
     if (warp == 0) {
       // ---------------------------------------------------------- loads
-      // B is free after dS, C after all products of its chunk, x after the y that took
-      // its place has left.  Each goes through the items at its own pace.
+      // in the order in which the places become free: B after dS, C after all products of
+      // its chunk, x after its part in y
       int n_b = 0, n_c = 0, n_x = 0;  // loads issued
-      Patience time;
-      auto free_at = [&](uint64_t* bar, int cc) {
-        return cc < 2 || __any_sync(0xFFFFFFFFu, mbar_test(bar + (cc & 1), ((cc >> 1) - 1) & 1));
-      };
-      struct Walk {
-        int it, left, row, h, p0;  // chunks left of the item, next row
-      };
-      auto enter = [&](Walk& k) {
-        const Item w = get_item<STATES>(p, k.it, ptiles);
-        k.left = w.nc;
-        k.row = static_cast<int>(w.sg.begin);
-        k.h = w.h;
-        k.p0 = w.p0;
-      };
-      // on to the next item when this one is through; whether there is a chunk
-      auto settle = [&](Walk& k) {
-        while (k.left == 0 && k.it < items) {
-          k.it += its;
-          if (k.it < items) enter(k);
-        }
-        return k.it < items;
-      };
-      Walk b{it0, 0, 0, 0, 0};
-      if (it0 < items) enter(b);
-      bool more_b = settle(b), more_x = more_b, more_c = !STATES && more_b;
-      Walk x = b, cw = b;
       const int per_group = p.heads / p.groups;
-      while (more_b || more_x || more_c) {
-        bool did = false;
-        if (more_b && free_at(bars->bfree, n_b)) {
-          const int s = n_b & 1, g = b.h / per_group;
+      bool ok = true;
+      for (int it = it0; it < items && ok; it += its) {
+        const Item w = get_item<STATES>(p, it, ptiles);
+        const int g = w.h / per_group;
+        int row = static_cast<int>(w.sg.begin);
+#pragma unroll 1
+        for (int c = 0; c < w.nc; ++c, row += kQ) {
+          const int s = n_b & 1;
+          const uint32_t st = sbase + s * L::kStage, par = ((n_b >> 1) - 1) & 1;
+          const bool first = n_b < 2;
+          ok = first || wait_bar<kNapLoad>(&bars->bfree[s], par, p, flag);
+          if (!ok) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(&bars->full_b[s], NA * kAtom);
 #pragma unroll
             for (int a = 0; a < NA; ++a)
-              tma_load_3d(sbase + s * L::kStage + stage_b + a * kAtom, &maps.b, &bars->full_b[s], a * 64, g, b.row);
+              tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_b[s], a * 64, g, row);
           }
-          ++n_b, --b.left, b.row += kQ;
-          more_b = settle(b);
-          did = true;
-        }
-        if (more_x && free_at(STATES ? bars->bfree : bars->xfree, n_x)) {
-          const int s = n_x & 1;
+          ++n_b;
+          if (!STATES) {
+            ok = first || wait_bar<kNapLoad>(&bars->done[s], par, p, flag);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&bars->full_c[s], NA * kAtom);
+#pragma unroll
+              for (int a = 0; a < NA; ++a)
+                tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_c[s], a * 64, g, row);
+            }
+            ++n_c;
+            ok = first || wait_bar<kNapLoad>(&bars->xfree[s], par, p, flag);
+            if (!ok) break;
+          }
           if (lane == 0) {
             mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
-            tma_load_3d(sbase + s * L::kStage + stage_x, &maps.x, &bars->full_x[s], x.p0, x.h, x.row);
+            tma_load_3d(st + stage_x, &maps.x, &bars->full_x[s], w.p0, w.h, row);
           }
-          ++n_x, --x.left, x.row += kQ;
-          more_x = settle(x);
-          did = true;
+          ++n_x;
         }
-        if (more_c && free_at(bars->done, n_c)) {
-          const int s = n_c & 1, g = cw.h / per_group;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars->full_c[s], NA * kAtom);
-#pragma unroll
-            for (int a = 0; a < NA; ++a)
-              tma_load_3d(sbase + s * L::kStage + stage_c + a * kAtom, &maps.c, &bars->full_c[s], a * 64, g, cw.row);
-          }
-          ++n_c, --cw.left, cw.row += kQ;
-          more_c = settle(cw);
-          did = true;
-        }
-        if (did)
-          time.progress();
-        else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitProducer)))
-          break;
-        else
-          __nanosleep(kNapLoad);
       }
       // after an abort, copies in flight land before the CTA leaves
       if (*flag && lane == 0) {
@@ -398,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idS = make_idesc(kFmtBF16, 128, 128, 0, 0);
       constexpr uint32_t idY = make_idesc(kFmtBF16, 128, kP, 0, 1);
       constexpr uint32_t idD = make_idesc(kFmtBF16, 128, kP, 1, 1);
-      const int ksteps = (N + 15) / 16;
+      const uint32_t ksteps = (N + 15) / 16;
       const uint32_t leader = elect_one();
       int total = 0;
       for (int it = it0; it < items; it += its) total += get_item<STATES>(p, it, ptiles).nc;
@@ -410,83 +379,92 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t dM = make_smem_desc(sbase, kAtom, 1024, kLayoutSw128);  // MN-major
       const uint32_t hK = static_cast<uint32_t>(dK >> 32), hM = static_cast<uint32_t>(dM >> 32);
       auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xFFFFFFFFu, mbar_test(bar, parity)) != 0; };
-      // terms k0 .. k1 - 1 (of 8 steps each) of dS = B^T Xw
-      auto ds_steps = [&](int s, int k0, int k1) {
+      // one of the three terms of dS = B^T Xw
+      auto ds_term = [&](int s, auto tc) {
+        constexpr uint32_t term = decltype(tc)::value * (kAtom >> 4);
+        constexpr bool more = decltype(tc)::value > 0;
         const uint32_t base = lo(dM) + s * kSt;
-#pragma unroll 2
-        for (int k = k0; k < k1; ++k)
-          umma_ss(leader, tmem + kColDs, base + (stage_b >> 4) + (k & 7) * 128, hM, lo(dM) + (L::kXw >> 4) + k * 128, hM,
-                  idD, k);
+        steps<8>([&](auto kc) {
+          constexpr uint32_t k = decltype(kc)::value;
+          umma_ss<(stage_b >> 4) + k * 128, (L::kXw >> 4) + term + k * 128, more || (k > 0)>(leader, tmem + kColDs, base,
+                                                                                          hM, lo(dM), hM, idD);
+        });
       };
-      int s_next = STATES ? total : 0, g_next = 0, sub = 0;
-      Patience time;
-      while (g_next < total) {
-        bool did = false;
-        if (!STATES && s_next < total && s_next < g_next + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
+      // Whatever has its operands: S up to a chunk ahead of the rest (the order fixed at its
+      // usual one, with blocking waits, was a tenth slower).
+      int s_next = STATES ? total : 0, cc = 0, sub = 0;
+      uint32_t idle = 0;
+      uint64_t t0 = 0;
+      while (cc < total) {
+        bool did = true;
+        const int s = cc & 1;
+        const uint32_t par = (cc >> 1) & 1;
+        if (!STATES && s_next < total && s_next < cc + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
             ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1)) {
-          // C was loaded once every product of chunk c - 2 was done: S's place, where its G was, is free
+          // C was loaded once every product of chunk cc - 2 was done: S's place, where its G was, is free
           tc_fence_after_sync();
-          const int s = s_next & 1;
-          const uint32_t base = lo(dK) + s * kSt;
-#pragma unroll 2
-          for (int k = 0; k < ksteps; ++k) {
-            const uint32_t off = base + (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
-            umma_ss(leader, tmem + kColS + s * 128, off + (stage_c >> 4), hK, off + (stage_b >> 4), hK, idS, k);
-          }
-          umma_commit_by(leader, &bars->s_full[s]);
+          const int sn = s_next & 1;
+          const uint32_t base = lo(dK) + sn * kSt;
+          steps<4 * NA>([&](auto kc) {
+            constexpr uint32_t k = decltype(kc)::value, off = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
+            if (k < ksteps)
+              umma_ss<(stage_c >> 4) + off, (stage_b >> 4) + off, (k > 0)>(leader, tmem + kColS + sn * 128, base, hK, base,
+                                                                           hK, idS);
+          });
+          umma_commit_by(leader, &bars->s_full[sn]);
           ++s_next;
-          did = true;
-        } else if (STATES || g_next < s_next) {
-          const int cc = g_next, s = cc & 1;
-          const uint32_t par = (cc >> 1) & 1;
-          if (sub == 0) {
-            if (ready(&bars->xw_full, cc & 1) && (cc == 0 || ready(&bars->ds_free, (cc - 1) & 1)) &&
-                ready(&bars->full_b[s], par) && ready(&bars->full_x[s], par)) {
-              tc_fence_after_sync();
-              ds_steps(s, 0, 16);
-              sub = 1;
-              did = true;
+        } else if (sub == 0 && ready(&bars->xw_full, cc & 1) && (cc == 0 || ready(&bars->ds_free, (cc - 1) & 1)) &&
+                   ready(&bars->full_b[s], par) && ready(&bars->full_x[s], par)) {
+          tc_fence_after_sync();
+          ds_term(s, std::integral_constant<int, 0>{});
+          ds_term(s, std::integral_constant<int, 1>{});
+          sub = 1;
+        } else if (sub == 1 && ready(&bars->xl_full, cc & 1)) {
+          tc_fence_after_sync();
+          ds_term(s, std::integral_constant<int, 2>{});
+          umma_commit_by(leader, &bars->ds_full);
+          umma_commit_by(leader, &bars->bfree[s]);
+          sub = 2;
+          if (STATES) sub = 0, ++cc;
+        } else if (sub == 2 && ready(&bars->g_full[s], par)) {
+          tc_fence_after_sync();
+          const uint32_t base = lo(dM) + s * kSt;
+          steps<8>([&](auto kc) {
+            constexpr uint32_t k = decltype(kc)::value;
+            umma_ts<(k >> 2) * 64 + (k & 3) * 8, (stage_x >> 4) + k * 128, (k > 0)>(
+                leader, tmem + kColY + s * kP, tmem + kColS + s * 128, base, hM, idY);
+          });
+          sub = 3;
+        } else if (sub == 3 && ready(&bars->h_full, cc & 1) && (cc == 0 || ready(&bars->yo_free, (cc - 1) & 1))) {
+          tc_fence_after_sync();
+          const uint32_t base = lo(dK) + s * kSt;
+          steps<4 * NA>([&](auto kc) {
+            constexpr uint32_t k = decltype(kc)::value, off = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
+            if (k < ksteps)
+              umma_ss<(stage_c >> 4) + off, (L::kH >> 4) + k * 128, (k > 0)>(leader, tmem + kColYo, base, hK, lo(dM), hM,
+                                                                            idY);
+          });
+          umma_commit_by(leader, &bars->done[s]);
+          sub = 0;
+          ++cc;
+        } else {
+          did = false;
+        }
+        if (did) {
+          idle = 0;
+        } else {
+          __nanosleep(kNapMma);
+          if ((++idle & 255u) == 0) {  // the timer is slow to read
+            if (__any_sync(0xFFFFFFFFu, *flag != 0)) break;
+            const uint64_t now = globaltimer_ns();
+            if (idle == 256u) t0 = now;
+            if (__any_sync(0xFFFFFFFFu, now - t0 > p.wait_limit_ns)) {
+              *flag = 1;
+              if (p.status && lane == 0) atomicOr(p.status, kDevErrTimeout | kWaitMma);
+              break;
             }
-          } else if (sub == 1) {
-            if (ready(&bars->xl_full, cc & 1)) {
-              tc_fence_after_sync();
-              ds_steps(s, 16, 24);
-              umma_commit_by(leader, &bars->ds_full);
-              umma_commit_by(leader, &bars->bfree[s]);
-              sub = 2;
-              if (STATES) sub = 0, ++g_next;
-              did = true;
-            }
-          } else if (sub == 2) {
-            if (ready(&bars->g_full[s], par)) {
-              tc_fence_after_sync();
-              const uint32_t base = lo(dM) + s * kSt;
-#pragma unroll 2
-              for (int k = 0; k < 8; ++k)
-                umma_ts(leader, tmem + kColY + s * kP, tmem + kColS + s * 128 + (k >> 2) * 64 + (k & 3) * 8,
-                        base + (stage_x >> 4) + k * 128, hM, idY, k);
-              sub = 3;
-              did = true;
-            }
-          } else if (ready(&bars->h_full, cc & 1) && (cc == 0 || ready(&bars->yo_free, (cc - 1) & 1))) {
-            tc_fence_after_sync();
-            const uint32_t base = lo(dK) + s * kSt;
-#pragma unroll 2
-            for (int k = 0; k < ksteps; ++k)
-              umma_ss(leader, tmem + kColYo, base + (stage_c >> 4) + (k >> 2) * (kAtom >> 4) + (k & 3) * 2, hK,
-                      lo(dM) + (L::kH >> 4) + k * 128, hM, idY, k);
-            umma_commit_by(leader, &bars->done[s]);
-            sub = 0;
-            ++g_next;
-            did = true;
           }
         }
-        if (did)
-          time.progress();
-        else if (__any_sync(0xFFFFFFFFu, time.out(p, flag, kWaitMma)))
-          break;
-        else
-          __nanosleep(kNapMma);
       }
       // every product has completed, and its arrivals have landed, before the CTA leaves
       umma_commit_by(leader, &bars->drain);
@@ -513,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c = first; c < w.nc; c += 2) {
           const int cc = cc0 + c, b3 = cc % 3;
-          ok = cc < 3 || wait_bar<kNapDecay>(&bars->sc_free[b3], (cc / 3 - 1) & 1, flag);
+          ok = cc < 3 || wait_bar<kNapDecay>(&bars->sc_free[b3], (cc / 3 - 1) & 1, p, flag);
           if (!ok) break;
           Scal& sc = scal[b3];
           const long long left = w.sg.end - w.sg.begin - static_cast<long long>(c) * kQ - lane;
@@ -573,8 +551,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t lanes = static_cast<uint32_t>(32 * q) << 16;
       const uint32_t sYo = tmem + lanes + kColYo + 32 * half;
       const bool gated = p.z != nullptr;
-      const long long zstep = static_cast<long long>(kQ) * p.ldz, ystep = static_cast<long long>(kQ) * p.ldy;
-      const bool wide = p.dim % 16 == 0 && p.ldy % 16 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 31) == 0;
+      const long long zstep = 8 * p.ldz, ystep = 8 * p.ldy;  // eight rows
+      const int col8 = 8 * (lane & 3);
       int cc0 = 0;
       bool ok = true;
       for (int it = it0; it < items && ok; it += its) {
@@ -583,25 +561,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float Dh = p.D ? __ldg(p.D + w.h) : 0.0f;
         const unsigned long long D2 = pack2(Dh, Dh);
         const long long col = static_cast<long long>(w.h) * p.dim + w.p0 + 32 * half;
-        const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + (w.sg.begin + t) * p.ldz + col;
-        __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + (w.sg.begin + t) * p.ldy + col;
+        const long long row = w.sg.begin + 32 * q + (lane >> 2);
+        const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + row * p.ldz + col + col8;
+        __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + row * p.ldy + col + col8;
         const int rows = static_cast<int>(w.sg.end - w.sg.begin);
         const int wdims = w.pdims - 32 * half;  // columns of this half
 #pragma unroll 1
         for (int c = 0; c <= w.nc; ++c) {
-          // z's own row for the chunk before, on its way while G is formed
+          // z of the chunk before, on its way while G is formed: four lanes to the 64 bytes of
+          // a row, eight rows at a time
           uint4 zv[4];
+          const int r0 = (c - 1) * kQ + 32 * q + (lane >> 2);  // this lane's first row in the segment
           if (gated && c > 0) {
-            const uint4* zr = reinterpret_cast<const uint4*>(gz);
-            const int have = (c - 1) * kQ + t < rows ? wdims : 0;
+            const __nv_bfloat16* zr = gz;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) zv[i] = 8 * i < have ? __ldg(zr + i) : make_uint4(0, 0, 0, 0);
-            gz += zstep;
+            for (int i = 0; i < 4; ++i, zr += zstep)
+              zv[i] = col8 < wdims && r0 + 8 * i < rows ? __ldg(reinterpret_cast<const uint4*>(zr))
+                                                        : make_uint4(0, 0, 0, 0);
+            gz = zr + 12 * zstep;
           }
           if (c < w.nc) {
             const int cc = cc0 + c, b3 = cc % 3, s = cc & 1;
-            ok = wait_bar<kNapG>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
-                 wait_bar<kNapG>(&bars->s_full[s], (cc >> 1) & 1, flag);
+            ok = wait_bar<kNapG>(&bars->sc_full[b3], (cc / 3) & 1, p, flag) &&
+                 wait_bar<kNapG>(&bars->s_full[s], (cc >> 1) & 1, p, flag);
             if (!ok) break;
             tc_fence_after_sync();
             const Scal& sc = scal[b3];
@@ -653,31 +635,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (c > 0) {
             const int d = cc0 + c - 1, b3 = d % 3, s = d & 1;
-            ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag) &&
-                 wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag);
+            ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, p, flag) &&
+                 wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, p, flag);
             if (!ok) break;
             tc_fence_after_sync();
-            // x's own row for D x, and the tile's place goes back: the next x but one comes
-            // into it, and dS of that chunk waits for it.  (With y leaving through the same
-            // place as a TMA tile that wait was the longest of a chunk's.)
-            const uint8_t* xt = smem + s * L::kStage + stage_x;
+            // x's own row for D x.  Its place then takes z and after that y on their way between
+            // the layout of global memory and a row to a lane (a lane's own row of z and y
+            // to and from global memory touched four times the lines).
+            uint8_t* xt = smem + s * L::kStage + stage_x;
             uint4 xv[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) xv[i] = *reinterpret_cast<const uint4*>(xt + swz_offset(t, 4 * half + i, 128));
             const float e = scal[b3].e[t];
             const unsigned long long e2 = pack2(e, e);
             const uint32_t sY = tmem + lanes + kColY + s * kP + 32 * half;
-            const int have = (c - 1) * kQ + t < rows ? wdims : 0;
-            __nv_bfloat16* yr = gy;
-            gy += ystep;
+            __syncwarp();
+            if (gated) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint4*>(xt + swz_offset(32 * q + 8 * i + (lane >> 2), 4 * half + (lane & 3), 128)) = zv[i];
+              __syncwarp();
+            }
 #pragma unroll 1
             for (int k = 0; k < 2; ++k) {
-              uint32_t ry[16], ro[16], out[8];
+              uint32_t ry[16], ro[16], out[8], zw[8];
               tmem_ld_32x32b_x16(sY + 16 * k, ry);
               tmem_ld_32x32b_x16(sYo + 16 * k, ro);
+              const uint32_t o0 = swz_offset(t, 4 * half + 2 * k, 128), o1 = swz_offset(t, 4 * half + 2 * k + 1, 128);
               const uint32_t xw[8] = {xv[0].x, xv[0].y, xv[0].z, xv[0].w, xv[1].x, xv[1].y, xv[1].z, xv[1].w};
-              const uint32_t zw[8] = {zv[0].x, zv[0].y, zv[0].z, zv[0].w, zv[1].x, zv[1].y, zv[1].z, zv[1].w};
-              xv[0] = xv[2], xv[1] = xv[3], zv[0] = zv[2], zv[1] = zv[3];
+              xv[0] = xv[2], xv[1] = xv[3];
+              if (gated) {
+                *reinterpret_cast<uint4*>(zw) = *reinterpret_cast<const uint4*>(xt + o0);
+                *reinterpret_cast<uint4*>(zw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
+              }
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
@@ -687,30 +677,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (gated) v = mul2(v, silu2(widen2(zw[i])));
                 out[i] = narrow2(v);
               }
-              // a lane's own row, whole sectors where rows are aligned to them
-              if (wide && have >= 16 * k + 16) {
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(yr + 16 * k), "r"(out[0]),
-                             "r"(out[1]), "r"(out[2]), "r"(out[3]), "r"(out[4]), "r"(out[5]), "r"(out[6]), "r"(out[7])
-                             : "memory");
-              } else {
-                if (have > 16 * k)
-                  *reinterpret_cast<uint4*>(yr + 16 * k) = make_uint4(out[0], out[1], out[2], out[3]);
-                if (have > 16 * k + 8)
-                  *reinterpret_cast<uint4*>(yr + 16 * k + 8) = make_uint4(out[4], out[5], out[6], out[7]);
-              }
-              if (k == 0) {
-                // Here, where the loaded registers have been used: an arrival does not wait
-                // for loads on their way, and the next tile then overtook them.
-                __syncwarp();
-                if (lane == 0) {
-                  mbar_arrive(&bars->xfree[s]);
-                  mbar_arrive(&bars->sc_free[b3]);
-                }
-              }
+              *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
+              *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i, gy += ystep)
+              if (col8 < wdims && r0 + 8 * i < rows)
+                *reinterpret_cast<uint4*>(gy) =
+                    *reinterpret_cast<const uint4*>(xt + swz_offset(32 * q + 8 * i + (lane >> 2), 4 * half + (lane & 3), 128));
+            gy += 12 * ystep;
+            fence_proxy_async_smem();  // the tile's next content comes by TMA
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->yo_free);
+            if (lane == 0) {
+              mbar_arrive(&bars->yo_free);
+              mbar_arrive(&bars->xfree[s]);
+              mbar_arrive(&bars->sc_free[b3]);
+            }
           }
         }
         cc0 += w.nc;
@@ -730,11 +714,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b3 = cc % 3, sb = cc & 1;
         const uint32_t st = sbase + sb * L::kStage;
         const int left = static_cast<int>(w.sg.end - w.sg.begin) - c * kQ;
-        ok = wait_bar<kNapXw>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
-             wait_bar<kNapXw>(&bars->full_x[sb], (cc >> 1) & 1, flag);
+        ok = wait_bar<kNapXw>(&bars->sc_full[b3], (cc / 3) & 1, p, flag) &&
+             wait_bar<kNapXw>(&bars->full_x[sb], (cc >> 1) & 1, p, flag);
         if (!ok) break;
         const float ws = scal[b3].f[3][s];
-        ok = cc < 1 || wait_bar<kNapXw>(&bars->ds_full, (cc - 1) & 1, flag);
+        ok = cc < 1 || wait_bar<kNapXw>(&bars->ds_full, (cc - 1) & 1, p, flag);
         if (!ok) break;
         const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
         uint32_t vl[16];
@@ -757,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (left < kQ) {
           // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-          ok = wait_bar<kNapXw>(&bars->full_b[sb], (cc >> 1) & 1, flag);
+          ok = wait_bar<kNapXw>(&bars->full_b[sb], (cc >> 1) & 1, p, flag);
           if (!ok) break;
           if (s >= left) {
 #pragma unroll
@@ -781,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the third term's place is H's until the chunk before is done
         if (!STATES) {
-          ok = cc < 1 || wait_bar<kNapXw>(&bars->done[(cc - 1) & 1], ((cc - 1) >> 1) & 1, flag);
+          ok = cc < 1 || wait_bar<kNapXw>(&bars->done[(cc - 1) & 1], ((cc - 1) >> 1) & 1, p, flag);
           if (!ok) break;
         }
 #pragma unroll
@@ -842,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < w.nc; ++c, ++cc) {
         const int b3 = cc % 3;
-        ok = wait_bar<kNapState>(&bars->ds_full, cc & 1, flag);
+        ok = wait_bar<kNapState>(&bars->ds_full, cc & 1, p, flag);
         if (!ok) break;
         if (!STATES) {
           // H, the state before the chunk, where the third term of Xw has been read
@@ -857,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->h_full);
         }
-        ok = wait_bar<kNapState>(&bars->sc_full[b3], (cc / 3) & 1, flag);
+        ok = wait_bar<kNapState>(&bars->sc_full[b3], (cc / 3) & 1, p, flag);
         if (!ok) break;
         const float decay = scal[b3].total;
         log_sum += scal[b3].log2;
@@ -938,7 +922,7 @@ int launch_one(const Tmaps& maps, const ScanParams& p, int items, int ptiles, cu
   if (dev < 64) std::call_once(once[dev], set);
   else set();
   SMM_CUDA_TRY(err, "selective scan shared memory size");
-  kern<<<std::min(items, kSms), kThreads, Smem<NA>::kBytes, st>>>(maps, p, items, ptiles);
+  kern<<<items, kThreads, Smem<NA>::kBytes, st>>>(maps, p, items, ptiles);
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "selective scan (tensor core) launch");
   return SMM_OK;
