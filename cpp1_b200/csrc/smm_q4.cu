@@ -203,16 +203,16 @@ __global__ void __launch_bounds__(NT == 1 ? 1024 : 512, 1) q4_kernel(const Q4Par
     if (c_first < c_end) fetch(c_first);
   }
   if constexpr (XS) {
-    for (int n = 0; n < nx; ++n) {
-      const T* row = static_cast<const T*>(p.x) + (b0 + n) * p.ldx;
+    // over rows and words alike, so that four loads of a thread are in flight
+    const int all = nx * words;
 #pragma unroll 4
-      for (int w = threadIdx.x; w < words; w += blockDim.x) {
-        XWord<T> x;
-        x.load(row + 8 * w);
+    for (int i = threadIdx.x; i < all; i += blockDim.x) {
+      const int n = i / words, w = i - n * words;
+      XWord<T> x;
+      x.load(static_cast<const T*>(p.x) + (b0 + n) * p.ldx + 8 * w);
 #pragma unroll
-        for (int part = 0; part < kParts; ++part)
-          sx[(((w / (4 * V) * V + w % V) * kParts + part) * nb + n) * 4 + w / V % 4] = x.b[part];
-      }
+      for (int part = 0; part < kParts; ++part)
+        sx[(((w / (4 * V) * V + w % V) * kParts + part) * nb + n) * 4 + w / V % 4] = x.b[part];
     }
     __syncthreads();
   }

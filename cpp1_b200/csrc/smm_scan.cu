@@ -4,6 +4,7 @@
 #include "smm_scan.cuh"
 
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 namespace smm {
@@ -16,20 +17,20 @@ using F2 = unsigned long long;  // two fp32 lanes
 // not reach) and for shapes the tensor-core kernel does not take.  Three
 // packed multiply-adds per two state elements and token; bound by their issue.
 //
-// A CTA holds the states of one head and 8 dims per warp in registers: lane
-// (pg, ng) has 2 dims x NPL state elements, in 16-byte pieces strided by the 8
+// A CTA holds the states of one head and 4 PPL dims per warp in registers: lane
+// (pg, ng) has PPL dims x NPL state elements, in 16-byte pieces strided by the 8
 // lanes ng so that reading B and C from shared memory has no bank conflict and
 // each value serves four lanes.  Tokens pass in tiles of 16: the next tile's B, C,
 // x, z and dt are loaded into registers while the present one is computed, four
-// tokens at a time, whose eight sums over the lanes ng are made together.  (Token by
+// tokens at a time, whose sums over the lanes ng are made together.  (Token by
 // token, the chain of one token's sum and its shuffles showed: 4096 tokens of 64
 // heads of 64 x 128 took 1.21 ms.)
 constexpr int kTile = 16;
 
-template <typename T, int NPL, int THREADS, bool STATES>
+template <typename T, int NPL, int THREADS, int PPL, bool STATES>
 __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int ptiles) {
   constexpr int NP = 8 * NPL;                  // padded state_dim
-  constexpr int PT = THREADS / 4;              // dims per CTA
+  constexpr int PT = THREADS / 8 * PPL;        // dims per CTA
   constexpr int NE = kTile * NP / THREADS > 0 ? kTile * NP / THREADS : 1;
   constexpr int XE = kTile * PT / THREADS;     // 4
   constexpr int CH = NPL >= 4 ? 4 : 2;         // consecutive state elements of a lane
@@ -56,7 +57,8 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
   if (!sg.valid) return;
   const int g = h / (p.heads / p.groups);
   const int p0 = pt * PT;
-  const int pl = p0 + warp * 8 + pg * 2;       // this lane's first dim
+  const int pw = warp * 4 * PPL + pg * PPL;    // this lane's first dim in the CTA's
+  const int pl = p0 + pw;
   const int N = p.state_dim;
   const float A = __ldg(p.A + h);
   const bool last = sg.j == sg.count - 1;
@@ -69,14 +71,14 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
   const long long per_slot = static_cast<long long>(p.heads) * p.dim * N;
 
   // state before the segment
-  float hv[2][NPL];
+  float hv[PPL][NPL];
 #pragma unroll
-  for (int pp = 0; pp < 2; ++pp)
+  for (int pp = 0; pp < PPL; ++pp)
 #pragma unroll
     for (int i = 0; i < NPL; ++i) hv[pp][i] = 0.0f;
   auto add_state = [&](const float* src, float decay) {
 #pragma unroll
-    for (int pp = 0; pp < 2; ++pp)
+    for (int pp = 0; pp < PPL; ++pp)
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         const int n = n_of(i / CH, i % CH);
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
   };
   auto put_state = [&](float* dst) {
 #pragma unroll
-    for (int pp = 0; pp < 2; ++pp)
+    for (int pp = 0; pp < PPL; ++pp)
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         const int n = n_of(i / CH, i % CH);
@@ -111,9 +113,9 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
       add_state(p.seg_state + (sg.first + k) * per_slot,
                 expf(p.seg_log[static_cast<long long>(sg.first + k) * p.heads + h]));
   }
-  F2 hst[2][NPL / 2];
+  F2 hst[PPL][NPL / 2];
 #pragma unroll
-  for (int pp = 0; pp < 2; ++pp)
+  for (int pp = 0; pp < PPL; ++pp)
 #pragma unroll
     for (int i = 0; i < NPL / 2; ++i) hst[pp][i] = pack2(hv[pp][2 * i], hv[pp][2 * i + 1]);
 
@@ -181,14 +183,18 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
     if (more) fetch(t0 + kTile);
 #pragma unroll 1
     for (int t = 0; t < nt; t += 4) {  // tokens behind the last one do nothing: decay 1, d 0
-      float ys[8];                     // [token][dim]
+      float ys[4 * PPL];               // [token][dim]
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float2 ad = sad[t + u];
-        const float2 xv = *reinterpret_cast<const float2*>(sx + (t + u) * PT + warp * 8 + pg * 2);
         const F2 a2 = pack2(ad.x, ad.x);
-        const F2 d0 = pack2(xv.x * ad.y, xv.x * ad.y), d1 = pack2(xv.y * ad.y, xv.y * ad.y);
-        F2 y0 = pack2(0.0f, 0.0f), y1 = y0;
+        F2 d[PPL], y[PPL][2];
+#pragma unroll
+        for (int pp = 0; pp < PPL; ++pp) {
+          const float dx = sx[(t + u) * PT + pw + pp] * ad.y;
+          d[pp] = pack2(dx, dx);
+          y[pp][0] = y[pp][1] = pack2(0.0f, 0.0f);
+        }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           F2 b[CH / 2], cc[CH / 2];
@@ -203,31 +209,35 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
 #pragma unroll
           for (int q = 0; q < CH / 2; ++q) {
             const int k = c * (CH / 2) + q;
-            hst[0][k] = fma2(hst[0][k], a2, mul2(d0, b[q]));
-            hst[1][k] = fma2(hst[1][k], a2, mul2(d1, b[q]));
-            if constexpr (!STATES) {
-              y0 = fma2(hst[0][k], cc[q], y0);
-              y1 = fma2(hst[1][k], cc[q], y1);
+#pragma unroll
+            for (int pp = 0; pp < PPL; ++pp) {
+              hst[pp][k] = fma2(hst[pp][k], a2, mul2(d[pp], b[q]));
+              if constexpr (!STATES) y[pp][q] = fma2(hst[pp][k], cc[q], y[pp][q]);
             }
           }
         }
-        float lo, hi;
-        unpack2(y0, lo, hi);
-        ys[2 * u] = lo + hi;
-        unpack2(y1, lo, hi);
-        ys[2 * u + 1] = lo + hi;
+        if constexpr (!STATES) {
+#pragma unroll
+          for (int pp = 0; pp < PPL; ++pp) {
+            float lo, hi;
+            unpack2(add2(y[pp][0], y[pp][1]), lo, hi);
+            ys[PPL * u + pp] = lo + hi;
+          }
+        }
       }
       if constexpr (!STATES) {
-        // sums over the 8 lanes ng, of which lane ng keeps the one of token ng / 2, dim ng % 2
-        float s4[4], s2[2];
+        // sums over the 8 lanes ng, of which lane ng keeps the one of token ng / 2 (and dim ng % 2)
+        constexpr int H = 2 * PPL, Q = PPL;
+        float s4[H], s2[Q];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s4[i] = ((ng & 4) ? ys[4 + i] : ys[i]) + __shfl_xor_sync(0xFFFFFFFFu, (ng & 4) ? ys[i] : ys[4 + i], 4);
+        for (int i = 0; i < H; ++i)
+          s4[i] = ((ng & 4) ? ys[H + i] : ys[i]) + __shfl_xor_sync(0xFFFFFFFFu, (ng & 4) ? ys[i] : ys[H + i], 4);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          s2[i] = ((ng & 2) ? s4[2 + i] : s4[i]) + __shfl_xor_sync(0xFFFFFFFFu, (ng & 2) ? s4[i] : s4[2 + i], 2);
-        const float sum = ((ng & 1) ? s2[1] : s2[0]) + __shfl_xor_sync(0xFFFFFFFFu, (ng & 1) ? s2[0] : s2[1], 1);
-        sy[(t + (ng >> 1)) * PT + warp * 8 + pg * 2 + (ng & 1)] = sum;
+        for (int i = 0; i < Q; ++i)
+          s2[i] = ((ng & 2) ? s4[Q + i] : s4[i]) + __shfl_xor_sync(0xFFFFFFFFu, (ng & 2) ? s4[i] : s4[Q + i], 2);
+        const float mine = (PPL == 2 && (ng & 1)) ? s2[Q - 1] : s2[0];
+        const float sum = mine + __shfl_xor_sync(0xFFFFFFFFu, (PPL == 2 && !(ng & 1)) ? s2[Q - 1] : s2[0], 1);
+        if (PPL == 2 || !(ng & 1)) sy[(t + (ng >> 1)) * PT + pw + (PPL == 2 ? (ng & 1) : 0)] = sum;
       }
     }
     __syncthreads();
@@ -249,7 +259,7 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
     __syncthreads();
   }
 #pragma unroll
-  for (int pp = 0; pp < 2; ++pp)
+  for (int pp = 0; pp < PPL; ++pp)
 #pragma unroll
     for (int i = 0; i < NPL / 2; ++i) unpack2(hst[pp][i], hv[pp][2 * i], hv[pp][2 * i + 1]);
   if constexpr (STATES) {
@@ -264,19 +274,19 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
   }
 }
 
-template <typename T, int NPL, int THREADS>
+template <typename T, int NPL, int THREADS, int PPL>
 int launch_scan(const ScanParams& p, long long segs, cudaStream_t st) {
-  constexpr int NP = 8 * NPL, PT = THREADS / 4;
+  constexpr int NP = 8 * NPL, PT = THREADS / 8 * PPL;
   const int ptiles = (p.dim + PT - 1) / PT;
   const long long blocks = segs * p.heads * ptiles;
   if (blocks > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "selective scan too large for one launch");
   const unsigned grid = static_cast<unsigned>(blocks);
   const size_t full = sizeof(float) * kTile * (2 * NP + 2 * PT + 2);
   if (p.split) {
-    scan_kernel<T, NPL, THREADS, true><<<grid, THREADS, full, st>>>(p, ptiles);
+    scan_kernel<T, NPL, THREADS, PPL, true><<<grid, THREADS, full, st>>>(p, ptiles);
     count_launch();
   }
-  scan_kernel<T, NPL, THREADS, false><<<grid, THREADS, full, st>>>(p, ptiles);
+  scan_kernel<T, NPL, THREADS, PPL, false><<<grid, THREADS, full, st>>>(p, ptiles);
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "selective scan launch");
   return SMM_OK;
@@ -286,9 +296,13 @@ template <typename T>
 int launch_scan_type(const ScanParams& p, long long segs, cudaStream_t st) {
   auto go = [&](auto npl) {
     constexpr int NPL = decltype(npl)::value;
-    // 32 dims to a CTA where 64 would leave SMs without one (or a head has no more)
-    const bool small = p.dim <= 32 || segs * p.heads * ((p.dim + 63) / 64) < 2 * 148;
-    return small ? launch_scan<T, NPL, 128>(p, segs, st) : launch_scan<T, NPL, 256>(p, segs, st);
+    // Two dims to a lane read B and C half as often; one makes twice the warps, which is
+    // faster while there are few (38 -> 36 us for 390 warps of two dims, but 0.79 ->
+    // 0.91 ms for 512 that run eight times as long).  Then 32 dims to a CTA where 64
+    // would leave SMs without one.
+    if (segs * p.heads * ((p.dim + 7) / 8) < 400) return launch_scan<T, NPL, 256, 1>(p, segs, st);
+    if (p.dim <= 32 || segs * p.heads * ((p.dim + 63) / 64) < 2 * 148) return launch_scan<T, NPL, 128, 2>(p, segs, st);
+    return launch_scan<T, NPL, 256, 2>(p, segs, st);
   };
   if (p.state_dim <= 16) return go(std::integral_constant<int, 2>{});
   if (p.state_dim <= 32) return go(std::integral_constant<int, 4>{});
@@ -299,90 +313,250 @@ int launch_scan_type(const ScanParams& p, long long segs, cudaStream_t st) {
 
 // ------------------------------------------------------------ one token
 // S = exp(d A) S + d x (outer) B, y = S C: the state is read once and written
-// once (8 bytes per element against 5 operations), which bounds it.  A warp takes
-// whole rows of the state (16 bytes per lane; several rows side by side where
-// state_dim is short), four at a time so that their loads are in flight
-// together, before anything that depends on dt is computed.
-constexpr int kStepThreads = 128;
-constexpr int kStepRows = 4;  // rows in flight per lane
+// once (8 bytes per element against 5 operations), which bounds it.  A row of the
+// state takes LANES lanes with 16 bytes each (twice where NV is 2).  A warp walks a
+// run of tiles of 4 KB, a few rows of one head each, its lanes copying their own
+// pieces up to two tiles ahead into shared memory (cp.async: no register holds them,
+// and as a lane reads back only what it copied, no barrier is needed).  671 MB of
+// states take 122 us, 85 % of a copy's rate; a short CTA for every few rows, which
+// waits for slot, states, then dt, B and C, took 164 us, and 4.5 instead of 4.1 for
+// 4 MB.  Sums over a row's lanes are made for all rows together: 9 exchanges, not 40
+// (122 us against 149, with two tiles of loads in flight and x and z one tile ahead).
+constexpr int kStepThreads = 256, kStepCtas = 2, kStepStages = 3, kStepTile = 4096;
+constexpr int kStepSmem = kStepThreads / 32 * kStepStages * kStepTile;
 
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, int lanes, int rows_per_cta,
-                                                            int ptiles) {
+template <typename T, int LANES, int NV>
+__global__ void __launch_bounds__(kStepThreads, kStepCtas) step_kernel(const ScanParams p, int tph,
+                                                                       long long tiles) {
+  constexpr int R = kStepTile / 512 / NV;         // rows of a lane in a tile, LANES lanes to a row
+  constexpr int H = R < LANES ? R : LANES;        // lanes that end with sums of their own
+  constexpr int KEEP = R / H, SHARE = LANES / H;  // rows of each, lanes with the same ones
+  constexpr int rstep = 32 / LANES;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 31, sub = lane % LANES, row0 = lane / LANES, mine = sub / SHARE * KEEP;
+  const int N = p.state_dim, per_group = p.heads / p.groups;
+  const long long warp = static_cast<long long>(blockIdx.x) * (kStepThreads / 32) + (threadIdx.x >> 5);
+  const long long warps = static_cast<long long>(gridDim.x) * (kStepThreads / 32);
+  const long long t0 = tiles * warp / warps, t1 = tiles * (warp + 1) / warps;
+  if (t0 >= t1) return;
+  float4* const ring = reinterpret_cast<float4*>(smem + (threadIdx.x >> 5) * kStepStages * kStepTile) + lane;
+  constexpr int kPieces = kStepTile / 16;
+
+  struct Place {
+    int b, h, pt, slot;
+  };
+  auto place = [&](long long t) {
+    Place c;
+    c.pt = static_cast<int>(t % tph);
+    const long long hb = t / tph;
+    c.h = static_cast<int>(hb % p.heads);
+    c.b = static_cast<int>(hb / p.heads);
+    c.slot = seq_slot(p.slots, c.b, p.nslots, p.status);
+    return c;
+  };
+  auto advance = [&](Place& c, bool live) {
+    if (++c.pt < tph) return;
+    c.pt = 0;
+    if (++c.h < p.heads) return;
+    c.h = 0;
+    ++c.b;
+    if (live) c.slot = seq_slot(p.slots, c.b, p.nslots, p.status);
+  };
+  auto state_at = [&](const Place& c) {
+    return (static_cast<long long>(c.slot) * p.heads + c.h) * p.dim * N;
+  };
+  Place ahead = place(t0), cur = ahead;
+  int fill = 0;
+  auto issue = [&](long long t) {
+    if (t < t1) {
+      const float* in = p.state_in && ahead.slot >= 0 ? p.state_in + state_at(ahead) : nullptr;
+      float4* dst = ring + fill * kPieces;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int q = ahead.pt * R * rstep + r * rstep + row0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int n = (k * LANES + sub) * 4;
+          if (in && q < p.dim && n < N)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + (r * NV + k) * 32)),
+                         "l"(in + static_cast<long long>(q) * N + n)
+                         : "memory");
+          else
+            dst[(r * NV + k) * 32] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+      fill = fill + 1 == kStepStages ? 0 : fill + 1;
+      advance(ahead, t + 1 < t1);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStepStages - 1; ++i) issue(t0 + i);
+
+  // x and z of the rows that this lane finishes, one tile ahead
+  T xn[KEEP], zn[KEEP];
+  auto load_xz = [&](const Place& c) {
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int q = (c.pt * R + mine + i) * rstep + row0;
+      const long long col = static_cast<long long>(c.h) * p.dim + q;
+      xn[i] = zn[i] = from_f32<T>(0.0f);
+      if (q < p.dim) xn[i] = static_cast<const T*>(p.x)[c.b * p.ldx + col];
+      if (q < p.dim && p.z) zn[i] = static_cast<const T*>(p.z)[c.b * p.ldz + col];
+    }
+  };
+  load_xz(cur);
+  float bv[NV][4], cv[NV][4], d = 0.0f, a = 0.0f, Dh = 0.0f;
+  int stage = 0;
+  for (long long t = t0; t < t1; ++t) {
+    issue(t + kStepStages - 1);
+    float xs[KEEP], zs[KEEP];
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) xs[i] = to_f32(xn[i]), zs[i] = to_f32(zn[i]);
+    if (t == t0 || cur.pt == 0) {
+      const int g = cur.h / per_group;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = (k * LANES + sub) * 4 + i;
+          const long long col = static_cast<long long>(g) * N + n;
+          bv[k][i] = n < N ? to_f32(static_cast<const T*>(p.B)[cur.b * p.ldb + col]) : 0.0f;
+          cv[k][i] = n < N ? to_f32(static_cast<const T*>(p.C)[cur.b * p.ldc + col]) : 0.0f;
+        }
+      d = scan_dt(p, scan_dt_raw(p, cur.b, cur.h), p.dt_bias ? __ldg(p.dt_bias + cur.h) : 0.0f);
+      a = expf(d * __ldg(p.A + cur.h));
+      Dh = p.D ? __ldg(p.D + cur.h) : 0.0f;
+    }
+    const Place at = cur;
+    advance(cur, t + 1 < t1);
+    if (t + 1 < t1) load_xz(cur);
+    float* out = p.state_out && at.slot >= 0 ? p.state_out + state_at(at) : nullptr;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStepStages - 1) : "memory");
+    const float4* src = ring + stage * kPieces;
+    float ys[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int q = (at.pt * R + r) * rstep + row0;
+      const float dx = d * __shfl_sync(0xFFFFFFFFu, xs[r % KEEP], row0 * LANES + r / KEEP * SHARE);
+      float y = 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int n = (k * LANES + sub) * 4;
+        float4 f = src[(r * NV + k) * 32];
+        f.x = fmaf(f.x, a, dx * bv[k][0]), f.y = fmaf(f.y, a, dx * bv[k][1]);
+        f.z = fmaf(f.z, a, dx * bv[k][2]), f.w = fmaf(f.w, a, dx * bv[k][3]);
+        y = fmaf(f.x, cv[k][0], y), y = fmaf(f.y, cv[k][1], y);
+        y = fmaf(f.z, cv[k][2], y), y = fmaf(f.w, cv[k][3], y);
+        if (out && q < p.dim && n < N) __stcs(reinterpret_cast<float4*>(out + static_cast<long long>(q) * N + n), f);
+      }
+      ys[r] = y;
+    }
+    // Sums over the LANES lanes of all rows together: each exchange halves the rows
+    // of a lane, then the lanes that share a row add up.
+    int o = LANES / 2;
+#pragma unroll
+    for (int half = R / 2; half >= KEEP; half /= 2, o /= 2) {
+      const bool up = sub & o;
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const float got = __shfl_xor_sync(0xFFFFFFFFu, up ? ys[i] : ys[i + half], o);
+        ys[i] = (up ? ys[i + half] : ys[i]) + got;
+      }
+    }
+#pragma unroll
+    for (; o > 0; o /= 2) ys[0] += __shfl_xor_sync(0xFFFFFFFFu, ys[0], o);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      const int q = (at.pt * R + mine + i) * rstep + row0;
+      if (sub % SHARE != 0 || q >= p.dim) continue;
+      float y = fmaf(Dh, xs[i], ys[i]);
+      if (p.z) y *= silu(zs[i]);
+      static_cast<T*>(p.y)[at.b * p.ldy + static_cast<long long>(at.h) * p.dim + q] = from_f32<T>(y);
+    }
+    stage = stage + 1 == kStepStages ? 0 : stage + 1;
+  }
+}
+
+template <typename T, int LANES, int NV>
+int launch_step_tiles(const ScanParams& p, long long heads, cudaStream_t st) {
+  auto kern = step_kernel<T, LANES, NV>;
+  constexpr int rows = kStepTile / 512 / NV * (32 / LANES);
+  const int tph = (p.dim + rows - 1) / rows;
+  static std::once_flag once[64];
+  int dev = 0;
+  SMM_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
+  cudaError_t err = cudaSuccess;
+  auto set = [&] { err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStepSmem); };
+  if (dev < 64) std::call_once(once[dev], set);
+  else set();
+  SMM_CUDA_TRY(err, "selective step shared memory size");
+  const int grid = static_cast<int>(std::min<long long>(heads * tph, kStepCtas * 148));
+  kern<<<grid, kStepThreads, kStepSmem, st>>>(p, tph, heads * tph);
+  count_launch();
+  SMM_CUDA_TRY(cudaGetLastError(), "selective step launch");
+  return SMM_OK;
+}
+
+
+// Any other state_dim, one element at a time.
+constexpr int kOddThreads = 128, kOddRows = 4;
+template <typename T, int NV>
+__global__ void __launch_bounds__(kOddThreads) step_odd_kernel(const ScanParams p, int lanes, int rows_per_cta,
+                                                                int ptiles) {
   const int pt = static_cast<int>(blockIdx.x % ptiles);
   const int hb = static_cast<int>(blockIdx.x / ptiles);
   const int h = hb % p.heads, b = hb / p.heads;
   const int g = h / (p.heads / p.groups);
   const int N = p.state_dim;
-  const int sub = threadIdx.x % lanes, row0 = threadIdx.x / lanes, rstep = kStepThreads / lanes;
+  const int sub = threadIdx.x % lanes, row0 = threadIdx.x / lanes, rstep = kOddThreads / lanes;
   const int slot = seq_slot(p.slots, b, p.nslots, p.status);
   const long long base = (static_cast<long long>(slot) * p.heads + h) * p.dim * N;
   const float* in = p.state_in && slot >= 0 ? p.state_in + base : nullptr;
   float* out = p.state_out && slot >= 0 ? p.state_out + base : nullptr;
   const int pend = (pt + 1) * rows_per_cta < p.dim ? (pt + 1) * rows_per_cta : p.dim;
 
-  float hv[kStepRows][NV][VEC], xv[kStepRows], bv[NV][VEC], cv[NV][VEC];
+  float hv[kOddRows][NV], xv[kOddRows], bv[NV], cv[NV];
   auto load_rows = [&](int r0) {
 #pragma unroll
-    for (int r = 0; r < kStepRows; ++r) {
+    for (int r = 0; r < kOddRows; ++r) {
       const int q = r0 + r * rstep;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int n = (k * lanes + sub) * VEC;
-        if (in && q < pend && n < N) {
-          if constexpr (VEC == 4) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(in + static_cast<long long>(q) * N + n));
-            hv[r][k][0] = f.x, hv[r][k][1] = f.y, hv[r][k][2] = f.z, hv[r][k][3] = f.w;
-          } else {
-            hv[r][k][0] = in[static_cast<long long>(q) * N + n];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) hv[r][k][i] = 0.0f;
-        }
+        const int n = k * lanes + sub;
+        hv[r][k] = in && q < pend && n < N ? in[static_cast<long long>(q) * N + n] : 0.0f;
       }
     }
 #pragma unroll
-    for (int r = 0; r < kStepRows; ++r) {
+    for (int r = 0; r < kOddRows; ++r) {
       const int q = r0 + r * rstep;
       xv[r] = q < pend ? to_f32(static_cast<const T*>(p.x)[b * p.ldx + static_cast<long long>(h) * p.dim + q]) : 0.0f;
     }
   };
   load_rows(pt * rows_per_cta + row0);
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int n = (k * lanes + sub) * VEC + i;
-      bv[k][i] = n < N ? to_f32(static_cast<const T*>(p.B)[b * p.ldb + static_cast<long long>(g) * N + n]) : 0.0f;
-      cv[k][i] = n < N ? to_f32(static_cast<const T*>(p.C)[b * p.ldc + static_cast<long long>(g) * N + n]) : 0.0f;
-    }
+  for (int k = 0; k < NV; ++k) {
+    const int n = k * lanes + sub;
+    bv[k] = n < N ? to_f32(static_cast<const T*>(p.B)[b * p.ldb + static_cast<long long>(g) * N + n]) : 0.0f;
+    cv[k] = n < N ? to_f32(static_cast<const T*>(p.C)[b * p.ldc + static_cast<long long>(g) * N + n]) : 0.0f;
+  }
   const float d = scan_dt(p, scan_dt_raw(p, b, h), p.dt_bias ? __ldg(p.dt_bias + h) : 0.0f);
   const float a = expf(d * __ldg(p.A + h));
   const float Dh = p.D ? __ldg(p.D + h) : 0.0f;
   // every thread of the CTA makes the same number of turns (the shuffles)
-  for (int base_row = pt * rows_per_cta; base_row < pend; base_row += kStepRows * rstep) {
+  for (int base_row = pt * rows_per_cta; base_row < pend; base_row += kOddRows * rstep) {
     if (base_row != pt * rows_per_cta) load_rows(base_row + row0);
 #pragma unroll
-    for (int r = 0; r < kStepRows; ++r) {
+    for (int r = 0; r < kOddRows; ++r) {
       const int q = base_row + row0 + r * rstep;
       const float dx = d * xv[r];
       float y = 0.0f;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          hv[r][k][i] = fmaf(hv[r][k][i], a, dx * bv[k][i]);
-          y = fmaf(hv[r][k][i], cv[k][i], y);
-        }
-        const int n = (k * lanes + sub) * VEC;
-        if (out && q < pend && n < N) {
-          if constexpr (VEC == 4)
-            __stcs(reinterpret_cast<float4*>(out + static_cast<long long>(q) * N + n),
-                   make_float4(hv[r][k][0], hv[r][k][1], hv[r][k][2], hv[r][k][3]));
-          else
-            out[static_cast<long long>(q) * N + n] = hv[r][k][0];
-        }
+        hv[r][k] = fmaf(hv[r][k], a, dx * bv[k]);
+        y = fmaf(hv[r][k], cv[k], y);
+        const int n = k * lanes + sub;
+        if (out && q < pend && n < N) out[static_cast<long long>(q) * N + n] = hv[r][k];
       }
       for (int o = lanes >> 1; o > 0; o >>= 1) y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
       if (sub == 0 && q < pend) {
@@ -397,25 +571,23 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const ScanParams p, 
 
 template <typename T>
 int launch_step(const ScanParams& p, int batch, cudaStream_t st) {
-  const bool vec = p.state_dim % 4 == 0 && aligned_to(p.state_in, 16) && aligned_to(p.state_out, 16);
-  const int pieces = vec ? p.state_dim / 4 : p.state_dim;
+  const long long heads = static_cast<long long>(batch) * p.heads;
+  if (p.state_dim % 4 == 0 && p.state_dim > 8 && aligned_to(p.state_in, 16) && aligned_to(p.state_out, 16)) {
+    if (p.state_dim <= 16) return launch_step_tiles<T, 4, 1>(p, heads, st);
+    if (p.state_dim <= 32) return launch_step_tiles<T, 8, 1>(p, heads, st);
+    if (p.state_dim <= 64) return launch_step_tiles<T, 16, 1>(p, heads, st);
+    return p.state_dim <= 128 ? launch_step_tiles<T, 32, 1>(p, heads, st) : launch_step_tiles<T, 32, 2>(p, heads, st);
+  }
   int lanes = 1;
-  while (lanes < 32 && lanes < pieces) lanes *= 2;
-  const int nv = (pieces + lanes - 1) / lanes;
-  // one round of rows per CTA: the most CTAs, and the shortest wait for one token
-  const int rows = kStepRows * kStepThreads / lanes;
+  while (lanes < 32 && lanes < p.state_dim) lanes *= 2;
+  const int rows = kOddRows * kOddThreads / lanes;
   const int ptiles = (p.dim + rows - 1) / rows;
-  const long long blocks = static_cast<long long>(batch) * p.heads * ptiles;
-  if (blocks > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "selective step too large for one launch");
-  const unsigned grid = static_cast<unsigned>(blocks);
-  if (vec && nv == 1)
-    step_kernel<T, 4, 1><<<grid, kStepThreads, 0, st>>>(p, lanes, rows, ptiles);
-  else if (vec)
-    step_kernel<T, 4, 2><<<grid, kStepThreads, 0, st>>>(p, lanes, rows, ptiles);
-  else if (nv == 1)
-    step_kernel<T, 1, 1><<<grid, kStepThreads, 0, st>>>(p, lanes, rows, ptiles);
+  if (heads * ptiles > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "selective step too large for one launch");
+  const unsigned grid = static_cast<unsigned>(heads * ptiles);
+  if (p.state_dim <= 32)
+    step_odd_kernel<T, 1><<<grid, kOddThreads, 0, st>>>(p, lanes, rows, ptiles);
   else
-    step_kernel<T, 1, 8><<<grid, kStepThreads, 0, st>>>(p, lanes, rows, ptiles);
+    step_odd_kernel<T, 8><<<grid, kOddThreads, 0, st>>>(p, lanes, rows, ptiles);
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "selective step launch");
   return SMM_OK;

@@ -930,13 +930,23 @@ int launch_one(const Tmaps& maps, const ScanParams& p, int items, int ptiles, cu
 
 }  // namespace
 
-// bf16, whole 16-byte pieces everywhere, state_dim of one 128-row tile, and prompts
-// long enough that tiles of 128 tokens are not mostly empty.
+// bf16, whole 16-byte pieces everywhere, state_dim of one 128-row tile, and sequences
+// long enough.  Time here goes with the chunks, a started one counting in full, and on
+// the fp32 pipes with tokens * dim * (state_dim + 40).  For many sequences of dim 64 the
+// two cross near 42 tokens each with state_dim 128 (32 sequences of 64 heads, fp32 pipes
+// against this kernel: 188 and 200 us at 40 tokens, 280 and 203 at 64) and near 125 with
+// state_dim 16 (87 and 198 us at 64; 227 and 91 us for 4 of 1024).  While the CTAs fit
+// the GPU at once this kernel's one chunk is 10 us, and they cross earlier (one sequence,
+// state_dim 128: 11.8 and 9.9 us at 24 tokens, 32 and 10 at 128).
 bool scan_umma_fits(const ScanParams& p, int dtype) {
-  return dtype == SMM_DTYPE_BF16 && p.dim % 8 == 0 && p.state_dim % 8 == 0 && p.state_dim <= 128 && p.ldx % 8 == 0 &&
-         p.ldb % 8 == 0 && p.ldc % 8 == 0 && p.ldy % 8 == 0 && (!p.z || p.ldz % 8 == 0) && aligned_to(p.x, 16) &&
-         aligned_to(p.B, 16) && aligned_to(p.C, 16) && aligned_to(p.y, 16) && aligned_to(p.z, 16) &&
-         p.tokens >= 16LL * p.nseq;
+  if (dtype != SMM_DTYPE_BF16 || p.dim % 8 || p.state_dim % 8 || p.state_dim > 128) return false;
+  if (p.ldx % 8 || p.ldb % 8 || p.ldc % 8 || p.ldy % 8 || (p.z && p.ldz % 8)) return false;
+  if (!aligned_to(p.x, 16) || !aligned_to(p.B, 16) || !aligned_to(p.C, 16) || !aligned_to(p.y, 16) ||
+      !aligned_to(p.z, 16))
+    return false;
+  const long long ptiles = (p.dim + kP - 1) / kP;
+  const long long item = 1LL * p.nseq * p.heads * ptiles <= 148 ? 2500 : 7000;
+  return p.tokens * (p.state_dim + 40) * p.dim >= p.nseq * item * kP * ptiles;
 }
 
 // Segment length of the tensor-core kernel: whole chunks, so that the waves of
