@@ -385,6 +385,63 @@ def test_step_matches_definition(cuda, dtype, batch, h, p, g_, n):
     assert torch.equal(keep, pool)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("batch,h,p,g_,n", [(60, 64, 64, 8, 128), (70, 48, 50, 2, 100), (40, 64, 40, 1, 200), (150, 40, 64, 1, 16),
+                                            (50, 64, 72, 4, 36), (3, 300, 64, 1, 64), (90, 64, 33, 1, 45)])
+def test_step_over_many_tiles(cuda, dtype, batch, h, p, g_, n):
+    """States that every warp walks several tiles of, some without a slot."""
+    a = make_scan(batch + n, batch, h, p, g_, n, dtype)
+    pool = rnd(gen(n), batch, h, p, n)
+    keep = pool.clone()
+    slots = torch.randperm(batch, generator=torch.Generator().manual_seed(1))
+    slots[batch // 2] = -1
+    st = pool[slots]
+    st[batch // 2] = 0
+    ref, mag, (fin, fmag) = scan_ref(a, list(range(batch + 1)), st)
+    y = ops.selective_step(**a, state=pool, slots=i32(slots.tolist()))
+    within(y, ref, scan_tol(ref, mag, n, 1, TYPES[dtype], False), "y")
+    live = slots >= 0
+    within(pool[slots[live]], fin[live], state_tol(fin[live], fmag[live], 1, False), "state")
+    keep[slots[live]] = pool[slots[live]]
+    assert torch.equal(keep, pool)
+
+
+@pytest.mark.parametrize("dtype,lens,h,g_,n,gate", [
+    ("bf16", [700, 37, 260], 160, 8, 128, True), ("bf16", [130, 900, 1, 0, 128], 200, 1, 64, False),
+    ("bf16", [60] * 40, 24, 3, 128, True), ("bf16", [9] * 30, 64, 1, 16, True), ("bf16", [300] * 6, 64, 1, 16, True),
+    ("fp32", [500, 37, 130], 160, 8, 128, True), ("fp32", [200] * 5, 64, 2, 64, False), ("fp32", [400], 16, 1, 128, True)])
+def test_scan_on_every_sm_repeats_itself(cuda, dtype, lens, h, g_, n, gate):
+    """All SMs at work, several items to each: right, and the same bits every time."""
+    b = offs(lens)
+    a = make_scan(h + n, b[-1], h, 64, g_, n, dtype, z=gate)
+    st = rnd(gen(h), len(lens), h, 64, n)
+    ref, mag, (fin, fmag) = scan_ref(a, b, st)
+    so = torch.empty_like(st)
+    y = ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so)
+    tensor = dtype == "bf16"
+    within(y, ref, scan_tol(ref, mag, n, max(lens), TYPES[dtype], tensor), "y")
+    within(so, fin, state_tol(fin, fmag, max(lens), tensor), "state")
+    for _ in range(20):
+        so2 = torch.empty_like(st)
+        y2 = ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so2)
+        assert torch.equal(y2, y) and torch.equal(so2, so)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,channels,width", [([3, 130, 64, 1, 0, 65, 7000], 4352, 4), ([4000, 63, 65, 2500, 500], 4400, 8),
+                                                 ([7129], 4354, 2)])
+def test_conv_long_runs(cuda, dtype, lens, channels, width):
+    dt = TYPES[dtype]
+    g = gen(channels)
+    b = offs(lens)
+    x, w, bias = rnd(g, b[-1], channels, dtype=dt), rnd(g, channels, width, dtype=dt), rnd(g, channels, dtype=dt)
+    st = rnd(g, len(lens), channels, width - 1, dtype=dt)
+    ref, mag, final = conv_ref(x, w, bias, b, st, True)
+    y = ops.causal_conv(x, w, bias, offsets=i32(b), state=st)
+    within(y, ref, conv_tol(ref, mag, width, dt), "y")
+    assert torch.equal(st.double(), final)
+
+
 def test_step_bad_slot_is_reported(cuda):
     a = make_scan(1, 3, 2, 16, 1, 8, "fp32")
     st = rnd(gen(1), 3, 2, 16, 8)
