@@ -22,17 +22,19 @@ using F2 = unsigned long long;  // two fp32 lanes
 // lanes ng so that reading B and C from shared memory has no bank conflict and
 // each value serves four lanes.  Tokens pass in tiles of 16: the next tile's B, C,
 // x, z and dt are loaded into registers while the present one is computed, four
-// tokens at a time, whose sums over the lanes ng are made together.  (Token by
-// token, the chain of one token's sum and its shuffles showed: 4096 tokens of 64
-// heads of 64 x 128 took 1.21 ms.)
+// tokens at a time, whose sums over the lanes ng are made together: 4096 tokens of 64
+// heads of 64 x 128 take 0.77 ms.  (Token by token, the chain of one token's sum and its
+// shuffles showed: 1.21 ms.)
 constexpr int kTile = 16;
 
+// bf16 comes here with short sequences, whose start and end want a second CTA on the SM
+// (16 tokens of 64 heads, 32 sequences: 188 -> 121 us); fp32 wants the registers.
 template <typename T, int NPL, int THREADS, int PPL, bool STATES>
-__global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int ptiles) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 512 / THREADS : 1) scan_kernel(const ScanParams p, int ptiles) {
   constexpr int NP = 8 * NPL;                  // padded state_dim
   constexpr int PT = THREADS / 8 * PPL;        // dims per CTA
   constexpr int NE = kTile * NP / THREADS > 0 ? kTile * NP / THREADS : 1;
-  constexpr int XE = kTile * PT / THREADS;     // 4
+  constexpr int XE = kTile * PT / THREADS;
   constexpr int CH = NPL >= 4 ? 4 : 2;         // consecutive state elements of a lane
   constexpr int NC = NPL / CH;
   extern __shared__ float sm[];
@@ -76,13 +78,15 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
   for (int pp = 0; pp < PPL; ++pp)
 #pragma unroll
     for (int i = 0; i < NPL; ++i) hv[pp][i] = 0.0f;
-  auto add_state = [&](const float* src, float decay) {
+  // (a multiply-add to zero where a load would do: with the plain load the compiler
+  // schedules the whole loop differently, and 4096 tokens of 64 heads take 0.87 ms, not 0.77)
+  auto get_state = [&](const float* src) {
 #pragma unroll
     for (int pp = 0; pp < PPL; ++pp)
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         const int n = n_of(i / CH, i % CH);
-        if (pl + pp < p.dim && n < N) hv[pp][i] = fmaf(hv[pp][i], decay, src[state_at(pp, n)]);
+        if (pl + pp < p.dim && n < N) hv[pp][i] = fmaf(hv[pp][i], 0.0f, src[state_at(pp, n)]);
       }
   };
   auto put_state = [&](float* dst) {
@@ -100,18 +104,15 @@ __global__ void __launch_bounds__(THREADS) scan_kernel(const ScanParams p, int p
     // second launch may overwrite it while other segments still need it.
     if (last) {
       if (sg.count > 1) {
-        if (in) add_state(in, 0.0f);
+        if (in) get_state(in);
         put_state(p.seg_state + seg * per_slot);
       }
       return;
     }
-  } else if (sg.count == 1) {
-    if (in) add_state(in, 0.0f);
-  } else {
-    add_state(p.seg_state + (sg.first + sg.count - 1) * per_slot, 0.0f);
-    for (int k = 0; k < sg.j; ++k)
-      add_state(p.seg_state + (sg.first + k) * per_slot,
-                expf(p.seg_log[static_cast<long long>(sg.first + k) * p.heads + h]));
+  } else if (sg.count > 1) {
+    get_state(p.seg_state + seg * per_slot);
+  } else if (in) {
+    get_state(in);
   }
   F2 hst[PPL][NPL / 2];
 #pragma unroll
@@ -285,6 +286,8 @@ int launch_scan(const ScanParams& p, long long segs, cudaStream_t st) {
   if (p.split) {
     scan_kernel<T, NPL, THREADS, PPL, true><<<grid, THREADS, full, st>>>(p, ptiles);
     count_launch();
+    SMM_CUDA_TRY(cudaGetLastError(), "selective scan launch");
+    if (int rc = scan_combine(p, st)) return rc;
   }
   scan_kernel<T, NPL, THREADS, PPL, false><<<grid, THREADS, full, st>>>(p, ptiles);
   count_launch();
@@ -635,6 +638,66 @@ int check_scan(const char* who, const ScanParams& p, int dtype, int dt_dtype, bo
   return SMM_OK;
 }
 
+// The state before segment j from the final states F_k of those before it (each from
+// zero) and S_in, which lies in the last one's place: a thread walks one element's
+// segments, eight elements' loads at a time.  Memory-bound: 8 bytes an element and segment.
+constexpr int kCombineThreads = 256;
+
+template <int V>  // elements of a thread
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const ScanParams p, int tiles, long long nsegs) {
+  __shared__ int sfirst;
+  const int s = static_cast<int>(blockIdx.x / tiles);
+  const int per_head = p.dim * p.state_dim;
+  const long long per_slot = static_cast<long long>(p.heads) * per_head;
+  const long long e = (static_cast<long long>(blockIdx.x % tiles) * kCombineThreads + threadIdx.x) * V;
+  long long first = 0;
+  if (s > 0) {
+    if (threadIdx.x == 0) sfirst = 0;
+    __syncthreads();
+    int before = 0;
+    for (int q = threadIdx.x; q < s; q += kCombineThreads) {
+      long long b, end;
+      seq_range(p.offsets, q, p.tokens, &b, &end);
+      before += segments_of(p, b, end);
+    }
+    if (before) atomicAdd(&sfirst, before);
+    __syncthreads();
+    first = sfirst;
+  }
+  long long b, end;
+  seq_range(p.offsets, s, p.tokens, &b, &end);
+  const int count = segments_of(p, b, end);
+  // sequences that overlap (offsets that decrease) may count past the workspace's segments
+  if (count == 1 || first + count > nsegs || e >= per_slot) return;
+  using E = typename std::conditional<V == 4, float4, float>::type;
+  const float* log = p.seg_log + first * p.heads + e / per_head;
+  float* at = p.seg_state + first * per_slot + e;
+  auto get = [&](int j, float(&v)[V]) { *reinterpret_cast<E*>(v) = *reinterpret_cast<const E*>(at + j * per_slot); };
+  auto put = [&](int j, const float(&v)[V]) { *reinterpret_cast<E*>(at + j * per_slot) = *reinterpret_cast<const E*>(v); };
+  alignas(16) float run[V];
+  get(count - 1, run);
+  constexpr int U = 8 / V;
+  for (int j0 = 0; j0 < count - 1; j0 += U) {
+    alignas(16) float f[U][V];
+    float a[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j0 + u < count - 1) {
+        get(j0 + u, f[u]);
+        a[u] = log[static_cast<long long>(j0 + u) * p.heads];
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j0 + u < count - 1) {
+        put(j0 + u, run);
+        const float decay = expf(a[u]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) run[i] = fmaf(run[i], decay, f[u][i]);
+      }
+  }
+  put(count - 1, run);
+}
+
 size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 
 // Segment length on the fp32 pipes.  The first launch costs over half of the
@@ -651,6 +714,22 @@ int simt_seg_len(long long tokens, int nseq, int heads, int dim) {
 }
 
 }  // namespace
+
+int scan_combine(const ScanParams& p, cudaStream_t st) {
+  const bool vec = p.dim * p.state_dim % 4 == 0;  // the workspace's alignment is checked
+  const long long per_cta = kCombineThreads * (vec ? 4 : 1);
+  const long long tiles = (static_cast<long long>(p.heads) * p.dim * p.state_dim + per_cta - 1) / per_cta;
+  if (tiles * p.nseq > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "selective scan too large for one launch");
+  const unsigned grid = static_cast<unsigned>(tiles * p.nseq);
+  const long long nsegs = max_segments(p.tokens, p.nseq, p.seg_len);
+  if (vec)
+    combine_kernel<4><<<grid, kCombineThreads, 0, st>>>(p, static_cast<int>(tiles), nsegs);
+  else
+    combine_kernel<1><<<grid, kCombineThreads, 0, st>>>(p, static_cast<int>(tiles), nsegs);
+  count_launch();
+  SMM_CUDA_TRY(cudaGetLastError(), "selective scan combine launch");
+  return SMM_OK;
+}
 
 // smm_scan_umma.cu
 int umma_seg_len(long long tokens, int nseq, int heads, int dim);

@@ -23,12 +23,19 @@
 // where the plain fp32 form has 0.2 to 1.7e-6).  The state itself stays in fp32
 // registers, S, Y, Yo and dS are fp32 in tensor memory.
 //
-// Persistent: a CTA an SM walks its share of the (segment, head, 64 dims) items as one
-// stream of chunks, so that the next item's loads and S are under way while an item
-// ends.  Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the decays in
-// turn, 4-11 form G and write y of the chunk before, half of the columns each, 12-19
-// form Xw, 20-23 carry the state.  Every wait is bounded; on expiry the CTA records it
-// and leaves.
+// A CTA takes one (segment, head, 64 dims), the hardware hands out the next as an SM
+// becomes free.  (A CTA an SM that walked a fixed share of them as one stream of chunks
+// saved their starts but shared out ragged ones badly: prompts of 16 tokens 195 -> 170 us,
+// but 8190 ragged tokens of 24 sequences 107 -> 126, before the states were
+// loaded all at once.)  Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the
+// decays in turn, 4-11 form G and write y of the chunk before, half of the columns each,
+// 12-19 form Xw, 20-23 carry the state.  Every wait is bounded; on expiry the CTA records
+// it and leaves.
+//
+// 4096 tokens of 64 heads of 64 x 128 take 101 us, 8190 ragged ones of 32 heads 83 us,
+// 32768 of 80 heads 0.78 ms: 3.3 us a chunk, no one unit's time but the mix of a chunk's way
+// through the roles (6000 clocks), shared memory (4000) and the issue of 3000
+// instructions a scheduler.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -68,20 +75,25 @@ struct Scal {
 
 struct Bars {
   uint64_t full_b[2], full_c[2], full_x[2], bfree[2], xfree[2], done[2], s_full[2], g_full[2];
-  uint64_t xw_full, xl_full, ds_full, ds_free, h_full, yo_free;
+  uint64_t xw_full[2], xl_full[2], ds_full[2], ds_free[2];  // by the chunk's parity
+  uint64_t h_full, yo_free;
   uint64_t sc_full[3], sc_free[3];
   uint64_t drain;
   uint32_t tmem;
   int abort_flag;
 };
 
-// NA: 64-wide tiles that state_dim takes (1 or 2)
-template <int NA>
+// NA: 64-wide tiles that state_dim takes (1 or 2).  The first launch of a split scan
+// needs no C and no H; it has two places for Xw and dS, so that a chunk's Xw is formed
+// while the product of the one before runs.
+template <int NA, bool STATES>
 struct Smem {
-  static constexpr uint32_t kStage = (2 * NA + 1) * kAtom;  // C, B, x
-  static constexpr uint32_t kXw = 2 * kStage;               // first and second term
-  static constexpr uint32_t kH = kXw + 2 * kAtom;           // third term of Xw, then H (in turn)
-  static constexpr uint32_t kScal = kH + kAtom;
+  static constexpr uint32_t kC = 0, kB = STATES ? 0 : NA * kAtom, kX = kB + NA * kAtom;  // in a stage
+  static constexpr uint32_t kStage = kX + kAtom;
+  static constexpr uint32_t kXw = 2 * kStage;                  // three terms
+  static constexpr uint32_t kXwNext = STATES ? 3 * kAtom : 0;  // from one place to the other
+  static constexpr uint32_t kH = kXw + 2 * kAtom;              // the third term of Xw, then H (in turn)
+  static constexpr uint32_t kScal = kXw + 3 * kAtom + kXwNext;
   static constexpr uint32_t kBars = kScal + 3 * sizeof(Scal);
   static constexpr uint32_t kBytes = kBars + sizeof(Bars) + 1024;  // + alignment
 };
@@ -251,7 +263,7 @@ __device__ __forceinline__ Item get_item(const ScanParams& p, int it, int ptiles
 template <int NA, bool STATES>
 __global__ void __launch_bounds__(kThreads, 1)
     scan_umma_kernel(const __grid_constant__ Tmaps maps, const ScanParams p, int items, int ptiles) {
-  using L = Smem<NA>;
+  using L = Smem<NA, STATES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -274,11 +286,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->done[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->g_full[i], 8);
+      mbar_init(&bars->xw_full[i], 8);
+      mbar_init(&bars->xl_full[i], 8);
+      mbar_init(&bars->ds_full[i], 1);
+      mbar_init(&bars->ds_free[i], 4);
     }
-    mbar_init(&bars->xw_full, 8);
-    mbar_init(&bars->xl_full, 8);
-    mbar_init(&bars->ds_full, 1);
-    mbar_init(&bars->ds_free, 4);
     mbar_init(&bars->h_full, 4);
     mbar_init(&bars->yo_free, 8);
     for (int i = 0; i < 3; ++i) {
@@ -296,7 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, bars->tmem, 0);
 
   volatile int* const flag = &bars->abort_flag;
-  constexpr uint32_t stage_c = 0, stage_b = NA * kAtom, stage_x = 2 * NA * kAtom;
+  constexpr uint32_t stage_c = L::kC, stage_b = L::kB, stage_x = L::kX;
+  constexpr int kDs = STATES ? 2 : 1;  // places for Xw and dS: a chunk's is free kDs chunks later
   const int it0 = blockIdx.x, its = gridDim.x;
 
   // In every role below, c counts the chunks of an item and cc those of the CTA: stages,
@@ -380,14 +393,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t hK = static_cast<uint32_t>(dK >> 32), hM = static_cast<uint32_t>(dM >> 32);
       auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xFFFFFFFFu, mbar_test(bar, parity)) != 0; };
       // one of the three terms of dS = B^T Xw
-      auto ds_term = [&](int s, auto tc) {
+      auto ds_term = [&](int s, uint32_t xw, uint32_t ds, auto tc) {
         constexpr uint32_t term = decltype(tc)::value * (kAtom >> 4);
         constexpr bool more = decltype(tc)::value > 0;
         const uint32_t base = lo(dM) + s * kSt;
         steps<8>([&](auto kc) {
           constexpr uint32_t k = decltype(kc)::value;
-          umma_ss<(stage_b >> 4) + k * 128, (L::kXw >> 4) + term + k * 128, more || (k > 0)>(leader, tmem + kColDs, base,
-                                                                                          hM, lo(dM), hM, idD);
+          umma_ss<(stage_b >> 4) + k * 128, (L::kXw >> 4) + term + k * 128, more || (k > 0)>(leader, ds, base, hM,
+                                                                                          xw, hM, idD);
         });
       };
       // Whatever has its operands: S up to a chunk ahead of the rest (the order fixed at its
@@ -399,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool did = true;
         const int s = cc & 1;
         const uint32_t par = (cc >> 1) & 1;
+        const uint32_t xw = lo(dM) + s * (L::kXwNext >> 4), ds = tmem + kColDs + (STATES ? s * kP : 0);
         if (!STATES && s_next < total && s_next < cc + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
             ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1)) {
           // C was loaded once every product of chunk cc - 2 was done: S's place, where its G was, is free
@@ -413,16 +427,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           });
           umma_commit_by(leader, &bars->s_full[sn]);
           ++s_next;
-        } else if (sub == 0 && ready(&bars->xw_full, cc & 1) && (cc == 0 || ready(&bars->ds_free, (cc - 1) & 1)) &&
+        } else if (sub == 0 && ready(&bars->xw_full[s], par) &&
+                   (cc < kDs || ready(&bars->ds_free[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1)) &&
                    ready(&bars->full_b[s], par) && ready(&bars->full_x[s], par)) {
           tc_fence_after_sync();
-          ds_term(s, std::integral_constant<int, 0>{});
-          ds_term(s, std::integral_constant<int, 1>{});
+          ds_term(s, xw, ds, std::integral_constant<int, 0>{});
+          ds_term(s, xw, ds, std::integral_constant<int, 1>{});
           sub = 1;
-        } else if (sub == 1 && ready(&bars->xl_full, cc & 1)) {
+        } else if (sub == 1 && ready(&bars->xl_full[s], par)) {
           tc_fence_after_sync();
-          ds_term(s, std::integral_constant<int, 2>{});
-          umma_commit_by(leader, &bars->ds_full);
+          ds_term(s, xw, ds, std::integral_constant<int, 2>{});
+          umma_commit_by(leader, &bars->ds_full[s]);
           umma_commit_by(leader, &bars->bfree[s]);
           sub = 2;
           if (STATES) sub = 0, ++cc;
@@ -718,8 +733,9 @@ __global__ void __launch_bounds__(kThreads, 1)
              wait_bar<kNapXw>(&bars->full_x[sb], (cc >> 1) & 1, p, flag);
         if (!ok) break;
         const float ws = scal[b3].f[3][s];
-        ok = cc < 1 || wait_bar<kNapXw>(&bars->ds_full, (cc - 1) & 1, p, flag);
+        ok = cc < kDs || wait_bar<kNapXw>(&bars->ds_full[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1, p, flag);
         if (!ok) break;
+        const uint32_t xw = L::kXw + sb * L::kXwNext;
         const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
         uint32_t vl[16];
 #pragma unroll
@@ -736,8 +752,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             vm[k] = narrow2(r);
             vl[4 * i + k] = narrow2(fma2(neg, widen2(vm[k]), r));
           }
-          *reinterpret_cast<uint4*>(smem + L::kXw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
-          *reinterpret_cast<uint4*>(smem + L::kXw + kAtom + off) = make_uint4(vm[0], vm[1], vm[2], vm[3]);
+          *reinterpret_cast<uint4*>(smem + xw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
+          *reinterpret_cast<uint4*>(smem + xw + kAtom + off) = make_uint4(vm[0], vm[1], vm[2], vm[3]);
         }
         if (left < kQ) {
           // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
@@ -750,8 +766,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = i0; i < i0 + 4; ++i) {
               const uint32_t off = swz_offset(s, i, 128);
               st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
-              st_shared_v4(sbase + L::kXw + off, 0, 0, 0, 0);
-              st_shared_v4(sbase + L::kXw + kAtom + off, 0, 0, 0, 0);
+              st_shared_v4(sbase + xw + off, 0, 0, 0, 0);
+              st_shared_v4(sbase + xw + kAtom + off, 0, 0, 0, 0);
 #pragma unroll
               for (int a = 0; a < NA; ++a) st_shared_v4(st + stage_b + a * kAtom + off, 0, 0, 0, 0);
             }
@@ -760,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bars->xw_full);
+          mbar_arrive(&bars->xw_full[sb]);
           mbar_arrive(&bars->sc_free[b3]);
         }
         // the third term's place is H's until the chunk before is done
@@ -770,10 +786,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          st_shared_v4(sbase + L::kH + swz_offset(s, i0 + i, 128), vl[4 * i], vl[4 * i + 1], vl[4 * i + 2], vl[4 * i + 3]);
+          st_shared_v4(sbase + xw + 2 * kAtom + swz_offset(s, i0 + i, 128), vl[4 * i], vl[4 * i + 1], vl[4 * i + 2], vl[4 * i + 3]);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->xl_full);
+        if (lane == 0) mbar_arrive(&bars->xl_full[sb]);
       }
     }
   } else {
@@ -794,39 +810,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       float hv[kP];
 #pragma unroll
       for (int i = 0; i < kP; ++i) hv[i] = 0.0f;
-      // What the state starts from: Horner over the earlier segments' final states, whose
-      // first term is the sequence's own start.  The first launch starts from zero, but
-      // copies the sequence's start into the last segment's place: the second launch
+      // What the state starts from.  The first launch of a split scan starts from zero, but
+      // copies the sequence's start into the last segment's place: the last launch
       // may overwrite it while other segments still need it.
-      const float* src = STATES || w.sg.count == 1
-                             ? in
-                             : p.seg_state + (w.sg.first + w.sg.count - 1) * per_slot + w.head_at;
-      int terms = w.sg.count > 1 ? 1 + w.sg.j : 1;
-      if (STATES) terms = w.last && w.sg.count > 1 ? 1 : 0;
-      if (!src) terms = 0;
-#pragma unroll 1
-      for (int k = 0; k < terms; ++k) {
-        const float decay = k ? expf(p.seg_log[static_cast<long long>(w.sg.first + k - 1) * p.heads + w.h]) : 0.0f;
-        // eight rows at a time (pdims is a multiple of 8): more loads in flight would not fit the registers
+      const float* src = w.sg.count == 1 ? in : p.seg_state + w.seg * per_slot + w.head_at;
+      if (STATES) src = w.last && w.sg.count > 1 ? in : nullptr;
+      if (src && live) {
+        src += n;
 #pragma unroll
-        for (int g8 = 0; g8 < kP / 8; ++g8) {
-          if (live && 8 * g8 < w.pdims) {
-            const float* at = src + 8 * g8 * N + n;
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = at[i * N];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) hv[8 * g8 + i] = fmaf(hv[8 * g8 + i], decay, v[i]);
-          }
-          asm volatile("" ::: "memory");
-        }
-        if (k + 1 < terms) src = p.seg_state + (w.sg.first + k) * per_slot + w.head_at;
+        for (int i = 0; i < kP; ++i)
+          if (i < w.pdims) hv[i] = src[i * N];
       }
       float log_sum = 0.0f;
 #pragma unroll 1
       for (int c = 0; c < w.nc; ++c, ++cc) {
         const int b3 = cc % 3;
-        ok = wait_bar<kNapState>(&bars->ds_full, cc & 1, p, flag);
+        ok = wait_bar<kNapState>(&bars->ds_full[cc & 1], (cc >> 1) & 1, p, flag);
         if (!ok) break;
         if (!STATES) {
           // H, the state before the chunk, where the third term of Xw has been read
@@ -851,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int pc = 0; pc < 4; ++pc) {
             uint32_t r[16];
-            tmem_ld_32x32b_x16(sD + 16 * pc, r);
+            tmem_ld_32x32b_x16(sD + (STATES ? (cc & 1) * kP : 0) + 16 * pc, r);
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -863,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bars->ds_free);
+          mbar_arrive(&bars->ds_free[cc & 1]);
           mbar_arrive(&bars->sc_free[b3]);
         }
       }
@@ -876,14 +875,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else if (w.last && p.state_out && slot >= 0) {
         dst = p.state_out + slot * per_slot + w.head_at;
       }
+      if (dst && live) {
+        dst += n;
 #pragma unroll
-      for (int g8 = 0; g8 < kP / 8; ++g8) {
-        if (dst && live && 8 * g8 < w.pdims) {
-          float* at = dst + 8 * g8 * N + n;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) at[i * N] = hv[8 * g8 + i];
-        }
-        asm volatile("" ::: "memory");
+        for (int i = 0; i < kP; ++i)
+          if (i < w.pdims) dst[i * N] = hv[i];
       }
     }
   }
@@ -918,11 +914,11 @@ int launch_one(const Tmaps& maps, const ScanParams& p, int items, int ptiles, cu
   int dev = 0;
   SMM_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
   cudaError_t err = cudaSuccess;
-  auto set = [&] { err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NA>::kBytes); };
+  auto set = [&] { err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NA, STATES>::kBytes); };
   if (dev < 64) std::call_once(once[dev], set);
   else set();
   SMM_CUDA_TRY(err, "selective scan shared memory size");
-  kern<<<items, kThreads, Smem<NA>::kBytes, st>>>(maps, p, items, ptiles);
+  kern<<<items, kThreads, Smem<NA, STATES>::kBytes, st>>>(maps, p, items, ptiles);
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "selective scan (tensor core) launch");
   return SMM_OK;
@@ -931,13 +927,12 @@ int launch_one(const Tmaps& maps, const ScanParams& p, int items, int ptiles, cu
 }  // namespace
 
 // bf16, whole 16-byte pieces everywhere, state_dim of one 128-row tile, and sequences
-// long enough.  Time here goes with the chunks, a started one counting in full, and on
-// the fp32 pipes with tokens * dim * (state_dim + 40).  For many sequences of dim 64 the
-// two cross near 42 tokens each with state_dim 128 (32 sequences of 64 heads, fp32 pipes
-// against this kernel: 188 and 200 us at 40 tokens, 280 and 203 at 64) and near 125 with
-// state_dim 16 (87 and 198 us at 64; 227 and 91 us for 4 of 1024).  While the CTAs fit
-// the GPU at once this kernel's one chunk is 10 us, and they cross earlier (one sequence,
-// state_dim 128: 11.8 and 9.9 us at 24 tokens, 32 and 10 at 128).
+// long enough.  Time here goes with the chunks, a started one counting in full (32 sequences
+// of 64 heads of 64: 132 to 140 us for up to 64 tokens each), on the fp32 pipes
+// with the tokens, and state_dim adds to it.  The two cross near 19 tokens with state_dim 128
+// (fp32 pipes against this kernel: 121 and 132 us at 16 tokens, 149 and 132 at 24)
+// and near 90 with 16 (96 and 133 us at 64; 220 and 82 for 4 sequences of 1024); for one
+// sequence no later (12.3 and 10.2 us at 24 tokens).
 bool scan_umma_fits(const ScanParams& p, int dtype) {
   if (dtype != SMM_DTYPE_BF16 || p.dim % 8 || p.state_dim % 8 || p.state_dim > 128) return false;
   if (p.ldx % 8 || p.ldb % 8 || p.ldc % 8 || p.ldy % 8 || (p.z && p.ldz % 8)) return false;
@@ -945,8 +940,7 @@ bool scan_umma_fits(const ScanParams& p, int dtype) {
       !aligned_to(p.z, 16))
     return false;
   const long long ptiles = (p.dim + kP - 1) / kP;
-  const long long item = 1LL * p.nseq * p.heads * ptiles <= 148 ? 2500 : 7000;
-  return p.tokens * (p.state_dim + 40) * p.dim >= p.nseq * item * kP * ptiles;
+  return p.tokens * (p.state_dim + 15) * p.dim >= 2750 * static_cast<long long>(p.nseq) * kP * ptiles;
 }
 
 // Segment length of the tensor-core kernel: whole chunks, so that the waves of
@@ -981,12 +975,16 @@ int scan_umma_launch(ScanParams& p, cudaStream_t st) {
   if (int rc = make_map(&maps.c, p.C, p.state_dim, p.groups, p.tokens, p.ldc, "C")) return rc;
   const int items = static_cast<int>(blocks);
   if (p.state_dim <= 64) {
-    if (p.split)
+    if (p.split) {
       if (int rc = launch_one<1, true>(maps, p, items, ptiles, st)) return rc;
+      if (int rc = scan_combine(p, st)) return rc;
+    }
     return launch_one<1, false>(maps, p, items, ptiles, st);
   }
-  if (p.split)
+  if (p.split) {
     if (int rc = launch_one<2, true>(maps, p, items, ptiles, st)) return rc;
+    if (int rc = scan_combine(p, st)) return rc;
+  }
   return launch_one<2, false>(maps, p, items, ptiles, st);
 }
 

@@ -467,6 +467,21 @@ def test_bad_offsets_stay_in_bounds(cuda, dtype):
     ops.device_status()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_overlapping_sequences_of_a_split_scan_stay_in_bounds(cuda, dtype):
+    """Offsets that decrease can count more segments than the workspace holds."""
+    t, h, n = 6000, 1, 128
+    a = make_scan(2, t, h, 64, 1, n, dtype)
+    for o in ([0, t, 10, t], [0, t, 0, t, 0, t], [t, 0, t, 0]):
+        nseq = len(o) - 1
+        assert _lib.load().smm_selective_scan_workspace_size(t, nseq, h, 64, 1, n, 0 if dtype == "fp32" else 1) > 0
+        so = torch.zeros(nseq, h, 64, n, device="cuda")
+        ops.selective_scan(**a, offsets=i32(o), state=rnd(gen(1), nseq, h, 64, n), state_out=so)
+    ops.device_status()
+    ref = ops.selective_scan(**a)
+    assert ref.isfinite().all()
+
+
 def test_no_sequences_and_no_tokens(cuda):
     a = make_scan(1, 0, 2, 64, 1, 128, "bf16")
     st = rnd(gen(1), 1, 2, 64, 128)
