@@ -1,5 +1,6 @@
 """Tensor-level API over libsmm: each function takes torch CUDA tensors
-(row-major fp32, contiguous), calls one C ABI entry point on the current
+(row-major fp32, contiguous; the state-space operators and the 4-bit product also
+bf16 and strided rows), calls one C ABI entry point on the current
 stream, and returns the output tensor.
 
 Storage conventions follow the reference DSL (src/dsl/layout_functions.py):
