@@ -3,7 +3,7 @@
 // packed prompts, and for one new token of each sequence.
 //
 // Bound by memory: each element is read once and written once (W multiplies
-// per element), with the activation's exponential and reciprocal next (half of their
+// per element), with the activation's exponential and reciprocal next (59 % of their
 // pipe's time).  A thread owns four channels and walks down a run of
 // consecutive tokens with the last W-1 rows in registers, so a row is read
 // from memory once and W-1 rows per run again from L2.  While it computes the rows
