@@ -6,7 +6,8 @@ magnitudes of an output's terms (computed beside it in 64 bits):
   - exp, log1p and the quotient of silu are within a few u relative, and an
     exponent's own error reaches the result as at most 0.37 times it (x exp(-x));
   - a product on the tensor cores whose operand was rounded to bf16 adds 2^-8 M,
-    one whose operand was split in two bf16 terms 2^-16 M;
+    one whose operand is the sum of three bf16 terms 2^-27 M, and its 24 products of
+    16 terms with truncated additions less than 2^-16 M;
   - the result's rounding is half a step of its type, eps/2.
 """
 import pytest
