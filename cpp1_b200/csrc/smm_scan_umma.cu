@@ -404,7 +404,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         });
       };
       // Whatever has its operands: S up to a chunk ahead of the rest (the order fixed at its
-      // usual one, with blocking waits, was a tenth slower).
+      // usual one, with blocking waits, was a tenth slower).  A chunk's dS never goes before its
+      // S, which may still wait for C then: the commit behind dS gives B's place to the
+      // next load, and has to cover both products that read B.
       int s_next = STATES ? total : 0, cc = 0, sub = 0;
       uint32_t idle = 0;
       uint64_t t0 = 0;
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           });
           umma_commit_by(leader, &bars->s_full[sn]);
           ++s_next;
-        } else if (sub == 0 && ready(&bars->xw_full[s], par) &&
+        } else if (sub == 0 && s_next > cc && ready(&bars->xw_full[s], par) &&
                    (cc < kDs || ready(&bars->ds_free[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1)) &&
                    ready(&bars->full_b[s], par) && ready(&bars->full_x[s], par)) {
           tc_fence_after_sync();
