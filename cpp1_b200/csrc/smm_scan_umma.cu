@@ -17,10 +17,10 @@
 // off the diagonal blocks, and exp(l_t - l_s) d_s on them, l being sums within
 // the block; w_s = f[4][s].  So a quarter of the exponentials remains.
 //
-// Roundings: G and H to bf16 as operands of products (relative 2^-8 of
-// each term of y, which is itself rounded to bf16); Xw as the sum of three bf16 terms
-// (2^-24; two left an error of 2.3e-6 in the states, an fp32 result that is carried on,
-// where the plain fp32 form has 0.2 to 1.7e-6).  The state itself stays in fp32
+// Roundings: G and H as operands of products are the sum of two bf16 terms (2^-17 of each
+// term of y, which is itself rounded to bf16; one term, 2^-9, added up to 1e-3 to y's error of
+// 1.7e-3 from its own rounding); Xw is the sum of three (2^-24; two left an error of 2.3e-6 in the
+// states, an fp32 result that is carried on, where the plain fp32 form has 0.2 to 1.7e-6).  The state itself stays in fp32
 // registers, S, Y, Yo and dS are fp32 in tensor memory.
 //
 // A CTA takes one (segment, head, 64 dims), the hardware hands out the next as an SM
@@ -74,8 +74,8 @@ struct Scal {
 };
 
 struct Bars {
-  uint64_t full_b[2], full_c[2], full_x[2], bfree[2], xfree[2], done[2], s_full[2], g_full[2];
-  uint64_t xw_full[2], xl_full[2], ds_full[2], ds_free[2];  // by the chunk's parity
+  uint64_t full_bc[2], full_x[2], xfree[2], done[2], s_full[2], g_full[2];
+  uint64_t xw_full[2], ds_full[2], ds_free[2];  // by the chunk's parity
   uint64_t h_full, yo_free;
   uint64_t sc_full[3], sc_free[3];
   uint64_t drain;
@@ -92,7 +92,7 @@ struct Smem {
   static constexpr uint32_t kStage = kX + kAtom;
   static constexpr uint32_t kXw = 2 * kStage;                  // three terms
   static constexpr uint32_t kXwNext = STATES ? 3 * kAtom : 0;  // from one place to the other
-  static constexpr uint32_t kH = kXw + 2 * kAtom;              // the third term of Xw, then H (in turn)
+  static constexpr uint32_t kH = NA * kAtom / 2;               // a term of H: two fill B's place in the stage
   static constexpr uint32_t kScal = kXw + 3 * kAtom + kXwNext;
   static constexpr uint32_t kBars = kScal + 3 * sizeof(Scal);
   static constexpr uint32_t kBytes = kBars + sizeof(Bars) + 1024;  // + alignment
@@ -215,9 +215,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
+// Two bf16 terms of a pair: their sum is within 2^-17 of it, relative.
+__device__ __forceinline__ void split2(unsigned long long v, uint32_t& hi, uint32_t& lo) {
+  hi = narrow2(v);
+  lo = narrow2(fma2(pack2(-1.0f, -1.0f), widen2(hi), v));
 }
 // 32 lanes x 32 consecutive columns of tensor memory into registers.
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -278,16 +279,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->full_b[i], 1);
-      mbar_init(&bars->full_c[i], 1);
+      mbar_init(&bars->full_bc[i], 1);
       mbar_init(&bars->full_x[i], 1);
-      mbar_init(&bars->bfree[i], 1);
       mbar_init(&bars->xfree[i], 8);
       mbar_init(&bars->done[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->g_full[i], 8);
       mbar_init(&bars->xw_full[i], 8);
-      mbar_init(&bars->xl_full[i], 8);
       mbar_init(&bars->ds_full[i], 1);
       mbar_init(&bars->ds_free[i], 4);
     }
@@ -317,15 +315,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   //
   // The launch's 6 x 80 registers per warpgroup's thread, shared out by need.
   // A spill costs a trip to L2 here: shared memory leaves L1 too small for the stacks.
-  constexpr int kRegsMisc = 48, kRegsG = STATES ? 24 : 104, kRegsXw = 64, kRegsState = STATES ? 152 : 96;
+  constexpr int kRegsMisc = 48, kRegsG = STATES ? 24 : 112, kRegsXw = 56, kRegsState = STATES ? 152 : 96;
   static_assert(kRegsMisc + 2 * kRegsG + 2 * kRegsXw + kRegsState <= 6 * 80, "more registers than the launch has");
   if (warp < 4) {
     regs_dec<kRegsMisc>();
     if (warp == 0) {
       // ---------------------------------------------------------- loads
-      // in the order in which the places become free: B after dS, C after all products of
-      // its chunk, x after its part in y
-      int n_b = 0, n_c = 0, n_x = 0;  // loads issued
+      // in the order in which the places become free: B and C after all products of their
+      // chunk (in the first launch of a split scan after dS, the only one), x after its part in y
+      int n_bc = 0, n_x = 0;  // loads issued
       const int per_group = p.heads / p.groups;
       bool ok = true;
       for (int it = it0; it < items && ok; it += its) {
@@ -334,28 +332,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         int row = static_cast<int>(w.sg.begin);
 #pragma unroll 1
         for (int c = 0; c < w.nc; ++c, row += kQ) {
-          const int s = n_b & 1;
-          const uint32_t st = sbase + s * L::kStage, par = ((n_b >> 1) - 1) & 1;
-          const bool first = n_b < 2;
-          ok = first || wait_bar<kNapLoad>(&bars->bfree[s], par, p, flag);
+          const int s = n_bc & 1;
+          const uint32_t st = sbase + s * L::kStage, par = ((n_bc >> 1) - 1) & 1;
+          const bool first = n_bc < 2;
+          ok = first || wait_bar<kNapLoad>(STATES ? &bars->ds_full[s] : &bars->done[s], par, p, flag);
           if (!ok) break;
           if (lane == 0) {
-            mbar_arrive_expect_tx(&bars->full_b[s], NA * kAtom);
+            mbar_arrive_expect_tx(&bars->full_bc[s], (STATES ? 1 : 2) * NA * kAtom);
 #pragma unroll
-            for (int a = 0; a < NA; ++a)
-              tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_b[s], a * 64, g, row);
-          }
-          ++n_b;
-          if (!STATES) {
-            ok = first || wait_bar<kNapLoad>(&bars->done[s], par, p, flag);
-            if (!ok) break;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&bars->full_c[s], NA * kAtom);
-#pragma unroll
-              for (int a = 0; a < NA; ++a)
-                tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_c[s], a * 64, g, row);
+            for (int a = 0; a < NA; ++a) {
+              tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_bc[s], a * 64, g, row);
+              if (!STATES) tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_bc[s], a * 64, g, row);
             }
-            ++n_c;
+          }
+          ++n_bc;
+          if (!STATES) {
             ok = first || wait_bar<kNapLoad>(&bars->xfree[s], par, p, flag);
             if (!ok) break;
           }
@@ -368,11 +359,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // after an abort, copies in flight land before the CTA leaves
       if (*flag && lane == 0) {
-        const int n[3] = {n_b, n_c, n_x};
+        const int n[2] = {n_bc, n_x};
 #pragma unroll 1
-        for (int k = 0; k < 6; ++k) {  // full_b, full_c, full_x, two of each
+        for (int k = 0; k < 4; ++k) {  // full_bc, full_x, two of each
           const int last_use = ((n[k >> 1] - (k & 1) + 1) >> 1) - 1;
-          if (last_use >= 0) drain_bar(&bars->full_b[0] + k, last_use & 1, p, flag);
+          if (last_use >= 0) drain_bar(&bars->full_bc[0] + k, last_use & 1, p, flag);
         }
       }
     } else if (warp == 1) {
@@ -405,8 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // Whatever has its operands: S up to a chunk ahead of the rest (the order fixed at its
       // usual one, with blocking waits, was a tenth slower).  A chunk's dS never goes before its
-      // S, which may still wait for C then: the commit behind dS gives B's place to the
-      // next load, and has to cover both products that read B.
+      // S: the commit behind dS gives B's place to H, and has to cover both products that read B.
       int s_next = STATES ? total : 0, cc = 0, sub = 0;
       uint32_t idle = 0;
       uint64_t t0 = 0;
@@ -415,8 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int s = cc & 1;
         const uint32_t par = (cc >> 1) & 1;
         const uint32_t xw = lo(dM) + s * (L::kXwNext >> 4), ds = tmem + kColDs + (STATES ? s * kP : 0);
-        if (!STATES && s_next < total && s_next < cc + 2 && ready(&bars->full_c[s_next & 1], (s_next >> 1) & 1) &&
-            ready(&bars->full_b[s_next & 1], (s_next >> 1) & 1)) {
+        if (!STATES && s_next < total && s_next < cc + 2 && ready(&bars->full_bc[s_next & 1], (s_next >> 1) & 1)) {
           // C was loaded once every product of chunk cc - 2 was done: S's place, where its G was, is free
           tc_fence_after_sync();
           const int sn = s_next & 1;
@@ -431,35 +420,34 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++s_next;
         } else if (sub == 0 && s_next > cc && ready(&bars->xw_full[s], par) &&
                    (cc < kDs || ready(&bars->ds_free[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1)) &&
-                   ready(&bars->full_b[s], par) && ready(&bars->full_x[s], par)) {
+                   ready(&bars->full_bc[s], par) && ready(&bars->full_x[s], par)) {
           tc_fence_after_sync();
           ds_term(s, xw, ds, std::integral_constant<int, 0>{});
           ds_term(s, xw, ds, std::integral_constant<int, 1>{});
-          sub = 1;
-        } else if (sub == 1 && ready(&bars->xl_full[s], par)) {
-          tc_fence_after_sync();
           ds_term(s, xw, ds, std::integral_constant<int, 2>{});
           umma_commit_by(leader, &bars->ds_full[s]);
-          umma_commit_by(leader, &bars->bfree[s]);
-          sub = 2;
-          if (STATES) sub = 0, ++cc;
-        } else if (sub == 2 && ready(&bars->g_full[s], par)) {
+          if (STATES)
+            ++cc;
+          else
+            sub = 1;
+        } else if (sub == 1 && ready(&bars->g_full[s], par)) {
           tc_fence_after_sync();
           const uint32_t base = lo(dM) + s * kSt;
-          steps<8>([&](auto kc) {
-            constexpr uint32_t k = decltype(kc)::value;
-            umma_ts<(k >> 2) * 64 + (k & 3) * 8, (stage_x >> 4) + k * 128, (k > 0)>(
+          steps<16>([&](auto kc) {  // both terms of G
+            constexpr uint32_t k = decltype(kc)::value & 7, term = decltype(kc)::value >> 3;
+            umma_ts<(k >> 1) * 32 + (k & 1) * 8 + term * 16, (stage_x >> 4) + k * 128, (term + k > 0)>(
                 leader, tmem + kColY + s * kP, tmem + kColS + s * 128, base, hM, idY);
           });
-          sub = 3;
-        } else if (sub == 3 && ready(&bars->h_full, cc & 1) && (cc == 0 || ready(&bars->yo_free, (cc - 1) & 1))) {
+          sub = 2;
+        } else if (sub == 2 && ready(&bars->h_full, cc & 1) && (cc == 0 || ready(&bars->yo_free, (cc - 1) & 1))) {
           tc_fence_after_sync();
-          const uint32_t base = lo(dK) + s * kSt;
-          steps<4 * NA>([&](auto kc) {
-            constexpr uint32_t k = decltype(kc)::value, off = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
+          const uint32_t base = lo(dK) + s * kSt, base_h = lo(dM) + s * kSt;
+          steps<8 * NA>([&](auto kc) {  // both terms of H
+            constexpr uint32_t k = decltype(kc)::value % (4 * NA), term = decltype(kc)::value / (4 * NA);
+            constexpr uint32_t off = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
             if (k < ksteps)
-              umma_ss<(stage_c >> 4) + off, (L::kH >> 4) + k * 128, (k > 0)>(leader, tmem + kColYo, base, hK, lo(dM), hM,
-                                                                            idY);
+              umma_ss<(stage_c >> 4) + off, ((stage_b + term * L::kH) >> 4) + k * 128, (term + k > 0)>(
+                  leader, tmem + kColYo, base, hK, base_h, hM, idY);
           });
           umma_commit_by(leader, &bars->done[s]);
           sub = 0;
@@ -609,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int i2 = 0; i2 < 2; ++i2) {
               const int b = 2 * half + i2;  // block of 32 columns: off the diagonal for b < q
-              uint32_t o[16];
+              uint32_t o[16], ol[16];        // G's first and second term
               if (b <= q) {
                 uint32_t r[32];
                 tmem_ld_32x32b_x32(sS + 32 * i2, r);
@@ -621,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                   for (int i = 0; i < 16; ++i) {
                     const unsigned long long s2 = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                    o[i] = narrow2(mul2(mul2(s2, f[i]), u2));
+                    split2(mul2(mul2(s2, f[i]), u2), o[i], ol[i]);
                   }
                 } else {
                   const unsigned long long* ls = reinterpret_cast<const unsigned long long*>(sc.l + 32 * b);
@@ -635,15 +623,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     unpack2(fma2(ls[i], neg, lt2), a, z);
                     const unsigned long long w2 = mul2(pack2(ex2(a), ex2(z)), f[i]);
                     unpack2(mul2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), w2), a, z);
-                    o[i] = bf16_pair(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f);
+                    split2(pack2(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f), o[i], ol[i]);
                   }
                 }
               } else {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = 0;
+                for (int i = 0; i < 16; ++i) o[i] = ol[i] = 0;
               }
               // these columns of S have been read by this lane already
-              tmem_st_32x32b_x16(sS + 16 * i2, o);
+              tmem_st_32x32b_x16(sS + 32 * i2, o);
+              tmem_st_32x32b_x16(sS + 32 * i2 + 16, ol);
             }
             tmem_wait_st();
             tc_fence_before_sync();
@@ -739,37 +728,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const uint32_t xw = L::kXw + sb * L::kXwNext;
         const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
-        uint32_t vl[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t off = swz_offset(s, i0 + i, 128);
           const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-          uint32_t vh[4], vm[4];
+          uint32_t vh[4], vm[4], vl[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const unsigned long long v = mul2(w2, widen2(xs[k]));
             vh[k] = narrow2(v);
-            const unsigned long long r = fma2(neg, widen2(vh[k]), v);
-            vm[k] = narrow2(r);
-            vl[4 * i + k] = narrow2(fma2(neg, widen2(vm[k]), r));
+            split2(fma2(neg, widen2(vh[k]), v), vm[k], vl[k]);
           }
           *reinterpret_cast<uint4*>(smem + xw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
           *reinterpret_cast<uint4*>(smem + xw + kAtom + off) = make_uint4(vm[0], vm[1], vm[2], vm[3]);
+          *reinterpret_cast<uint4*>(smem + xw + 2 * kAtom + off) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
         }
         if (left < kQ) {
           // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-          ok = wait_bar<kNapXw>(&bars->full_b[sb], (cc >> 1) & 1, p, flag);
+          ok = wait_bar<kNapXw>(&bars->full_bc[sb], (cc >> 1) & 1, p, flag);
           if (!ok) break;
           if (s >= left) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) vl[i] = 0;
 #pragma unroll 1
             for (int i = i0; i < i0 + 4; ++i) {
               const uint32_t off = swz_offset(s, i, 128);
               st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
               st_shared_v4(sbase + xw + off, 0, 0, 0, 0);
               st_shared_v4(sbase + xw + kAtom + off, 0, 0, 0, 0);
+              st_shared_v4(sbase + xw + 2 * kAtom + off, 0, 0, 0, 0);
 #pragma unroll
               for (int a = 0; a < NA; ++a) st_shared_v4(st + stage_b + a * kAtom + off, 0, 0, 0, 0);
             }
@@ -781,17 +767,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&bars->xw_full[sb]);
           mbar_arrive(&bars->sc_free[b3]);
         }
-        // the third term's place is H's until the chunk before is done
-        if (!STATES) {
-          ok = cc < 1 || wait_bar<kNapXw>(&bars->done[(cc - 1) & 1], ((cc - 1) >> 1) & 1, p, flag);
-          if (!ok) break;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          st_shared_v4(sbase + xw + 2 * kAtom + swz_offset(s, i0 + i, 128), vl[4 * i], vl[4 * i + 1], vl[4 * i + 2], vl[4 * i + 3]);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->xl_full[sb]);
       }
     }
   } else {
@@ -830,13 +805,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = wait_bar<kNapState>(&bars->ds_full[cc & 1], (cc >> 1) & 1, p, flag);
         if (!ok) break;
         if (!STATES) {
-          // H, the state before the chunk, where the third term of Xw has been read
-          if (n < 64 * NA) {
+          // H, the state before the chunk, in the place of B, which has been read
+          // (hidden from the compiler, or it keeps eight offsets in registers through the loop)
+          uint32_t row = n, at = sbase + (cc & 1) * L::kStage + stage_b;
+          asm volatile("" : "+r"(row), "+r"(at));
+          if (row < 64 * NA) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              st_shared_v4(sbase + L::kH + swz_offset(n, i, 128), bf16_pair(hv[8 * i], hv[8 * i + 1]),
-                           bf16_pair(hv[8 * i + 2], hv[8 * i + 3]), bf16_pair(hv[8 * i + 4], hv[8 * i + 5]),
-                           bf16_pair(hv[8 * i + 6], hv[8 * i + 7]));
+            for (int i = 0; i < 8; ++i) {
+              uint32_t vh[4], vl[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) split2(pack2(hv[8 * i + 2 * k], hv[8 * i + 2 * k + 1]), vh[k], vl[k]);
+              const uint32_t off = swz_offset(row, i, 128);
+              st_shared_v4(at + off, vh[0], vh[1], vh[2], vh[3]);
+              st_shared_v4(at + L::kH + off, vl[0], vl[1], vl[2], vl[3]);
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();

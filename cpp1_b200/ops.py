@@ -604,7 +604,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     x, z, y (tokens, heads, dim) and B, C (tokens, groups, state_dim) float32 or
     bfloat16, dt (tokens, heads) of the same type or float32; A, D, dt_bias
     (heads) float32.  dim and state_dim are 1 to 256.  Rows may be strided (x, B and
-    C columns of one matrix).  Sums, decays and states are float32.
+    C columns of one matrix).  Sums, decays and states are float32; longer bfloat16 prompts go through
+    the tensor cores, where scores and states enter products as two bfloat16 terms (2^-17 relative).
 
     offsets, slots, out, state (entries, heads, dim, state_dim; float32) and state_out are as in causal_conv.
     A non-finite input makes the rest of its sequence non-finite, and may

@@ -517,6 +517,11 @@ int smm_causal_conv_step(const void* x, const void* w, const void* bias, const v
  * dt_bias are fp32.  D, z and dt_bias may be NULL.  A state is heads x dim x
  * state_dim fp32.  dim and state_dim are 1..256.  dt_dtype is dt's own type.
  *
+ * Sums, decays and states are fp32.  bf16 prompts that are long enough go through the
+ * tensor cores, where the scores C B^T and the state enter products as the sum of two bf16
+ * terms (2^-17 relative).  Which path a call takes goes by its sizes, so the last bits of a
+ * sequence's outputs can differ between batches.
+ *
  * A non-finite x, B, C or dt of a token makes the rest of its sequence
  * non-finite, and may do so for the up to 127 tokens before it as well.
  *

@@ -36,3 +36,39 @@ def test_scan_beside_busy_memory(cuda, lens, h, n):
         y2 = ops.selective_scan(**a, offsets=o, state=st, state_out=so2)
         torch.cuda.synchronize()
         assert torch.equal(y2, y) and torch.equal(so2, so)
+
+
+# ---------------------------------------------------------------- accuracy
+def on_tensor_cores(a, lens):
+    """The rule by which bf16 prompts take the tensor cores (aligned pieces, one tile of state)."""
+    t, _, p = a["x"].shape
+    n = a["B"].shape[2]
+    return (a["x"].dtype is BF and p % 8 == 0 and n % 8 == 0 and n <= 128
+            and t * (n + 15) * p >= 2750 * len(lens) * 64 * ((p + 63) // 64))
+
+
+def once_rounded_tol(ref, mag, n, longest, dtype):
+    """One rounding to the output's type, and behind it what 32-bit sums leave: the recurrence's
+    roundings as in scan_tol; on the tensor cores two terms of 2^-17 each for the scores and the state,
+    and 40 additions truncated to 2^-23 of the sum, 2^-17.7."""
+    return scan_tol(ref, mag, n, longest, dtype, False) + (2.0 ** -16 + 2.0 ** -17.7) * mag
+
+
+@pytest.mark.parametrize("lens,h,p,g_,n", [
+    ([128], 4, 64, 1, 128), ([127, 129, 1, 0, 256], 4, 64, 2, 128), ([300, 100], 8, 64, 8, 64), ([513], 2, 128, 1, 128),
+    ([200, 131], 3, 96, 1, 96), ([260], 5, 40, 1, 24), ([1000], 2, 64, 1, 128), ([64] * 9, 2, 32, 1, 16),
+    ([600, 1400], 1, 64, 1, 8), ([700, 37, 260], 160, 64, 8, 128), ([130, 900, 1, 0, 128], 200, 64, 1, 64)])
+@pytest.mark.parametrize("with_state", [False, True])
+def test_bf16_scan_rounds_its_outputs_alone(cuda, lens, h, p, g_, n, with_state):
+    """Scores, decays and states are not cut to the inputs' 8 bits on their way: where the terms
+    of an output cancel, its error stays that of its own rounding."""
+    b = offs(lens)
+    a = make_scan(h + n, b[-1], h, p, g_, n, "bf16", z=h % 2 == 0)
+    st = rnd(gen(n), len(lens), h, p, n) if with_state else None
+    ref, mag, (fin, fmag) = scan_ref(a, b, st)
+    so = torch.empty(len(lens), h, p, n, device="cuda")
+    y = ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so)
+    within(y, ref, once_rounded_tol(ref, mag, n, max(lens), BF), "y")
+    # a rounding of the exact result, and 2^-16 of the terms beside it
+    best = float((ref.to(BF).double() - ref).norm())
+    assert float((y.double() - ref).norm()) <= best + 2.0 ** -16 * float(mag.norm())
