@@ -24,6 +24,8 @@ void count_launch(unsigned n = 1);
 uint32_t* device_status_word();
 // Wait limit handed to the pipelined kernels (ns); SMM_WAIT_LIMIT_MS overrides.
 unsigned long long wait_limit_ns();
+// The same for one call: the limit that smm_debug_wait_limit_next set, which this takes, or the above.
+unsigned long long take_wait_limit_ns();
 
 inline cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 

@@ -178,6 +178,12 @@ thread_local unsigned long long g_wait_next = 0;
 
 }  // namespace
 
+unsigned long long take_wait_limit_ns() {
+  const unsigned long long v = g_wait_next ? g_wait_next : wait_limit_ns();
+  g_wait_next = 0;
+  return v;
+}
+
 // cuTensorMapEncodeTiled, or null (for the translation units with maps of their own).
 void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
 
@@ -249,11 +255,10 @@ int run_contraction(AKind ak, BKind bk, int mode, const Operand& a, const Operan
   // so a group spans every row tile and each B column slab is read once.
   p.raster_group = ak == AKind::Toeplitz ? std::max(p.row_tiles, 1) : 8;
   p.status = device_status_word();
-  p.wait_limit_ns = g_wait_next ? g_wait_next : wait_limit_ns();
+  p.wait_limit_ns = take_wait_limit_ns();
   p.drain_limit_ns = std::max(p.wait_limit_ns, kMinDrainNs);
   p.trace = g_trace;
   g_trace = nullptr;
-  g_wait_next = 0;
   cudaEvent_t ev_before = g_ev_before, ev_after = g_ev_after;
   g_ev_before = g_ev_after = nullptr;
   if (!p.status) return set_error(SMM_ERR_CUDA, "device status word unavailable");
@@ -762,9 +767,9 @@ extern "C" int smm_debug_time_next(void* event_before, void* event_after) {
   return SMM_OK;
 }
 
-// Failure-path test: the next contraction kernel launched from this thread
-// gives every pipeline wait `wait_limit_ns` nanoseconds instead of the
-// default (teardown waits keep at least a second).  0 restores the default.
+// Failure-path test: the next contraction kernel (or tensor-core selective
+// scan, in all of its launches) launched from this thread gives every
+// pipeline wait `wait_limit_ns` nanoseconds instead of the default (teardown waits keep at least a second).  0 restores the default.
 extern "C" int smm_debug_wait_limit_next(unsigned long long wait_limit_ns) {
   if (wait_limit_ns > 10ull * 1000000000ull)
     return set_error(SMM_ERR_INVALID, "smm_debug_wait_limit_next: limit must be at most 10 s");

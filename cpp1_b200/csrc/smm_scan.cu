@@ -770,7 +770,6 @@ extern "C" int smm_selective_scan(const void* x, const void* dt, const float* A,
   p.softplus = dt_softplus != 0;
   if (int rc = check_scan("smm_selective_scan", p, dtype, dt_dtype, false)) return rc;
   if (heads == 0 || nseq == 0) return SMM_OK;
-  p.wait_limit_ns = wait_limit_ns();
   const bool umma = scan_umma_fits(p, dtype);
   p.seg_len = umma ? umma_seg_len(tokens, nseq, heads, dim) : simt_seg_len(tokens, nseq, heads, dim);
   p.split = p.seg_len < tokens;
@@ -786,7 +785,10 @@ extern "C" int smm_selective_scan(const void* x, const void* dt, const float* A,
   }
   p.status = device_status_word();
   if (!p.status) return set_error(SMM_ERR_CUDA, "device status word unavailable");
-  if (umma) return scan_umma_launch(p, as_stream(stream));
+  if (umma) {
+    p.wait_limit_ns = take_wait_limit_ns();
+    return scan_umma_launch(p, as_stream(stream));
+  }
   return dtype == SMM_DTYPE_F32 ? launch_scan_type<float>(p, segs, as_stream(stream))
                                 : launch_scan_type<__nv_bfloat16>(p, segs, as_stream(stream));
 }

@@ -173,14 +173,16 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // Waits of all roles.  A sleep follows every fruitless try: the tries return at once, and
 // a dozen waiting warps' loops would take issue slots from those that compute.  Every
 // wait depends on loads or products still to come, so the warp that issues the products
-// keeps the time (TIMED), and raises the flag for all: the code of a dozen timers is
-// what instruction fetches have no room for.
+// keeps the time, and raises the flag for all: the code of a dozen timers is
+// what instruction fetches have no room for.  The answer is the whole warp's: lanes that saw the
+// flag and lanes that saw the phase must not part, as what follows (tcgen05.ld and .st, shuffles)
+// needs them all.
 template <int NS>
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const ScanParams& p, volatile int* abort_flag) {
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   const uint32_t a = smem_u32(bar);
-  while (!mbar_try_wait(a, parity)) {
+  while (!__all_sync(0xFFFFFFFFu, mbar_try_wait(a, parity))) {
     __nanosleep(NS);
-    if (*abort_flag) return false;
+    if (__any_sync(0xFFFFFFFFu, *abort_flag != 0)) return false;
   }
   return true;
 }
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int s = n_bc & 1;
           const uint32_t st = sbase + s * L::kStage, par = ((n_bc >> 1) - 1) & 1;
           const bool first = n_bc < 2;
-          ok = first || wait_bar<kNapLoad>(STATES ? &bars->ds_full[s] : &bars->done[s], par, p, flag);
+          ok = first || wait_bar<kNapLoad>(STATES ? &bars->ds_full[s] : &bars->done[s], par, flag);
           if (!ok) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(&bars->full_bc[s], (STATES ? 1 : 2) * NA * kAtom);
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ++n_bc;
           if (!STATES) {
-            ok = first || wait_bar<kNapLoad>(&bars->xfree[s], par, p, flag);
+            ok = first || wait_bar<kNapLoad>(&bars->xfree[s], par, flag);
             if (!ok) break;
           }
           if (lane == 0) {
@@ -357,8 +359,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++n_x;
         }
       }
-      // after an abort, copies in flight land before the CTA leaves
-      if (*flag && lane == 0) {
+      // Copies in flight land before the CTA leaves, whichever role gives up and when; without
+      // that, all have been waited for by those that read them.
+      if (lane == 0) {
         const int n[2] = {n_bc, n_x};
 #pragma unroll 1
         for (int k = 0; k < 4; ++k) {  // full_bc, full_x, two of each
@@ -398,6 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       // usual one, with blocking waits, was a tenth slower).  A chunk's dS never goes before its
       // S: the commit behind dS gives B's place to H, and has to cover both products that read B.
       int s_next = STATES ? total : 0, cc = 0, sub = 0;
+      // the timer is slow to read: every so many idle turns, unless the limit is a short one
+      const uint32_t look = p.wait_limit_ns < 1000000ull ? 0u : 255u;
       uint32_t idle = 0;
       uint64_t t0 = 0;
       while (cc < total) {
@@ -457,12 +462,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (did) {
           idle = 0;
+          t0 = 0;
         } else {
           __nanosleep(kNapMma);
-          if ((++idle & 255u) == 0) {  // the timer is slow to read
+          if ((++idle & look) == 0) {
             if (__any_sync(0xFFFFFFFFu, *flag != 0)) break;
             const uint64_t now = globaltimer_ns();
-            if (idle == 256u) t0 = now;
+            if (t0 == 0) t0 = now;
             if (__any_sync(0xFFFFFFFFu, now - t0 > p.wait_limit_ns)) {
               *flag = 1;
               if (p.status && lane == 0) atomicOr(p.status, kDevErrTimeout | kWaitMma);
@@ -496,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int c = first; c < w.nc; c += 2) {
           const int cc = cc0 + c, b3 = cc % 3;
-          ok = cc < 3 || wait_bar<kNapDecay>(&bars->sc_free[b3], (cc / 3 - 1) & 1, p, flag);
+          ok = cc < 3 || wait_bar<kNapDecay>(&bars->sc_free[b3], (cc / 3 - 1) & 1, flag);
           if (!ok) break;
           Scal& sc = scal[b3];
           const long long left = w.sg.end - w.sg.begin - static_cast<long long>(c) * kQ - lane;
@@ -587,8 +593,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (c < w.nc) {
             const int cc = cc0 + c, b3 = cc % 3, s = cc & 1;
-            ok = wait_bar<kNapG>(&bars->sc_full[b3], (cc / 3) & 1, p, flag) &&
-                 wait_bar<kNapG>(&bars->s_full[s], (cc >> 1) & 1, p, flag);
+            ok = wait_bar<kNapG>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
+                 wait_bar<kNapG>(&bars->s_full[s], (cc >> 1) & 1, flag);
             if (!ok) break;
             tc_fence_after_sync();
             const Scal& sc = scal[b3];
@@ -641,8 +647,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (c > 0) {
             const int d = cc0 + c - 1, b3 = d % 3, s = d & 1;
-            ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, p, flag) &&
-                 wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, p, flag);
+            ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag) &&
+                 wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag);
             if (!ok) break;
             tc_fence_after_sync();
             // x's own row for D x.  Its place then takes z and after that y on their way between
@@ -720,11 +726,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int b3 = cc % 3, sb = cc & 1;
         const uint32_t st = sbase + sb * L::kStage;
         const int left = static_cast<int>(w.sg.end - w.sg.begin) - c * kQ;
-        ok = wait_bar<kNapXw>(&bars->sc_full[b3], (cc / 3) & 1, p, flag) &&
-             wait_bar<kNapXw>(&bars->full_x[sb], (cc >> 1) & 1, p, flag);
+        ok = wait_bar<kNapXw>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
+             wait_bar<kNapXw>(&bars->full_x[sb], (cc >> 1) & 1, flag);
         if (!ok) break;
         const float ws = scal[b3].f[3][s];
-        ok = cc < kDs || wait_bar<kNapXw>(&bars->ds_full[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1, p, flag);
+        ok = cc < kDs || wait_bar<kNapXw>(&bars->ds_full[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1, flag);
         if (!ok) break;
         const uint32_t xw = L::kXw + sb * L::kXwNext;
         const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
@@ -746,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (left < kQ) {
           // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-          ok = wait_bar<kNapXw>(&bars->full_bc[sb], (cc >> 1) & 1, p, flag);
+          ok = wait_bar<kNapXw>(&bars->full_bc[sb], (cc >> 1) & 1, flag);
           if (!ok) break;
           if (s >= left) {
 #pragma unroll 1
@@ -802,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < w.nc; ++c, ++cc) {
         const int b3 = cc % 3;
-        ok = wait_bar<kNapState>(&bars->ds_full[cc & 1], (cc >> 1) & 1, p, flag);
+        ok = wait_bar<kNapState>(&bars->ds_full[cc & 1], (cc >> 1) & 1, flag);
         if (!ok) break;
         if (!STATES) {
           // H, the state before the chunk, in the place of B, which has been read
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->h_full);
         }
-        ok = wait_bar<kNapState>(&bars->sc_full[b3], (cc / 3) & 1, p, flag);
+        ok = wait_bar<kNapState>(&bars->sc_full[b3], (cc / 3) & 1, flag);
         if (!ok) break;
         const float decay = scal[b3].total;
         log_sum += scal[b3].log2;

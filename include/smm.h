@@ -609,12 +609,12 @@ int smm_debug_trace_next(unsigned* trace);
  * (src/dsl/codegen_cuda.py:257-275). */
 int smm_debug_time_next(void* event_before, void* event_after);
 
-/* Failure-path test: the next tensor-core contraction kernel launched from
- * the calling thread gives each pipeline wait `wait_limit_ns` nanoseconds
- * instead of the default (SMM_WAIT_LIMIT_MS, 2000 ms when unset); teardown
+/* Failure-path test: the next tensor-core contraction kernel (or tensor-core
+ * selective scan, in all of its launches) launched from the calling thread
+ * gives each pipeline wait `wait_limit_ns` nanoseconds instead of the default (SMM_WAIT_LIMIT_MS, 2000 ms when unset); teardown
  * waits for copies and MMAs already issued keep at least one second.  A limit
  * shorter than the first TMA round trip makes the kernel give up, record
- * the expiry, write no output and exit cleanly; smm_device_status then
+ * the expiry, write no (a scan: not every) output and exit cleanly; smm_device_status then
  * returns SMM_ERR_DEVICE_TIMEOUT.  0 restores the default; at most 10 s. */
 int smm_debug_wait_limit_next(unsigned long long wait_limit_ns);
 

@@ -3,7 +3,7 @@ accuracy, decays, non-finite values, calls from several threads and streams, lim
 import pytest
 import torch
 
-from cpp1_b200 import ops
+from cpp1_b200 import _lib, ops
 from test_gpu_state_space import gen, i32, make_scan, offs, rnd, scan_ref, scan_tol, state_tol, within
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +72,29 @@ def test_bf16_scan_rounds_its_outputs_alone(cuda, lens, h, p, g_, n, with_state)
     # a rounding of the exact result, and 2^-16 of the terms beside it
     best = float((ref.to(BF).double() - ref).norm())
     assert float((y.double() - ref).norm()) <= best + 2.0 ** -16 * float(mag.norm())
+
+
+# ---------------------------------------------------------------- giving up
+@pytest.mark.parametrize("lens,h,n", [([700, 37, 260], 160, 128), ([100] * 40, 24, 64), ([6000], 2, 128), ([5000, 90], 3, 64)])
+def test_scan_that_gives_up_leaves_cleanly(cuda, lens, h, n):
+    """With a wait limit of a microsecond some wait of the tensor-core scan runs out: the
+    expiry is reported once, whatever was under way has landed, and the next call is right."""
+    L = _lib.load()
+    b = offs(lens)
+    a = make_scan(h, b[-1], h, 64, 1, n, "bf16")
+    assert on_tensor_cores(a, lens)
+    o = i32(b)
+    so = torch.empty(len(lens), h, 64, n, device="cuda")
+    y = ops.selective_scan(**a, offsets=o, state_out=so)
+    ops.device_status()
+    for _ in range(3):
+        so2 = torch.empty_like(so)
+        assert L.smm_debug_wait_limit_next(1000) == _lib.SMM_OK
+        ops.selective_scan(**a, offsets=o, state_out=so2)
+        with pytest.raises(_lib.SmmError) as e:
+            ops.device_status()
+        assert e.value.status == _lib.SMM_ERR_DEVICE_TIMEOUT
+        ops.device_status()  # consumed
+        y2 = ops.selective_scan(**a, offsets=o, state_out=so2)
+        ops.device_status()  # and the limit was for one call
+        assert torch.equal(y2, y) and torch.equal(so2, so)
