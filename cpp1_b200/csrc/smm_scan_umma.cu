@@ -11,11 +11,13 @@
 // next chunk's S and G are under way while this one's products run.
 //
 // Decays are products of factors exp(<= 0 when A <= 0) whose exponents are sums over
-// at most 128 tokens that lie between s and t, never differences of long sums:
-// within blocks of 32 tokens u_t = exp(sum from the block's start to t),
+// at most 128 tokens that lie between s and t: within blocks of 32 tokens
+// u_t = exp(sum from the block's start to t),
 // f[b][s] = d_s exp(sum from behind s to the start of block b).  G is S u_t f[b][s]
-// off the diagonal blocks, and exp(l_t - l_s) d_s on them, l being sums within
-// the block; w_s = f[4][s].  So a quarter of the exponentials remains.
+// off the diagonal blocks; w_s = f[4][s].  On the diagonal blocks it is exp(l_t - l_s) d_s, l being sums
+// within the block: differences, so a token's exponent is cut at -130 binary orders, below which its
+// factor is zero in any case, and l stays small enough for the tokens behind a
+// strong one (uncut, |d A| of 1e5 put an error of 1e-2 on them).  So a quarter of the exponentials remains.
 //
 // Roundings: G and H as operands of products are the sum of two bf16 terms (2^-17 of each
 // term of y, which is itself rounded to bf16; one term, 2^-9, added up to 1e-3 to y's error of
@@ -512,7 +514,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float d = 32 * b < left ? scan_dt(p, raw[0], bias) : 0.0f;
             raw[0] = raw[1], raw[1] = raw[2], raw[2] = raw[3];
             // sums within the block: inclusive up to the token, exclusive behind it
-            float inc = d * A2, suf = inc;
+            // 2^-130 counts as zero already; a stronger decay would only take bits from the sums
+            // whose differences are the decays of the tokens behind it
+            float inc = d * A2;
+            if (inc < -130.0f) inc = -130.0f;
+            float suf = inc;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
               const float x = __shfl_up_sync(0xFFFFFFFFu, inc, o), z = __shfl_down_sync(0xFFFFFFFFu, suf, o);

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from cpp1_b200 import _lib, ops
-from test_gpu_state_space import gen, i32, make_scan, offs, rnd, scan_ref, scan_tol, state_tol, within
+from test_gpu_state_space import TYPES, U, gen, i32, make_scan, offs, rnd, scan_ref, scan_tol, state_tol, within
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,33 @@ def test_scan_that_gives_up_leaves_cleanly(cuda, lens, h, n):
         y2 = ops.selective_scan(**a, offsets=o, state_out=so2)
         ops.device_status()  # and the limit was for one call
         assert torch.equal(y2, y) and torch.equal(so2, so)
+
+
+# ---------------------------------------------------------------- strong resets
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("strength", [1e3, 1e4, 1e5, 1e6, 1e9, 1e30])
+@pytest.mark.parametrize("empty", [False, True])
+def test_tokens_behind_a_reset(cuda, dtype, strength, empty):
+    """A token whose d A is large and negative forgets the state; what it adds itself (nothing, if
+    its x is zero) and the tokens behind it decay as they would without it."""
+    lens, h, n = [300, 140], 4, 128
+    b = offs(lens)
+    a = make_scan(3, b[-1], h, 64, 1, n, dtype, strided=False, dt_f32=True)
+    a["dt"] = 0.01 + 0.1 * torch.rand(b[-1], h, generator=gen(5), device="cuda")
+    a["dt_bias"], a["dt_softplus"] = None, False
+    a["A"] = torch.tensor([-1.0, -0.01, -8.0, -0.5], device="cuda")
+    resets = [0, 5, 37, 38, 64, 200, 255, 300 + 1, 300 + 70, 300 + 99]
+    for r in resets:
+        a["dt"][r] = strength
+        if empty:
+            a["x"][r] = 0
+    st = rnd(gen(4), 2, h, 64, n)
+    ref, mag, (fin, fmag) = scan_ref(a, b, st)
+    so = torch.empty_like(st)
+    y = ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so)
+    # Exponents within 32 tokens are differences of two sums of five additions each.  Two
+    # resets in a row count as 130 binary orders each at most, what is below is zero.
+    sums = 10 * U * 0.7 * (2 * 130 + 32 * 0.11 * 8 * 1.45)
+    tol = once_rounded_tol(ref, mag, n, 300, TYPES[dtype]) + (sums * mag if dtype == "bf16" else 0)
+    within(y, ref, tol, "y")
+    within(so, fin, state_tol(fin, fmag, 300, False) + sums * fmag, "state")
