@@ -83,6 +83,9 @@ struct Bars {
   uint64_t drain;
   uint32_t tmem;
   int abort_flag;
+  // Non-finite elements of x, by the chunk's parity: the last chunk that has one (plus 1), and by
+  // dim the chunk (x 256) and 128 less its first such row.  Higher is later, so nothing is reset.
+  uint32_t bad[2], bad_from[2][kP];
 };
 
 // NA: 64-wide tiles that state_dim takes (1 or 2).  The first launch of a split scan
@@ -304,6 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc(&bars->tmem, kCols);
+  if (warp >= 4 && threadIdx.x < 128 + 2 * kP) bars->bad_from[0][threadIdx.x - 128] = 0;
+  if (threadIdx.x >= 64 && threadIdx.x < 66) bars->bad[threadIdx.x - 64] = 0;
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -654,9 +659,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (c > 0) {
             const int d = cc0 + c - 1, b3 = d % 3, s = d & 1;
             ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag) &&
+                 wait_bar<kNapG>(&bars->xw_full[s], (d >> 1) & 1, flag) &&
                  wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag);
             if (!ok) break;
             tc_fence_after_sync();
+            const bool bad = bars->bad[s] == d + 1u;
             // x's own row for D x.  Its place then takes z and after that y on their way between
             // the layout of global memory and a row to a lane (a lane's own row of z and y
             // to and from global memory touched four times the lines).
@@ -697,6 +704,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
               *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
+            }
+            if (bad) {
+#pragma unroll 1
+              for (int i = 32 * half; i < 32 * half + 32; ++i) {
+                const uint32_t from = bars->bad_from[s][i];
+                if ((from >> 8) == d && t >= 128 - static_cast<int>(from & 255))
+                  *reinterpret_cast<unsigned short*>(xt + t * 128 + ((2 * i) ^ ((t & 7) << 4))) = 0x7FFF;
+              }
             }
             __syncwarp();
 #pragma unroll
@@ -740,6 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const uint32_t xw = L::kXw + sb * L::kXwNext;
         const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
+        unsigned long long chk = 0;  // stays zero while all products are finite
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t off = swz_offset(s, i0 + i, 128);
@@ -749,12 +765,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const unsigned long long v = mul2(w2, widen2(xs[k]));
+            if (!STATES) chk = fma2(v, 0ull, chk);
             vh[k] = narrow2(v);
             split2(fma2(neg, widen2(vh[k]), v), vm[k], vl[k]);
           }
           *reinterpret_cast<uint4*>(smem + xw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
           *reinterpret_cast<uint4*>(smem + xw + kAtom + off) = make_uint4(vm[0], vm[1], vm[2], vm[3]);
           *reinterpret_cast<uint4*>(smem + xw + 2 * kAtom + off) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
+        }
+        if (!STATES) {
+          // In G x every row of x meets zeros of G, for the tokens before it, and a non-finite
+          // element would pass them.  It is taken out here (the state gets it through Xw), and y is
+          // made NaN in its dim from its token on.
+          float c0, c1;
+          unpack2(chk, c0, c1);
+          if (c0 + c1 != 0.0f && s < left) {
+#pragma unroll 1
+            for (int e = 8 * i0; e < 8 * i0 + 32; ++e) {
+              unsigned short* x = reinterpret_cast<unsigned short*>(smem + sb * L::kStage + stage_x +
+                                                                    swz_offset(s, e / 8, 128) + 2 * (e % 8));
+              if ((*x & 0x7F80) != 0x7F80) continue;
+              *x = 0;
+              atomicMax(&bars->bad_from[sb][e], (static_cast<uint32_t>(cc) << 8) | (128u - s));
+              bars->bad[sb] = cc + 1u;
+            }
+          }
         }
         if (left < kQ) {
           // rows behind the sequence hold what lies there; a zero factor would not stop a NaN

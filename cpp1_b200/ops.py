@@ -608,8 +608,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     the tensor cores, where scores and states enter products as two bfloat16 terms (2^-17 relative).
 
     offsets, slots, out, state (entries, heads, dim, state_dim; float32) and state_out are as in causal_conv.
-    A non-finite input makes the rest of its sequence non-finite, and may
-    do so for up to 127 tokens before it."""
+    What depends on a non-finite input is not finite (NaN at times where an infinity would do); the
+    tokens before it do not depend on it."""
     tokens, heads, dim, groups, n, ty, dty = _scan_args(x, dt, A, B, C, D, z, dt_bias)
     state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out)
     offsets, nseq = _sequences(offsets, x)

@@ -522,8 +522,8 @@ int smm_causal_conv_step(const void* x, const void* w, const void* bias, const v
  * terms (2^-17 relative).  Which path a call takes goes by its sizes, so the last bits of a
  * sequence's outputs can differ between batches.
  *
- * A non-finite x, B, C or dt of a token makes the rest of its sequence
- * non-finite, and may do so for the up to 127 tokens before it as well.
+ * What depends on a non-finite x, B, C or dt of a token is not finite (NaN at times
+ * where an infinity would do); the tokens before it do not depend on it.
  *
  * The workspace holds the states between the parts that a long sequence is
  * split into (0 bytes: no split at these sizes).  No counterpart in the reference. */

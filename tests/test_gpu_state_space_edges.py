@@ -128,3 +128,58 @@ def test_tokens_behind_a_reset(cuda, dtype, strength, empty):
     tol = once_rounded_tol(ref, mag, n, 300, TYPES[dtype]) + (sums * mag if dtype == "bf16" else 0)
     within(y, ref, tol, "y")
     within(so, fin, state_tol(fin, fmag, 300, False) + sums * fmag, "state")
+
+
+# ---------------------------------------------------------------- non-finite inputs
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,h,p,n", [([140, 70, 300], 2, 64, 128), ([128, 128], 3, 128, 64), ([5, 9, 16], 4, 64, 16), ([6000], 2, 64, 128)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_non_finite_values_reach_no_token_before_them(cuda, dtype, lens, h, p, n, value):
+    """What does not depend on a non-finite element keeps its bits, what does is not finite."""
+    b = offs(lens)
+    t = b[-1]
+    dt = TYPES[dtype]
+    clean = make_scan(6, t, h, p, 1, n, dtype, strided=False, dt_f32=True)
+    st = rnd(gen(4), len(lens), h, p, n)
+
+    def call(a):
+        so = torch.empty_like(st)
+        return ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so), so
+
+    good, gst = call(clean)
+    seq = len(lens) - 1
+    toks = sorted({b[seq], b[seq] + 3, b[seq + 1] - 1, b[seq] + lens[seq] // 2})
+    for what in ("x", "B", "C", "dt", "z"):
+        a = dict(clean)
+        a[what] = clean[what].clone()
+        hit = torch.zeros(t, h, p, dtype=torch.bool, device="cuda")  # outputs that depend on it
+        hst = torch.zeros(h, p, n, dtype=torch.bool, device="cuda")
+        for i, k in enumerate(toks[1:3] if what in ("B", "dt") else toks):
+            head, dim = i % h, (7 * i + 3) % p
+            if what == "x":
+                a["x"][k, head, dim] = value
+                hit[k:, head, dim] = True
+                hst[head, dim] = True
+            elif what == "z":
+                a["z"][k, head, dim] = value
+                hit[k, head, dim] = True
+            elif what == "dt":
+                a["dt"][k, head] = float("nan")
+                hit[k:, head] = True
+                hst[head] = True
+            elif what == "B":
+                a["B"][k, 0, i] = value
+                hit[k:] = True
+                hst[:, :, i] = True
+            else:
+                a["C"][k, 0, i] = value
+                hit[k] = True
+        y, so = call(a)
+        if what == "z" and value == float("-inf"):
+            hit &= ~y.isfinite()  # a gate of minus infinity is zero at its limit, or no number
+        assert torch.equal(y[~hit], good[~hit]), what
+        assert not y[hit].isfinite().any(), what
+        assert torch.equal(so[:seq], gst[:seq])
+        assert torch.equal(so[seq][~hst], gst[seq][~hst]), what
+        assert not so[seq][hst].isfinite().any(), what
+    assert y.dtype == dt
