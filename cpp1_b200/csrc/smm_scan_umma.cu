@@ -247,7 +247,7 @@ __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y,
 // One (segment, head, 64 dims) of the work.
 struct Item {
   Segment sg;
-  int seg, h, p0, pdims, nc;  // nc: chunks
+  int seg, h, p0, pdims, nc;  // nc: chunks (none for the last segment in the first launch of a split scan)
   long long head_at;          // of this head's and these dims' state in an entry
   bool last;                  // the sequence's last segment
 };
@@ -270,7 +270,7 @@ __device__ __forceinline__ Item get_item(const ScanParams& p, int it, int ptiles
 // STATES: the first launch of a split scan (B, x and the state only).
 template <int NA, bool STATES>
 __global__ void __launch_bounds__(kThreads, 1)
-    scan_umma_kernel(const __grid_constant__ Tmaps maps, const ScanParams p, int items, int ptiles) {
+    scan_umma_kernel(const __grid_constant__ Tmaps maps, const ScanParams p, int ptiles) {
   using L = Smem<NA, STATES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -283,6 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int N = p.state_dim;
   const long long per_slot = static_cast<long long>(p.heads) * p.dim * N;
+  const Item w = get_item<STATES>(p, blockIdx.x, ptiles);
+  if (!w.sg.valid) return;  // the grid provides for more segments than there are
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -317,10 +319,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* const flag = &bars->abort_flag;
   constexpr uint32_t stage_c = L::kC, stage_b = L::kB, stage_x = L::kX;
   constexpr int kDs = STATES ? 2 : 1;  // places for Xw and dS: a chunk's is free kDs chunks later
-  const int it0 = blockIdx.x, its = gridDim.x;
 
-  // In every role below, c counts the chunks of an item and cc those of the CTA: stages,
-  // buffers and barriers' phases go by cc.
+  // In every role below, stages, buffers and barriers' phases go by the chunk c.
   //
   // The launch's 6 x 80 registers per warpgroup's thread, shared out by need.
   // A spill costs a trip to L2 here: shared memory leaves L1 too small for the stacks.
@@ -333,38 +333,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       // in the order in which the places become free: B and C after all products of their
       // chunk (in the first launch of a split scan after dS, the only one), x after its part in y
       int n_bc = 0, n_x = 0;  // loads issued
-      const int per_group = p.heads / p.groups;
       bool ok = true;
-      for (int it = it0; it < items && ok; it += its) {
-        const Item w = get_item<STATES>(p, it, ptiles);
-        const int g = w.h / per_group;
-        int row = static_cast<int>(w.sg.begin);
+      const int g = w.h / (p.heads / p.groups);
+      int row = static_cast<int>(w.sg.begin);
 #pragma unroll 1
-        for (int c = 0; c < w.nc; ++c, row += kQ) {
-          const int s = n_bc & 1;
-          const uint32_t st = sbase + s * L::kStage, par = ((n_bc >> 1) - 1) & 1;
-          const bool first = n_bc < 2;
-          ok = first || wait_bar<kNapLoad>(STATES ? &bars->ds_full[s] : &bars->done[s], par, flag);
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars->full_bc[s], (STATES ? 1 : 2) * NA * kAtom);
+      for (int c = 0; c < w.nc; ++c, row += kQ) {
+        const int s = c & 1;
+        const uint32_t st = sbase + s * L::kStage, par = ((c >> 1) - 1) & 1;
+        const bool first = c < 2;
+        ok = first || wait_bar<kNapLoad>(STATES ? &bars->ds_full[s] : &bars->done[s], par, flag);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->full_bc[s], (STATES ? 1 : 2) * NA * kAtom);
 #pragma unroll
-            for (int a = 0; a < NA; ++a) {
-              tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_bc[s], a * 64, g, row);
-              if (!STATES) tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_bc[s], a * 64, g, row);
-            }
+          for (int a = 0; a < NA; ++a) {
+            tma_load_3d(st + stage_b + a * kAtom, &maps.b, &bars->full_bc[s], a * 64, g, row);
+            if (!STATES) tma_load_3d(st + stage_c + a * kAtom, &maps.c, &bars->full_bc[s], a * 64, g, row);
           }
-          ++n_bc;
-          if (!STATES) {
-            ok = first || wait_bar<kNapLoad>(&bars->xfree[s], par, flag);
-            if (!ok) break;
-          }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
-            tma_load_3d(st + stage_x, &maps.x, &bars->full_x[s], w.p0, w.h, row);
-          }
-          ++n_x;
         }
+        ++n_bc;
+        if (!STATES) {
+          ok = first || wait_bar<kNapLoad>(&bars->xfree[s], par, flag);
+          if (!ok) break;
+        }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->full_x[s], kAtom);
+          tma_load_3d(st + stage_x, &maps.x, &bars->full_x[s], w.p0, w.h, row);
+        }
+        ++n_x;
       }
       // Copies in flight land before the CTA leaves, whichever role gives up and when; without
       // that, all have been waited for by those that read them.
@@ -383,8 +379,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idD = make_idesc(kFmtBF16, 128, kP, 1, 1);
       const uint32_t ksteps = (N + 15) / 16;
       const uint32_t leader = elect_one();
-      int total = 0;
-      for (int it = it0; it < items; it += its) total += get_item<STATES>(p, it, ptiles).nc;
       // descriptors of stage 0; a stage is kSt further.  Only the low word, the
       // start address in 16-byte units, changes with stage and step.
       constexpr uint32_t kSt = L::kStage >> 4;
@@ -407,18 +401,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Whatever has its operands: S up to a chunk ahead of the rest (the order fixed at its
       // usual one, with blocking waits, was a tenth slower).  A chunk's dS never goes before its
       // S: the commit behind dS gives B's place to H, and has to cover both products that read B.
-      int s_next = STATES ? total : 0, cc = 0, sub = 0;
+      int s_next = STATES ? w.nc : 0, c = 0, sub = 0;
       // the timer is slow to read: every so many idle turns, unless the limit is a short one
       const uint32_t look = p.wait_limit_ns < 1000000ull ? 0u : 255u;
       uint32_t idle = 0;
       uint64_t t0 = 0;
-      while (cc < total) {
+      while (c < w.nc) {
         bool did = true;
-        const int s = cc & 1;
-        const uint32_t par = (cc >> 1) & 1;
+        const int s = c & 1;
+        const uint32_t par = (c >> 1) & 1;
         const uint32_t xw = lo(dM) + s * (L::kXwNext >> 4), ds = tmem + kColDs + (STATES ? s * kP : 0);
-        if (!STATES && s_next < total && s_next < cc + 2 && ready(&bars->full_bc[s_next & 1], (s_next >> 1) & 1)) {
-          // C was loaded once every product of chunk cc - 2 was done: S's place, where its G was, is free
+        if (!STATES && s_next < w.nc && s_next < c + 2 && ready(&bars->full_bc[s_next & 1], (s_next >> 1) & 1)) {
+          // C was loaded once every product of chunk c - 2 was done: S's place, where its G was, is free
           tc_fence_after_sync();
           const int sn = s_next & 1;
           const uint32_t base = lo(dK) + sn * kSt;
@@ -430,8 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           });
           umma_commit_by(leader, &bars->s_full[sn]);
           ++s_next;
-        } else if (sub == 0 && s_next > cc && ready(&bars->xw_full[s], par) &&
-                   (cc < kDs || ready(&bars->ds_free[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1)) &&
+        } else if (sub == 0 && s_next > c && ready(&bars->xw_full[s], par) &&
+                   (c < kDs || ready(&bars->ds_free[(c - kDs) & 1], ((c - kDs) >> 1) & 1)) &&
                    ready(&bars->full_bc[s], par) && ready(&bars->full_x[s], par)) {
           tc_fence_after_sync();
           ds_term(s, xw, ds, std::integral_constant<int, 0>{});
@@ -439,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ds_term(s, xw, ds, std::integral_constant<int, 2>{});
           umma_commit_by(leader, &bars->ds_full[s]);
           if (STATES)
-            ++cc;
+            ++c;
           else
             sub = 1;
         } else if (sub == 1 && ready(&bars->g_full[s], par)) {
@@ -451,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 leader, tmem + kColY + s * kP, tmem + kColS + s * 128, base, hM, idY);
           });
           sub = 2;
-        } else if (sub == 2 && ready(&bars->h_full, cc & 1) && (cc == 0 || ready(&bars->yo_free, (cc - 1) & 1))) {
+        } else if (sub == 2 && ready(&bars->h_full, c & 1) && (c == 0 || ready(&bars->yo_free, (c - 1) & 1))) {
           tc_fence_after_sync();
           const uint32_t base = lo(dK) + s * kSt, base_h = lo(dM) + s * kSt;
           steps<8 * NA>([&](auto kc) {  // both terms of H
@@ -463,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           });
           umma_commit_by(leader, &bars->done[s]);
           sub = 0;
-          ++cc;
+          ++c;
         } else {
           did = false;
         }
@@ -489,79 +483,74 @@ __global__ void __launch_bounds__(kThreads, 1)
       drain_bar(&bars->drain, 0, p, flag);
     } else {
       // ---------------------------------------------------------- decays
-      // lane -> token 32 b + lane of each block b; even chunks of the stream by warp 2, odd ones by warp 3
-      int cc0 = 0;
+      // lane -> token 32 b + lane of each block b; even chunks by warp 2, odd ones by warp 3
       bool ok = true;
-      for (int it = it0; it < items && ok; it += its) {
-        const Item w = get_item<STATES>(p, it, ptiles);
-        const float A2 = w.nc > 0 ? __ldg(p.A + w.h) * kLog2e : 0.0f;
-        const float bias = w.nc > 0 && p.dt_bias ? __ldg(p.dt_bias + w.h) : 0.0f;
-        uint32_t raw[4] = {};
-        auto fetch = [&](int c) {
+      const float A2 = __ldg(p.A + w.h) * kLog2e;
+      const float bias = p.dt_bias ? __ldg(p.dt_bias + w.h) : 0.0f;
+      uint32_t raw[4] = {};
+      auto fetch = [&](int c) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const long long t = w.sg.begin + static_cast<long long>(c) * kQ + 32 * i + lane;
-            if (t < w.sg.end) raw[i] = scan_dt_raw(p, t, w.h);
-          }
-        };
-        const int first = (cc0 & 1) == (warp & 1) ? 0 : 1;
-        if (first < w.nc) fetch(first);
-#pragma unroll 1
-        for (int c = first; c < w.nc; c += 2) {
-          const int cc = cc0 + c, b3 = cc % 3;
-          ok = cc < 3 || wait_bar<kNapDecay>(&bars->sc_free[b3], (cc / 3 - 1) & 1, flag);
-          if (!ok) break;
-          Scal& sc = scal[b3];
-          const long long left = w.sg.end - w.sg.begin - static_cast<long long>(c) * kQ - lane;
-          float bt[4], head = 0.0f;
-#pragma unroll 1
-          for (int b = 0; b < 4; ++b) {
-            const float d = 32 * b < left ? scan_dt(p, raw[0], bias) : 0.0f;
-            raw[0] = raw[1], raw[1] = raw[2], raw[2] = raw[3];
-            // sums within the block: inclusive up to the token, exclusive behind it
-            // 2^-130 counts as zero already; a stronger decay would only take bits from the sums
-            // whose differences are the decays of the tokens behind it
-            float inc = d * A2;
-            if (inc < -130.0f) inc = -130.0f;
-            float suf = inc;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const float x = __shfl_up_sync(0xFFFFFFFFu, inc, o), z = __shfl_down_sync(0xFFFFFFFFu, suf, o);
-              if (lane >= o) inc += x;
-              if (lane + o < 32) suf += z;
-            }
-            bt[0] = bt[1], bt[1] = bt[2], bt[2] = bt[3], bt[3] = __shfl_sync(0xFFFFFFFFu, inc, 31);
-            suf = __shfl_down_sync(0xFFFFFFFFu, suf, 1);
-            const int t = 32 * b + lane;
-            sc.l[t] = inc;
-            sc.u[t] = ex2(inc);
-            sc.e[t] = ex2(head + inc);
-            sc.d[t] = d;
-            sc.f[3][t] = lane < 31 ? suf : 0.0f;  // the exponent, until the blocks' sums are known
-            head += bt[3];
-          }
-          if (c + 2 < w.nc) fetch(c + 2);
-#pragma unroll 1
-          for (int b = 0; b < 4; ++b) {
-            const int t = 32 * b + lane;
-            const float suf = sc.f[3][t], d = sc.d[t];
-            float between = 0.0f;
-#pragma unroll
-            for (int k = 1; k <= 4; ++k) {
-              if (k > b) {
-                if (k - 1 > b) between += bt[k - 1];
-                sc.f[k - 1][t] = d * ex2(suf + between);
-              }
-            }
-          }
-          if (lane == 0) {
-            sc.total = ex2(head);
-            sc.log2 = head;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->sc_full[b3]);
+        for (int i = 0; i < 4; ++i) {
+          const long long t = w.sg.begin + static_cast<long long>(c) * kQ + 32 * i + lane;
+          if (t < w.sg.end) raw[i] = scan_dt_raw(p, t, w.h);
         }
-        cc0 += w.nc;
+      };
+      const int first = warp & 1;
+      if (first < w.nc) fetch(first);
+#pragma unroll 1
+      for (int c = first; c < w.nc; c += 2) {
+        const int b3 = c % 3;
+        ok = c < 3 || wait_bar<kNapDecay>(&bars->sc_free[b3], (c / 3 - 1) & 1, flag);
+        if (!ok) break;
+        Scal& sc = scal[b3];
+        const long long left = w.sg.end - w.sg.begin - static_cast<long long>(c) * kQ - lane;
+        float bt[4], head = 0.0f;
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          const float d = 32 * b < left ? scan_dt(p, raw[0], bias) : 0.0f;
+          raw[0] = raw[1], raw[1] = raw[2], raw[2] = raw[3];
+          // sums within the block: inclusive up to the token, exclusive behind it
+          // 2^-130 counts as zero already; a stronger decay would only take bits from the sums
+          // whose differences are the decays of the tokens behind it
+          float inc = d * A2;
+          if (inc < -130.0f) inc = -130.0f;
+          float suf = inc;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const float x = __shfl_up_sync(0xFFFFFFFFu, inc, o), z = __shfl_down_sync(0xFFFFFFFFu, suf, o);
+            if (lane >= o) inc += x;
+            if (lane + o < 32) suf += z;
+          }
+          bt[0] = bt[1], bt[1] = bt[2], bt[2] = bt[3], bt[3] = __shfl_sync(0xFFFFFFFFu, inc, 31);
+          suf = __shfl_down_sync(0xFFFFFFFFu, suf, 1);
+          const int t = 32 * b + lane;
+          sc.l[t] = inc;
+          sc.u[t] = ex2(inc);
+          sc.e[t] = ex2(head + inc);
+          sc.d[t] = d;
+          sc.f[3][t] = lane < 31 ? suf : 0.0f;  // the exponent, until the blocks' sums are known
+          head += bt[3];
+        }
+        if (c + 2 < w.nc) fetch(c + 2);
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          const int t = 32 * b + lane;
+          const float suf = sc.f[3][t], d = sc.d[t];
+          float between = 0.0f;
+#pragma unroll
+          for (int k = 1; k <= 4; ++k) {
+            if (k > b) {
+              if (k - 1 > b) between += bt[k - 1];
+              sc.f[k - 1][t] = d * ex2(suf + between);
+            }
+          }
+        }
+        if (lane == 0) {
+          sc.total = ex2(head);
+          sc.log2 = head;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->sc_full[b3]);
       }
     }
   } else if (warp < 12) {
@@ -575,162 +564,156 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool gated = p.z != nullptr;
       const long long zstep = 8 * p.ldz, ystep = 8 * p.ldy;  // eight rows
       const int col8 = 8 * (lane & 3);
-      int cc0 = 0;
       bool ok = true;
-      for (int it = it0; it < items && ok; it += its) {
-        const Item w = get_item<STATES>(p, it, ptiles);
-        if (w.nc == 0) continue;
-        const float Dh = p.D ? __ldg(p.D + w.h) : 0.0f;
-        const unsigned long long D2 = pack2(Dh, Dh);
-        const long long col = static_cast<long long>(w.h) * p.dim + w.p0 + 32 * half;
-        const long long row = w.sg.begin + 32 * q + (lane >> 2);
-        const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + row * p.ldz + col + col8;
-        __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + row * p.ldy + col + col8;
-        const int rows = static_cast<int>(w.sg.end - w.sg.begin);
-        const int wdims = w.pdims - 32 * half;  // columns of this half
+      const float Dh = p.D ? __ldg(p.D + w.h) : 0.0f;
+      const unsigned long long D2 = pack2(Dh, Dh);
+      const long long col = static_cast<long long>(w.h) * p.dim + w.p0 + 32 * half;
+      const long long row = w.sg.begin + 32 * q + (lane >> 2);
+      const __nv_bfloat16* gz = static_cast<const __nv_bfloat16*>(p.z) + row * p.ldz + col + col8;
+      __nv_bfloat16* gy = static_cast<__nv_bfloat16*>(p.y) + row * p.ldy + col + col8;
+      const int rows = static_cast<int>(w.sg.end - w.sg.begin);
+      const int wdims = w.pdims - 32 * half;  // columns of this half
 #pragma unroll 1
-        for (int c = 0; c <= w.nc; ++c) {
-          // z of the chunk before, on its way while G is formed: four lanes to the 64 bytes of
-          // a row, eight rows at a time
-          uint4 zv[4];
-          const int r0 = (c - 1) * kQ + 32 * q + (lane >> 2);  // this lane's first row in the segment
-          if (gated && c > 0) {
-            const __nv_bfloat16* zr = gz;
+      for (int c = 0; c <= w.nc; ++c) {
+        // z of the chunk before, on its way while G is formed: four lanes to the 64 bytes of
+        // a row, eight rows at a time
+        uint4 zv[4];
+        const int r0 = (c - 1) * kQ + 32 * q + (lane >> 2);  // this lane's first row in the segment
+        if (gated && c > 0) {
+          const __nv_bfloat16* zr = gz;
 #pragma unroll
-            for (int i = 0; i < 4; ++i, zr += zstep)
-              zv[i] = col8 < wdims && r0 + 8 * i < rows ? __ldg(reinterpret_cast<const uint4*>(zr))
-                                                        : make_uint4(0, 0, 0, 0);
-            gz = zr + 12 * zstep;
-          }
-          if (c < w.nc) {
-            const int cc = cc0 + c, b3 = cc % 3, s = cc & 1;
-            ok = wait_bar<kNapG>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
-                 wait_bar<kNapG>(&bars->s_full[s], (cc >> 1) & 1, flag);
-            if (!ok) break;
-            tc_fence_after_sync();
-            const Scal& sc = scal[b3];
-            const float u = sc.u[t], lt = sc.l[t];
-            const uint32_t sS = tmem + lanes + kColS + s * 128 + 64 * half;
+          for (int i = 0; i < 4; ++i, zr += zstep)
+            zv[i] = col8 < wdims && r0 + 8 * i < rows ? __ldg(reinterpret_cast<const uint4*>(zr))
+                                                      : make_uint4(0, 0, 0, 0);
+          gz = zr + 12 * zstep;
+        }
+        if (c < w.nc) {
+          const int b3 = c % 3, s = c & 1;
+          ok = wait_bar<kNapG>(&bars->sc_full[b3], (c / 3) & 1, flag) &&
+               wait_bar<kNapG>(&bars->s_full[s], (c >> 1) & 1, flag);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const Scal& sc = scal[b3];
+          const float u = sc.u[t], lt = sc.l[t];
+          const uint32_t sS = tmem + lanes + kColS + s * 128 + 64 * half;
 #pragma unroll 1
-            for (int i2 = 0; i2 < 2; ++i2) {
-              const int b = 2 * half + i2;  // block of 32 columns: off the diagonal for b < q
-              uint32_t o[16], ol[16];        // G's first and second term
-              if (b <= q) {
-                uint32_t r[32];
-                tmem_ld_32x32b_x32(sS + 32 * i2, r);
-                const unsigned long long* f =
-                    reinterpret_cast<const unsigned long long*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
-                if (b < q) {
-                  const unsigned long long u2 = pack2(u, u);
-                  tmem_wait_ld();
+          for (int i2 = 0; i2 < 2; ++i2) {
+            const int b = 2 * half + i2;  // block of 32 columns: off the diagonal for b < q
+            uint32_t o[16], ol[16];        // G's first and second term
+            if (b <= q) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(sS + 32 * i2, r);
+              const unsigned long long* f =
+                  reinterpret_cast<const unsigned long long*>((b < q ? sc.f[q - 1] : sc.d) + 32 * b);
+              if (b < q) {
+                const unsigned long long u2 = pack2(u, u);
+                tmem_wait_ld();
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const unsigned long long s2 = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                    split2(mul2(mul2(s2, f[i]), u2), o[i], ol[i]);
-                  }
-                } else {
-                  const unsigned long long* ls = reinterpret_cast<const unsigned long long*>(sc.l + 32 * b);
-                  const unsigned long long lt2 = pack2(lt, lt), neg = pack2(-1.0f, -1.0f);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    // Columns up to this row.  The factors are formed for all of them and the rest is
-                    // selected away: an exponential inside a condition becomes a branch of its own.
-                    float a, z;
-                    unpack2(fma2(ls[i], neg, lt2), a, z);
-                    const unsigned long long w2 = mul2(pack2(ex2(a), ex2(z)), f[i]);
-                    unpack2(mul2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), w2), a, z);
-                    split2(pack2(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f), o[i], ol[i]);
-                  }
+                for (int i = 0; i < 16; ++i) {
+                  const unsigned long long s2 = pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                  split2(mul2(mul2(s2, f[i]), u2), o[i], ol[i]);
                 }
               } else {
+                const unsigned long long* ls = reinterpret_cast<const unsigned long long*>(sc.l + 32 * b);
+                const unsigned long long lt2 = pack2(lt, lt), neg = pack2(-1.0f, -1.0f);
+                tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = ol[i] = 0;
+                for (int i = 0; i < 16; ++i) {
+                  // Columns up to this row.  The factors are formed for all of them and the rest is
+                  // selected away: an exponential inside a condition becomes a branch of its own.
+                  float a, z;
+                  unpack2(fma2(ls[i], neg, lt2), a, z);
+                  const unsigned long long w2 = mul2(pack2(ex2(a), ex2(z)), f[i]);
+                  unpack2(mul2(pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), w2), a, z);
+                  split2(pack2(2 * i <= lane ? a : 0.0f, 2 * i + 1 <= lane ? z : 0.0f), o[i], ol[i]);
+                }
               }
-              // these columns of S have been read by this lane already
-              tmem_st_32x32b_x16(sS + 32 * i2, o);
-              tmem_st_32x32b_x16(sS + 32 * i2 + 16, ol);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = ol[i] = 0;
             }
-            tmem_wait_st();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->g_full[s]);
+            // these columns of S have been read by this lane already
+            tmem_st_32x32b_x16(sS + 32 * i2, o);
+            tmem_st_32x32b_x16(sS + 32 * i2 + 16, ol);
           }
-          if (c > 0) {
-            const int d = cc0 + c - 1, b3 = d % 3, s = d & 1;
-            ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag) &&
-                 wait_bar<kNapG>(&bars->xw_full[s], (d >> 1) & 1, flag) &&
-                 wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag);
-            if (!ok) break;
-            tc_fence_after_sync();
-            const bool bad = bars->bad[s] == d + 1u;
-            // x's own row for D x.  Its place then takes z and after that y on their way between
-            // the layout of global memory and a row to a lane (a lane's own row of z and y
-            // to and from global memory touched four times the lines).
-            uint8_t* xt = smem + s * L::kStage + stage_x;
-            uint4 xv[4];
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->g_full[s]);
+        }
+        if (c > 0) {
+          const int d = c - 1, b3 = d % 3, s = d & 1;
+          ok = wait_bar<kNapG>(&bars->full_x[s], (d >> 1) & 1, flag) &&
+               wait_bar<kNapG>(&bars->xw_full[s], (d >> 1) & 1, flag) &&
+               wait_bar<kNapG>(&bars->done[s], (d >> 1) & 1, flag);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const bool bad = bars->bad[s] == d + 1u;
+          // x's own row for D x.  Its place then takes z and after that y on their way between
+          // the layout of global memory and a row to a lane (a lane's own row of z and y
+          // to and from global memory touched four times the lines).
+          uint8_t* xt = smem + s * L::kStage + stage_x;
+          uint4 xv[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) xv[i] = *reinterpret_cast<const uint4*>(xt + swz_offset(t, 4 * half + i, 128));
-            const float e = scal[b3].e[t];
-            const unsigned long long e2 = pack2(e, e);
-            const uint32_t sY = tmem + lanes + kColY + s * kP + 32 * half;
+          for (int i = 0; i < 4; ++i) xv[i] = *reinterpret_cast<const uint4*>(xt + swz_offset(t, 4 * half + i, 128));
+          const float e = scal[b3].e[t];
+          const unsigned long long e2 = pack2(e, e);
+          const uint32_t sY = tmem + lanes + kColY + s * kP + 32 * half;
+          __syncwarp();
+          if (gated) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(xt + swz_offset(32 * q + 8 * i + (lane >> 2), 4 * half + (lane & 3), 128)) = zv[i];
             __syncwarp();
+          }
+#pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            uint32_t ry[16], ro[16], out[8], zw[8];
+            tmem_ld_32x32b_x16(sY + 16 * k, ry);
+            tmem_ld_32x32b_x16(sYo + 16 * k, ro);
+            const uint32_t o0 = swz_offset(t, 4 * half + 2 * k, 128), o1 = swz_offset(t, 4 * half + 2 * k + 1, 128);
+            const uint32_t xw[8] = {xv[0].x, xv[0].y, xv[0].z, xv[0].w, xv[1].x, xv[1].y, xv[1].z, xv[1].w};
+            xv[0] = xv[2], xv[1] = xv[3];
             if (gated) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint4*>(xt + swz_offset(32 * q + 8 * i + (lane >> 2), 4 * half + (lane & 3), 128)) = zv[i];
-              __syncwarp();
+              *reinterpret_cast<uint4*>(zw) = *reinterpret_cast<const uint4*>(xt + o0);
+              *reinterpret_cast<uint4*>(zw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
             }
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              unsigned long long v = fma2(e2, pack2(__uint_as_float(ro[2 * i]), __uint_as_float(ro[2 * i + 1])),
+                                          pack2(__uint_as_float(ry[2 * i]), __uint_as_float(ry[2 * i + 1])));
+              v = fma2(D2, widen2(xw[i]), v);
+              if (gated) v = mul2(v, silu2(widen2(zw[i])));
+              out[i] = narrow2(v);
+            }
+            *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
+            *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
+          }
+          if (bad) {
 #pragma unroll 1
-            for (int k = 0; k < 2; ++k) {
-              uint32_t ry[16], ro[16], out[8], zw[8];
-              tmem_ld_32x32b_x16(sY + 16 * k, ry);
-              tmem_ld_32x32b_x16(sYo + 16 * k, ro);
-              const uint32_t o0 = swz_offset(t, 4 * half + 2 * k, 128), o1 = swz_offset(t, 4 * half + 2 * k + 1, 128);
-              const uint32_t xw[8] = {xv[0].x, xv[0].y, xv[0].z, xv[0].w, xv[1].x, xv[1].y, xv[1].z, xv[1].w};
-              xv[0] = xv[2], xv[1] = xv[3];
-              if (gated) {
-                *reinterpret_cast<uint4*>(zw) = *reinterpret_cast<const uint4*>(xt + o0);
-                *reinterpret_cast<uint4*>(zw + 4) = *reinterpret_cast<const uint4*>(xt + o1);
-              }
-              tmem_wait_ld();
+            for (int i = 32 * half; i < 32 * half + 32; ++i) {
+              const uint32_t from = bars->bad_from[s][i];
+              if ((from >> 8) == d && t >= 128 - static_cast<int>(from & 255))
+                *reinterpret_cast<unsigned short*>(xt + t * 128 + ((2 * i) ^ ((t & 7) << 4))) = 0x7FFF;
+            }
+          }
+          __syncwarp();
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                unsigned long long v = fma2(e2, pack2(__uint_as_float(ro[2 * i]), __uint_as_float(ro[2 * i + 1])),
-                                            pack2(__uint_as_float(ry[2 * i]), __uint_as_float(ry[2 * i + 1])));
-                v = fma2(D2, widen2(xw[i]), v);
-                if (gated) v = mul2(v, silu2(widen2(zw[i])));
-                out[i] = narrow2(v);
-              }
-              *reinterpret_cast<uint4*>(xt + o0) = make_uint4(out[0], out[1], out[2], out[3]);
-              *reinterpret_cast<uint4*>(xt + o1) = make_uint4(out[4], out[5], out[6], out[7]);
-            }
-            if (bad) {
-#pragma unroll 1
-              for (int i = 32 * half; i < 32 * half + 32; ++i) {
-                const uint32_t from = bars->bad_from[s][i];
-                if ((from >> 8) == d && t >= 128 - static_cast<int>(from & 255))
-                  *reinterpret_cast<unsigned short*>(xt + t * 128 + ((2 * i) ^ ((t & 7) << 4))) = 0x7FFF;
-              }
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i, gy += ystep)
-              if (col8 < wdims && r0 + 8 * i < rows)
-                *reinterpret_cast<uint4*>(gy) =
-                    *reinterpret_cast<const uint4*>(xt + swz_offset(32 * q + 8 * i + (lane >> 2), 4 * half + (lane & 3), 128));
-            gy += 12 * ystep;
-            fence_proxy_async_smem();  // the tile's next content comes by TMA
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(&bars->yo_free);
-              mbar_arrive(&bars->xfree[s]);
-              mbar_arrive(&bars->sc_free[b3]);
-            }
+          for (int i = 0; i < 4; ++i, gy += ystep)
+            if (col8 < wdims && r0 + 8 * i < rows)
+              *reinterpret_cast<uint4*>(gy) =
+                  *reinterpret_cast<const uint4*>(xt + swz_offset(32 * q + 8 * i + (lane >> 2), 4 * half + (lane & 3), 128));
+          gy += 12 * ystep;
+          fence_proxy_async_smem();  // the tile's next content comes by TMA
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bars->yo_free);
+            mbar_arrive(&bars->xfree[s]);
+            mbar_arrive(&bars->sc_free[b3]);
           }
         }
-        cc0 += w.nc;
       }
     }
   } else if (warp < 20) {
@@ -738,82 +721,78 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ Xw
     const int s = (threadIdx.x - 384) & 127;     // row
     const int i0 = warp < 16 ? 0 : 4;            // first of this thread's 16-byte pieces
-    int cc = 0;
     bool ok = true;
-    for (int it = it0; it < items && ok; it += its) {
-      const Item w = get_item<STATES>(p, it, ptiles);
 #pragma unroll 1
-      for (int c = 0; c < w.nc; ++c, ++cc) {
-        const int b3 = cc % 3, sb = cc & 1;
-        const uint32_t st = sbase + sb * L::kStage;
-        const int left = static_cast<int>(w.sg.end - w.sg.begin) - c * kQ;
-        ok = wait_bar<kNapXw>(&bars->sc_full[b3], (cc / 3) & 1, flag) &&
-             wait_bar<kNapXw>(&bars->full_x[sb], (cc >> 1) & 1, flag);
+    for (int c = 0; c < w.nc; ++c) {
+      const int b3 = c % 3, sb = c & 1;
+      const uint32_t st = sbase + sb * L::kStage;
+      const int left = static_cast<int>(w.sg.end - w.sg.begin) - c * kQ;
+      ok = wait_bar<kNapXw>(&bars->sc_full[b3], (c / 3) & 1, flag) &&
+           wait_bar<kNapXw>(&bars->full_x[sb], (c >> 1) & 1, flag);
+      if (!ok) break;
+      const float ws = scal[b3].f[3][s];
+      ok = c < kDs || wait_bar<kNapXw>(&bars->ds_full[(c - kDs) & 1], ((c - kDs) >> 1) & 1, flag);
+      if (!ok) break;
+      const uint32_t xw = L::kXw + sb * L::kXwNext;
+      const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
+      unsigned long long chk = 0;  // stays zero while all products are finite
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t off = swz_offset(s, i0 + i, 128);
+        const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+        uint32_t vh[4], vm[4], vl[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned long long v = mul2(w2, widen2(xs[k]));
+          if (!STATES) chk = fma2(v, 0ull, chk);
+          vh[k] = narrow2(v);
+          split2(fma2(neg, widen2(vh[k]), v), vm[k], vl[k]);
+        }
+        *reinterpret_cast<uint4*>(smem + xw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
+        *reinterpret_cast<uint4*>(smem + xw + kAtom + off) = make_uint4(vm[0], vm[1], vm[2], vm[3]);
+        *reinterpret_cast<uint4*>(smem + xw + 2 * kAtom + off) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
+      }
+      if (!STATES) {
+        // In G x every row of x meets zeros of G, for the tokens before it, and a non-finite
+        // element would pass them.  It is taken out here (the state gets it through Xw), and y is
+        // made NaN in its dim from its token on.
+        float c0, c1;
+        unpack2(chk, c0, c1);
+        if (c0 + c1 != 0.0f && s < left) {
+#pragma unroll 1
+          for (int e = 8 * i0; e < 8 * i0 + 32; ++e) {
+            unsigned short* x = reinterpret_cast<unsigned short*>(smem + sb * L::kStage + stage_x +
+                                                                  swz_offset(s, e / 8, 128) + 2 * (e % 8));
+            if ((*x & 0x7F80) != 0x7F80) continue;
+            *x = 0;
+            atomicMax(&bars->bad_from[sb][e], (static_cast<uint32_t>(c) << 8) | (128u - s));
+            bars->bad[sb] = c + 1u;
+          }
+        }
+      }
+      if (left < kQ) {
+        // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
+        ok = wait_bar<kNapXw>(&bars->full_bc[sb], (c >> 1) & 1, flag);
         if (!ok) break;
-        const float ws = scal[b3].f[3][s];
-        ok = cc < kDs || wait_bar<kNapXw>(&bars->ds_full[(cc - kDs) & 1], ((cc - kDs) >> 1) & 1, flag);
-        if (!ok) break;
-        const uint32_t xw = L::kXw + sb * L::kXwNext;
-        const unsigned long long w2 = pack2(ws, ws), neg = pack2(-1.0f, -1.0f);
-        unsigned long long chk = 0;  // stays zero while all products are finite
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t off = swz_offset(s, i0 + i, 128);
-          const uint4 x = *reinterpret_cast<const uint4*>(smem + sb * L::kStage + stage_x + off);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-          uint32_t vh[4], vm[4], vl[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const unsigned long long v = mul2(w2, widen2(xs[k]));
-            if (!STATES) chk = fma2(v, 0ull, chk);
-            vh[k] = narrow2(v);
-            split2(fma2(neg, widen2(vh[k]), v), vm[k], vl[k]);
-          }
-          *reinterpret_cast<uint4*>(smem + xw + off) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
-          *reinterpret_cast<uint4*>(smem + xw + kAtom + off) = make_uint4(vm[0], vm[1], vm[2], vm[3]);
-          *reinterpret_cast<uint4*>(smem + xw + 2 * kAtom + off) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
-        }
-        if (!STATES) {
-          // In G x every row of x meets zeros of G, for the tokens before it, and a non-finite
-          // element would pass them.  It is taken out here (the state gets it through Xw), and y is
-          // made NaN in its dim from its token on.
-          float c0, c1;
-          unpack2(chk, c0, c1);
-          if (c0 + c1 != 0.0f && s < left) {
+        if (s >= left) {
 #pragma unroll 1
-            for (int e = 8 * i0; e < 8 * i0 + 32; ++e) {
-              unsigned short* x = reinterpret_cast<unsigned short*>(smem + sb * L::kStage + stage_x +
-                                                                    swz_offset(s, e / 8, 128) + 2 * (e % 8));
-              if ((*x & 0x7F80) != 0x7F80) continue;
-              *x = 0;
-              atomicMax(&bars->bad_from[sb][e], (static_cast<uint32_t>(cc) << 8) | (128u - s));
-              bars->bad[sb] = cc + 1u;
-            }
-          }
-        }
-        if (left < kQ) {
-          // rows behind the sequence hold what lies there; a zero factor would not stop a NaN
-          ok = wait_bar<kNapXw>(&bars->full_bc[sb], (cc >> 1) & 1, flag);
-          if (!ok) break;
-          if (s >= left) {
-#pragma unroll 1
-            for (int i = i0; i < i0 + 4; ++i) {
-              const uint32_t off = swz_offset(s, i, 128);
-              st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
-              st_shared_v4(sbase + xw + off, 0, 0, 0, 0);
-              st_shared_v4(sbase + xw + kAtom + off, 0, 0, 0, 0);
-              st_shared_v4(sbase + xw + 2 * kAtom + off, 0, 0, 0, 0);
+          for (int i = i0; i < i0 + 4; ++i) {
+            const uint32_t off = swz_offset(s, i, 128);
+            st_shared_v4(st + stage_x + off, 0, 0, 0, 0);
+            st_shared_v4(sbase + xw + off, 0, 0, 0, 0);
+            st_shared_v4(sbase + xw + kAtom + off, 0, 0, 0, 0);
+            st_shared_v4(sbase + xw + 2 * kAtom + off, 0, 0, 0, 0);
 #pragma unroll
-              for (int a = 0; a < NA; ++a) st_shared_v4(st + stage_b + a * kAtom + off, 0, 0, 0, 0);
-            }
+            for (int a = 0; a < NA; ++a) st_shared_v4(st + stage_b + a * kAtom + off, 0, 0, 0, 0);
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->xw_full[sb]);
-          mbar_arrive(&bars->sc_free[b3]);
-        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars->xw_full[sb]);
+        mbar_arrive(&bars->sc_free[b3]);
       }
     }
   } else {
@@ -824,94 +803,88 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool wlive = 32 * q < N;    // this warp has state elements
     const bool live = n < N;
     const uint32_t sD = tmem + (static_cast<uint32_t>(32 * q) << 16) + kColDs;
-    int cc = 0;
     bool ok = true;
-    for (int it = it0; it < items && ok; it += its) {
-      const Item w = get_item<STATES>(p, it, ptiles);
-      if (!w.sg.valid) continue;
-      const int slot = (p.state_in || p.state_out) ? seq_slot(p.slots, w.sg.seq, p.nslots, p.status) : -1;
-      const float* in = p.state_in && slot >= 0 ? p.state_in + slot * per_slot + w.head_at : nullptr;
-      float hv[kP];
+    const int slot = (p.state_in || p.state_out) ? seq_slot(p.slots, w.sg.seq, p.nslots, p.status) : -1;
+    const float* in = p.state_in && slot >= 0 ? p.state_in + slot * per_slot + w.head_at : nullptr;
+    float hv[kP];
 #pragma unroll
-      for (int i = 0; i < kP; ++i) hv[i] = 0.0f;
-      // What the state starts from.  The first launch of a split scan starts from zero, but
-      // copies the sequence's start into the last segment's place: the last launch
-      // may overwrite it while other segments still need it.
-      const float* src = w.sg.count == 1 ? in : p.seg_state + w.seg * per_slot + w.head_at;
-      if (STATES) src = w.last && w.sg.count > 1 ? in : nullptr;
-      if (src && live) {
-        src += n;
+    for (int i = 0; i < kP; ++i) hv[i] = 0.0f;
+    // What the state starts from.  The first launch of a split scan starts from zero, but
+    // copies the sequence's start into the last segment's place: the last launch
+    // may overwrite it while other segments still need it.
+    const float* src = w.sg.count == 1 ? in : p.seg_state + w.seg * per_slot + w.head_at;
+    if (STATES) src = w.last && w.sg.count > 1 ? in : nullptr;
+    if (src && live) {
+      src += n;
 #pragma unroll
-        for (int i = 0; i < kP; ++i)
-          if (i < w.pdims) hv[i] = src[i * N];
-      }
-      float log_sum = 0.0f;
+      for (int i = 0; i < kP; ++i)
+        if (i < w.pdims) hv[i] = src[i * N];
+    }
+    float log_sum = 0.0f;
 #pragma unroll 1
-      for (int c = 0; c < w.nc; ++c, ++cc) {
-        const int b3 = cc % 3;
-        ok = wait_bar<kNapState>(&bars->ds_full[cc & 1], (cc >> 1) & 1, flag);
-        if (!ok) break;
-        if (!STATES) {
-          // H, the state before the chunk, in the place of B, which has been read
-          // (hidden from the compiler, or it keeps eight offsets in registers through the loop)
-          uint32_t row = n, at = sbase + (cc & 1) * L::kStage + stage_b;
-          asm volatile("" : "+r"(row), "+r"(at));
-          if (row < 64 * NA) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint32_t vh[4], vl[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) split2(pack2(hv[8 * i + 2 * k], hv[8 * i + 2 * k + 1]), vh[k], vl[k]);
-              const uint32_t off = swz_offset(row, i, 128);
-              st_shared_v4(at + off, vh[0], vh[1], vh[2], vh[3]);
-              st_shared_v4(at + L::kH + off, vl[0], vl[1], vl[2], vl[3]);
-            }
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->h_full);
-        }
-        ok = wait_bar<kNapState>(&bars->sc_full[b3], (cc / 3) & 1, flag);
-        if (!ok) break;
-        const float decay = scal[b3].total;
-        log_sum += scal[b3].log2;
-        const unsigned long long decay2 = pack2(decay, decay);
-        tc_fence_after_sync();
-        if (wlive) {
-#pragma unroll
-          for (int pc = 0; pc < 4; ++pc) {
-            uint32_t r[16];
-            tmem_ld_32x32b_x16(sD + (STATES ? (cc & 1) * kP : 0) + 16 * pc, r);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              unpack2(fma2(pack2(hv[16 * pc + 2 * i], hv[16 * pc + 2 * i + 1]), decay2,
-                           pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]))),
-                      hv[16 * pc + 2 * i], hv[16 * pc + 2 * i + 1]);
-          }
-        }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->ds_free[cc & 1]);
-          mbar_arrive(&bars->sc_free[b3]);
-        }
-      }
+    for (int c = 0; c < w.nc; ++c) {
+      const int b3 = c % 3;
+      ok = wait_bar<kNapState>(&bars->ds_full[c & 1], (c >> 1) & 1, flag);
       if (!ok) break;
-      float* dst = nullptr;
-      if (STATES) {
-        if (w.sg.count > 1) dst = p.seg_state + w.seg * per_slot + w.head_at;
-        if (n == 0 && w.p0 == 0)
-          p.seg_log[static_cast<long long>(w.seg) * p.heads + w.h] = log_sum * (1.0f / kLog2e);
-      } else if (w.last && p.state_out && slot >= 0) {
-        dst = p.state_out + slot * per_slot + w.head_at;
-      }
-      if (dst && live) {
-        dst += n;
+      if (!STATES) {
+        // H, the state before the chunk, in the place of B, which has been read
+        // (hidden from the compiler, or it keeps eight offsets in registers through the loop)
+        uint32_t row = n, at = sbase + (c & 1) * L::kStage + stage_b;
+        asm volatile("" : "+r"(row), "+r"(at));
+        if (row < 64 * NA) {
 #pragma unroll
-        for (int i = 0; i < kP; ++i)
-          if (i < w.pdims) dst[i * N] = hv[i];
+          for (int i = 0; i < 8; ++i) {
+            uint32_t vh[4], vl[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) split2(pack2(hv[8 * i + 2 * k], hv[8 * i + 2 * k + 1]), vh[k], vl[k]);
+            const uint32_t off = swz_offset(row, i, 128);
+            st_shared_v4(at + off, vh[0], vh[1], vh[2], vh[3]);
+            st_shared_v4(at + L::kH + off, vl[0], vl[1], vl[2], vl[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->h_full);
       }
+      ok = wait_bar<kNapState>(&bars->sc_full[b3], (c / 3) & 1, flag);
+      if (!ok) break;
+      const float decay = scal[b3].total;
+      log_sum += scal[b3].log2;
+      const unsigned long long decay2 = pack2(decay, decay);
+      tc_fence_after_sync();
+      if (wlive) {
+#pragma unroll
+        for (int pc = 0; pc < 4; ++pc) {
+          uint32_t r[16];
+          tmem_ld_32x32b_x16(sD + (STATES ? (c & 1) * kP : 0) + 16 * pc, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            unpack2(fma2(pack2(hv[16 * pc + 2 * i], hv[16 * pc + 2 * i + 1]), decay2,
+                         pack2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]))),
+                    hv[16 * pc + 2 * i], hv[16 * pc + 2 * i + 1]);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars->ds_free[c & 1]);
+        mbar_arrive(&bars->sc_free[b3]);
+      }
+    }
+    float* dst = nullptr;  // stays null if the CTA gave up
+    if (STATES && ok) {
+      if (w.sg.count > 1) dst = p.seg_state + w.seg * per_slot + w.head_at;
+      if (n == 0 && w.p0 == 0)
+        p.seg_log[static_cast<long long>(w.seg) * p.heads + w.h] = log_sum * (1.0f / kLog2e);
+    } else if (ok && w.last && p.state_out && slot >= 0) {
+      dst = p.state_out + slot * per_slot + w.head_at;
+    }
+    if (dst && live) {
+      dst += n;
+#pragma unroll
+      for (int i = 0; i < kP; ++i)
+        if (i < w.pdims) dst[i * N] = hv[i];
     }
   }
   __syncwarp();
@@ -939,7 +912,7 @@ int make_map(CUtensorMap* m, const void* base, int inner, int mid, long long row
 }
 
 template <int NA, bool STATES>
-int launch_one(const Tmaps& maps, const ScanParams& p, int items, int ptiles, cudaStream_t st) {
+int launch_one(const Tmaps& maps, const ScanParams& p, unsigned grid, int ptiles, cudaStream_t st) {
   auto kern = scan_umma_kernel<NA, STATES>;
   static std::once_flag once[64];
   int dev = 0;
@@ -949,7 +922,7 @@ int launch_one(const Tmaps& maps, const ScanParams& p, int items, int ptiles, cu
   if (dev < 64) std::call_once(once[dev], set);
   else set();
   SMM_CUDA_TRY(err, "selective scan shared memory size");
-  kern<<<items, kThreads, Smem<NA, STATES>::kBytes, st>>>(maps, p, items, ptiles);
+  kern<<<grid, kThreads, Smem<NA, STATES>::kBytes, st>>>(maps, p, ptiles);
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "selective scan (tensor core) launch");
   return SMM_OK;
@@ -1004,19 +977,19 @@ int scan_umma_launch(ScanParams& p, cudaStream_t st) {
   if (int rc = make_map(&maps.x, p.x, p.dim, p.heads, p.tokens, p.ldx, "x")) return rc;
   if (int rc = make_map(&maps.b, p.B, p.state_dim, p.groups, p.tokens, p.ldb, "B")) return rc;
   if (int rc = make_map(&maps.c, p.C, p.state_dim, p.groups, p.tokens, p.ldc, "C")) return rc;
-  const int items = static_cast<int>(blocks);
+  const unsigned grid = static_cast<unsigned>(blocks);
   if (p.state_dim <= 64) {
     if (p.split) {
-      if (int rc = launch_one<1, true>(maps, p, items, ptiles, st)) return rc;
+      if (int rc = launch_one<1, true>(maps, p, grid, ptiles, st)) return rc;
       if (int rc = scan_combine(p, st)) return rc;
     }
-    return launch_one<1, false>(maps, p, items, ptiles, st);
+    return launch_one<1, false>(maps, p, grid, ptiles, st);
   }
   if (p.split) {
-    if (int rc = launch_one<2, true>(maps, p, items, ptiles, st)) return rc;
+    if (int rc = launch_one<2, true>(maps, p, grid, ptiles, st)) return rc;
     if (int rc = scan_combine(p, st)) return rc;
   }
-  return launch_one<2, false>(maps, p, items, ptiles, st);
+  return launch_one<2, false>(maps, p, grid, ptiles, st);
 }
 
 }  // namespace smm
