@@ -29,6 +29,7 @@
 #include "smm_seq.cuh"
 
 #include <algorithm>
+#include <mutex>
 
 namespace smm {
 namespace {
@@ -305,12 +306,21 @@ template <typename T, int V, int NT, bool XS>
 int launch_q4(const Q4Params& p, int nb, cudaStream_t st) {
   auto kern = q4_kernel<T, V, NT, XS>;
   constexpr int kThreads = NT == 1 ? 1024 : 512, kTeams = kThreads / (32 * kTeam);
-  const size_t smem = (XS ? static_cast<size_t>(p.cols) / 8 * XWord<T>::kParts * nb * sizeof(uint4) : 0) +
-                      kTeams * kTeam * NT * 128 * sizeof(float);
-  if (smem > 48 * 1024) {
-    // (a cheap call, and right for whichever device is current)
-    SMM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)),
-                 "q4_matvec shared memory size");
+  constexpr size_t sums = kTeams * kTeam * NT * 128 * sizeof(float);
+  const size_t smem = (XS ? static_cast<size_t>(p.cols) / 8 * XWord<T>::kParts * nb * sizeof(uint4) : 0) + sums;
+  if constexpr (XS) {
+    // The largest size, once: were it each call's own, another thread's smaller one could
+    // take its place before this launch.
+    static std::once_flag once[64];
+    int dev = 0;
+    SMM_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
+    cudaError_t err = cudaSuccess;
+    auto set = [&] {
+      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kQ4XBytes + sums));
+    };
+    if (dev < 64) std::call_once(once[dev], set);
+    else set();
+    SMM_CUDA_TRY(err, "q4_matvec shared memory size");
   }
   const int tiles = (p.rows + 15) / 16;
   // One CTA an SM.  Few tiles are spread over the SMs, one to a CTA.

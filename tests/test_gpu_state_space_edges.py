@@ -1,5 +1,7 @@
 """State-space operators and the 4-bit product where they can go wrong: busy memory,
 accuracy, decays, non-finite values, calls from several threads and streams, limits."""
+import threading
+
 import pytest
 import torch
 
@@ -183,3 +185,41 @@ def test_non_finite_values_reach_no_token_before_them(cuda, dtype, lens, h, p, n
         assert torch.equal(so[seq][~hst], gst[seq][~hst]), what
         assert not so[seq][hst].isfinite().any(), what
     assert y.dtype == dt
+
+
+# ---------------------------------------------------------------- several callers
+def test_q4_from_several_threads(cuda):
+    """Calls of one kernel with different amounts of shared memory, each thread on its own stream."""
+    L = _lib.load()
+    g = gen(2)
+    failed = []
+    start = threading.Barrier(6)
+
+    def work(args, stream):
+        torch.cuda.set_device(0)
+        start.wait()
+        bad = sum(L.smm_q4_matvec(*args, stream.cuda_stream) != _lib.SMM_OK for _ in range(20000))
+        if bad:
+            failed.append((bad, _lib.last_error()))
+
+    jobs = []
+    for i in range(6):
+        cols = (8192, 4096)[i % 2]  # 128 and 64 KB for x: both above the 48 that need no leave
+        q = torch.randint(0, 256, (16, cols // 2), generator=g, device="cuda", dtype=torch.uint8)
+        s = torch.rand(16, cols // 128, generator=g, device="cuda")
+        x = rnd(g, 8, cols, dtype=BF)
+        y = torch.empty(8, 16, device="cuda", dtype=BF)
+        ref = ops.q4_matvec(q, s, x)
+        args = (q.data_ptr(), s.data_ptr(), None, x.data_ptr(), y.data_ptr(), 8, 16, cols, 128, cols, 16,
+                _lib.DTYPE_BF16, _lib.DTYPE_F32)
+        jobs.append((args, torch.cuda.Stream(), y, ref, (q, s, x)))
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=j[:2]) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for _, _, y, ref, _ in jobs:
+        assert torch.equal(y, ref)
