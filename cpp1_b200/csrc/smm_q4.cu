@@ -12,7 +12,8 @@
 // (g, t) of a warp loads 4 V bytes of rows g and g+8 at k = 8 V t: V words of
 // eight codes with consecutive k.  Masking a word and its shifts by 4, 8 and 12
 // bits yields the code pairs (0,4), (1,5), (2,6), (3,7); OR 0x4300 makes each the
-// bf16 number 128 + code, and subtracting 128 + zero leaves code - zero, exactly.
+// bf16 number 128 + code, and subtracting 128 + zero leaves code - zero, exactly (for zero
+// points up to 127: 16 is common where a format keeps zero - 1 in four bits).
 // x's pairs are picked in the same order from one 16-byte load.  So products are
 // exact, and a group's sum is scaled in fp32 when the group's last product is
 // done, which also keeps the tensor cores' truncating additions to one group.
@@ -235,8 +236,8 @@ __global__ void __launch_bounds__(NT == 1 ? 1024 : 512, 1) q4_kernel(const Q4Par
         if (c >= c_end) break;
         uint32_t oa = 0x43084308u, ob = 0x43084308u;
         if (p.zeros) {
-          oa = 0x43004300u | ((__shfl_sync(0xFFFFFFFFu, k.za, u, 4) & 15u) * 0x10001u);
-          ob = 0x43004300u | ((__shfl_sync(0xFFFFFFFFu, k.zb, u, 4) & 15u) * 0x10001u);
+          oa = 0x43004300u | ((__shfl_sync(0xFFFFFFFFu, k.za, u, 4) & 127u) * 0x10001u);
+          ob = 0x43004300u | ((__shfl_sync(0xFFFFFFFFu, k.zb, u, 4) & 127u) * 0x10001u);
         }
         float acc[NT][4];
 #pragma unroll

@@ -669,7 +669,7 @@ def q4_matvec(q: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, zeros: Opt
     W[r, k] = (code[r, k] - zero[r, k // group]) * scales[r, k // group].
 
     q (rows, cols/2) uint8 holds code 2i of a row in the low half of byte i; scales
-    (rows, cols/group), of x's type or float32, and zeros (same shape, uint8, 0..15; None:
+    (rows, cols/group), of x's type or float32, and zeros (same shape, uint8, 0..127; None:
     8 everywhere) give the group, a multiple of 32.  x float32 or bfloat16; products are
     exact and sums float32 in both.  Returns (batch, rows)."""
     batch, cols = _dims("x", x, 2)

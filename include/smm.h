@@ -547,8 +547,8 @@ int smm_selective_step(const void* x, const void* dt, const float* A, const void
 
 /* y[b][r] = sum_k W[r][k] x[b][k], W[r][k] = (code[r][k] - zero[r][k/group]) scale[r][k/group]
  * (X W^T for a few rows x).  q holds rows x cols/2 bytes, code 2i of a row in
- * the low half of byte i; scales and zeros (bytes; NULL: 8 everywhere) are rows x
- * cols/group.  group is a multiple of 32 and divides cols.  x and y have dtype
+ * the low half of byte i; scales and zeros (bytes of 0 to 127; NULL: 8 everywhere)
+ * are rows x cols/group.  group is a multiple of 32 and divides cols.  x and y have dtype
  * elements, scales scale_dtype.  Products are exact and sums fp32, also for fp32 x.
  * q, x and x's rows are 16-byte aligned; batch is at most 65535.  y must not overlap
  * an input.  No counterpart in the reference. */

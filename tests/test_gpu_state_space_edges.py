@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from cpp1_b200 import _lib, ops
-from test_gpu_state_space import TYPES, U, gen, i32, make_scan, offs, rnd, scan_ref, scan_tol, state_tol, within
+from test_gpu_state_space import TYPES, U, gen, half_step, i32, make_scan, offs, q4_ref, rnd, scan_ref, scan_tol, state_tol, within
 
 pytestmark = pytest.mark.gpu
 
@@ -223,3 +223,23 @@ def test_q4_from_several_threads(cuda):
     assert not failed, failed
     for _, _, y, ref, _ in jobs:
         assert torch.equal(y, ref)
+
+
+# ---------------------------------------------------------------- 4-bit product: ranges
+def q4_tol(ref, mag, cols, group, dtype):
+    """As in test_q4_matches_definition."""
+    steps = 2 * 24 + 2 * cols // min(group, 128) / 8 + 16
+    return half_step(dtype) * ref.abs() * 1.01 + 2 * steps * U * mag + 1e-30
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("batch,group", [(1, 128), (8, 32), (12, 64)])
+def test_q4_zero_points_up_to_127(cuda, dtype, batch, group):
+    g = gen(group)
+    x = rnd(g, batch, 512, dtype=TYPES[dtype])
+    q = torch.randint(0, 256, (70, 256), generator=g, device="cuda", dtype=torch.uint8)
+    s = torch.rand(70, 512 // group, generator=g, device="cuda") * 0.02
+    z = torch.randint(0, 128, s.shape, generator=g, device="cuda", dtype=torch.uint8)
+    z[0], z[1], z[2], z[3] = 16, 127, 0, 15
+    ref, mag = q4_ref(q, s, z, x)
+    within(ops.q4_matvec(q, s, x, z), ref, q4_tol(ref, mag, 512, group, TYPES[dtype]))
