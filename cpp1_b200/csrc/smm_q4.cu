@@ -95,7 +95,8 @@ struct XWord<float> {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         hi[i] = __float_as_uint(v[i]) & 0xFFFF0000u;  // 8 of the 24 significant bits, truncated
-        // an infinity or NaN is all in its first term
+        // an infinity or NaN is all in its first term (a NaN may lie in the bits that were cut)
+        if (part == 0 && v[i] != v[i]) hi[i] = 0x7FC00000u;
         v[i] = (hi[i] & 0x7F800000u) == 0x7F800000u ? 0.0f : v[i] - __uint_as_float(hi[i]);
       }
       b[part] = make_uint4(__byte_perm(hi[0], hi[4], 0x7632), __byte_perm(hi[1], hi[5], 0x7632),

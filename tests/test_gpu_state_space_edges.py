@@ -243,3 +243,18 @@ def test_q4_zero_points_up_to_127(cuda, dtype, batch, group):
     z[0], z[1], z[2], z[3] = 16, 127, 0, 15
     ref, mag = q4_ref(q, s, z, x)
     within(ops.q4_matvec(q, s, x, z), ref, q4_tol(ref, mag, 512, group, TYPES[dtype]))
+
+
+def test_q4_keeps_every_nan(cuda):
+    """Not-a-numbers whose payload lies in their low bits alone, beside an infinity."""
+    g = gen(6)
+    q = torch.randint(0, 256, (40, 64), generator=g, device="cuda", dtype=torch.uint8)
+    s = torch.rand(40, 1, generator=g, device="cuda") + 0.01
+    x = rnd(g, 5, 128)
+    clean = ops.q4_matvec(q, s, x)
+    bits = x.view(torch.int32)
+    for row, v in ((0, 0x7F800001), (1, -0x007FFFFF), (2, 0x7FC00000), (3, 0x7F800000)):
+        bits[row, 9 * row + 4] = v
+    y = ops.q4_matvec(q, s, x)
+    assert y[:3].isnan().all()
+    assert not y[3].isfinite().any() and torch.equal(y[4], clean[4])
