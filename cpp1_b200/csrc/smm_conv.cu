@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(const ConvParam
   const int b = static_cast<int>(blockIdx.x / p.ctiles);
   const int c = (static_cast<int>(blockIdx.x % p.ctiles) * blockDim.x + threadIdx.x) * VEC;
   if (c >= p.channels) return;
-  const int slot = seq_slot(p.slots, b, p.nslots, p.status);
+  const int slot = p.state_in || p.state_out ? seq_slot(p.slots, b, p.nslots, p.status) : -1;
   const long long at = (static_cast<long long>(slot) * p.channels + c) * (W - 1);
   using Lane = ConvLane<T, VEC, W>;
   float old[VEC * (W - 1)];

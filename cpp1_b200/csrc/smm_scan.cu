@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas) step_kernel(const Sca
     const long long hb = t / tph;
     c.h = static_cast<int>(hb % p.heads);
     c.b = static_cast<int>(hb / p.heads);
-    c.slot = seq_slot(p.slots, c.b, p.nslots, p.status);
+    c.slot = p.state_in || p.state_out ? seq_slot(p.slots, c.b, p.nslots, p.status) : -1;
     return c;
   };
   auto advance = [&](Place& c, bool live) {
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtas) step_kernel(const Sca
     if (++c.h < p.heads) return;
     c.h = 0;
     ++c.b;
-    if (live) c.slot = seq_slot(p.slots, c.b, p.nslots, p.status);
+    if (live && (p.state_in || p.state_out)) c.slot = seq_slot(p.slots, c.b, p.nslots, p.status);
   };
   auto state_at = [&](const Place& c) {
     return (static_cast<long long>(c.slot) * p.heads + c.h) * p.dim * N;
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kOddThreads) step_odd_kernel(const ScanParams 
   const int g = h / (p.heads / p.groups);
   const int N = p.state_dim;
   const int sub = threadIdx.x % lanes, row0 = threadIdx.x / lanes, rstep = kOddThreads / lanes;
-  const int slot = seq_slot(p.slots, b, p.nslots, p.status);
+  const int slot = p.state_in || p.state_out ? seq_slot(p.slots, b, p.nslots, p.status) : -1;
   const long long base = (static_cast<long long>(slot) * p.heads + h) * p.dim * N;
   const float* in = p.state_in && slot >= 0 ? p.state_in + base : nullptr;
   float* out = p.state_out && slot >= 0 ? p.state_out + base : nullptr;

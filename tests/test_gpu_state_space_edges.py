@@ -258,3 +258,34 @@ def test_q4_keeps_every_nan(cuda):
     y = ops.q4_matvec(q, s, x)
     assert y[:3].isnan().all()
     assert not y[3].isfinite().any() and torch.equal(y[4], clean[4])
+
+
+# ---------------------------------------------------------------- C entries
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [128, 20, 7])
+def test_step_entries_without_states(cuda, dtype, n):
+    """No states at all (null pointers, no entries): every row starts from zero, and nothing is reported."""
+    L = _lib.load()
+    batch, h, p = 5, 3, 40
+    ty = _lib.DTYPE_F32 if dtype == "fp32" else _lib.DTYPE_BF16
+    a = make_scan(n, batch, h, p, 1, n, dtype, z=False, d=False, strided=False)
+    pool = rnd(gen(1), batch, h, p, n)
+    none = i32([-1] * batch)
+    ref = ops.selective_step(**a, state=pool, slots=none)
+    y = torch.full_like(ref, float("nan"))
+    ops.device_status()
+    rc = L.smm_selective_step(a["x"].data_ptr(), a["dt"].data_ptr(), a["A"].data_ptr(), a["B"].data_ptr(),
+                              a["C"].data_ptr(), None, None, a["dt_bias"].data_ptr(), None, None, None, y.data_ptr(),
+                              batch, 0, h, p, 1, n, h * p, h, n, n, 0, h * p, ty, ty, 1, None)
+    assert rc == _lib.SMM_OK
+    ops.device_status()
+    assert torch.equal(y, ref)
+    x, w = rnd(gen(2), batch, n, dtype=TYPES[dtype]), rnd(gen(3), n, 4, dtype=TYPES[dtype])
+    cs = rnd(gen(4), batch, n, 3, dtype=TYPES[dtype])
+    ref = ops.causal_conv_step(x, w, state=cs, slots=none)
+    y = torch.full_like(ref, float("nan"))
+    rc = L.smm_causal_conv_step(x.data_ptr(), w.data_ptr(), None, None, None, None, y.data_ptr(), batch, n, 4, 0, n, n,
+                                ty, 1, None)
+    assert rc == _lib.SMM_OK
+    ops.device_status()
+    assert torch.equal(y, ref)
