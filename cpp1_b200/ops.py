@@ -445,11 +445,9 @@ def _states(x, dtype, entry, state, state_out):
     return state, state if state_out is None else state_out, n or 0
 
 
-def _index(name: str, t: Optional[torch.Tensor], like: torch.Tensor, n: Optional[int]) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    _check_seq(name, t, like, torch.int32, _dims(name, t, 1) if n is None else (n,))
-    return t if t.is_contiguous() else t.contiguous()
+def _check_index(name: str, t: Optional[torch.Tensor], like: torch.Tensor, n: Optional[int]) -> None:
+    if t is not None:
+        _check_seq(name, t, like, torch.int32, _dims(name, t, 1) if n is None else (n,))
 
 
 def _opt(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -466,8 +464,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
 
 
 def _on(x: torch.Tensor, stream: Optional[torch.cuda.Stream], call):
-    """call(stream pointer) with x's device current.  Whatever call allocates belongs
-    to the stream that its kernels run on."""
+    """call(stream pointer) with x's device current.  Whatever call allocates and copies belongs
+    to the stream that its kernels run on, so nothing is copied outside of it."""
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
     index = x.device.index
@@ -482,13 +480,13 @@ def _on(x: torch.Tensor, stream: Optional[torch.cuda.Stream], call):
         return call(_raw_stream(index) or None)
 
 
-def _sequences(offsets, x):
+def _sequences(offsets, x) -> int:
     if offsets is None:
-        return None, 1
-    offsets = _index("offsets", offsets, x, None)
+        return 1
+    _check_index("offsets", offsets, x, None)
     if offsets.shape[0] < 1:
         raise ValueError("offsets must have at least one element")
-    return offsets, offsets.shape[0] - 1
+    return offsets.shape[0] - 1
 
 
 def _conv_args(x, weight, bias, activation):
@@ -524,15 +522,15 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     left as they are in `out`, and have no defined values without it."""
     tokens, channels, width, ty, act = _conv_args(x, weight, bias, activation)
     state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out)
-    offsets, nseq = _sequences(offsets, x)
-    slots = _index("slots", slots, x, nseq)
+    nseq = _sequences(offsets, x)
+    _check_index("slots", slots, x, nseq)
 
     def call(st):
         xr, ldx = _rows(x, channels)
-        w, b = _vec(weight), _vec(bias)
+        w, b, off, sl = _vec(weight), _vec(bias), _vec(offsets), _vec(slots)
         y, ldy = _seq_out(out, x, (tokens, channels), channels)
         _lib.check(_lib.load().smm_causal_conv(
-            xr.data_ptr(), w.data_ptr(), _opt(b), _opt(offsets), _opt(state), _opt(state_out), _opt(slots),
+            xr.data_ptr(), w.data_ptr(), _opt(b), _opt(off), _opt(state), _opt(state_out), _opt(sl),
             y.data_ptr(), tokens, channels, width, nseq, entries, ldx, ldy, ty, act, st), "smm_causal_conv")
         return y
     return _on(x, stream, call)
@@ -549,14 +547,14 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     if state is None:
         raise TypeError("state must be a torch.Tensor")
     state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out)
-    slots = _index("slots", slots, x, batch)
+    _check_index("slots", slots, x, batch)
 
     def call(st):
         xr, ldx = _rows(x, channels)
-        w, b = _vec(weight), _vec(bias)
+        w, b, sl = _vec(weight), _vec(bias), _vec(slots)
         y, ldy = _seq_out(out, x, (batch, channels), channels)
         _lib.check(_lib.load().smm_causal_conv_step(
-            xr.data_ptr(), w.data_ptr(), _opt(b), state.data_ptr(), state_out.data_ptr(), _opt(slots), y.data_ptr(),
+            xr.data_ptr(), w.data_ptr(), _opt(b), state.data_ptr(), state_out.data_ptr(), _opt(sl), y.data_ptr(),
             batch, channels, width, entries, ldx, ldy, ty, act, st), "smm_causal_conv_step")
         return y
     return _on(x, stream, call)
@@ -612,22 +610,22 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     tokens before it do not depend on it."""
     tokens, heads, dim, groups, n, ty, dty = _scan_args(x, dt, A, B, C, D, z, dt_bias)
     state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out)
-    offsets, nseq = _sequences(offsets, x)
-    slots = _index("slots", slots, x, nseq)
+    nseq = _sequences(offsets, x)
+    _check_index("slots", slots, x, nseq)
 
     def call(st):
         L = _lib.load()
         wx, wb = heads * dim, groups * n
         (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x, wx), _rows(dt, heads), _rows(B, wb), _rows(C, wb)
         zr, ldz = (None, 0) if z is None else _rows(z, wx)
-        a, dd, db = _vec(A), _vec(D), _vec(dt_bias)
+        a, dd, db, off, sl = _vec(A), _vec(D), _vec(dt_bias), _vec(offsets), _vec(slots)
         y, ldy = _seq_out(out, x, (tokens, heads, dim), wx)
         nws = L.smm_selective_scan_workspace_size(tokens, nseq, heads, dim, groups, n, ty)
         # of this call alone: streams and captured graphs share nothing
         ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
         _lib.check(L.smm_selective_scan(
             xr.data_ptr(), dr.data_ptr(), a.data_ptr(), br.data_ptr(), cr.data_ptr(), _opt(dd), _opt(zr), _opt(db),
-            _opt(offsets), _opt(state), _opt(state_out), _opt(slots), y.data_ptr(), tokens, nseq, entries, heads, dim,
+            _opt(off), _opt(state), _opt(state_out), _opt(sl), y.data_ptr(), tokens, nseq, entries, heads, dim,
             groups, n, ldx, ldd, ldb, ldc, ldz, ldy, ty, dty, 1 if dt_softplus else 0, _opt(ws), nws, st),
             "smm_selective_scan")
         return y
@@ -647,17 +645,17 @@ def selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if state is None:
         raise TypeError("state must be a torch.Tensor")
     state, state_out, entries = _states(x, torch.float32, (heads, dim, n), state, state_out)
-    slots = _index("slots", slots, x, batch)
+    _check_index("slots", slots, x, batch)
 
     def call(st):
         wx, wb = heads * dim, groups * n
         (xr, ldx), (dr, ldd), (br, ldb), (cr, ldc) = _rows(x, wx), _rows(dt, heads), _rows(B, wb), _rows(C, wb)
         zr, ldz = (None, 0) if z is None else _rows(z, wx)
-        a, dd, db = _vec(A), _vec(D), _vec(dt_bias)
+        a, dd, db, sl = _vec(A), _vec(D), _vec(dt_bias), _vec(slots)
         y, ldy = _seq_out(out, x, (batch, heads, dim), wx)
         _lib.check(_lib.load().smm_selective_step(
             xr.data_ptr(), dr.data_ptr(), a.data_ptr(), br.data_ptr(), cr.data_ptr(), _opt(dd), _opt(zr), _opt(db),
-            state.data_ptr(), state_out.data_ptr(), _opt(slots), y.data_ptr(), batch, entries, heads, dim, groups, n,
+            state.data_ptr(), state_out.data_ptr(), _opt(sl), y.data_ptr(), batch, entries, heads, dim, groups, n,
             ldx, ldd, ldb, ldc, ldz, ldy, ty, dty, 1 if dt_softplus else 0, st), "smm_selective_step")
         return y
     return _on(x, stream, call)

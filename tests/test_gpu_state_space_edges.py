@@ -289,3 +289,41 @@ def test_step_entries_without_states(cuda, dtype, n):
     assert rc == _lib.SMM_OK
     ops.device_status()
     assert torch.equal(y, ref)
+
+
+# ---------------------------------------------------------------- streams
+def test_strided_offsets_and_slots_on_another_stream(cuda):
+    """Arguments that have to be copied are copied on the stream that the call runs on,
+    however busy the current one is."""
+    h, p, n = 2, 64, 128
+    lens = [100, 30, 70]
+    b = offs(lens)
+    a = make_scan(1, b[-1], h, p, 1, n, "bf16")
+    x = rnd(gen(2), b[-1], 64)
+    w = rnd(gen(3), 64, 4)
+    st, cs = rnd(gen(4), 4, h, p, n), rnd(gen(5), 4, 64, 3)
+    one = {k: v[:3] if isinstance(v, torch.Tensor) and v.dim() > 1 else v for k, v in a.items()}
+    off, sl = i32(b), i32([3, 0, 2])
+    off2, sl2 = torch.stack([off, off * 0 + 7], 1)[:, 0], torch.stack([sl, sl * 0 + 1], 1)[:, 0]
+    assert not off2.is_contiguous() and not sl2.is_contiguous()
+
+    def calls(o, s, stream):
+        kw = dict(stream=stream)
+        so, co = torch.zeros_like(st), torch.zeros_like(cs)
+        s1, c1 = st.clone(), cs.clone()
+        if stream is not None:
+            stream.wait_stream(torch.cuda.current_stream())
+            torch.cuda._sleep(400_000_000)  # the current stream is busy from here on
+        res = [ops.selective_scan(**a, offsets=o, state=st, state_out=so, slots=s, **kw), so,
+               ops.causal_conv(x, w, offsets=o, state=cs, state_out=co, slots=s, **kw), co,
+               ops.selective_step(**one, state=s1, slots=s, **kw), s1,
+               ops.causal_conv_step(x[:3], w, state=c1, slots=s, **kw), c1]
+        if stream is not None:
+            stream.synchronize()
+            res = [r.cpu() for r in res]
+        return res
+
+    ref = [r.cpu() for r in calls(off, sl, None)]
+    got = calls(off2, sl2, torch.cuda.Stream())
+    for r, v in zip(ref, got):
+        assert torch.equal(r, v)
