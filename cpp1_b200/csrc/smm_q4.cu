@@ -365,8 +365,8 @@ extern "C" int smm_q4_matvec(const void* q, const void* scales, const void* zero
   if (!y || (cols > 0 && (!q || !scales || !x))) return set_error(SMM_ERR_INVALID, "smm_q4_matvec: null pointer");
   const size_t e = dtype_size(dtype);
   const size_t groups = static_cast<size_t>(rows) * (cols / group);
-  const Span ys{y, span_bytes(batch, rows, ldy, e)};
-  if (overlaps(ys, {x, span_bytes(batch, cols, ldx, e)}) || overlaps(ys, {q, static_cast<size_t>(rows) * (cols / 2)}) ||
+  const Span ys = row_span(y, batch, rows, ldy, e);
+  if (overlaps(ys, row_span(x, batch, cols, ldx, e)) || overlaps(ys, {q, static_cast<size_t>(rows) * (cols / 2)}) ||
       overlaps(ys, {scales, groups * dtype_size(scale_dtype)}) || overlaps(ys, {zeros, groups}))
     return set_error(SMM_ERR_INVALID, "smm_q4_matvec: y overlaps an input");
   if (!aligned_to(q, 16) || !aligned_to(x, 16) || (batch > 1 && ldx * e % 16 != 0))

@@ -621,12 +621,12 @@ int check_scan(const char* who, const ScanParams& p, int dtype, int dt_dtype, bo
     return set_error(SMM_ERR_INVALID, "%s: null pointer", who);
   const size_t e = dtype_size(dtype);
   const size_t sb = static_cast<size_t>(p.nslots) * hp * p.state_dim * sizeof(float);
-  const Span y{p.y, span_bytes(p.tokens, hp, p.ldy, e)}, so{p.state_out, sb}, si{p.state_in, sb};
-  const Span in[] = {{p.x, span_bytes(p.tokens, hp, p.ldx, e)},
-                     {p.z, span_bytes(p.tokens, hp, p.ldz, e)},
-                     {p.B, span_bytes(p.tokens, gn, p.ldb, e)},
-                     {p.C, span_bytes(p.tokens, gn, p.ldc, e)},
-                     {p.dt, span_bytes(p.tokens, p.heads, p.lddt, dtype_size(dt_dtype))},
+  const Span y = row_span(p.y, p.tokens, hp, p.ldy, e), so{p.state_out, sb}, si{p.state_in, sb};
+  const Span in[] = {row_span(p.x, p.tokens, hp, p.ldx, e),
+                     row_span(p.z, p.tokens, hp, p.ldz, e),
+                     row_span(p.B, p.tokens, gn, p.ldb, e),
+                     row_span(p.C, p.tokens, gn, p.ldc, e),
+                     row_span(p.dt, p.tokens, p.heads, p.lddt, dtype_size(dt_dtype)),
                      {p.A, p.heads * sizeof(float)},
                      {p.D, p.heads * sizeof(float)},
                      {p.dt_bias, p.heads * sizeof(float)},

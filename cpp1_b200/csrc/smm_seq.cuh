@@ -180,19 +180,31 @@ __device__ __forceinline__ int seq_slot(const int* __restrict__ slots, int s, in
 }
 
 // ---------------------------------------------------------------- host checks
+// Memory that a call touches: rows of `width` bytes, ld apart (one row: contiguous bytes).
 struct Span {
   const void* p;
-  size_t bytes;
+  size_t width;
+  long long rows = 1;
+  size_t ld = 0;
 };
-// Bytes from the first to behind the last element of `rows` rows of `width`
-// elements, ld apart.
-inline size_t span_bytes(long long rows, long long width, long long ld, size_t esz) {
-  return rows <= 0 || width <= 0 ? 0 : (static_cast<size_t>(rows - 1) * ld + width) * esz;
+inline Span row_span(const void* p, long long rows, long long width, long long ld, size_t esz) {
+  return {p, static_cast<size_t>(width) * esz, rows, static_cast<size_t>(ld) * esz};
 }
-inline bool overlaps(Span a, Span b) {
-  if (!a.p || !b.p || !a.bytes || !b.bytes) return false;
+// Whether two spans share a byte.  Columns of the same rows of one matrix may lie side
+// by side; rows of different strides count as whole.
+inline bool overlaps(const Span& a, const Span& b) {
+  if (!a.p || !b.p || !a.width || !b.width || a.rows <= 0 || b.rows <= 0) return false;
   const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-  return x < y + b.bytes && y < x + a.bytes;
+  const size_t an = (a.rows - 1) * a.ld + a.width, bn = (b.rows - 1) * b.ld + b.width;
+  if (x >= y + bn || y >= x + an) return false;
+  if ((a.rows == 1 && b.rows == 1) || (a.rows > 1 && b.rows > 1 && a.ld != b.ld)) return true;
+  const long long ld = a.rows > 1 ? a.ld : b.ld, aw = a.width, bw = b.width;
+  if (aw > ld || bw > ld) return true;
+  // b's row j begins d + (j - i) ld behind a's row i: some k = j - i with -bw < d + k ld < aw?
+  const long long d = static_cast<long long>(y - x);
+  for (long long k = -d / ld - 2; k <= -d / ld + 2; ++k)
+    if (k > -a.rows && k < b.rows && d + k * ld > -bw && d + k * ld < aw) return true;
+  return false;
 }
 inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 inline bool valid_dtype(int d) { return d == SMM_DTYPE_F32 || d == SMM_DTYPE_BF16; }

@@ -519,7 +519,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     (None: zeros), and state_out receives the rows that each one ends with (None:
     state is updated in place).  Sequence s uses entry slots[s] (int32; None: s;
     negative: no state); no two may share one.  Rows outside every sequence are
-    left as they are in `out`, and have no defined values without it."""
+    left as they are in `out`, and have no defined values without it.  `out` may be columns of
+    the matrix whose other columns are inputs."""
     tokens, channels, width, ty, act = _conv_args(x, weight, bias, activation)
     state, state_out, entries = _states(x, x.dtype, (channels, width - 1), state, state_out)
     nseq = _sequences(offsets, x)

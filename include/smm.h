@@ -491,7 +491,8 @@ typedef enum { SMM_ACT_NONE = 0, SMM_ACT_SILU = 1 } smm_act;
  *   (device ints; NULL: entry s).  A sequence with a negative slot starts from
  *   zero and leaves no state.  So does one whose slot is nslots or more, which
  *   also makes smm_device_status report SMM_ERR_BOUNDS.  Two sequences of one
- *   call must not share an entry.  Outputs must not overlap inputs. */
+ *   call must not share an entry.  Outputs must not overlap inputs; columns of the
+ *   same rows of one matrix (equal ld) may lie side by side. */
 
 /* y[t][c] = act(bias[c] + sum_j w[c][j] x[t-width+1+j][c]): per channel a banded
  * lower-triangular Toeplitz matrix of `width` (2..8) diagonals times a column.

@@ -327,3 +327,51 @@ def test_strided_offsets_and_slots_on_another_stream(cuda):
     got = calls(off2, sl2, torch.cuda.Stream())
     for r, v in zip(ref, got):
         assert torch.equal(r, v)
+
+
+# ---------------------------------------------------------------- one matrix for all
+@pytest.mark.parametrize("dtype,lens,h,n", [("bf16", [300, 41], 4, 64), ("bf16", [5, 2], 4, 64), ("fp32", [70, 30], 4, 20),
+                                            ("bf16", [4200], 1, 128), ("fp32", [3000], 1, 32)])
+def test_outputs_beside_inputs_in_one_matrix(cuda, dtype, lens, h, n):
+    """out= as columns of the rows that hold the inputs: the result, and no other column changed."""
+    dt, p = TYPES[dtype], 64
+    b = offs(lens)
+    t, hp = b[-1], h * p
+    a = make_scan(9, t, h, p, 1, n, dtype, strided=False)
+    ref = ops.selective_scan(**a, offsets=i32(b))
+    widths = dict(x=hp, y=hp, B=n, C=n, z=hp, dt=8)
+    m = rnd(gen(1), t, sum(widths.values()) + 8, dtype=dt)
+    col, at = {}, 0
+    for k, v in widths.items():
+        col[k], at = m[:, at:at + v], at + v
+    for k in ("x", "B", "C", "z"):
+        col[k].copy_(a[k].reshape(t, -1))
+    col["dt"][:, :h].copy_(a["dt"])
+    keep = m.clone()
+    args = dict(a, x=col["x"].unflatten(1, (h, p)), B=col["B"].unflatten(1, (1, n)), C=col["C"].unflatten(1, (1, n)),
+                z=col["z"].unflatten(1, (h, p)), dt=col["dt"][:, :h])
+    out = col["y"].unflatten(1, (h, p))
+    ops.selective_scan(**args, offsets=i32(b), out=out)
+    assert torch.equal(out, ref)
+    keep[:, hp:2 * hp] = ref.view(t, hp)
+    assert torch.equal(m, keep)
+    st = rnd(gen(2), t, h, p, n)
+    ops.selective_step(**args, state=st.clone(), out=out)
+    keep[:, hp:2 * hp] = ops.selective_step(**a, state=st.clone()).view(t, hp)
+    assert torch.equal(m, keep)
+    w, cs = rnd(gen(3), hp, 4, dtype=dt), rnd(gen(4), t, hp, 3, dtype=dt)
+    x = a["x"].reshape(t, hp)
+    ops.causal_conv(col["x"], w, offsets=i32(b), out=col["y"])
+    keep[:, hp:2 * hp] = ops.causal_conv(x, w, offsets=i32(b))
+    assert torch.equal(m, keep)
+    ops.causal_conv_step(col["x"], w, state=cs.clone(), out=col["y"])
+    keep[:, hp:2 * hp] = ops.causal_conv_step(x, w, state=cs.clone())
+    assert torch.equal(m, keep)
+    q = torch.randint(0, 256, (hp, hp // 2), generator=gen(5), device="cuda", dtype=torch.uint8)
+    s = torch.rand(hp, hp // 32, generator=gen(6), device="cuda")
+    ops.q4_matvec(q, s, col["x"], out=col["y"])
+    keep[:, hp:2 * hp] = ops.q4_matvec(q, s, x)
+    assert torch.equal(m, keep)
+    with pytest.raises(_lib.SmmError) as e:
+        ops.causal_conv(col["x"], w, offsets=i32(b), out=m[:, hp - 1:2 * hp - 1])
+    assert e.value.status == _lib.SMM_ERR_INVALID
