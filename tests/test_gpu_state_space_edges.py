@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from cpp1_b200 import _lib, ops
-from test_gpu_state_space import TYPES, U, gen, half_step, i32, make_scan, offs, q4_ref, rnd, scan_ref, scan_tol, state_tol, within
+from test_gpu_state_space import SCAN_CASES, TYPES, U, gen, half_step, i32, make_scan, offs, q4_ref, rnd, scan_ref, scan_tol, state_tol, within
 
 pytestmark = pytest.mark.gpu
 
@@ -74,6 +74,38 @@ def test_bf16_scan_rounds_its_outputs_alone(cuda, lens, h, p, g_, n, with_state)
     # a rounding of the exact result, and 2^-16 of the terms beside it
     best = float((ref.to(BF).double() - ref).norm())
     assert float((y.double() - ref).norm()) <= best + 2.0 ** -16 * float(mag.norm())
+
+
+@pytest.mark.parametrize("lens,h,p,n", [([2048], 16, 64, 128), ([700, 37, 260], 40, 64, 64), ([4097], 2, 64, 128),
+                                        ([300] * 6, 8, 128, 16)])
+def test_tensor_core_states_keep_32_bits(cuda, lens, h, p, n):
+    """Over all elements a final state is within 2^-20: three terms of the weighted x leave 2^-24, 24
+    truncated additions of random signs 5 x 2^-24, two exponentials 2^-22 each.  Two terms would leave 2^-18.7."""
+    b = offs(lens)
+    a = make_scan(n, b[-1], h, p, 1, n, "bf16")
+    assert on_tensor_cores(a, lens)
+    st = rnd(gen(h), len(lens), h, p, n)
+    _, _, (fin, _) = scan_ref(a, b, st)
+    so = torch.empty_like(st)
+    ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so)
+    assert float((so.double() - fin).norm()) <= 2.0 ** -20 * float(fin.norm())
+
+
+@pytest.mark.parametrize("lens,h,p,g_,n", SCAN_CASES)
+def test_bf16_recurrence_sums_in_32_bits(cuda, lens, h, p, g_, n):
+    """bf16 prompts that are too short or too odd for the tensor cores: the fp32 recurrence's tolerance."""
+    b = offs(lens)
+    a = make_scan(h + p + n, b[-1], h, p, g_, n, "bf16", strided=p % 32 != 0)
+    if on_tensor_cores(a, lens):
+        a = {k: v[..., 1:] if k in ("B", "C") else v for k, v in a.items()}  # an odd state size goes there too
+        n -= 1
+    st = rnd(gen(n), len(lens), h, p, n)
+    ref, mag, (fin, fmag) = scan_ref(a, b, st)
+    so = torch.empty_like(st)
+    y = ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so)
+    longest = max(max(lens), 1)
+    within(y, ref, scan_tol(ref, mag, n, longest, BF, False), "y")
+    within(so, fin, state_tol(fin, fmag, longest, False), "state")
 
 
 # ---------------------------------------------------------------- giving up
@@ -375,3 +407,19 @@ def test_outputs_beside_inputs_in_one_matrix(cuda, dtype, lens, h, n):
     with pytest.raises(_lib.SmmError) as e:
         ops.causal_conv(col["x"], w, offsets=i32(b), out=m[:, hp - 1:2 * hp - 1])
     assert e.value.status == _lib.SMM_ERR_INVALID
+
+
+# ---------------------------------------------------------------- long rows
+@pytest.mark.parametrize("dtype,cols", [("fp32", 32768), ("bf16", 98304)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("batch,zeros", [(2, True), (11, False)])
+def test_q4_rows_beyond_shared_memory(cuda, dtype, cols, group, batch, zeros):
+    """Rows of x of which one fills the shared memory's share, and longer ones that are read beside the products."""
+    for c in (cols, cols + group):
+        g = gen(c)
+        x = rnd(g, batch, c, dtype=TYPES[dtype])
+        q = torch.randint(0, 256, (33, c // 2), generator=g, device="cuda", dtype=torch.uint8)
+        s = torch.rand(33, c // group, generator=g, device="cuda") * 0.02
+        z = torch.randint(0, 16, s.shape, generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+        ref, mag = q4_ref(q, s, z, x)
+        within(ops.q4_matvec(q, s, x, z), ref, q4_tol(ref, mag, c, group, TYPES[dtype]))
