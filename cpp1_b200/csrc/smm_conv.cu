@@ -14,8 +14,9 @@
 // from, and the state it ends with may overwrite that.  Both are done by the
 // threads whose run holds the sequence's last token: they read the old state
 // first and write the new one last, so an update in place has no race, and
-// needs no second launch.  An empty sequence belongs to the run that holds
-// its position (the last run, behind the last row).
+// needs no second launch.  Empty sequences are dealt out over the runs, whatever their
+// position: a padded batch has hundreds of them in one place (2048 tokens of 16
+// sequences with 240 empty ones behind took 115 us when one run walked them all).
 #include "smm_seq.cuh"
 
 #include <type_traits>
@@ -162,7 +163,6 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
   if (c >= p.channels || r >= p.nruns) return;
   const long long t0 = r * p.run;
   const long long t1 = t0 + p.run < p.tokens ? t0 + p.run : p.tokens;
-  const bool last_run = r == p.nruns - 1;
   const T* x = static_cast<const T*>(p.x) + c;
   T* y = static_cast<T*>(p.y) + c;
   const bool act = p.silu != 0;
@@ -170,13 +170,13 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
   Lane lane;
   lane.load(p, c);
 
-  // first sequence that reaches into this run or is empty at its start
+  // first sequence that ends in this run or behind it
   int s = 0;
   if (p.offsets) {
     int lo = 0, hi = p.nseq;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (__ldg(p.offsets + mid + 1) > t0 || __ldg(p.offsets + mid) >= t0)
+      if (__ldg(p.offsets + mid + 1) > t0)
         hi = mid;
       else
         lo = mid + 1;
@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
   for (; s < p.nseq; ++s) {
     long long b, e;
     seq_range(p.offsets, s, p.tokens, &b, &e);
-    if (b > t1 || (b == t1 && !last_run)) break;
+    if (b >= t1) break;
+    if (e == b) continue;
     typename Lane::E win[W - 1][Lane::NP];
     const long long lo = b + W - 1 > t0 ? b + W - 1 : t0;
     const long long hi = e < t1 ? e : t1;
@@ -219,8 +220,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
         lane.row(win, cur, y + t * p.ldy, act);
       }
     }
-    const bool owner = e > b ? (e > t0 && e <= t1) : (b >= t0 && (b < t1 || last_run));
-    if (!owner) continue;
+    if (e > t1) continue;  // another run has the last token
     const int slot = (p.state_in || p.state_out) ? seq_slot(p.slots, s, p.nslots, p.status) : -1;
     const long long at = (static_cast<long long>(slot) * p.channels + c) * (W - 1);
     float old[VEC * (W - 1)];
@@ -249,6 +249,20 @@ __global__ void __launch_bounds__(kConvThreads) conv_kernel(const ConvParams p) 
       Lane::to_state(win, old);
       store_f32<T, VEC*(W - 1), kVec, Lane::kPiece>(static_cast<T*>(p.state_out) + at, old);
     }
+  }
+  // empty sequences: the state they start from is what they end with
+  if (!p.state_out) return;
+#pragma unroll 1
+  for (unsigned q = static_cast<unsigned>(r); q < static_cast<unsigned>(p.nseq); q += p.nruns) {
+    long long b, e;
+    seq_range(p.offsets, q, p.tokens, &b, &e);
+    if (e > b) continue;
+    const int slot = seq_slot(p.slots, q, p.nslots, p.status);
+    if (slot < 0 || p.state_in == p.state_out) continue;
+    const long long at = (static_cast<long long>(slot) * p.channels + c) * (W - 1);
+    float old[VEC * (W - 1)] = {};
+    if (p.state_in) load_f32<T, VEC*(W - 1), kVec, Lane::kPiece>(static_cast<const T*>(p.state_in) + at, old);
+    store_f32<T, VEC*(W - 1), kVec, Lane::kPiece>(static_cast<T*>(p.state_out) + at, old);
   }
 }
 

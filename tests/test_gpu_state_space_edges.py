@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from cpp1_b200 import _lib, ops
-from test_gpu_state_space import SCAN_CASES, TYPES, U, gen, half_step, i32, make_scan, offs, q4_ref, rnd, scan_ref, scan_tol, state_tol, within
+from test_gpu_state_space import SCAN_CASES, TYPES, U, conv_ref, conv_tol, gen, half_step, i32, make_scan, offs, q4_ref, rnd, scan_ref, scan_tol, state_tol, within
 
 pytestmark = pytest.mark.gpu
 
@@ -255,6 +255,52 @@ def test_q4_from_several_threads(cuda):
     assert not failed, failed
     for _, _, y, ref, _ in jobs:
         assert torch.equal(y, ref)
+
+
+# ---------------------------------------------------------------- padded batches
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,channels", [([0] * 70, 24), ([0] * 300 + [9, 0, 70] + [0] * 500, 40), ([3] + [0] * 90, 4352),
+                                           ([64, 64, 0, 0, 64] + [0] * 33, 130), ([1, 0] * 120, 33)])
+def test_many_empty_sequences(cuda, dtype, lens, channels):
+    """Empty sequences in front, between and behind: their states pass through the convolution and the
+    scan (zero where there is none), in place too, padded ones without a slot leave nothing."""
+    dt = TYPES[dtype]
+    b = offs(lens)
+    k = len(lens)
+    slots = torch.randperm(k, generator=torch.Generator().manual_seed(k)).tolist()
+    for i in range(0, k, 3):
+        slots[i] = -1
+    x, w = rnd(gen(1), b[-1], channels, dtype=dt), rnd(gen(2), channels, 4, dtype=dt)
+    st = rnd(gen(3), k, channels, 3, dtype=dt)
+    start = torch.stack([st[s] if s >= 0 else torch.zeros_like(st[0]) for s in slots])
+    ref, mag, final = conv_ref(x, w, None, b, start, True)
+    live = [i for i in range(k) if slots[i] >= 0]
+    rest = sorted(set(range(k)) - {slots[i] for i in live})
+    where = [slots[i] for i in live]
+    out = torch.full_like(st, 5.0)
+    y = ops.causal_conv(x, w, offsets=i32(b), state=st, state_out=out, slots=i32(slots))
+    within(y, ref, conv_tol(ref, mag, 4, dt), "y")
+    assert torch.equal(out[where].double(), final[live]) and (out[rest] == 5).all()
+    again = st.clone()
+    assert torch.equal(ops.causal_conv(x, w, offsets=i32(b), state=again, slots=i32(slots)), y)
+    assert torch.equal(again[where], out[where]) and torch.equal(again[rest], st[rest])
+    out.fill_(5.0)
+    ops.causal_conv(x, w, offsets=i32(b), state_out=out, slots=i32(slots))
+    for i in live:
+        if lens[i] == 0:
+            assert (out[slots[i]] == 0).all()
+    assert (out[rest] == 5).all()
+    h, p, n = 2, 16, 8
+    a = make_scan(4, b[-1], h, p, 1, n, dtype)
+    ss = rnd(gen(5), k, h, p, n)
+    start = torch.stack([ss[s] if s >= 0 else torch.zeros_like(ss[0]) for s in slots])
+    ref, mag, (fin, fmag) = scan_ref(a, b, start)
+    out = torch.full_like(ss, 5.0)
+    y = ops.selective_scan(**a, offsets=i32(b), state=ss, state_out=out, slots=i32(slots))
+    within(y, ref, scan_tol(ref, mag, n, max(lens), dt, dtype == "bf16"), "y")
+    within(out[where], fin[live], state_tol(fin[live], fmag[live], max(lens), False), "state")
+    assert (out[rest] == 5).all()
+    ops.device_status()
 
 
 # ---------------------------------------------------------------- 4-bit product: ranges
