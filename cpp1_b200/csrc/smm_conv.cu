@@ -332,6 +332,8 @@ int check_conv(const char* who, const ConvParams& p, int width, int dtype, int a
   if (p.channels == 0 || (p.tokens == 0 && p.nseq == 0)) return SMM_OK;
   if (!p.w || (p.tokens > 0 && (!p.x || !p.y))) return set_error(SMM_ERR_INVALID, "%s: null pointer", who);
   const size_t e = dtype_size(dtype);
+  if (!all_aligned_to(e, p.x, p.w, p.bias, p.state_in, p.state_out, p.y) || !all_aligned_to(4, p.offsets, p.slots))
+    return set_error(SMM_ERR_INVALID, "%s: a pointer is not aligned to its elements", who);
   const Span x = row_span(p.x, p.tokens, p.channels, p.ldx, e), y = row_span(p.y, p.tokens, p.channels, p.ldy, e);
   const size_t sb = static_cast<size_t>(p.nslots) * p.channels * (width - 1) * e;
   const Span si{p.state_in, sb}, so{p.state_out, sb};

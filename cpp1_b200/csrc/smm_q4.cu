@@ -364,6 +364,8 @@ extern "C" int smm_q4_matvec(const void* q, const void* scales, const void* zero
   if (batch == 0 || rows == 0) return SMM_OK;
   if (!y || (cols > 0 && (!q || !scales || !x))) return set_error(SMM_ERR_INVALID, "smm_q4_matvec: null pointer");
   const size_t e = dtype_size(dtype);
+  if (!aligned_to(y, e) || !aligned_to(scales, dtype_size(scale_dtype)))
+    return set_error(SMM_ERR_INVALID, "smm_q4_matvec: a pointer is not aligned to its elements");
   const size_t groups = static_cast<size_t>(rows) * (cols / group);
   const Span ys = row_span(y, batch, rows, ldy, e);
   if (overlaps(ys, row_span(x, batch, cols, ldx, e)) || overlaps(ys, {q, static_cast<size_t>(rows) * (cols / 2)}) ||

@@ -620,6 +620,9 @@ int check_scan(const char* who, const ScanParams& p, int dtype, int dt_dtype, bo
   if (!p.A || (p.tokens > 0 && (!p.x || !p.dt || !p.B || !p.C || !p.y)))
     return set_error(SMM_ERR_INVALID, "%s: null pointer", who);
   const size_t e = dtype_size(dtype);
+  if (!all_aligned_to(e, p.x, p.z, p.B, p.C, p.y) || !aligned_to(p.dt, dtype_size(dt_dtype)) ||
+      !all_aligned_to(4, p.A, p.D, p.dt_bias, p.state_in, p.state_out, p.offsets, p.slots))
+    return set_error(SMM_ERR_INVALID, "%s: a pointer is not aligned to its elements", who);
   const size_t sb = static_cast<size_t>(p.nslots) * hp * p.state_dim * sizeof(float);
   const Span y = row_span(p.y, p.tokens, hp, p.ldy, e), so{p.state_out, sb}, si{p.state_in, sb};
   const Span in[] = {row_span(p.x, p.tokens, hp, p.ldx, e),

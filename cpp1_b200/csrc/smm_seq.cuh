@@ -207,6 +207,11 @@ inline bool overlaps(const Span& a, const Span& b) {
   return false;
 }
 inline bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+// All of these pointers lie on a multiple of n bytes, an element's size (null does).
+template <typename... P>
+inline bool all_aligned_to(size_t n, P... p) {
+  return (aligned_to(p, n) && ...);
+}
 inline bool valid_dtype(int d) { return d == SMM_DTYPE_F32 || d == SMM_DTYPE_BF16; }
 inline size_t dtype_size(int d) { return d == SMM_DTYPE_F32 ? 4 : 2; }
 

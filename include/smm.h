@@ -492,7 +492,8 @@ typedef enum { SMM_ACT_NONE = 0, SMM_ACT_SILU = 1 } smm_act;
  *   zero and leaves no state.  So does one whose slot is nslots or more, which
  *   also makes smm_device_status report SMM_ERR_BOUNDS.  Two sequences of one
  *   call must not share an entry.  Outputs must not overlap inputs; columns of the
- *   same rows of one matrix (equal ld) may lie side by side. */
+ *   same rows of one matrix (equal ld) may lie side by side.  Pointers are aligned
+ *   to their elements. */
 
 /* y[t][c] = act(bias[c] + sum_j w[c][j] x[t-width+1+j][c]): per channel a banded
  * lower-triangular Toeplitz matrix of `width` (2..8) diagonals times a column.

@@ -1,5 +1,6 @@
-"""Which memory the state-space entry points and the 4-bit product take for overlapping: refusals
-of outputs that share bytes with inputs, counted by rows of a common stride, on the CPU."""
+"""What the state-space entry points and the 4-bit product refuse of the memory they are given, on the
+CPU: outputs that share bytes with inputs, counted by rows of a common stride, and pointers that
+are not aligned to their elements."""
 import ctypes
 import random
 
@@ -47,3 +48,38 @@ def test_scan_columns_that_share_elements(oy, ldx, ldy):
     rc = L.smm_selective_scan(x, FAR, FAR + 4096, FAR + 8192, FAR + 16384, None, None, None, None, None, None, None,
                               x + 4 * oy, 4, 1, 0, 2, 16, 1, 8, ldx, 2, 8, 8, 0, ldy, 0, 0, 0, None, 0, None)
     assert rc == _lib.SMM_ERR_INVALID and "overlaps" in _lib.last_error()
+
+
+Q = [P0 + 4096 * i for i in range(16)]  # places 4 KB apart
+
+
+@pytest.mark.parametrize("which", range(8))
+@pytest.mark.parametrize("dtype,shift", [(0, 2), (0, 1), (1, 1)])
+def test_conv_pointers_off_their_elements(which, dtype, shift):
+    ptrs = Q[:8]  # x, w, bias, offsets, state_in, state_out, slots, y
+    ptrs[which] += shift
+    rc = _lib.load().smm_causal_conv(*ptrs, 4, 8, 4, 1, 2, 8, 8, dtype, 0, None)
+    assert rc == _lib.SMM_ERR_INVALID and "not aligned" in _lib.last_error()
+
+
+@pytest.mark.parametrize("which", range(13))
+@pytest.mark.parametrize("dtype,shift", [(0, 2), (0, 1), (1, 1)])
+def test_scan_pointers_off_their_elements(which, dtype, shift):
+    # x, dt, A, B, C, D, z, dt_bias, offsets, state_in, state_out, slots, y
+    ptrs = Q[:13]
+    ptrs[which] += shift
+    rc = _lib.load().smm_selective_scan(*ptrs, 4, 1, 2, 2, 16, 1, 8, 32, 2, 8, 8, 32, 32, dtype, dtype, 0, None, 0, None)
+    assert rc == _lib.SMM_ERR_INVALID and "not aligned" in _lib.last_error()
+    if which == 8:
+        return
+    step = ptrs[:8] + ptrs[9:]
+    rc = _lib.load().smm_selective_step(*step, 2, 2, 2, 16, 1, 8, 32, 2, 8, 8, 32, 32, dtype, dtype, 0, None)
+    assert rc == _lib.SMM_ERR_INVALID and "not aligned" in _lib.last_error()
+
+
+@pytest.mark.parametrize("which,dtype,sd,shift", [(1, 0, 0, 2), (1, 0, 1, 1), (4, 0, 0, 2), (4, 1, 0, 1), (1, 1, 0, 2)])
+def test_q4_pointers_off_their_elements(which, dtype, sd, shift):
+    ptrs = Q[:5]  # q, scales, zeros, x, y
+    ptrs[which] += shift
+    rc = _lib.load().smm_q4_matvec(*ptrs, 2, 8, 64, 64, 64, 8, dtype, sd, None)
+    assert rc == _lib.SMM_ERR_INVALID and "not aligned" in _lib.last_error()
