@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(NT == 1 ? 1024 : 512, 1) q4_kernel(const Q4Par
   const int g = lane >> 2, t = lane & 3;
   const int b0 = blockIdx.y * nb;
   const int nx = p.batch - b0 < nb ? p.batch - b0 : nb;  // rows of x here
-  const int tiles = (p.rows + 15) / 16;
+  const int tiles = (p.rows - 1) / 16 + 1;  // (rows + 15 may pass 31 bits)
   const int groups = p.cols / p.group;
   const int chunks = p.cols / kChunk;
   const int ratio = p.group / kChunk;  // chunks per group
@@ -324,7 +324,7 @@ int launch_q4(const Q4Params& p, int nb, cudaStream_t st) {
     else set();
     SMM_CUDA_TRY(err, "q4_matvec shared memory size");
   }
-  const int tiles = (p.rows + 15) / 16;
+  const int tiles = (p.rows - 1) / 16 + 1;  // (rows + 15 may pass 31 bits)
   // One CTA an SM.  Few tiles are spread over the SMs, one to a CTA.
   const dim3 grid(std::min(tiles, 148), (p.batch + nb - 1) / nb);
   kern<<<grid, kThreads, smem, st>>>(p, nb);

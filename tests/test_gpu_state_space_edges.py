@@ -469,3 +469,23 @@ def test_q4_rows_beyond_shared_memory(cuda, dtype, cols, group, batch, zeros):
         z = torch.randint(0, 16, s.shape, generator=g, device="cuda", dtype=torch.uint8) if zeros else None
         ref, mag = q4_ref(q, s, z, x)
         within(ops.q4_matvec(q, s, x, z), ref, q4_tol(ref, mag, c, group, TYPES[dtype]))
+
+
+def test_q4_most_rows(cuda):
+    """Nearly 2^31 rows of 32 columns: 34 GB of codes."""
+    rows = (1 << 31) - 3
+    q = torch.zeros(rows, 16, device="cuda", dtype=torch.uint8)
+    s = torch.ones(rows, 1, device="cuda", dtype=BF)
+    g = gen(8)
+    some = (0, rows // 2, rows - 40)
+    for r in some:
+        q[r:r + 40] = torch.randint(0, 256, (40, 16), generator=g, device="cuda", dtype=torch.uint8)
+        s[r:r + 40] = torch.rand(40, 1, generator=g, device="cuda").to(BF)
+    x = rnd(g, 1, 32, dtype=BF)
+    y = ops.q4_matvec(q, s, x)
+    for r in some:
+        ref, mag = q4_ref(q[r:r + 40], s[r:r + 40], None, x)
+        within(y[:, r:r + 40], ref, q4_tol(ref, mag, 32, 32, BF))
+    ref, mag = q4_ref(q[100:101], s[100:101], None, x)
+    assert (y[:, 100:rows // 2] == y[:, 100:101]).all()
+    within(y[:, 100:101], ref, q4_tol(ref, mag, 32, 32, BF))
