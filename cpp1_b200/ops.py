@@ -389,6 +389,8 @@ def _dims(name: str, t: torch.Tensor, dims: int):
     shape = t.shape
     if len(shape) != dims:
         raise ValueError(f"{name} has shape {tuple(shape)}, expected {dims} dimensions")
+    if max(shape) > 0x7FFFFFFF:
+        raise ValueError(f"{name} has shape {tuple(shape)}, a dimension beyond 31 bits")
     return shape
 
 

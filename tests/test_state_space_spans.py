@@ -1,13 +1,13 @@
 """What the state-space entry points and the 4-bit product refuse of the memory they are given, on the
-CPU: outputs that share bytes with inputs, counted by rows of a common stride, and pointers that
-are not aligned to their elements."""
+CPU: outputs that share bytes with inputs, counted by rows of a common stride, pointers that
+are not aligned to their elements, dimensions that do not fit the entries' integers."""
 import ctypes
 import random
 
 import pytest
 import torch
 
-from cpp1_b200 import _lib
+from cpp1_b200 import _lib, ops
 
 BUF = ctypes.create_string_buffer(1 << 18)
 P0 = (ctypes.addressof(BUF) + 255) // 256 * 256
@@ -83,3 +83,28 @@ def test_q4_pointers_off_their_elements(which, dtype, sd, shift):
     ptrs[which] += shift
     rc = _lib.load().smm_q4_matvec(*ptrs, 2, 8, 64, 64, 64, 8, dtype, sd, None)
     assert rc == _lib.SMM_ERR_INVALID and "not aligned" in _lib.last_error()
+
+
+def huge(*shape, dtype=torch.float32):
+    """A tensor of one element seen as many."""
+    return torch.zeros((), dtype=dtype).expand(shape)
+
+
+MANY = (1 << 32) + 8  # would count as 8 in 32 bits
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ops.q4_matvec(huge(MANY, 16, dtype=torch.uint8), huge(MANY, 1), torch.zeros(1, 32)),
+    lambda: ops.q4_matvec(huge(4, 16, dtype=torch.uint8), huge(4, 1), huge(MANY, 32)),
+    lambda: ops.causal_conv(huge(MANY, 4), torch.zeros(4, 4)),
+    lambda: ops.causal_conv(torch.zeros(4, 4), torch.zeros(4, 4), state=huge(MANY, 4, 3)),
+    lambda: ops.causal_conv(torch.zeros(4, 4), torch.zeros(4, 4), offsets=huge(MANY, dtype=torch.int32)),
+    lambda: ops.causal_conv_step(huge(MANY, 4), torch.zeros(4, 4), state=huge(MANY, 4, 3)),
+    lambda: ops.causal_conv_step(huge(1, MANY), huge(MANY, 4), state=huge(1, MANY, 3)),
+    lambda: ops.selective_scan(huge(MANY, 2, 16), huge(MANY, 2), torch.zeros(2), huge(MANY, 1, 8), huge(MANY, 1, 8)),
+    lambda: ops.selective_step(torch.zeros(3, 2, 16), torch.zeros(3, 2), torch.zeros(2), torch.zeros(3, 1, 8),
+                               torch.zeros(3, 1, 8), state=huge(MANY, 2, 16, 8)),
+])
+def test_dimensions_beyond_31_bits(call):
+    with pytest.raises(ValueError, match="31 bits"):
+        call()
