@@ -943,11 +943,11 @@ int launch_one(const Tmaps& maps, const ScanParams& p, unsigned grid, int ptiles
 
 // bf16, whole 16-byte pieces everywhere, state_dim of one 128-row tile, and sequences
 // long enough.  Time here goes with the chunks, a started one counting in full (32 sequences
-// of 64 heads of 64: 132 to 140 us for up to 64 tokens each), on the fp32 pipes
-// with the tokens, and state_dim adds to it.  The two cross near 19 tokens with state_dim 128
-// (fp32 pipes against this kernel: 121 and 132 us at 16 tokens, 149 and 132 at 24)
-// and near 90 with 16 (96 and 133 us at 64; 220 and 82 for 4 sequences of 1024); for one
-// sequence no later (12.3 and 10.2 us at 24 tokens).
+// of 64 heads of 64 x 128: 151 to 157 us for 16 to 32 tokens each), on the fp32 pipes
+// with the tokens, and state_dim adds to it.  The two cross near 25 tokens with state_dim 128
+// (fp32 pipes against this kernel: 138 and 151 us at 20 tokens, 149 and 152 at 24, 186 and 157
+// at 32) and near 120 with 16 (127 and 156 us at 96, 160 and 165 at 128, 214 and 177 at 160; 220 and 88
+// for 4 sequences of 1024); for one sequence no later (9.9 and 12.0 us at 16 tokens, 12.7 and 12.2 at 24).
 bool scan_umma_fits(const ScanParams& p, int dtype) {
   if (dtype != SMM_DTYPE_BF16 || p.dim % 8 || p.state_dim % 8 || p.state_dim > 128) return false;
   if (p.ldx % 8 || p.ldb % 8 || p.ldc % 8 || p.ldy % 8 || (p.z && p.ldz % 8)) return false;
@@ -955,7 +955,7 @@ bool scan_umma_fits(const ScanParams& p, int dtype) {
       !aligned_to(p.z, 16))
     return false;
   const long long ptiles = (p.dim + kP - 1) / kP;
-  return p.tokens * (p.state_dim + 15) * p.dim >= 2750 * static_cast<long long>(p.nseq) * kP * ptiles;
+  return p.tokens * (p.state_dim + 15) * p.dim >= 3500 * static_cast<long long>(p.nseq) * kP * ptiles;
 }
 
 // Segment length of the tensor-core kernel: whole chunks, so that the waves of

@@ -46,7 +46,7 @@ def on_tensor_cores(a, lens):
     t, _, p = a["x"].shape
     n = a["B"].shape[2]
     return (a["x"].dtype is BF and p % 8 == 0 and n % 8 == 0 and n <= 128
-            and t * (n + 15) * p >= 2750 * len(lens) * 64 * ((p + 63) // 64))
+            and t * (n + 15) * p >= 3500 * len(lens) * 64 * ((p + 63) // 64))
 
 
 def once_rounded_tol(ref, mag, n, longest, dtype):
