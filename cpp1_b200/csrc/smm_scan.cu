@@ -299,11 +299,14 @@ template <typename T>
 int launch_scan_type(const ScanParams& p, long long segs, cudaStream_t st) {
   auto go = [&](auto npl) {
     constexpr int NPL = decltype(npl)::value;
-    // Two dims to a lane read B and C half as often; one makes twice the warps, which is
-    // faster while there are few (38 -> 36 us for 390 warps of two dims, but 0.79 ->
-    // 0.91 ms for 512 that run eight times as long).  Then 32 dims to a CTA where 64
-    // would leave SMs without one.
-    if (segs * p.heads * ((p.dim + 7) / 8) < 400) return launch_scan<T, NPL, 256, 1>(p, segs, st);
+    // Two dims to a lane read B and C half as often; one makes twice the warps, which is faster
+    // for small states while a scheduler has one warp of two dims at most (592 of them; state_dim
+    // 16, sequences of 200 tokens, 256 to 512 warps: 19.2 us against 20.2, of 800: 68 against 72; 624
+    // warps: 24.9 against 22.9; state_dim 32, 512 warps: 23.8 against 22.7, with 128 49 against 46).
+    // Then 32 dims to a CTA where 64 would leave SMs without one.
+    if constexpr (NPL == 2) {
+      if (segs * p.heads * ((p.dim + 7) / 8) <= 592) return launch_scan<T, NPL, 256, 1>(p, segs, st);
+    }
     if (p.dim <= 32 || segs * p.heads * ((p.dim + 63) / 64) < 2 * 148) return launch_scan<T, NPL, 128, 2>(p, segs, st);
     return launch_scan<T, NPL, 256, 2>(p, segs, st);
   };
