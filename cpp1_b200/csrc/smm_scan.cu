@@ -27,10 +27,10 @@ using F2 = unsigned long long;  // two fp32 lanes
 // shuffles showed: 1.21 ms.)
 constexpr int kTile = 16;
 
-// bf16 comes here with short sequences, whose start and end want a second CTA on the SM
-// (16 tokens of 64 heads, 32 sequences: 188 -> 121 us); fp32 wants the registers.
-template <typename T, int NPL, int THREADS, int PPL, bool STATES>
-__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 512 / THREADS : 1) scan_kernel(const ScanParams p, int ptiles) {
+// bf16 comes here with short sequences, whose start and end want a second CTA on the SM (TWO;
+// 16 tokens of 64 heads, 32 sequences: 188 -> 121 us); fp32 wants the registers.
+template <typename T, int NPL, int THREADS, int PPL, bool STATES, bool TWO>
+__global__ void __launch_bounds__(THREADS, TWO ? 512 / THREADS : 1) scan_kernel(const ScanParams p, int ptiles) {
   constexpr int NP = 8 * NPL;                  // padded state_dim
   constexpr int PT = THREADS / 8 * PPL;        // dims per CTA
   constexpr int NE = kTile * NP / THREADS > 0 ? kTile * NP / THREADS : 1;
@@ -275,24 +275,36 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 ? 512 / THREADS : 1) s
   }
 }
 
-template <typename T, int NPL, int THREADS, int PPL>
-int launch_scan(const ScanParams& p, long long segs, cudaStream_t st) {
+template <typename T, int NPL, int THREADS, int PPL, bool TWO>
+int launch_scan_ctas(const ScanParams& p, unsigned grid, int ptiles, cudaStream_t st) {
   constexpr int NP = 8 * NPL, PT = THREADS / 8 * PPL;
-  const int ptiles = (p.dim + PT - 1) / PT;
-  const long long blocks = segs * p.heads * ptiles;
-  if (blocks > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "selective scan too large for one launch");
-  const unsigned grid = static_cast<unsigned>(blocks);
   const size_t full = sizeof(float) * kTile * (2 * NP + 2 * PT + 2);
   if (p.split) {
-    scan_kernel<T, NPL, THREADS, PPL, true><<<grid, THREADS, full, st>>>(p, ptiles);
+    scan_kernel<T, NPL, THREADS, PPL, true, TWO><<<grid, THREADS, full, st>>>(p, ptiles);
     count_launch();
     SMM_CUDA_TRY(cudaGetLastError(), "selective scan launch");
     if (int rc = scan_combine(p, st)) return rc;
   }
-  scan_kernel<T, NPL, THREADS, PPL, false><<<grid, THREADS, full, st>>>(p, ptiles);
+  scan_kernel<T, NPL, THREADS, PPL, false, TWO><<<grid, THREADS, full, st>>>(p, ptiles);
   count_launch();
   SMM_CUDA_TRY(cudaGetLastError(), "selective scan launch");
   return SMM_OK;
+}
+
+template <typename T, int NPL, int THREADS, int PPL>
+int launch_scan(const ScanParams& p, long long segs, cudaStream_t st) {
+  constexpr int PT = THREADS / 8 * PPL;
+  const int ptiles = (p.dim + PT - 1) / PT;
+  const long long blocks = segs * p.heads * ptiles;
+  if (blocks > 0x7FFFFFFFLL) return set_error(SMM_ERR_INVALID, "selective scan too large for one launch");
+  const unsigned grid = static_cast<unsigned>(blocks);
+  // Half of the registers spill for state_dim above 128, which a second CTA on the SM makes up for, if
+  // there is one (64 heads of state_dim 256: one sequence of 4000 tokens 3.6 ms with half, 1.8 with all
+  // of them, two of 600 577 and 382 us, but eight of 500 898 and 956, 32 of 64 497 and 593).
+  if constexpr (sizeof(T) == 2 && NPL == 32) {
+    if (blocks * THREADS <= 148 * 256) return launch_scan_ctas<T, NPL, THREADS, PPL, false>(p, grid, ptiles, st);
+  }
+  return launch_scan_ctas<T, NPL, THREADS, PPL, sizeof(T) == 2>(p, grid, ptiles, st);
 }
 
 template <typename T>

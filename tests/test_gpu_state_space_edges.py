@@ -108,6 +108,22 @@ def test_bf16_recurrence_sums_in_32_bits(cuda, lens, h, p, g_, n):
     within(so, fin, state_tol(fin, fmag, longest, False), "state")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,h,p,n", [([40, 7, 65], 64, 64, 256), ([40, 7, 65], 16, 64, 256), ([30] * 9, 72, 20, 136),
+                                        ([200], 64, 64, 200), ([50, 90], 96, 64, 16), ([50, 90], 9, 64, 12)])
+def test_recurrence_variants(cuda, dtype, lens, h, p, n):
+    """Both sides of the recurrence's choices: one or two dims a lane, one or two CTAs on an SM."""
+    b = offs(lens)
+    a = make_scan(h + n, b[-1], h, p, 1, n, dtype)
+    st = rnd(gen(n), len(lens), h, p, n)
+    ref, mag, (fin, fmag) = scan_ref(a, b, st)
+    so = torch.empty_like(st)
+    y = ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so)
+    tensor = on_tensor_cores(a, lens)
+    within(y, ref, (once_rounded_tol if tensor else lambda *v: scan_tol(*v, False))(ref, mag, n, max(lens), TYPES[dtype]), "y")
+    within(so, fin, state_tol(fin, fmag, max(lens), tensor), "state")
+
+
 # ---------------------------------------------------------------- giving up
 @pytest.mark.parametrize("lens,h,n", [([700, 37, 260], 160, 128), ([100] * 40, 24, 64), ([6000], 2, 128), ([5000, 90], 3, 64)])
 def test_scan_that_gives_up_leaves_cleanly(cuda, lens, h, n):
