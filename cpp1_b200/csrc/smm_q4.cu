@@ -26,7 +26,9 @@
 // that the products take it.  64 registers a thread leave little to prefetch with:
 // the 32 warps' loads cover for one another.  8192 x 4096 with one row takes 9.3 us (1.2
 // for the launch, 0.7 for x, 4.3 until the codes are there, then the unpacking),
-// 8200 x 8192 with eight rows and zero points 19 us, with two sets of codes in turn 21.7.
+// 8200 x 8192 with eight rows and zero points 19 us (with two sets of codes in turn 8.9 and 21.1
+// where a set is one chunk, 10.6 and 23.3 where it is two).  Of the instances for fp32 x those of 1024
+// threads spill (4 to 124 bytes a thread).
 #include "smm_seq.cuh"
 
 #include <algorithm>

@@ -28,16 +28,15 @@
 // A CTA takes one (segment, head, 64 dims), the hardware hands out the next as an SM
 // becomes free.  (A CTA an SM that walked a fixed share of them as one stream of chunks
 // saved their starts but shared out ragged ones badly: prompts of 16 tokens 195 -> 170 us,
-// but 8190 ragged tokens of 24 sequences 107 -> 126, before the states were
-// loaded all at once.)  Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the
+// but 8190 ragged tokens of 24 sequences 107 -> 126, in an earlier form.)  Warps: 0 loads (TMA), 1 issues the products, 2 and 3 compute the
 // decays in turn, 4-11 form G and write y of the chunk before, half of the columns each,
 // 12-19 form Xw, 20-23 carry the state.  Every wait is bounded; on expiry the CTA records
 // it and leaves.
 //
-// 4096 tokens of 64 heads of 64 x 128 take 101 us, 8190 ragged ones of 32 heads 83 us,
-// 32768 of 80 heads 0.78 ms: 3.3 us a chunk, no one unit's time but the mix of a chunk's way
-// through the roles (6000 clocks), shared memory (4000) and the issue of 3000
-// instructions a scheduler.
+// 4096 tokens of 64 heads of 64 x 128 take 112 us, 8190 ragged ones of 32 heads 93 us,
+// 32768 of 80 heads 0.86 ms.  No one unit's time (tensor pipe 28 % busy, issue slots 44 %, shared
+// memory 46 %) but a chunk's way through the roles.  (With one bf16 term for G and H, and NaN of x
+// reaching the tokens before it: 101, 83 and 0.78.)
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -337,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // In every role below, stages, buffers and barriers' phases go by the chunk c.
   //
   // The launch's 6 x 80 registers per warpgroup's thread, shared out by need.
-  // A spill costs a trip to L2 here: shared memory leaves L1 too small for the stacks.
+  // A spill costs a trip to L2 here: shared memory leaves L1 too small for the stacks (64 bytes a
+  // thread remain in the last launch; splits that left 88 and 132 took 4 and 3 % longer).
   constexpr int kRegsMisc = 48, kRegsG = STATES ? 24 : 112, kRegsXw = 56, kRegsState = STATES ? 152 : 96;
   static_assert(kRegsMisc + 2 * kRegsG + 2 * kRegsXw + kRegsState <= 6 * 80, "more registers than the launch has");
   if (warp < 4) {

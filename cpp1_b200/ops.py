@@ -603,7 +603,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         y_t = (S_t C_t,g + D_h x_t) * silu(z_t)
 
     x, z, y (tokens, heads, dim) and B, C (tokens, groups, state_dim) float32 or
-    bfloat16, dt (tokens, heads) of the same type or float32; A, D, dt_bias
+    bfloat16, dt (tokens, heads) of the same type or float32; A (one decay rate a head), D, dt_bias
     (heads) float32.  dim and state_dim are 1 to 256.  Rows may be strided (x, B and
     C columns of one matrix).  Sums, decays and states are float32; longer bfloat16 prompts go through
     the tensor cores, where scores and states enter products as two bfloat16 terms (2^-17 relative).
@@ -672,7 +672,9 @@ def q4_matvec(q: torch.Tensor, scales: torch.Tensor, x: torch.Tensor, zeros: Opt
     q (rows, cols/2) uint8 holds code 2i of a row in the low half of byte i; scales
     (rows, cols/group), of x's type or float32, and zeros (same shape, uint8, 0..127; None:
     8 everywhere) give the group, a multiple of 32.  x float32 or bfloat16; products are
-    exact and sums float32 in both.  Returns (batch, rows)."""
+    exact and sums float32 in both (over x times codes, before the scale).  Returns (batch, rows).
+
+    For a few rows: at most 65535, and q is read again for every 8 or 16 of them."""
     batch, cols = _dims("x", x, 2)
     ty = _x_dtype(x)
     if cols % 2:

@@ -551,7 +551,8 @@ int smm_selective_step(const void* x, const void* dt, const float* A, const void
  * (X W^T for a few rows x).  q holds rows x cols/2 bytes, code 2i of a row in
  * the low half of byte i; scales and zeros (bytes of 0 to 127; NULL: 8 everywhere)
  * are rows x cols/group.  group is a multiple of 32 and divides cols.  x and y have dtype
- * elements, scales scale_dtype.  Products are exact and sums fp32, also for fp32 x.
+ * elements, scales scale_dtype.  Products are exact and sums fp32, also for fp32 x
+ * (over x times codes, before the scale).  q is read again for every 8 or 16 rows of x.
  * q, x and x's rows are 16-byte aligned; batch is at most 65535.  y must not overlap
  * an input.  No counterpart in the reference. */
 int smm_q4_matvec(const void* q, const void* scales, const void* zeros, const void* x, void* y, int batch, int rows,
