@@ -180,6 +180,44 @@ def test_tokens_behind_a_reset(cuda, dtype, strength, empty):
     within(so, fin, state_tol(fin, fmag, 300, False) + sums * fmag, "state")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("every", [2, 5])
+def test_resets_all_over(cuda, dtype, every):
+    """Every second (fifth) token forgets."""
+    t, h, n = 260, 4, 64
+    a = make_scan(4, t, h, 64, 1, n, dtype, strided=False, dt_f32=True)
+    a["dt"] = 0.01 + 0.1 * torch.rand(t, h, generator=gen(5), device="cuda")
+    a["dt"][1::every] = 2e4
+    a["x"][1::every] = 0
+    a["dt_bias"], a["dt_softplus"] = None, False
+    a["A"] = torch.tensor([-1.0, -0.01, -8.0, -0.5], device="cuda")
+    ref, mag, (fin, fmag) = scan_ref(a, [0, t], None)
+    so = torch.empty(1, h, 64, n, device="cuda")
+    y = ops.selective_scan(**a, state_out=so)
+    sums = 10 * U * 0.7 * (32 / every * 130 + 32 * 0.11 * 8 * 1.45)  # as in test_tokens_behind_a_reset
+    tol = once_rounded_tol(ref, mag, n, t, TYPES[dtype]) + (sums * mag if dtype == "bf16" else 0)
+    within(y, ref, tol, "y")
+    within(so, fin, state_tol(fin, fmag, t, False) + sums * fmag, "state")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,h", [([300, 17], 4), ([3000], 4)])
+def test_states_that_grow(cuda, dtype, lens, h):
+    """Steps of both signs and rates of both signs: states grow and shrink."""
+    b = offs(lens)
+    n = 128
+    a = make_scan(5, b[-1], h, 64, 1, n, dtype, strided=False, dt_f32=True)
+    a["dt"] = 0.6 * torch.rand(b[-1], h, generator=gen(7), device="cuda") - 0.3
+    a["dt_bias"], a["dt_softplus"] = None, False
+    a["A"] = torch.tensor([0.3, -0.3, 0.05, 0.0], device="cuda")
+    st = rnd(gen(8), len(lens), h, 64, n)
+    ref, mag, (fin, fmag) = scan_ref(a, b, st)
+    so = torch.empty_like(st)
+    y = ops.selective_scan(**a, offsets=i32(b), state=st, state_out=so)
+    within(y, ref, once_rounded_tol(ref, mag, n, max(lens), TYPES[dtype]), "y")
+    within(so, fin, state_tol(fin, fmag, max(lens), dtype == "bf16"), "state")
+
+
 # ---------------------------------------------------------------- non-finite inputs
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("lens,h,p,n", [([140, 70, 300], 2, 64, 128), ([128, 128], 3, 128, 64), ([5, 9, 16], 4, 64, 16), ([6000], 2, 64, 128)])
